@@ -363,6 +363,116 @@ int tt_attn_prefill_causal_selected(tt_context *ctx, tt_stream stream, const voi
                                     const uint32_t *keep_indices, uint32_t keep_index_stride,
                                     const uint32_t *keep_counts, const uint32_t *keep_rows);
 
+/* ------------------------------- attention over a bounded or shared cache */
+
+/* No counterparts in the reference, whose caches grow with every token of every session. The calls
+ * of this section are the operators of a server that bounds or shares them; they use the sessions,
+ * strides, streams, workspace and errors of the calls above, fp16 or bf16 rows, head_dim 64, 128 or
+ * 256 for decode. Batches of any size up to max_sessions; during a stream capture, decode batches of
+ * up to 64 sessions (8 prefix groups), whose tables travel in the kernel parameters (larger ones
+ * are refused with TT_ERR_UNSUPPORTED_SHAPE; accumulate and evict take any). Captured calls use the
+ * context's workspace when replayed: like calls, graphs of one context must not overlap on the GPU. */
+
+/* Sinks: row r of a session (causal end e = seq_len - (q_rows - 1 - r)) sees key j when j < e and
+ * (j < sink_tokens or j >= e - window); window 0 = no window. A row without visible keys gives
+ * zeros. Key j is cache row j, or with ring_capacity R > 0 (window > 0 then) row
+ * j < sink_tokens ? j : sink_tokens + (j - sink_tokens) % R, a cache of sink_tokens + R rows for an
+ * endless session; R >= window + q_rows - 1 once a session has wrapped. kv_start must be 0. Cache
+ * rows that no query row sees are not read and may hold anything. */
+int tt_attn_decode_sink_window(tt_context *ctx, tt_stream stream, const tt_attn_session *sessions,
+                               uint32_t n_sessions, const tt_attn_batch_params *params,
+                               uint32_t sink_tokens, uint32_t window, uint32_t ring_capacity);
+/* The keys such a session reads (host arithmetic): the first key of its rows' windows behind the
+ * sinks, and how many keys at least one of its rows may see. */
+int tt_attn_sink_keys(uint32_t seq_len, uint32_t q_rows, uint32_t sink_tokens, uint32_t window,
+                      uint32_t *out_window_start, uint32_t *out_keys);
+/* The same visibility for a prompt chunk (params as tt_attn_prefill_causal, sliding_window = the
+ * window, 16-bit rows). All rows of the chunk are in the cache: with a ring,
+ * R >= window + (kv_valid_count - start_position) - 1 once it has wrapped. Runs on the tcgen05
+ * kernel where tt_attn_prefill_causal does and R is a multiple of 64 (or 0), else on the generic
+ * kernel; tt_attn_prefill_sink_path tells which (1 / 0). Without a ring, rows between the sinks and
+ * the first query's window may hold anything; a ring's rows must be finite. */
+int tt_attn_prefill_sink_window(tt_context *ctx, tt_stream stream, const void *q, const void *k,
+                                const void *v, void *out, const tt_prefill_params *params,
+                                uint32_t sink_tokens, uint32_t ring_capacity, uint32_t io_dtype);
+int tt_attn_prefill_sink_path(const void *q, const void *k, const void *v, const void *out,
+                              const tt_prefill_params *params, uint32_t ring_capacity);
+
+/* Shared prefix: the sessions of a group continue the same prefix_len tokens, whose K/V rows exist
+ * once. Every query row sees the whole prefix of its group and the keys of its own session as in
+ * tt_attn_decode_batched (session k, v, seq_len describe the rows behind the prefix; seq_len may be
+ * q_rows - 1, kv_start must be 0). groups[g] owns the next n_sessions entries of `sessions`; the
+ * counts add up to the batch. The prefix is streamed once per 128 packed query rows of a KV head
+ * (sessions x q_rows x n_q_heads / n_kv_heads), not once per session. */
+typedef struct tt_attn_prefix {
+    const void *k; /* row 0 of the prefix, params->kv_token_stride_elements apart */
+    const void *v;
+    uint32_t prefix_len; /* 0: the group has no prefix */
+    uint32_t n_sessions;
+} tt_attn_prefix;
+int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const tt_attn_prefix *groups,
+                                 uint32_t n_groups, const tt_attn_session *sessions,
+                                 uint32_t n_sessions, const tt_attn_batch_params *params);
+/* The split of the prefix pass (host arithmetic): keys per work item (a multiple of 128) for groups
+ * of the given prefix lengths and query rows (sessions x q_rows), and the number of items.
+ * TT_ERR_OOM when the partials do not fit workspace_bytes (0 = no limit). */
+int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_t *query_rows,
+                               uint32_t n_groups, uint32_t head_dim, uint32_t n_q_heads,
+                               uint32_t n_kv_heads, uint32_t sm_count, size_t workspace_bytes,
+                               uint32_t *out_keys_per_item, uint32_t *out_n_items);
+
+/* tt_attn_decode_batched (kv_start 0) that also adds up how much attention every cached row gets:
+ * weights[h * head_stride + j] += the softmax weight of key j, summed over the session's query rows
+ * and the query heads of KV head h. The last fresh_rows rows of the session are new since the last
+ * call: their sums start from zero whatever stood there, and positions (when given) records their
+ * token positions, end_position - fresh_rows .. end_position - 1. A decode step has
+ * fresh_rows = q_rows; the first call after a prompt has fresh_rows = seq_len, with the prompt's
+ * last queries as its rows. Entries at seq_len and beyond are left alone. Sums are deterministic. */
+typedef struct tt_attn_weight_rows {
+    float *weights;      /* KV head 0; the heads are head_stride elements apart */
+    uint32_t *positions; /* nullable, same layout */
+    uint32_t fresh_rows;
+    uint32_t end_position;
+} tt_attn_weight_rows;
+int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt_attn_session *sessions,
+                              const tt_attn_weight_rows *weight_rows, uint32_t n_sessions,
+                              const tt_attn_batch_params *params, uint32_t head_stride);
+
+/* Eviction: every KV head of a session keeps `budget` of its `rows` cache rows -- those whose
+ * position is below sink_tokens or at least end_position - recent_tokens, then by weight descending
+ * (NaN last), ties to the lower row -- and the kept rows are compacted: a kept row below `budget`
+ * stays, the rows given up there are filled in ascending order by the kept rows above. K, V,
+ * weights and positions follow. Afterwards the session has min(rows, budget) rows per head, in an
+ * order of their own per head, which plain decode attention over min(rows, budget) keys does not
+ * see (keys carry their rotation). Each *_out is NULL or its input for in place, or a buffer that
+ * does not overlap the input; positions NULL = row j holds position j. Sessions with rows <= budget
+ * keep everything (and are copied where an *_out is given). Entries behind the kept rows are left
+ * as they were. head_dim 64, 128 or 256; sink_tokens + recent_tokens <= budget. Sessions must not
+ * share buffers. */
+typedef struct tt_kv_evict_session {
+    void *k; /* row 0 of the session */
+    void *v;
+    void *k_out;
+    void *v_out;
+    float *weights;
+    float *weights_out;
+    uint32_t *positions;
+    uint32_t *positions_out;
+    uint32_t rows;
+    uint32_t end_position; /* position of the next token */
+} tt_kv_evict_session;
+typedef struct tt_kv_evict_params {
+    uint32_t head_dim, n_kv_heads;
+    uint32_t budget, sink_tokens, recent_tokens;
+    uint32_t kv_token_stride_elements;     /* 0: n_kv_heads * head_dim */
+    uint32_t kv_out_token_stride_elements; /* 0: kv_token_stride_elements */
+    uint32_t weight_head_stride;           /* elements between the heads of weights / positions */
+    uint32_t weight_out_head_stride;       /* 0: weight_head_stride */
+    uint32_t reserved;
+} tt_kv_evict_params;
+int tt_kv_evict(tt_context *ctx, tt_stream stream, const tt_kv_evict_session *sessions,
+                uint32_t n_sessions, const tt_kv_evict_params *params);
+
 /* ----------------------------------------- sparse-attention block indexer */
 
 /* QSAIndexer's device work (sources/TinyTitan/Kernels/Attention/QSAIndexer.swift,

@@ -52,6 +52,26 @@ class AttnBatchParams(C.Structure):
                 ("out_row_stride_elements", C.c_uint32), ("scale", C.c_float), ("io_dtype", C.c_uint32)]
 
 
+class AttnPrefix(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("prefix_len", C.c_uint32), ("n_sessions", C.c_uint32)]
+
+
+class AttnWeightRows(C.Structure):
+    _fields_ = [("weights", C.c_void_p), ("positions", C.c_void_p), ("fresh_rows", C.c_uint32),
+                ("end_position", C.c_uint32)]
+
+
+class KVEvictSession(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_out", "v_out", "weights", "weights_out", "positions",
+                                          "positions_out")] + [("rows", C.c_uint32), ("end_position", C.c_uint32)]
+
+
+class KVEvictParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in (
+        "head_dim", "n_kv_heads", "budget", "sink_tokens", "recent_tokens", "kv_token_stride_elements",
+        "kv_out_token_stride_elements", "weight_head_stride", "weight_out_head_stride", "reserved")]
+
+
 class SplitGeometry(C.Structure):
     _fields_ = [("effective_length", C.c_uint32), ("num_chunks", C.c_uint32), ("chunk_length", C.c_uint32),
                 ("partial_threadgroups", C.c_uint32), ("use_swa_grouped_partial", C.c_uint32)]
@@ -177,6 +197,16 @@ SIGNATURES = {
     "tt_gdn_step": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(GdnShape), _u32, _u32, _vp]),
     "tt_gdn_step_batched": (C.c_int, [_vp, _vp, C.POINTER(GdnSession), _u32, _vp, _vp, C.POINTER(GdnShape), _u32,
                                       _u32]),
+    "tt_attn_decode_sink_window": (C.c_int, [_vp, _vp, _vp, _u32, C.POINTER(AttnBatchParams), _u32, _u32, _u32]),
+    "tt_attn_sink_keys": (C.c_int, [_u32, _u32, _u32, _u32, C.POINTER(_u32), C.POINTER(_u32)]),
+    "tt_attn_prefill_sink_window": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(PrefillParams), _u32, _u32,
+                                              _u32]),
+    "tt_attn_prefill_sink_path": (C.c_int, [_vp, _vp, _vp, _vp, C.POINTER(PrefillParams), _u32]),
+    "tt_attn_decode_shared_prefix": (C.c_int, [_vp, _vp, _vp, _u32, _vp, _u32, C.POINTER(AttnBatchParams)]),
+    "tt_attn_plan_prefix_splits": (C.c_int, [C.POINTER(_u32), C.POINTER(_u32), _u32, _u32, _u32, _u32, _u32,
+                                             C.c_size_t, C.POINTER(_u32), C.POINTER(_u32)]),
+    "tt_attn_decode_accumulate": (C.c_int, [_vp, _vp, _vp, _vp, _u32, C.POINTER(AttnBatchParams), _u32]),
+    "tt_kv_evict": (C.c_int, [_vp, _vp, _vp, _u32, C.POINTER(KVEvictParams)]),
     "tt_gdn_scan_chunked": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(GdnShape), _u32, _u32,
                                       _u32]),
     "tt_gdn_conv_mix": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, C.c_int]),

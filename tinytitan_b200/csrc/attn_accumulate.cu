@@ -1,0 +1,226 @@
+// Decode attention that also adds every cached row's attention weight to a running statistic.
+//
+// A cache of a fixed number of rows keeps the rows that attention has used: the statistic of row j of a KV head is
+// A[j] += sum over the session's query rows r and the head's query heads g of softmax(q_rg . K^T * scale)[j].
+// A weight needs the maximum and the sum of its whole row, which exist only after all splits of the key range are
+// done. Instead of reading K a second time, pass 1 (attn_pass1.cuh) leaves the raw scores behind (4 bytes per key and
+// query head next to the 4 * head_dim bytes of K and V it reads per key and KV head; they mostly stay in L2), the
+// usual merge writes the output rows, and the kernel below forms the weights from the scores. The sums it divides by
+// are those of the unrounded weights: the output divides by the sum of the ROUNDED ones its P.V product used, whose
+// error (2^-9 with bf16 weights) the statistic, in 32 bits, would otherwise collect step after step.
+// Every statistic is written by one thread in a fixed order, so results do not depend on the schedule.
+#include "attn_pass1.cuh"
+
+namespace {
+
+constexpr uint32_t kAccThreads = 256;
+constexpr uint32_t kAccKeys = 512;        // keys of one CTA
+
+struct AccSession {
+    const float *scores;
+    float *weights;              // row 0 of KV head 0
+    uint32_t *positions;         // nullable
+    uint32_t seq_len;            // keys the scores cover
+    uint32_t total_len;          // keys of the whole session (>= seq_len when its rows are taken in several passes)
+    uint32_t q_rows;
+    uint32_t n_parts, partial_base;
+    uint32_t fresh_begin;        // rows from here on start at zero (total_len: none)
+    uint32_t end_position;
+    uint32_t block_begin;        // CTAs of the sessions before this one
+};
+
+struct AccTable {
+    AccSession s[kParamSessions];
+    uint32_t n;
+};
+
+// grid = sum over sessions of (KV heads x key chunks). One thread per key; the rows' normalisers are merged from the
+// parts' (max, sum) by one warp per row first.
+__global__ void __launch_bounds__(kAccThreads)
+attn_accumulate_kernel(const __grid_constant__ AccTable table, const float *__restrict__ part_m2,
+                       const float *__restrict__ part_l2, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t row_pad,
+                       uint32_t head_stride, float scale_log2) {
+    extern __shared__ float norm[];           // log2 of the softmax denominator of every packed row
+    pdl_launch_dependents();
+    pdl_wait();
+    uint32_t lo = 0, hi = table.n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (table.s[mid].block_begin <= blockIdx.x) lo = mid; else hi = mid;
+    }
+    const AccSession &ses = table.s[lo];
+    const uint32_t local = blockIdx.x - ses.block_begin;
+    const uint32_t kv_head = local % n_kv_heads, chunk = local / n_kv_heads;
+    const uint32_t group = n_q_heads / n_kv_heads;
+    const uint32_t rows = ses.q_rows * group, rows_padded = (rows + row_pad - 1) / row_pad * row_pad;
+    const uint32_t rows_total = ses.q_rows * n_q_heads;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (uint32_t r = warp; r < rows; r += kAccThreads / 32) {
+        const size_t base = (size_t)ses.partial_base + (r / group) * n_q_heads + kv_head * group + r % group;
+        float m = -INFINITY;
+        for (uint32_t c = lane; c < ses.n_parts; c += 32) m = fmaxf(m, part_m2[base + (size_t)c * rows_total]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        float l = 0.f;
+        if (m != -INFINITY)
+            for (uint32_t c = lane; c < ses.n_parts; c += 32) {
+                const size_t at = base + (size_t)c * rows_total;
+                l += part_l2[at] * exp2f(part_m2[at] - m);
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) norm[r] = l > 0.f ? m + log2f(l) : INFINITY;      // a row that sees nothing weighs nothing
+    }
+    __syncthreads();
+    const float *scores = ses.scores + (size_t)kv_head * ses.seq_len * rows_padded;
+    const uint32_t key_end = min(ses.total_len, (chunk + 1) * kAccKeys);
+    for (uint32_t key = chunk * kAccKeys + threadIdx.x; key < key_end; key += kAccThreads) {
+        float sum = 0.f;
+        if (key < ses.seq_len) {
+            const float *row = scores + (size_t)key * rows_padded;
+            // query row w of q_rows sees keys below seq_len - (q_rows - 1 - w)
+            const uint32_t hidden = key + ses.q_rows > ses.seq_len ? key + ses.q_rows - ses.seq_len : 0u;   // first rows that do not see it
+            for (uint32_t r = hidden * group / 4 * 4; r < rows; r += 4) {
+                const float4 s = *reinterpret_cast<const float4 *>(row + r);
+                const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (r + j < rows && r + j >= hidden * group) sum += exp2f(fmaf(v[j], scale_log2, -norm[r + j]));
+            }
+        }
+        const size_t at = (size_t)kv_head * head_stride + key;
+        const bool fresh = key >= ses.fresh_begin;
+        if (fresh && ses.positions != nullptr) ses.positions[at] = ses.end_position - (ses.total_len - key);
+        ses.weights[at] = fresh ? sum : ses.weights[at] + sum;
+    }
+}
+
+uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+}  // namespace
+
+cudaError_t tt_launch_pass1_scores(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items, const TTDecodeSession *sessions,
+                                   const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t *status,
+                                   const TTSessionTable &table, uint32_t table_keys, bool wide_rows, uint32_t hpc) {
+    PassExtra<kPassScores> extra;
+    extra.part_m2 = form.part_m2;
+    extra.part_l2 = form.part_l2;
+    if (p->io_dtype == TT_F16)
+        return launch_partial_hd<__half>(stream, n_items, items, sessions, form.part_o, form.part_m, form.part_l, p, status,
+                                         table, table_keys, wide_rows, hpc, extra);
+    return launch_partial_hd<__nv_bfloat16>(stream, n_items, items, sessions, form.part_o, form.part_m, form.part_l, p, status,
+                                            table, table_keys, wide_rows, hpc, extra);
+}
+
+TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt_attn_session *sessions,
+                                     const tt_attn_weight_rows *weight_rows, uint32_t n_sessions,
+                                     const tt_attn_batch_params *params, uint32_t head_stride) {
+    TT_ENTER(ctx);
+    if (params == nullptr || ((sessions == nullptr || weight_rows == nullptr) && n_sessions != 0))
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "sessions, weight rows and params must not be null");
+    if (params->n_kv_heads == 0 || params->n_q_heads == 0 || params->n_q_heads % params->n_kv_heads != 0)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_q_heads must be a multiple of n_kv_heads");
+    if (params->n_q_heads > 96) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_q_heads exceeds 96");
+    if (!(params->scale > 0.f)) return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "accumulated weights need a positive scale");
+    const uint32_t group = params->n_q_heads / params->n_kv_heads;
+    for (uint32_t i = 0; i < n_sessions; ++i) {
+        const tt_attn_session &s = sessions[i];
+        const tt_attn_weight_rows &w = weight_rows[i];
+        if (s.kv_start != 0) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: kv_start must be 0", i);
+        if (s.q_rows == 0 || s.q_rows > 64) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: q_rows must be in 1..64", i);
+        if (s.seq_len > (uint32_t)INT32_MAX || s.seq_len + 1 < s.q_rows)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: seq_len %u cannot hold %u query rows", i, s.seq_len, s.q_rows);
+        if (w.weights == nullptr) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has no weight row", i);
+        if (((uintptr_t)w.weights | (uintptr_t)w.positions) & 3)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: weight and position rows must be 4-byte aligned", i);
+        if (s.seq_len > head_stride)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: %u keys do not fit a weight row of %u", i, s.seq_len, head_stride);
+        if (w.fresh_rows > s.seq_len)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: %u fresh rows of %u", i, w.fresh_rows, s.seq_len);
+    }
+    // The scores of one pass share the workspace with its split partials: at most half of it. A batch that needs more
+    // is taken in several passes, by sessions first, then by the query rows of one session.
+    const size_t score_budget = ctx->workspace_bytes / 2 / 16 * 16;
+    static thread_local AccTable table;
+    uint32_t i = 0, row_done = 0;
+    while (i < n_sessions) {
+        bool wide_rows = false;
+        // rows taken per session decide the padding (8 packed rows, or 16 as soon as one session has more)
+        size_t bytes = 0;
+        uint32_t count = 0, rows_of_first = 0;
+        TTDecodeSession *tmp = ctx->h_sessions_in;
+        for (uint32_t pass = 0; pass < 2; ++pass) {
+            // pass 0: with 8-row padding when every session of the call fits it; pass 1: 16-row padding
+            const uint32_t pad = pass == 0 ? 8u : 16u;
+            bytes = 0; count = 0; wide_rows = false;
+            for (uint32_t k = i; k < n_sessions && count < kParamSessions; ++k) {
+                uint32_t rows = sessions[k].q_rows - (k == i ? row_done : 0u);
+                auto need = [&](uint32_t r) {
+                    return (size_t)params->n_kv_heads * sessions[k].seq_len * ((r * group + pad - 1) / pad * pad) * sizeof(float);
+                };
+                if (bytes + need(rows) > score_budget) {
+                    if (count != 0) break;
+                    while (rows > 1 && need(rows) > score_budget) --rows;
+                    if (need(rows) > score_budget)
+                        return tt_set_error(ctx, TT_ERR_OOM, "the scores of session %u do not fit the context workspace", k);
+                }
+                bytes += (need(rows) + 15) / 16 * 16;
+                wide_rows |= rows * group > 8;
+                if (count == 0) rows_of_first = rows;
+                ++count;
+                if (rows != sessions[k].q_rows - (k == i ? row_done : 0u)) break;      // a session cut by rows ends its pass
+            }
+            if (!wide_rows) break;
+        }
+        const uint32_t pad = wide_rows ? 16u : 8u;
+        float *scores = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->partials) + (ctx->workspace_bytes / 16 * 16 - (bytes + 255) / 256 * 256));
+        table.n = count;
+        uint32_t blocks = 0, max_rows = 0;
+        for (uint32_t c = 0; c < count; ++c) {
+            const tt_attn_session &s = sessions[i + c];
+            const uint32_t skip = c == 0 ? row_done : 0u, rows = c == 0 ? rows_of_first : s.q_rows;
+            TTDecodeSession &d = tmp[c];
+            d.q = reinterpret_cast<const unsigned char *>(s.q) + (size_t)skip * params->q_row_stride_elements * 2;
+            d.out = reinterpret_cast<unsigned char *>(s.out) + (size_t)skip * params->out_row_stride_elements * 2;
+            if (s.q == nullptr || s.out == nullptr) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has a null buffer", i + c);
+            d.k = s.k; d.v = s.v;
+            d.seq_len = s.seq_len - (s.q_rows - skip - rows); d.q_rows = rows; d.kv_start = 0;
+            d.n_parts = 0; d.partial_base = 0; d.ring_capacity = 0; d.keep = nullptr; d.scores = scores;
+            AccSession &a = table.s[c];
+            a.scores = scores;
+            a.weights = weight_rows[i + c].weights; a.positions = weight_rows[i + c].positions;
+            a.seq_len = d.seq_len; a.total_len = s.seq_len; a.q_rows = rows;
+            a.fresh_begin = skip == 0 ? s.seq_len - weight_rows[i + c].fresh_rows : s.seq_len;
+            a.end_position = weight_rows[i + c].end_position;
+            a.block_begin = blocks;
+            blocks += ceil_div(s.seq_len, kAccKeys) * params->n_kv_heads;
+            const uint32_t padded = (rows * group + pad - 1) / pad * pad;
+            scores += ((size_t)params->n_kv_heads * d.seq_len * padded + 3) / 4 * 4;
+            if (rows * group > max_rows) max_rows = rows * group;
+        }
+        TTDecodeForm form;
+        form.form = kPassScores;
+        form.reserved_bytes = (bytes + 255) / 256 * 256 + 16;
+        int rc = tt_launch_decode(ctx, (cudaStream_t)stream, tmp, count, params, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &form);
+        if (rc != TT_OK) return rc;
+        for (uint32_t c = 0; c < count; ++c) {
+            table.s[c].n_parts = ctx->h_sessions[c].n_parts;
+            table.s[c].partial_base = ctx->h_sessions[c].partial_base;
+        }
+        if (blocks != 0) {
+            const cudaError_t e = tt_launch_pdl(attn_accumulate_kernel, dim3(blocks), dim3(kAccThreads), max_rows * sizeof(float),
+                                                (cudaStream_t)stream, table, form.part_m2, form.part_l2, params->n_q_heads,
+                                                params->n_kv_heads, pad, head_stride, params->scale * kLog2e);
+            if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_accumulate launch");
+            ctx->launches++;
+        }
+        // the next pass: the rest of a cut session, or the sessions behind it
+        if (count == 1 && row_done + rows_of_first < sessions[i].q_rows) {
+            row_done += rows_of_first;
+        } else {
+            i += count;
+            row_done = 0;
+        }
+    }
+    return TT_OK;
+}

@@ -14,7 +14,7 @@
 // with quad shuffles. Pass 2 merges the items of a session by log-sum-exp. A call with one
 // session carries it in the kernel parameters (no table upload), which also makes that call
 // capturable in a CUDA graph.
-#include "tt_sm100.h"
+#include "attn_pass1.cuh"
 
 #include <algorithm>
 #include <cstdlib>
@@ -22,393 +22,7 @@
 
 namespace {
 
-constexpr int kKeysPerBlock = 16;   // keys per warp pipeline stage
-constexpr int kStages = 3;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr));
-}
-
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr));
-}
-
-template <typename T>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                          uint32_t b1);
-
-template <>
-__device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t (&a)[4],
-                                                  uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <>
-__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4],
-                                                         uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Shared memory of the fp16/bf16 pass-1 kernel for HPC KV heads per CTA.
-template <int HD, int HPC>
-struct DecodeSmem {
-    static constexpr int kPitch = HPC * HD + 8;                    // elements per staged row (all HPC heads of a key)
-    static constexpr int kRowBytes = kPitch * 2;
-    static constexpr int kTileBytes = kKeysPerBlock * kRowBytes;   // one K (or V) block
-    static constexpr int kVRing = kStages * kTileBytes;            // K ring first, V ring behind it
-    static constexpr int kRingBytes = 2 * kStages * kTileBytes;
-    static constexpr int kScorePitch = 24;                         // floats per query row of a handed-over score tile
-    static constexpr int kScoreTile = 16 * kScorePitch;            // [query row][key]
-    static constexpr int kScoreBytes = HPC * 2 * kScoreTile * 4;   // [head][buffer]
-    static constexpr int kBars = 4 * kStages + 4 * HPC;            // k_full, v_full, k_empty, v_empty [kStages]; s_full, s_empty [HPC][2]
-    static constexpr int kTotal = kRingBytes + kScoreBytes + kBars * 8;
-};
-
 __device__ __forceinline__ void pair_barrier() { asm volatile("bar.sync 1, 64;" ::: "memory"); }
-
-// ---------------------------------------------------------------------------------------
-// Pass 1. grid = items, block = 2 * HPC warps; 4 / HPC CTAs per SM.
-//
-// A work item is (session, HPC adjacent KV heads, up to 16 packed query rows per head, key range).
-// With HPC = 2 a CTA streams whole cache rows (both KV heads of a key, 1 KB at head_dim 256) so
-// that DRAM is read in long contiguous pieces; a pure streaming read of 512-byte pieces at a 1 KB
-// pitch measured 6.6 TB/s on this part against 7.1 TB/s for whole rows.
-//
-// The warps of a CTA have different jobs and run one block apart. Both products are TRANSPOSED so
-// that the 8-wide N dimension of mma.m16n8k16 is the query rows of one KV head (8 with a GQA group
-// of 8, two n-tiles for up to 16 packed rows) and the 16-wide M dimension is filled by keys
-// (Q.K^T) or head dimensions (P.V) -- nothing is padding:
-//   warps 0 .. HPC-1      (one per KV head) form S^T = K . Q^T from the K ring (A = the K block read
-//                         with ldmatrix, B = the query rows held in registers) and hand the
-//                         16 x 8 score tile over through shared memory;
-//   warps HPC .. 2 HPC-1  take the score tile in the B-operand layout (one query row per lane
-//                         quad-row, so a row's maximum is two shuffles), run the online softmax
-//                         and accumulate O^T += V^T . P^T from the V ring (A = the V block read
-//                         with ldmatrix.trans); they end with (m, l) and the whole output tile.
-// K and V have their own 3-stage rings of bulk copies (one per key row, completion on the stage's
-// mbarrier). Warp 0 refills a K stage once every K.Q^T warp has released it, warp HPC a V stage
-// once every P.V warp has; the score tiles are double buffered per head. Every wait is bounded.
-// ---------------------------------------------------------------------------------------
-template <int HD, int NT, int HPC, typename T>
-__global__ void __launch_bounds__(64 * HPC, 4 / HPC)
-attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
-                           const TTDecodeSession *__restrict__ sessions, float *__restrict__ part_o,
-                           float *__restrict__ part_m, float *__restrict__ part_l,
-                           uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t kv_stride_bytes,
-                           uint32_t q_row_stride, float scale_log2, uint32_t *__restrict__ status,
-                           const __grid_constant__ TTSessionTable table, uint32_t table_keys_per_item) {
-    using S = DecodeSmem<HD, HPC>;
-    constexpr int KS = HD / 16;         // k-steps of K.Q^T and m-tiles of V^T.P^T
-    extern __shared__ __align__(128) unsigned char smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = lane >> 2, t = lane & 3;
-    const int role = warp / HPC, head = warp % HPC;   // role 0: K.Q^T, role 1: softmax + V^T.P^T
-
-    const uint32_t group = n_q_heads / n_kv_heads;
-    const uint32_t n_kv_groups = n_kv_heads / HPC;
-    // Calls with up to kParamSessions sessions carry them in the kernel parameters and derive the
-    // work item from the block index (the items of a session are equal slices, item_prefix says
-    // where each session's items start), so no table is copied to the device and a CTA starts
-    // without two dependent global loads.
-    pdl_launch_dependents();
-    TTDecodeItem item;
-    TTDecodeSession ses;
-    if (table.n != 0) {
-        uint32_t lo = 0, hi = table.n;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (table.item_prefix[mid] <= blockIdx.x) lo = mid; else hi = mid;
-        }
-        ses = table.s[lo];
-        const uint32_t local = blockIdx.x - table.item_prefix[lo];
-        const uint32_t packed_rows = ses.q_rows * group;
-        const uint32_t row_tiles = (packed_rows + 15) / 16;
-        const uint32_t rt = local % row_tiles, kvg = (local / row_tiles) % n_kv_groups;
-        const uint32_t part = local / (row_tiles * n_kv_groups);
-        item.session = lo; item.kv_head = kvg * HPC; item.part_index = part; item.partial_base = ses.partial_base;
-        item.key_begin = min(ses.seq_len, ses.kv_start + part * table_keys_per_item);
-        item.key_end = min(ses.seq_len, item.key_begin + table_keys_per_item);
-        item.row_begin = rt * 16;
-        item.row_count = min(16u, packed_rows - rt * 16);
-    } else {
-        item = items[blockIdx.x];
-        ses = sessions[item.session];
-    }
-    const uint32_t kv_head = item.kv_head + head;      // the head this warp serves
-
-    unsigned char *k_ring = smem;
-    unsigned char *v_ring = smem + S::kVRing;
-    float *score = reinterpret_cast<float *>(smem + S::kRingBytes) + head * 2 * S::kScoreTile;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kRingBytes + S::kScoreBytes);
-    uint64_t *k_full = bars, *v_full = bars + kStages, *k_empty = bars + 2 * kStages, *v_empty = bars + 3 * kStages;
-    uint64_t *s_full = bars + 4 * kStages + head * 4, *s_empty = s_full + 2;
-
-    if (threadIdx.x == 0) {
-        for (int b = 0; b < 2 * kStages; ++b) mbar_init(&bars[b], 1);                   // filled by one expect_tx arrival
-        for (int b = 2 * kStages; b < 4 * kStages; ++b) mbar_init(&bars[b], HPC);       // released by every reader warp
-        for (int b = 4 * kStages; b < S::kBars; ++b) mbar_init(&bars[b], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
-    // everything above overlapped the tail of the kernel before this one in the stream; its
-    // results (the query rows, the newest K/V rows, partials being merged) are read from here on
-    pdl_wait();
-
-    const uint32_t n_keys = item.key_end - item.key_begin;
-    const uint32_t n_blocks = (n_keys + kKeysPerBlock - 1) / kKeysPerBlock;
-    auto block_valid = [&](uint32_t i) { return min((uint32_t)kKeysPerBlock, n_keys - i * kKeysPerBlock); };
-    // lanes 0..15 of the issuing warp fetch one row each (all HPC heads of the key) of block i
-    auto issue = [&](uint32_t i, unsigned char *ring, const unsigned char *base, uint64_t *full, bool zero_fill) {
-        const uint32_t valid = block_valid(i), stage = i % kStages;
-        if (lane == 0) mbar_expect_tx(&full[stage], valid * (uint32_t)(HPC * HD * 2));
-        __syncwarp();
-        if (lane < kKeysPerBlock) {
-            unsigned char *dst = ring + stage * S::kTileBytes + lane * S::kRowBytes;
-            if ((uint32_t)lane < valid) {
-                uint32_t p = item.key_begin + i * kKeysPerBlock + lane;
-                if (ses.row_index != nullptr) p = ses.row_index[p];
-                if (ses.ring_capacity) p %= ses.ring_capacity;
-                // read once: evict-first in L2, so that the stream does not push out the partials, the query
-                // rows and what the neighbouring kernels of the step keep there (measured on the config-2
-                // step: 0.1854 -> 0.1778 ms)
-                bulk_copy_g2s_stream(dst, base + (size_t)p * kv_stride_bytes, HPC * HD * 2, &full[stage]);
-            } else if (zero_fill) {
-                // a V row that is never fetched must still be finite: it meets p == 0 in P.V
-                const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-                for (int c = 0; c < HPC * HD / 8; ++c) reinterpret_cast<uint4 *>(dst)[c] = z;
-            }
-        }
-    };
-    bool timed_out = false;
-    uint32_t consumed = 0, issued = 0;      // blocks of the ring this warp fills (warps 0 and HPC only)
-
-    if (role == 0) {
-        // ================= K . Q^T =================
-        const unsigned char *kbase = reinterpret_cast<const unsigned char *>(ses.k) + (size_t)item.kv_head * HD * 2;
-        // the query rows as B fragments: lane (g, t) holds dims 2t, 2t+1 (+8) of row g of every n-tile
-        uint32_t qf[NT][KS][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t r = nt * 8 + g;
-            const T *qp = nullptr;
-            if (r < item.row_count) {
-                const uint32_t packed = item.row_begin + r;
-                qp = reinterpret_cast<const T *>(ses.q) + (size_t)(packed / group) * q_row_stride +
-                     (size_t)(kv_head * group + packed % group) * HD + t * 2;
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                qf[nt][ks][0] = qp ? *reinterpret_cast<const uint32_t *>(qp + ks * 16) : 0u;
-                qf[nt][ks][1] = qp ? *reinterpret_cast<const uint32_t *>(qp + ks * 16 + 8) : 0u;
-            }
-        }
-        if (head == 0)
-            for (; issued < n_blocks && issued < (uint32_t)kStages; ++issued) issue(issued, k_ring, kbase, k_full, false);
-        // A fragment of a K block: matrix j = lane / 8 covers keys 8 (j & 1) .. +7, dims 8 (j >> 1) .. +7
-        const uint32_t k_off = ((lane & 7) + ((lane >> 3) & 1) * 8) * S::kRowBytes + (lane >> 4) * 16 + head * HD * 2;
-        for (uint32_t i = 0; i < n_blocks; ++i) {
-            if (!warp_all(mbar_wait(&k_full[i % kStages], (i / kStages) & 1))) { timed_out = true; break; }
-            const uint32_t stage = smem_u32(k_ring + (i % kStages) * S::kTileBytes);
-            // two accumulator chains per n-tile (even / odd k-steps) halve the dependent MMA depth
-            float s0[NT][4], s1[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) { s0[nt][0] = s0[nt][1] = s0[nt][2] = s0[nt][3] = 0.f; s1[nt][0] = s1[nt][1] = s1[nt][2] = s1[nt][3] = 0.f; }
-#pragma unroll
-            for (int ks = 0; ks < KS; ks += 2) {
-                uint32_t a[4], b[4];
-                ldmatrix_x4(a, stage + k_off + ks * 32);
-                ldmatrix_x4(b, stage + k_off + (ks + 1) * 32);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma_16816<T>(s0[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
-                    mma_16816<T>(s1[nt], b, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
-                }
-            }
-            __syncwarp();                                   // every lane has its fragments: this warp releases the stage
-            if (lane == 0) mbar_arrive(&k_empty[i % kStages]);
-            if (head == 0) consumed = i + 1;
-            // hand the tile over: element (query row r, key k) at score[buffer][r][k]
-            if (i >= 2 && !warp_all(mbar_wait(&s_empty[i & 1], ((i >> 1) - 1) & 1))) { timed_out = true; break; }
-            float *sb = score + (i & 1) * S::kScoreTile;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float *r0 = sb + (nt * 8 + 2 * t) * S::kScorePitch, *r1 = r0 + S::kScorePitch;
-                r0[g] = s0[nt][0] + s1[nt][0]; r1[g] = s0[nt][1] + s1[nt][1];
-                r0[g + 8] = s0[nt][2] + s1[nt][2]; r1[g + 8] = s0[nt][3] + s1[nt][3];
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_full[i & 1]);
-            if (head == 0 && issued < n_blocks) {           // block i + kStages goes into the stage block i just left
-                if (!warp_all(mbar_wait(&k_empty[i % kStages], (i / kStages) & 1))) { timed_out = true; break; }
-                issue(issued, k_ring, kbase, k_full, false);
-                ++issued;
-            }
-        }
-        if (timed_out) {
-            // blocks issued into the ring and not yet waited for may still be landing
-            for (uint32_t b = consumed; b < issued; ++b) mbar_wait(&k_full[b % kStages], (b / kStages) & 1, 1u << 16);
-            if (lane == 0) atomicOr(status, TT_DEV_WAIT_TIMEOUT);
-        }
-        return;
-    }
-
-    // ================= softmax and V^T . P^T =================
-    const unsigned char *vbase = reinterpret_cast<const unsigned char *>(ses.v) + (size_t)item.kv_head * HD * 2;
-    if (head == 0)
-        for (; issued < n_blocks && issued < (uint32_t)kStages; ++issued) issue(issued, v_ring, vbase, v_full, true);
-
-    float acc[NT][KS][4];               // O^T: dims 16 mt + g (+8) x query rows 2t, 2t+1 of n-tile nt
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int mt = 0; mt < KS; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.f;
-    float m_run[NT], l_run[NT];         // of query row 8 nt + g; l is this lane's share (keys 2t, 2t+1, 2t+8, 2t+9)
-    uint32_t limit[NT];                 // visible-key limit of that row
-    const uint32_t w_first = item.row_begin / group;
-    const uint32_t limit_min = ses.seq_len - (ses.q_rows - 1 - w_first);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        m_run[nt] = -INFINITY; l_run[nt] = 0.f;
-        const uint32_t r = nt * 8 + g;
-        // rows past row_count are never written: they take the tile's smallest limit and need no masking of their own
-        limit[nt] = r < item.row_count ? ses.seq_len - (ses.q_rows - 1 - (item.row_begin + r) / group) : limit_min;
-    }
-    // A fragment of V^T: matrix j = lane / 8 covers keys 8 (j >> 1) .. +7, dims 8 (j & 1) .. +7 (read transposed)
-    const uint32_t v_off = ((lane & 7) + (lane >> 4) * 8) * S::kRowBytes + ((lane >> 3) & 1) * 16 + head * HD * 2;
-
-    for (uint32_t i = 0; i < n_blocks; ++i) {
-        if (!warp_all(mbar_wait(&s_full[i & 1], (i >> 1) & 1))) { timed_out = true; break; }
-        const float *sb = score + (i & 1) * S::kScoreTile;
-        float sv[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const float2 lo = *reinterpret_cast<const float2 *>(sb + (nt * 8 + g) * S::kScorePitch + 2 * t);
-            const float2 hi = *reinterpret_cast<const float2 *>(sb + (nt * 8 + g) * S::kScorePitch + 2 * t + 8);
-            sv[nt][0] = lo.x; sv[nt][1] = lo.y; sv[nt][2] = hi.x; sv[nt][3] = hi.y;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[i & 1]);
-
-        // ---- mask + online softmax of row 8 nt + g over this lane's four keys ----
-        const uint32_t blk_key0 = item.key_begin + i * kKeysPerBlock;
-        const bool plain = (blk_key0 + kKeysPerBlock <= limit_min) && (blk_key0 + kKeysPerBlock <= item.key_end) &&
-                           (ses.keep == nullptr);
-        uint32_t pb[NT][2];
-        float alpha[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float s = sv[nt][j] * scale_log2;
-                if (!plain) {
-                    const uint32_t key = blk_key0 + 2 * t + (j >> 1) * 8 + (j & 1);
-                    bool ok = key < limit[nt] && key < item.key_end;
-                    if (ok && ses.keep != nullptr) ok = ses.keep[key] != 0;
-                    s = ok ? s : -INFINITY;
-                }
-                sv[nt][j] = s;
-                mx = fmaxf(mx, s);
-            }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m_run[nt], mx);
-            const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
-            alpha[nt] = fast_exp2(m_run[nt] - m_use);
-            m_run[nt] = m_new;
-            pb[nt][0] = pack2<T>(fast_exp2(sv[nt][0] - m_use), fast_exp2(sv[nt][1] - m_use));
-            pb[nt][1] = pack2<T>(fast_exp2(sv[nt][2] - m_use), fast_exp2(sv[nt][3] - m_use));
-            // row sums from the ROUNDED weights the MMA consumes: O / l stays a convex combination
-            l_run[nt] = l_run[nt] * alpha[nt] + sum2<T>(pb[nt][0]) + sum2<T>(pb[nt][1]);
-        }
-        // the accumulators hold query rows 2t, 2t+1: their factors live in the lanes of quad rows 2t and 2t+1
-        bool rescale = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) rescale |= alpha[nt] != 1.f;
-        if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float a0 = __shfl_sync(0xffffffffu, alpha[nt], 8 * t), a1 = __shfl_sync(0xffffffffu, alpha[nt], 8 * t + 4);
-#pragma unroll
-                for (int mt = 0; mt < KS; ++mt) {
-                    acc[nt][mt][0] *= a0; acc[nt][mt][1] *= a1;
-                    acc[nt][mt][2] *= a0; acc[nt][mt][3] *= a1;
-                }
-            }
-        }
-
-        // ---- O^T += V^T P^T ----
-        if (!warp_all(mbar_wait(&v_full[i % kStages], (i / kStages) & 1))) { timed_out = true; break; }
-        const uint32_t stage = smem_u32(v_ring + (i % kStages) * S::kTileBytes);
-#pragma unroll
-        for (int mt = 0; mt < KS; ++mt) {
-            uint32_t a[4];
-            ldmatrix_x4_trans(a, stage + v_off + mt * 32);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816<T>(acc[nt][mt], a, pb[nt][0], pb[nt][1]);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_empty[i % kStages]);
-        if (head == 0) {
-            consumed = i + 1;
-            if (issued < n_blocks) {
-                if (!warp_all(mbar_wait(&v_empty[i % kStages], (i / kStages) & 1))) { timed_out = true; break; }
-                issue(issued, v_ring, vbase, v_full, true);
-                ++issued;
-            }
-        }
-    }
-
-    if (timed_out) {
-        for (uint32_t b = consumed; b < issued; ++b) mbar_wait(&v_full[b % kStages], (b / kStages) & 1, 1u << 16);
-        if (lane == 0) atomicOr(status, TT_DEV_WAIT_TIMEOUT);
-    }
-
-    // ---- write the partial: (m, l) of row 8 nt + g by the quad's first lane, O^T by everyone ----
-    const uint32_t rows_total = ses.q_rows * n_q_heads;
-    auto partial_row = [&](uint32_t r) {
-        const uint32_t packed = item.row_begin + r;
-        const uint32_t rho = (packed / group) * n_q_heads + kv_head * group + packed % group;
-        return (size_t)ses.partial_base + (size_t)item.part_index * rows_total + rho;
-    };
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float l = l_run[nt];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const uint32_t r = nt * 8 + g;
-        if (t == 0 && r < item.row_count) {
-            const size_t prow = partial_row(r);
-            part_m[prow] = m_run[nt] * kLn2;   // natural-log domain, the reference's partial format
-            part_l[prow] = l;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t ro = nt * 8 + 2 * t + h;
-            if (ro >= item.row_count) continue;
-            float *dst = part_o + partial_row(ro) * HD + g;
-#pragma unroll
-            for (int mt = 0; mt < KS; ++mt) {
-                dst[mt * 16] = acc[nt][mt][h];
-                dst[mt * 16 + 8] = acc[nt][mt][2 + h];
-            }
-        }
-    }
-}
 
 // Shared memory of the quantised-KV variant: a ring of RAW rows (this head's packed values followed by
 // the row's scale/bias block), plus one private fp16 tile pair per warp holding the dequantised halves.
@@ -887,33 +501,6 @@ __global__ void attn_combine_parts_kernel(const float *__restrict__ m, const flo
     }
 }
 
-template <int HD, int NT, int HPC, typename T>
-cudaError_t launch_partial_nt(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items,
-                              const TTDecodeSession *sessions, float *part_o, float *part_m,
-                              float *part_l, const tt_attn_batch_params *p, uint32_t *status,
-                              const TTSessionTable &table, uint32_t table_keys) {
-    auto kernel = attn_decode_partial_kernel<HD, NT, HPC, T>;
-    const int smem = DecodeSmem<HD, HPC>::kTotal;
-    cudaError_t e = tt_set_smem_once(kernel, smem);
-    if (e != cudaSuccess) return e;
-    return tt_launch_pdl(kernel, dim3(n_items), dim3(64 * HPC), (size_t)smem, stream, items, sessions, part_o, part_m, part_l,
-                         p->n_q_heads, p->n_kv_heads, p->kv_token_stride_elements * 2u, p->q_row_stride_elements,
-                         p->scale * kLog2e, status, table, table_keys);
-}
-
-// `wide_rows`: some session has more than 8 packed query rows per KV head (two n-tiles per item);
-// `hpc`: KV heads served by one CTA (tt_decode_heads_per_cta)
-template <int HD, typename T>
-cudaError_t launch_partial(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items,
-                           const TTDecodeSession *sessions, float *part_o, float *part_m,
-                           float *part_l, const tt_attn_batch_params *p, uint32_t *status,
-                           const TTSessionTable &table, uint32_t table_keys, bool wide_rows, uint32_t hpc) {
-#define TT_P(NT, HPC) launch_partial_nt<HD, NT, HPC, T>(stream, n_items, items, sessions, part_o, part_m, part_l, p, status, table, table_keys)
-    if (hpc == 2) return wide_rows ? TT_P(2, 2) : TT_P(1, 2);
-    return wide_rows ? TT_P(2, 1) : TT_P(1, 1);
-#undef TT_P
-}
-
 template <int HD, int BITS>
 cudaError_t launch_partial_quant_one(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items,
                                      const TTDecodeSession *sessions, float *part_o, float *part_m, float *part_l,
@@ -937,19 +524,6 @@ cudaError_t launch_partial_quant(cudaStream_t stream, uint32_t n_items, const TT
     if (p->head_dim == 256) return quant->bits == 8 ? TT_Q(256, 8) : TT_Q(256, 4);
     return quant->bits == 8 ? TT_Q(128, 8) : TT_Q(128, 4);
 #undef TT_Q
-}
-
-template <typename T>
-cudaError_t launch_partial_hd(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items,
-                              const TTDecodeSession *sessions, float *part_o, float *part_m,
-                              float *part_l, const tt_attn_batch_params *p, uint32_t *status,
-                              const TTSessionTable &table, uint32_t table_keys, bool wide_rows, uint32_t hpc) {
-    switch (p->head_dim) {
-        case 64: return launch_partial<64, T>(stream, n_items, items, sessions, part_o, part_m, part_l, p, status, table, table_keys, wide_rows, hpc);
-        case 128: return launch_partial<128, T>(stream, n_items, items, sessions, part_o, part_m, part_l, p, status, table, table_keys, wide_rows, hpc);
-        case 256: return launch_partial<256, T>(stream, n_items, items, sessions, part_o, part_m, part_l, p, status, table, table_keys, wide_rows, hpc);
-        default: return cudaErrorInvalidValue;
-    }
 }
 
 }  // namespace
@@ -1255,7 +829,8 @@ static bool plan_wide(tt_context *ctx, const TTDecodeSession *in_sessions, uint3
 // with the cross-GPU exchange (`exchange`).
 int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *in_sessions,
                      uint32_t n_sessions, const tt_attn_batch_params *p, int mode, float *m_out,
-                     float *d_out, float *o_out, const TTKvQuant *quant, const tt_attn_exchange *exchange) {
+                     float *d_out, float *o_out, const TTKvQuant *quant, const tt_attn_exchange *exchange,
+                     TTDecodeForm *form) {
     if (n_sessions == 0) return TT_OK;
     if (mode == 2 && (exchange == nullptr || n_sessions != 1 || in_sessions[0].q_rows != 1))
         return tt_set_error(ctx, TT_ERR_INVALID_ARG, "the fused exchange serves one session with one query row");
@@ -1306,11 +881,12 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
         if (((uintptr_t)s.q | (uintptr_t)s.k | (uintptr_t)s.v | (uintptr_t)s.out) & 15)
             return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "session %u: buffers must be 16-byte aligned", i);
         keys[i] = s.seq_len > s.kv_start ? s.seq_len - s.kv_start : 0u;
+        if (form != nullptr && form->form == kPassSink) keys[i] += s.seq_len < form->sink ? s.seq_len : form->sink;
         rows[i] = s.q_rows;
     }
     // Verify batches (17..128 packed rows per KV head, head_dim 256, plain 16-bit rows) take the
     // tensor-core pass 1: one item serves all packed rows of a (session, kv head, key range).
-    bool wide = !quantised && p->head_dim == 256 && getenv("TT_VERIFY_FORCE_MMA_SYNC") == nullptr;
+    bool wide = !quantised && form == nullptr && p->head_dim == 256 && getenv("TT_VERIFY_FORCE_MMA_SYNC") == nullptr;
     bool wide128 = false;       // some session has more than 64 packed rows: the 128-row form of the kernel
     for (uint32_t i = 0; wide && i < n_sessions; ++i) {
         const TTDecodeSession &s = in_sessions[i];
@@ -1331,9 +907,20 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     // derives its item from the block index).
     const bool in_params = wide ? n_sessions <= kVerifyParamSessions : n_sessions <= kParamSessions;
     const uint32_t hpc = tt_decode_heads_per_cta(p->n_kv_heads, quantised);
+    size_t partial_bytes = ctx->workspace_bytes;
+    if (form != nullptr) {
+        if (!in_params && tt_stream_is_capturing(stream))
+            return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE,
+                                "more than %u sessions cannot be captured: their table is uploaded from host memory",
+                                kParamSessions);
+        if (form->reserved_bytes >= partial_bytes)
+            return tt_set_error(ctx, TT_ERR_OOM, "the context workspace is too small for this call");
+        partial_bytes -= form->reserved_bytes;
+        if (form->form == kPassScores) partial_bytes = partial_bytes / (p->head_dim + 4) * (p->head_dim + 2);   // two more floats a row
+    }
     if (!wide) {
         int rc = plan_splits(keys, rows, n_sessions, p->head_dim, p->n_q_heads, p->n_kv_heads, (uint32_t)ctx->sm_count,
-                             ctx->workspace_bytes, hpc, &keys_per_item, &n_items);
+                             partial_bytes, hpc, &keys_per_item, &n_items);
         if (rc != TT_OK) return tt_set_error(ctx, rc, "split-KV partials do not fit the context workspace");
         if (!in_params && n_items > ctx->max_items)
             return tt_set_error(ctx, TT_ERR_OOM, "%u work items exceed the context's item table (%u)", n_items,
@@ -1356,10 +943,12 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
                 table.item_prefix[i] = item_cursor;
                 item_cursor += parts * (p->n_kv_heads / hpc) * ceil_div_u32(packed_rows, rows_per_item);
             } else {
+                const bool compact = form != nullptr && form->form == kPassSink;     // item ranges index the visible keys
+                const uint32_t key0 = compact ? 0u : s.kv_start, limit = compact ? keys[i] : s.seq_len;
                 for (uint32_t part = 0; part < parts; ++part) {
-                    const uint32_t kb = s.kv_start + part * keys_per_item;
+                    const uint32_t kb = key0 + part * keys_per_item;
                     uint32_t ke = kb + keys_per_item;
-                    if (ke > s.seq_len) ke = s.seq_len;
+                    if (ke > limit) ke = limit;
                     if (ke < kb) ke = kb;
                     for (uint32_t kvh = 0; kvh < p->n_kv_heads; kvh += hpc)
                         for (uint32_t rb = 0; rb < packed_rows; rb += rows_per_item) {
@@ -1383,6 +972,11 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     float *part_o = ctx->partials;
     float *part_m = part_o + (size_t)partial_cursor * p->head_dim;
     float *part_l = part_m + partial_cursor;
+
+    if (form != nullptr) {
+        form->part_o = part_o; form->part_m = part_m; form->part_l = part_l;
+        form->part_m2 = part_l + partial_cursor; form->part_l2 = form->part_m2 + partial_cursor;
+    }
 
     const uint32_t table_keys = in_params ? keys_per_item : 0u;
     bool wide_rows = false;             // more than 8 packed query rows per KV head somewhere: two n-tiles per item
@@ -1409,16 +1003,20 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     } else if (quantised)
         e = launch_partial_quant(stream, n_items, ctx->items, ctx->sessions, part_o, part_m, part_l, p, ctx->status,
                                  table, table_keys, quant, meta_bytes);
+    else if (form != nullptr && form->form == kPassSink)
+        e = tt_launch_pass1_sink(stream, n_items, ctx->items, ctx->sessions, *form, p, ctx->status, table, table_keys, wide_rows, hpc);
+    else if (form != nullptr && form->form == kPassScores)
+        e = tt_launch_pass1_scores(stream, n_items, ctx->items, ctx->sessions, *form, p, ctx->status, table, table_keys, wide_rows, hpc);
     else if (p->io_dtype == TT_F16)
         e = launch_partial_hd<__half>(stream, n_items, ctx->items, ctx->sessions, part_o, part_m, part_l, p, ctx->status,
-                                      table, table_keys, wide_rows, hpc);
+                                      table, table_keys, wide_rows, hpc, PassExtra<kPassPlain>());
     else
         e = launch_partial_hd<__nv_bfloat16>(stream, n_items, ctx->items, ctx->sessions, part_o, part_m, part_l, p,
-                                             ctx->status, table, table_keys, wide_rows, hpc);
+                                             ctx->status, table, table_keys, wide_rows, hpc, PassExtra<kPassPlain>());
     if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_decode_partial launch");
     timer.stop();
     ctx->launches++;
-    if (direct) return TT_OK;
+    if (direct || (form != nullptr && form->partials_only)) return TT_OK;
     if (mode == 2)
         return tt_launch_merge_exchange(ctx, stream, part_o, part_m, part_l, ctx->h_sessions[0].n_parts, exchange,
                                         p->n_q_heads, p->head_dim, p->io_dtype);
@@ -1677,7 +1275,7 @@ TT_API int tt_attn_decode_noalloc(tt_stream stream, const void *q, const void *k
     p.kv_token_stride_elements = n_kv_heads * head_dim; p.q_row_stride_elements = n_q_heads * head_dim;
     p.out_row_stride_elements = n_q_heads * head_dim; p.scale = scale; p.io_dtype = TT_F16;
     if (launch_partial_hd<__half>(s, grid, nullptr, nullptr, part_o, part_m, part_l, &p, status, table, keys_per_item,
-                                  group > 8, hpc) != cudaSuccess)
+                                  group > 8, hpc, PassExtra<kPassPlain>()) != cudaSuccess)
         return TT_ERR_CUDA;
     attn_decode_combine_kernel<__half><<<dim3(1, n_q_heads, (head_dim / 4 + 15) / 16), 256, 0, s>>>(
         nullptr, part_o, part_m, part_l, n_q_heads, head_dim, n_q_heads * head_dim, 0, nullptr, nullptr, nullptr, table,

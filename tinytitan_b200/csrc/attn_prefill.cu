@@ -9,7 +9,7 @@
 #include "tt_common.h"
 
 int tt_launch_prefill_tc(tt_context *ctx, cudaStream_t stream, const void *q, const void *k, const void *v,
-                         void *out, const tt_prefill_params *p, uint32_t io_dtype);
+                         void *out, const tt_prefill_params *p, uint32_t io_dtype, const TTPrefillSink *sink = nullptr);
 
 namespace {
 
@@ -64,6 +64,7 @@ struct PrefillSelection {
     const uint32_t *counts;
     uint32_t index_stride;
     const uint32_t *rows;
+    uint32_t sink = 0;      // mode 0: keys below it stay visible beside the window, the ring lies behind their rows
 };
 
 // One warp per (query row, q head). Keys are taken 32 at a time: lane j scores key j (a full
@@ -98,7 +99,8 @@ attn_prefill_generic_kernel(const T *__restrict__ q, const T *__restrict__ k, co
 
     // steps of the row: visible keys, or the entries of its compact list
     const bool compact = sel.mode >= 2;
-    const uint32_t steps = compact ? sel.counts[t] : (last > first ? last - first : 0u);
+    const uint32_t sinks = min(sel.sink, min(first, last));     // sinks the window does not cover
+    const uint32_t steps = compact ? sel.counts[t] : sinks + (last > first ? last - first : 0u);
     for (uint32_t step0 = 0; step0 < steps; step0 += 32) {
         const uint32_t step = step0 + lane;
         float s = -INFINITY;
@@ -111,9 +113,9 @@ attn_prefill_generic_kernel(const T *__restrict__ q, const T *__restrict__ k, co
                 valid = key >= first && key < last;
                 phys = sel.mode == 3 ? sel.rows[(size_t)t * sel.index_stride + step] : (ring ? key % ring : key);
             } else {
-                key = first + step;
+                key = step < sinks ? step : first + (step - sinks);
                 valid = sel.mode == 0 || sel.keep[(size_t)t * sel.keep_stride + key] != 0;
-                phys = ring ? key % ring : key;
+                phys = ring && key >= sel.sink ? sel.sink + (key - sel.sink) % ring : key;
             }
             if (valid) {
                 float dot = 0.f;
@@ -237,7 +239,7 @@ TT_API int tt_attn_prefill_causal(tt_context *ctx, tt_stream stream, const void 
     if (rc != TT_OK) return rc;
     if (tt_attn_prefill_path(q, k, v, out, params, kv_ring_capacity) == 1 && getenv("TT_PREFILL_FORCE_GENERIC") == nullptr)
         return tt_launch_prefill_tc(ctx, (cudaStream_t)stream, q, k, v, out, params, io_dtype);
-    PrefillSelection none = {0, nullptr, 0, nullptr, nullptr, 0, nullptr};
+    PrefillSelection none = {0, nullptr, 0, nullptr, nullptr, 0, nullptr, 0};
     return launch_generic(ctx, (cudaStream_t)stream, q, k, v, out, params, kv_ring_capacity, io_dtype, none);
 }
 
@@ -250,7 +252,7 @@ TT_API int tt_attn_prefill_causal_selected(tt_context *ctx, tt_stream stream, co
     int rc = validate_prefill(ctx, q, k, v, out, params, io_dtype);
     if (rc != TT_OK) return rc;
     // the mode follows from what was bound, as in PrefillAttention.encodeCausal (PrefillAttention.swift:214-226)
-    PrefillSelection sel = {0, keep_mask, keep_stride, keep_indices, keep_counts, keep_index_stride, keep_rows};
+    PrefillSelection sel = {0, keep_mask, keep_stride, keep_indices, keep_counts, keep_index_stride, keep_rows, 0};
     const bool compacted = keep_indices != nullptr && keep_counts != nullptr;
     if (compacted) sel.mode = keep_rows != nullptr ? 3u : 2u;
     else if (keep_mask != nullptr) sel.mode = 1u;
@@ -265,4 +267,33 @@ TT_API int tt_attn_prefill_causal_selected(tt_context *ctx, tt_stream stream, co
             return tt_launch_prefill_tc(ctx, (cudaStream_t)stream, q, k, v, out, params, io_dtype);
     }
     return launch_generic(ctx, (cudaStream_t)stream, q, k, v, out, params, kv_ring_capacity, io_dtype, sel);
+}
+
+TT_API int tt_attn_prefill_sink_path(const void *q, const void *k, const void *v, const void *out,
+                                     const tt_prefill_params *p, uint32_t ring_capacity) {
+    // a 64-key box of the tensor-core kernel must not run over the ring's end
+    return ring_capacity % 64 == 0 ? tt_attn_prefill_path(q, k, v, out, p, 0) : 0;
+}
+
+TT_API int tt_attn_prefill_sink_window(tt_context *ctx, tt_stream stream, const void *q, const void *k, const void *v,
+                                       void *out, const tt_prefill_params *params, uint32_t sink_tokens,
+                                       uint32_t ring_capacity, uint32_t io_dtype) {
+    TT_ENTER(ctx);
+    int rc = validate_prefill(ctx, q, k, v, out, params, io_dtype);
+    if (rc != TT_OK) return rc;
+    if (params->kv_bits != 16)
+        return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "attention with sinks reads 16-bit rows, not %u-bit ones", params->kv_bits);
+    if (params->kv_valid_count > (uint32_t)INT32_MAX || sink_tokens > (uint32_t)INT32_MAX)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "kvValidCount and sink_tokens must be below 2^31");
+    const uint64_t newest = (uint64_t)params->kv_valid_count - params->start_position;     // rows written from the first query's own on
+    if (ring_capacity != 0 && params->kv_valid_count > (uint64_t)sink_tokens + ring_capacity &&
+        (params->sliding_window == 0 || (uint64_t)ring_capacity < (uint64_t)params->sliding_window + newest - 1))
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "a ring of %u rows cannot hold a window of %u for %u new rows", ring_capacity,
+                            params->sliding_window, (uint32_t)newest);
+    if (tt_attn_prefill_sink_path(q, k, v, out, params, ring_capacity) == 1 && getenv("TT_PREFILL_FORCE_GENERIC") == nullptr) {
+        const TTPrefillSink sink = {sink_tokens, ring_capacity};
+        return tt_launch_prefill_tc(ctx, (cudaStream_t)stream, q, k, v, out, params, io_dtype, &sink);
+    }
+    const PrefillSelection sel = {0, nullptr, 0, nullptr, nullptr, 0, nullptr, sink_tokens};
+    return launch_generic(ctx, (cudaStream_t)stream, q, k, v, out, params, ring_capacity, io_dtype, sel);
 }

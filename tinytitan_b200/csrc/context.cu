@@ -20,6 +20,11 @@ bool tt_pdl_enabled() {
     return enabled;
 }
 
+bool tt_stream_is_capturing(cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(stream, &status) == cudaSuccess && status != cudaStreamCaptureStatusNone;
+}
+
 int tt_check_cuda(tt_context *ctx, cudaError_t e, const char *what) {
     if (e == cudaSuccess) return TT_OK;
     const int code = (e == cudaErrorMemoryAllocation) ? TT_ERR_OOM : TT_ERR_CUDA;
@@ -80,6 +85,7 @@ static void context_free(tt_context *ctx) {
     if (ctx == nullptr) return;
     cudaFree(ctx->partials);
     cudaFree(ctx->tables);
+    cudaFree(ctx->prefix_tables);
     cudaFree(ctx->gdn_sessions);
     cudaFree(ctx->status);
     if (ctx->profile_begin) {
@@ -91,6 +97,9 @@ static void context_free(tt_context *ctx) {
         free(ctx->profile_end);
     }
     free(ctx->h_tables);
+    free(ctx->h_prefix_tables);
+    free(ctx->h_prefix_lens);
+    free(ctx->h_prefix_rows);
     free(ctx->h_sessions_in);
     free(ctx->h_keys);
     free(ctx->h_rows);
@@ -123,6 +132,8 @@ TT_API tt_context *tt_context_create(int device, const tt_context_options *optio
     ctx->table_bytes = (sizeof(TTDecodeSession) * ctx->max_sessions + 127) / 128 * 128 + (size_t)256 * ctx->max_sessions +
                        sizeof(TTDecodeItem) * ctx->max_items;
     ok = ok && cudaMalloc(&ctx->tables, ctx->table_bytes) == cudaSuccess;
+    ctx->prefix_table_bytes = (size_t)512 * ctx->max_sessions + 256;   // at most 376 bytes a session (one group each)
+    ok = ok && cudaMalloc(&ctx->prefix_tables, ctx->prefix_table_bytes) == cudaSuccess;
     ok = ok && cudaMalloc(&ctx->gdn_sessions, sizeof(tt_gdn_session) * ctx->max_sessions) == cudaSuccess;
     ok = ok && cudaMalloc(&ctx->status, sizeof(uint32_t)) == cudaSuccess;
     ok = ok && cudaMemset(ctx->status, 0, sizeof(uint32_t)) == cudaSuccess;
@@ -130,6 +141,10 @@ TT_API tt_context *tt_context_create(int device, const tt_context_options *optio
     ctx->h_sessions_in = (TTDecodeSession *)malloc(sizeof(TTDecodeSession) * ctx->max_sessions);
     ctx->h_keys = (uint32_t *)malloc(sizeof(uint32_t) * ctx->max_sessions);
     ctx->h_rows = (uint32_t *)malloc(sizeof(uint32_t) * ctx->max_sessions);
+    ctx->h_prefix_tables = (unsigned char *)aligned_alloc(128, (ctx->prefix_table_bytes + 127) / 128 * 128);
+    ctx->h_prefix_lens = (uint32_t *)malloc(sizeof(uint32_t) * ctx->max_sessions);
+    ctx->h_prefix_rows = (uint32_t *)malloc(sizeof(uint32_t) * ctx->max_sessions);
+    ok = ok && ctx->h_prefix_tables && ctx->h_prefix_lens && ctx->h_prefix_rows;
     ok = ok && ctx->h_tables && ctx->h_sessions_in && ctx->h_keys && ctx->h_rows;
     if (ok) tt_bind_decode_tables(ctx, ctx->max_sessions, true);
     if (!ok) {

@@ -1,0 +1,389 @@
+// Eviction from a KV cache by accumulated attention weight: choose the rows to keep per KV head, compact them.
+//
+// Every (session, KV head) has its own statistic A[row] (tt_attn_decode_accumulate) and keeps `budget` of its `rows`
+// rows: the protected ones (token position below `sink_tokens`, or among the last `recent_tokens`), then by A
+// descending, ties to the lower row. Attention over a cache whose keys carry their rotation already does not depend
+// on the order of its rows, so nothing is shifted: a kept row below `budget` stays where it is, and the rows given up
+// there ("holes") are filled, in ascending order, by the kept rows above it. At most min(budget, rows - budget) rows
+// move, one when a full cache takes in one token; sources lie at or above `budget` and destinations below it, so the
+// moves are free of order and the same in place and into other buffers.
+//
+// kv_evict_select_kernel: one thread-block cluster per (session, KV head). The selection key of a row is 32 bits whose
+//   unsigned order is the order above; a CTA keeps its slice of keys in shared memory, so the statistic and the
+//   positions are read once. The budget-th largest key is found by three histogram rounds (11 + 11 + 10 bits, counts
+//   of the cluster's CTAs added through distributed shared memory), then one pass gives ties their rank in row order
+//   and one numbers holes and fills. A thread owns consecutive rows, an odd number of them, so that ranks need one
+//   block scan and the strided shared-memory reads meet no bank twice. Bound: latency of about a dozen block or
+//   cluster barriers for the usual few thousand rows.
+// kv_evict_move_kernel: a warp per 32 destination rows copies what changes, 16 bytes a lane; bound by HBM.
+#include "tt_sm100.h"
+
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+constexpr uint32_t kSelThreads = 512;
+constexpr uint32_t kSelWarps = kSelThreads / 32;
+constexpr uint32_t kBins = 2048;
+constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kSelSliceKeys = 50000;          // keys a CTA holds: 200,000 bytes beside the histogram and the counters
+constexpr uint32_t kHoleFlag = 0x80000000u;
+
+struct EvictSession {
+    const unsigned char *k, *v;
+    unsigned char *k_out, *v_out;
+    const float *weights;
+    float *weights_out;
+    const uint32_t *positions;
+    uint32_t *positions_out;
+    uint32_t rows;
+    uint32_t end_position;
+    uint32_t map_begin;          // first entry of KV head 0's map; a head's map and fill list take `map_pitch` entries
+    uint32_t map_pitch;
+};
+
+struct EvictTable {
+    EvictSession s[kParamSessions];
+    uint32_t n;
+};
+
+struct EvictParams {
+    uint32_t budget, sink, recent, n_kv_heads;
+    uint32_t weight_stride, weight_out_stride;      // elements between the heads of a session
+    uint32_t row_bytes;                             // one head of one row
+    uint32_t held_keys;                             // selection keys a CTA's shared memory has room for
+    size_t in_stride, out_stride;                   // bytes between token rows
+};
+
+// Unsigned order = order of preference. Protected rows above every weight; NaN below every weight.
+__device__ __forceinline__ uint32_t evict_key(float w, bool is_protected) {
+    if (is_protected) return 0xffffffffu;
+    if (w != w) return 0u;
+    const uint32_t b = __float_as_uint(w + 0.0f);          // -0 counts as 0
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// Exclusive block scan of one value per thread; *total gets the sum. Two barriers.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *warp_sums, uint32_t *total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= (uint32_t)o) inc += up;
+    }
+    __syncthreads();                                       // the previous use of warp_sums is over
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSelWarps; ++w) {
+        const uint32_t s = warp_sums[w];
+        before += w < warp ? s : 0u;
+        all += s;
+    }
+    *total = all;
+    return before + inc - x;
+}
+
+struct __align__(16) SelShared {
+    uint32_t hist[kBins];
+    uint32_t warp_sums[kSelWarps];
+    uint32_t counts[4];          // this CTA's ties, holes, fills (read by the cluster)
+    uint32_t pick[2];            // the bin that holds the budget-th key, keys above it
+};
+
+__global__ void __launch_bounds__(kSelThreads)
+kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, uint32_t *__restrict__ maps) {
+    extern __shared__ uint32_t keys[];
+    __shared__ SelShared sh;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t size = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t pair = blockIdx.x / size;
+    const EvictSession &ses = table.s[pair / p.n_kv_heads];
+    const uint32_t head = pair % p.n_kv_heads;
+    pdl_launch_dependents();
+    pdl_wait();
+    if (ses.rows <= p.budget) return;                      // nothing is given up (the whole cluster leaves)
+
+    const float *weights = ses.weights + (size_t)head * p.weight_stride;
+    const uint32_t *positions = ses.positions ? ses.positions + (size_t)head * p.weight_stride : nullptr;
+    uint32_t *map = maps + ses.map_begin + (size_t)head * ses.map_pitch;
+    uint32_t *fills = map + p.budget;
+    const uint32_t slice = (ses.rows + size - 1) / size;
+    const uint32_t begin = min(ses.rows, rank * slice), n = min(ses.rows, begin + slice) - begin;
+    const bool held = slice <= p.held_keys;                // else every round reads the statistic again
+    auto key_at = [&](uint32_t i) {
+        const uint32_t row = begin + i;
+        const uint32_t pos = positions ? positions[row] : row;
+        return evict_key(weights[row], pos < p.sink || (uint64_t)pos + p.recent >= ses.end_position);
+    };
+    if (held) {
+        for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) keys[i] = key_at(i);
+    }
+    auto key_of = [&](uint32_t i) { return held ? keys[i] : key_at(i); };
+
+    // ---- the budget-th largest key: three rounds over its bits from the top ----
+    uint32_t prefix = 0, want = p.budget;                  // key bits fixed so far; rank wanted among the keys that share them
+#pragma unroll 1
+    for (int round = 0; round < 3; ++round) {
+        const uint32_t bits = round < 2 ? 11u : 10u, shift = round == 0 ? 21u : round == 1 ? 10u : 0u;
+        for (uint32_t b = threadIdx.x; b < kBins; b += kSelThreads) sh.hist[b] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) {
+            const uint32_t key = key_of(i);
+            if (round == 0 || key >> (shift + bits) == prefix) atomicAdd(&sh.hist[(key >> shift) & ((1u << bits) - 1)], 1u);
+        }
+        cluster.sync();
+        // thread t adds up bins 4t .. 4t+3 counted from the top, over the CTAs of the cluster
+        uint32_t c[4] = {0u, 0u, 0u, 0u};
+        const uint32_t top = kBins - 4 * (threadIdx.x + 1);
+        for (uint32_t r = 0; r < size; ++r) {
+            const uint4 h = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(sh.hist, r) + top);
+            c[0] += h.w; c[1] += h.z; c[2] += h.y; c[3] += h.x;
+        }
+        uint32_t total;
+        const uint32_t above = block_scan(c[0] + c[1] + c[2] + c[3], sh.warp_sums, &total);
+        if (above < want && want <= above + c[0] + c[1] + c[2] + c[3]) {
+            uint32_t seen = above;
+            int j = 0;
+            while (j < 3 && seen + c[j] < want) seen += c[j++];
+            sh.pick[0] = top + 3 - j;
+            sh.pick[1] = seen;
+        }
+        cluster.sync();                                    // the picked bin is known here, and no CTA still reads these counts
+        prefix = (prefix << bits) | sh.pick[0];
+        want -= sh.pick[1];
+        __syncthreads();
+    }
+    const uint32_t threshold = prefix, ties_kept = want;   // keys above it stay, and the first `ties_kept` equal to it
+
+    // ---- consecutive rows per thread: rank of ties, then of holes and fills, in row order ----
+    const uint32_t per = ((n + kSelThreads - 1) / kSelThreads) | 1u;
+    const uint32_t i0 = min(n, threadIdx.x * per), i1 = min(n, i0 + per);
+    uint32_t ties = 0;
+    for (uint32_t i = i0; i < i1; ++i) ties += key_of(i) == threshold;
+    uint32_t total;
+    uint32_t tie_rank = block_scan(ties, sh.warp_sums, &total);
+    if (threadIdx.x == 0) sh.counts[0] = total;
+    cluster.sync();
+    for (uint32_t r = 0; r < rank; ++r) tie_rank += *cluster.map_shared_rank(&sh.counts[0], r);
+
+    uint32_t holes = 0, kept_above = 0, t = tie_rank;
+    for (uint32_t i = i0; i < i1; ++i) {
+        const uint32_t key = key_of(i);
+        const bool keep = key > threshold || (key == threshold && t < ties_kept);
+        t += key == threshold;
+        if (begin + i < p.budget) holes += !keep; else kept_above += keep;
+    }
+    uint32_t total_holes, total_fills;
+    uint32_t hole = block_scan(holes, sh.warp_sums, &total_holes);
+    uint32_t fill = block_scan(kept_above, sh.warp_sums, &total_fills);
+    if (threadIdx.x == 0) { sh.counts[1] = total_holes; sh.counts[2] = total_fills; }
+    cluster.sync();
+    for (uint32_t r = 0; r < rank; ++r) {
+        const uint32_t *other = cluster.map_shared_rank(sh.counts, r);
+        hole += other[1];
+        fill += other[2];
+    }
+    t = tie_rank;
+    for (uint32_t i = i0; i < i1; ++i) {
+        const uint32_t key = key_of(i), row = begin + i;
+        const bool keep = key > threshold || (key == threshold && t < ties_kept);
+        t += key == threshold;
+        if (row < p.budget) map[row] = keep ? row : kHoleFlag | hole++;
+        else if (keep) fills[fill++] = row;
+    }
+    cluster.sync();                                        // a CTA's counters outlive their readers
+}
+
+// grid = (blocks of 256 destination rows, sessions x KV heads), a warp per 32 of them.
+template <int ROW_BYTES>
+__global__ void __launch_bounds__(256)
+kv_evict_move_kernel(const __grid_constant__ EvictTable table, EvictParams p, const uint32_t *__restrict__ maps) {
+    constexpr uint32_t kLanes = ROW_BYTES / 16, kRowsAtOnce = 32 / kLanes;
+    __shared__ uint8_t todo_list[8][32];            // the lanes whose row is copied, packed
+    const EvictSession &ses = table.s[blockIdx.y / p.n_kv_heads];
+    const uint32_t head = blockIdx.y % p.n_kv_heads;
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 32;
+    const uint32_t kept = min(ses.rows, p.budget);
+    if (j0 >= kept) return;
+    const bool selected = ses.rows > p.budget;
+    const uint32_t *map = maps + ses.map_begin + (size_t)head * ses.map_pitch;
+    const uint32_t j = j0 + lane;
+    uint32_t src = j;
+    bool hole = false;
+    if (selected && j < kept) {
+        const uint32_t e = map[j];
+        hole = (e & kHoleFlag) != 0;
+        if (hole) src = map[p.budget + (e & ~kHoleFlag)];
+    }
+    if (j < kept) {
+        const size_t at = (size_t)head * p.weight_stride + src, to = (size_t)head * p.weight_out_stride + j;
+        if (hole || ses.weights_out != ses.weights) ses.weights_out[to] = ses.weights[at];
+        if (ses.positions_out != nullptr && (hole || ses.positions_out != ses.positions))
+            ses.positions_out[to] = ses.positions ? ses.positions[at] : src;
+    }
+    // rows to copy: the holes, and every row where the destination is another buffer
+    const bool all_k = ses.k_out != ses.k, all_v = ses.v_out != ses.v;
+    const uint32_t live = __ballot_sync(0xffffffffu, j < kept), holes = __ballot_sync(0xffffffffu, hole);
+    const uint32_t todo = (all_k || all_v) ? live : holes;
+    const size_t head_off = (size_t)head * ROW_BYTES + (lane % kLanes) * 16;
+    const uint32_t n = __popc(todo);
+    uint8_t *list = todo_list[threadIdx.x >> 5];
+    if ((todo >> lane) & 1u) list[__popc(todo & ((1u << lane) - 1))] = (uint8_t)lane;
+    __syncwarp();
+#pragma unroll 4
+    for (uint32_t i = 0; i < n; i += kRowsAtOnce) {
+        const uint32_t nth = i + lane / kLanes;
+        const uint32_t at = nth < n ? list[nth] : 0u;
+        const uint32_t from = __shfl_sync(0xffffffffu, src, at);
+        if (nth >= n) continue;
+        const bool moved = (holes >> at) & 1u;
+        const size_t in = (size_t)from * p.in_stride + head_off, out = (size_t)(j0 + at) * p.out_stride + head_off;
+        if (moved || all_k) *reinterpret_cast<uint4 *>(ses.k_out + out) = *reinterpret_cast<const uint4 *>(ses.k + in);
+        if (moved || all_v) *reinterpret_cast<uint4 *>(ses.v_out + out) = *reinterpret_cast<const uint4 *>(ses.v + in);
+    }
+}
+
+// CTAs per (session, KV head): one per 4096 rows while the machine has SMs for them, and enough that the slices fit
+// shared memory.
+uint32_t cluster_size(uint32_t max_rows, uint32_t pairs, uint32_t sm_count) {
+    uint32_t c = 1;
+    while (c < kMaxCluster && ((max_rows > c * 4096u && pairs * c * 2 <= sm_count) || (uint64_t)c * kSelSliceKeys < max_rows)) c *= 2;
+    return c;
+}
+
+bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
+cudaError_t launch_evict(tt_context *ctx, cudaStream_t stream, const EvictTable &table, EvictParams p, uint32_t max_rows,
+                         bool select, uint32_t *maps) {
+    const uint32_t pairs = table.n * p.n_kv_heads;
+    cudaError_t e = cudaSuccess;
+    if (select) {
+        const uint32_t c = cluster_size(max_rows, pairs, (uint32_t)ctx->sm_count);
+        const uint32_t slice = (max_rows + c - 1) / c;
+        p.held_keys = slice <= kSelSliceKeys ? slice : kSelSliceKeys;
+        const size_t smem = sizeof(uint32_t) * p.held_keys;
+        e = tt_set_smem_once(kv_evict_select_kernel, (int)(kSelSliceKeys * sizeof(uint32_t)));
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(pairs * c); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = tt_pdl_enabled() ? 2 : 1;
+        e = cudaLaunchKernelEx(&cfg, kv_evict_select_kernel, table, p, maps);
+        if (e != cudaSuccess) return e;
+        ctx->launches++;
+    }
+    const uint32_t kept = max_rows < p.budget ? max_rows : p.budget;
+    if (kept == 0) return cudaSuccess;
+    const dim3 grid((kept + 255) / 256, pairs);
+    switch (p.row_bytes) {
+        case 128: e = tt_launch_pdl(kv_evict_move_kernel<128>, grid, dim3(256), 0, stream, table, p, maps); break;
+        case 256: e = tt_launch_pdl(kv_evict_move_kernel<256>, grid, dim3(256), 0, stream, table, p, maps); break;
+        default: e = tt_launch_pdl(kv_evict_move_kernel<512>, grid, dim3(256), 0, stream, table, p, maps); break;
+    }
+    if (e == cudaSuccess) ctx->launches++;
+    return e;
+}
+
+}  // namespace
+
+TT_API int tt_kv_evict(tt_context *ctx, tt_stream stream, const tt_kv_evict_session *sessions, uint32_t n_sessions,
+                       const tt_kv_evict_params *params) {
+    TT_ENTER(ctx);
+    if (params == nullptr || (sessions == nullptr && n_sessions != 0))
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "sessions and params must not be null");
+    const tt_kv_evict_params &q = *params;
+    if (q.head_dim != 64 && q.head_dim != 128 && q.head_dim != 256)
+        return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "eviction supports head_dim 64/128/256, got %u", q.head_dim);
+    if (q.n_kv_heads == 0 || q.n_kv_heads > 96) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_kv_heads must be in 1..96");
+    if (q.budget == 0 || q.budget > (uint32_t)INT32_MAX) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "budget must be in 1..2^31-1");
+    if ((uint64_t)q.sink_tokens + q.recent_tokens > q.budget)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "%u sinks and %u recent rows exceed the budget of %u rows", q.sink_tokens,
+                            q.recent_tokens, q.budget);
+    const uint64_t width = (uint64_t)q.n_kv_heads * q.head_dim;
+    const uint64_t in_stride = q.kv_token_stride_elements ? q.kv_token_stride_elements : width;
+    const uint64_t out_stride = q.kv_out_token_stride_elements ? q.kv_out_token_stride_elements : in_stride;
+    const uint32_t weight_out_stride = q.weight_out_head_stride ? q.weight_out_head_stride : q.weight_head_stride;
+    if (in_stride < width || out_stride < width) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "a row stride is smaller than its tight width");
+    if (in_stride % 8 || out_stride % 8) return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "row strides must keep rows 16-byte aligned");
+    for (uint32_t i = 0; i < n_sessions; ++i) {
+        const tt_kv_evict_session &s = sessions[i];
+        if (s.k == nullptr || s.v == nullptr || s.weights == nullptr)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has a null buffer", i);
+        if (((uintptr_t)s.k | (uintptr_t)s.v | (uintptr_t)s.k_out | (uintptr_t)s.v_out) & 15)
+            return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "session %u: K and V must be 16-byte aligned", i);
+        if (((uintptr_t)s.weights | (uintptr_t)s.weights_out | (uintptr_t)s.positions | (uintptr_t)s.positions_out) & 3)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: weights and positions must be 4-byte aligned", i);
+        if (s.rows > (uint32_t)INT32_MAX || s.rows > q.weight_head_stride)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: %u rows do not fit a weight row of %u", i, s.rows, q.weight_head_stride);
+        const uint32_t kept = s.rows < q.budget ? s.rows : q.budget;
+        if (kept > weight_out_stride)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: %u kept rows do not fit a weight row of %u", i, kept, weight_out_stride);
+        if ((s.k_out == nullptr || s.k_out == s.k || s.v_out == nullptr || s.v_out == s.v) && out_stride != in_stride)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: in place, the row strides must be equal", i);
+        const bool w_in = s.weights_out == nullptr || s.weights_out == s.weights;
+        const bool p_in = s.positions != nullptr && (s.positions_out == nullptr || s.positions_out == s.positions);
+        if ((w_in || p_in) && weight_out_stride != q.weight_head_stride)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: in place, the weight strides must be equal", i);
+        const size_t in_bytes = (size_t)s.rows * in_stride * 2, out_bytes = (size_t)kept * out_stride * 2;
+        const size_t w_bytes = ((size_t)(q.n_kv_heads - 1) * q.weight_head_stride + s.rows) * 4;
+        const size_t wo_bytes = ((size_t)(q.n_kv_heads - 1) * weight_out_stride + kept) * 4;
+        if ((s.k_out != nullptr && s.k_out != s.k && overlaps(s.k, in_bytes, s.k_out, out_bytes)) ||
+            (s.v_out != nullptr && s.v_out != s.v && overlaps(s.v, in_bytes, s.v_out, out_bytes)) ||
+            (!w_in && overlaps(s.weights, w_bytes, s.weights_out, wo_bytes)) ||
+            (s.positions != nullptr && !p_in && overlaps(s.positions, w_bytes, s.positions_out, wo_bytes)))
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: an output overlaps its input without being it", i);
+    }
+    EvictParams p;
+    p.budget = q.budget; p.sink = q.sink_tokens; p.recent = q.recent_tokens; p.n_kv_heads = q.n_kv_heads;
+    p.weight_stride = q.weight_head_stride; p.weight_out_stride = weight_out_stride;
+    p.row_bytes = q.head_dim * 2; p.held_keys = 0;
+    p.in_stride = in_stride * 2; p.out_stride = out_stride * 2;
+    // the maps of one launch pair live in the workspace; a batch that needs more is taken in several
+    const uint64_t map_room = ctx->workspace_bytes / sizeof(uint32_t);
+    static thread_local EvictTable table;
+    uint32_t i = 0;
+    while (i < n_sessions) {
+        uint64_t used = 0;
+        uint32_t max_rows = 0;
+        bool select = false;
+        table.n = 0;
+        for (; i < n_sessions && table.n < kParamSessions; ++i) {
+            const tt_kv_evict_session &s = sessions[i];
+            uint64_t pitch = 0;
+            if (s.rows > q.budget) pitch = (uint64_t)q.budget + (s.rows - q.budget < q.budget ? s.rows - q.budget : q.budget);
+            if (used + pitch * q.n_kv_heads > map_room || used + pitch * q.n_kv_heads > UINT32_MAX) {
+                if (table.n != 0) break;
+                return tt_set_error(ctx, TT_ERR_OOM, "the row map of session %u does not fit the context workspace", i);
+            }
+            EvictSession &d = table.s[table.n++];
+            d.k = (const unsigned char *)s.k; d.v = (const unsigned char *)s.v;
+            d.k_out = (unsigned char *)(s.k_out ? s.k_out : s.k); d.v_out = (unsigned char *)(s.v_out ? s.v_out : s.v);
+            d.weights = s.weights; d.weights_out = s.weights_out ? s.weights_out : s.weights;
+            d.positions = s.positions; d.positions_out = s.positions_out ? s.positions_out : s.positions;
+            d.rows = s.rows; d.end_position = s.end_position;
+            d.map_begin = (uint32_t)used; d.map_pitch = (uint32_t)pitch;
+            used += pitch * q.n_kv_heads;
+            select |= pitch != 0;
+            if (s.rows > max_rows) max_rows = s.rows;
+        }
+        const cudaError_t e = launch_evict(ctx, (cudaStream_t)stream, table, p, max_rows, select, reinterpret_cast<uint32_t *>(ctx->partials));
+        if (e != cudaSuccess) return tt_check_cuda(ctx, e, "kv_evict launch");
+    }
+    return TT_OK;
+}

@@ -46,7 +46,10 @@ struct TTDecodeSession {
     uint32_t partial_base;   // first partial row of this session in the workspace
     uint32_t ring_capacity;
     const uint8_t *keep;     // nullable
-    const uint32_t *row_index;  // nullable: key s lives at row row_index[s] (compact selection)
+    union {
+        const uint32_t *row_index;  // nullable: key s lives at row row_index[s] (compact selection)
+        float *scores;              // the form of pass 1 that keeps the scores: [kv head][key][packed row, padded]
+    };
 };
 
 // Sessions of a batched decode call that travel in the kernel parameters instead of a device
@@ -93,6 +96,12 @@ struct tt_context {
     uint32_t *h_keys = nullptr;
     uint32_t *h_rows = nullptr;
     void *h_tensor_maps = nullptr;
+    // shared-prefix calls too large for the kernel parameters: maps | groups | sessions | merge entries
+    unsigned char *prefix_tables = nullptr;
+    unsigned char *h_prefix_tables = nullptr;
+    size_t prefix_table_bytes = 0;
+    uint32_t *h_prefix_lens = nullptr;  // [max_sessions]
+    uint32_t *h_prefix_rows = nullptr;
     TTSessionTable session_table;       // the parameter form of the current decode call's sessions
     TTVerifyMaps verify_maps;           // ... and of a verify batch's tensor maps
     uint64_t launches = 0;
@@ -184,11 +193,41 @@ struct TTKvQuant {
     uint32_t value_bytes = 0;    // packed values of the whole row; scales and biases follow
 };
 
+// A variant of pass 1 and what its caller shares with the launcher (attn_sink.cu, attn_accumulate.cu,
+// attn_prefix.cu). Fields under "out" are set by tt_launch_decode.
+struct TTDecodeForm {
+    int form = 0;                    // kPassPlain / kPassSink / kPassScores (attn_pass1.cuh)
+    uint32_t sink = 0, window = 0;   // kPassSink
+    size_t reserved_bytes = 0;       // the end of the workspace, which the caller keeps for itself
+    bool partials_only = false;      // leave the split partials for the caller to merge
+    // out: where this call's partials are
+    float *part_o = nullptr, *part_m = nullptr, *part_l = nullptr;
+    float *part_m2 = nullptr, *part_l2 = nullptr;   // kPassScores
+};
+
+// Prefill over the first `tokens` keys and a sliding window: cache rows [0, tokens) hold the sinks, the rows behind
+// them a ring of `ring` rows (0: one row per key).
+struct TTPrefillSink {
+    uint32_t tokens;
+    uint32_t ring;
+};
+
+// Calls whose tables do not fit the kernel parameters upload them from host memory that the next call
+// rewrites: inside a stream capture the graph would replay whatever stands there by then, so the entry points
+// that take a TTDecodeForm refuse it.
+bool tt_stream_is_capturing(cudaStream_t stream);
+
 // Launchers implemented in the .cu files.
+cudaError_t tt_launch_pass1_sink(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items, const TTDecodeSession *sessions,
+                                 const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t *status,
+                                 const TTSessionTable &table, uint32_t table_keys, bool wide_rows, uint32_t hpc);
+cudaError_t tt_launch_pass1_scores(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items, const TTDecodeSession *sessions,
+                                   const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t *status,
+                                   const TTSessionTable &table, uint32_t table_keys, bool wide_rows, uint32_t hpc);
 int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *h_sessions,
                      uint32_t n_sessions, const tt_attn_batch_params *p, int mode,
                      float *m_out, float *d_out, float *o_out, const TTKvQuant *quant = nullptr,
-                     const tt_attn_exchange *exchange = nullptr);
+                     const tt_attn_exchange *exchange = nullptr, TTDecodeForm *form = nullptr);
 int tt_launch_merge_exchange(tt_context *ctx, cudaStream_t stream, const float *part_o, const float *part_m,
                              const float *part_l, uint32_t n_parts, const tt_attn_exchange *x, uint32_t n_q_heads,
                              uint32_t head_dim, uint32_t io_dtype);

@@ -18,6 +18,8 @@ import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
+import numpy as np
+
 from . import _lib as L
 
 
@@ -98,6 +100,20 @@ class Context:
         """Polls (~0.25 us each) the exchange kernels wait for peers before giving up; 0 = default."""
         self.check(L.lib().tt_ctx_set_exchange_poll_limit(self.handle, polls))
 
+    def stream(self, command_buffer=None) -> int:
+        """The stream handle of a call: `command_buffer`, else torch's current stream of THIS context's device."""
+        if command_buffer is not None:
+            return int(getattr(command_buffer, "cuda_stream", command_buffer))
+        import torch
+        return int(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def check_device(self, *holders):
+        """Refuses tensors (or tables over tensors) that are not on this context's device."""
+        for t in holders:
+            device = getattr(t, "device", None)
+            if device is not None and (device.type != "cuda" or device.index != self.device):
+                raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a buffer is on {device}, the context on cuda:{self.device}")
+
     @property
     def launch_count(self) -> int:
         return int(L.lib().tt_ctx_launch_count(self.handle))
@@ -134,6 +150,159 @@ class DecodeSession:
     out_offset: int = 0
     k_offset: int = 0
     v_offset: int = 0
+
+
+@dataclass
+class PrefixGroup:
+    """The shared prefix of the next `n_sessions` sessions of a call (tt_attn_prefix)."""
+    k: object
+    v: object
+    prefix_len: int
+    n_sessions: int
+    k_offset: int = 0
+    v_offset: int = 0
+
+
+def _row_stride(name: str, t, dims: int) -> int:
+    """Elements between the rows (dimension 1) of a [batch, rows, heads, head_dim] tensor with tight rows."""
+    if t.dim() != dims or t.stride(-1) != 1 or t.stride(-2) != t.shape[-1]:
+        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must be [batch, rows, heads, head_dim] with tight rows")
+    return int(t.stride(1))
+
+
+def _batch_addresses(t, index=None):
+    """Device addresses of t[i] (or t[index[i]]) for every i of the first dimension."""
+    i = np.arange(t.shape[0], dtype=np.uint64) if index is None else np.asarray(index, dtype=np.uint64)
+    return np.uint64(t.data_ptr()) + i * np.uint64(t.stride(0) * t.element_size())
+
+
+def _same_kind(what: str, *tensors):
+    first = tensors[0]
+    for t in tensors[1:]:
+        if t.dtype != first.dtype or t.device != first.device:
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{what} must share one dtype and one device")
+    if str(first.dtype) not in ("torch.float16", "torch.bfloat16"):
+        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{what} must be fp16 or bf16, not {first.dtype}")
+
+
+def _counts(name: str, values, n: int):
+    """One non-negative 32-bit number per session from a sequence, or the same for all from an int."""
+    a = np.asarray(values, dtype=np.int64)
+    if a.ndim == 0:
+        a = np.full(n, int(a), dtype=np.int64)
+    if a.shape != (n,) or (n and (int(a.min()) < 0 or int(a.max()) > 0xFFFFFFFF)):
+        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must be {n} numbers in 0..2^32-1")
+    return a.astype(np.uint32)
+
+
+class SessionTable:
+    """The sessions of a batched decode call as one block of tt_attn_session, built from whole tensors.
+
+    Call sites whose sessions live in the slots of one cache build the block without a Python object per
+    session; it is accepted wherever a list of DecodeSession is. The tensors must outlive the call."""
+
+    record = np.dtype([("q", "u8"), ("out", "u8"), ("k", "u8"), ("v", "u8"), ("seq_len", "u4"), ("q_rows", "u4"),
+                       ("kv_start", "u4"), ("reserved", "u4")])
+
+    def __init__(self, records, kv_stride=None, q_stride=None, out_stride=None, io_dtype=None, capacity=None, device=None):
+        self.records, self.kv_stride, self.q_stride, self.out_stride = records, kv_stride, q_stride, out_stride
+        self.io_dtype, self.capacity, self.device = io_dtype, capacity, device
+
+    def __len__(self):
+        return len(self.records)
+
+    @property
+    def pointer(self) -> int:
+        return self.records.ctypes.data
+
+    @classmethod
+    def over_cache(cls, q, out, k, v, seq_lens, slots=None) -> "SessionTable":
+        """q, out: [n, q_rows, n_q_heads, head_dim]; k, v: [slots, capacity, n_kv_heads, head_dim], session i in
+        slot i or slots[i]; seq_lens[i] keys are visible to the last of its rows."""
+        _same_kind("q, out, k and v", q, out, k, v)
+        q_stride, out_stride = _row_stride("q", q, 4), _row_stride("out", out, 4)
+        kv_stride = _row_stride("k", k, 4)
+        n = q.shape[0]
+        if out.shape != q.shape or v.shape != k.shape or _row_stride("v", v, 4) != kv_stride:
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "out must be shaped like q, and v laid out like k")
+        if slots is None and k.shape[0] < n:
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{n} sessions, but the cache has {k.shape[0]} slots")
+        if slots is not None and (len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k.shape[0]))):
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"slots must name {n} of the cache's {k.shape[0]} slots")
+        r = np.zeros(n, dtype=cls.record)
+        r["q"], r["out"] = _batch_addresses(q), _batch_addresses(out)
+        r["k"], r["v"] = _batch_addresses(k, slots if slots is not None else range(n)), _batch_addresses(v, slots if slots is not None else range(n))
+        r["seq_len"], r["q_rows"] = _counts("seq_lens", seq_lens, n), q.shape[1]
+        return cls(r, kv_stride, q_stride, out_stride, _dtype_of(q), int(k.shape[1]), k.device)
+
+    @classmethod
+    def of(cls, sessions) -> "SessionTable":
+        if isinstance(sessions, cls):
+            return sessions
+        r = np.zeros(len(sessions), dtype=cls.record)
+        for i, s in enumerate(sessions):
+            r[i] = (_addr(s.q, s.q_offset), _addr(s.out, s.out_offset), _addr(s.k, s.k_offset), _addr(s.v, s.v_offset),
+                    s.seq_len, s.q_rows, s.kv_start, 0)
+        return cls(r, io_dtype=_dtype_of(sessions[0].q) if len(sessions) else None)
+
+    def params(self, attention, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
+               out_row_stride_elements, scale, io_dtype) -> "L.AttnBatchParams":
+        tight_q = num_q_heads * head_dim
+        dtype = io_dtype if io_dtype is not None else self.io_dtype
+        return L.AttnBatchParams(head_dim, num_q_heads, num_kv_heads,
+                                 kv_token_stride_elements or self.kv_stride or num_kv_heads * head_dim,
+                                 q_row_stride_elements or self.q_stride or tight_q,
+                                 out_row_stride_elements or self.out_stride or tight_q,
+                                 attention.default_scale(head_dim) if scale is None else scale,
+                                 dtype if dtype is not None else L.TT_F16)
+
+    def check_capacity(self, rows=None):
+        """Refuses sessions that reach past their slot; `rows`: the rows a ring cache has."""
+        if self.capacity is None or not len(self.records):
+            return
+        need = int(self.records["seq_len"].max())
+        need = need if rows is None else min(need, rows)
+        if need > self.capacity:
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a session needs {need} rows, its slot has {self.capacity}")
+
+
+class PrefixTable:
+    """The groups of a shared-prefix call as one block of tt_attn_prefix."""
+
+    record = np.dtype([("k", "u8"), ("v", "u8"), ("prefix_len", "u4"), ("n_sessions", "u4")])
+
+    def __init__(self, records, device=None):
+        self.records, self.device = records, device
+
+    def __len__(self):
+        return len(self.records)
+
+    @property
+    def pointer(self) -> int:
+        return self.records.ctypes.data
+
+    @classmethod
+    def over_cache(cls, k, v, prefix_lens, n_sessions) -> "PrefixTable":
+        """k, v: [groups, capacity, n_kv_heads, head_dim]; n_sessions: per group, or one number for all."""
+        _same_kind("k and v", k, v)
+        if v.shape != k.shape or _row_stride("v", v, 4) != _row_stride("k", k, 4):
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "v must be laid out like k")
+        g = k.shape[0]
+        r = np.zeros(g, dtype=cls.record)
+        r["k"], r["v"] = _batch_addresses(k), _batch_addresses(v)
+        r["prefix_len"], r["n_sessions"] = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
+        if g and int(r["prefix_len"].max()) > k.shape[1]:
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a prefix is longer than the {k.shape[1]} rows of its slot")
+        return cls(r, k.device)
+
+    @classmethod
+    def of(cls, groups) -> "PrefixTable":
+        if isinstance(groups, cls):
+            return groups
+        r = np.zeros(len(groups), dtype=cls.record)
+        for i, g in enumerate(groups):
+            r[i] = (_addr(g.k, g.k_offset), _addr(g.v, g.v_offset), g.prefix_len, g.n_sessions)
+        return cls(r)
 
 
 class Attention:
@@ -240,6 +409,69 @@ class Attention:
         self.context.check(L.lib().tt_attn_decode_batched(self.context.handle, _stream(command_buffer), arr, n,
                                                           C.byref(p)))
 
+    def _table(self, sessions) -> SessionTable:
+        table = SessionTable.of(sessions)
+        self.context.check_device(table)
+        return table
+
+    def encode_sink_window(self, sessions, head_dim, num_q_heads, num_kv_heads, sink_tokens, window, ring_capacity=0,
+                           kv_token_stride_elements=None, q_row_stride_elements=None, out_row_stride_elements=None,
+                           scale=None, io_dtype=None, command_buffer=None):
+        """Decode / few-token attention over the first `sink_tokens` keys and the last `window` ones
+        (tt_attn_decode_sink_window). `sessions`: DecodeSession list or SessionTable; with `ring_capacity` R a
+        session's cache has sink_tokens + R rows and key j >= sink_tokens is row sink_tokens + (j - sink_tokens) % R."""
+        t = self._table(sessions)
+        t.check_capacity(sink_tokens + ring_capacity if ring_capacity else None)
+        p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
+                     out_row_stride_elements, scale, io_dtype)
+        self.context.check(L.lib().tt_attn_decode_sink_window(
+            self.context.handle, self.context.stream(command_buffer), t.pointer, len(t), C.byref(p), sink_tokens, window,
+            ring_capacity))
+
+    def encode_shared_prefix(self, groups, sessions, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements=None,
+                             q_row_stride_elements=None, out_row_stride_elements=None, scale=None, io_dtype=None,
+                             command_buffer=None):
+        """Decode / few-token attention of sessions that continue shared prefixes (tt_attn_decode_shared_prefix).
+        `groups`: PrefixGroup list or PrefixTable, each owning the next n_sessions of `sessions`, whose k, v and
+        seq_len describe the rows behind the prefix. Prefix and session rows have one row stride."""
+        t, g = self._table(sessions), PrefixTable.of(groups)
+        self.context.check_device(g)
+        t.check_capacity()
+        p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
+                     out_row_stride_elements, scale, io_dtype)
+        self.context.check(L.lib().tt_attn_decode_shared_prefix(
+            self.context.handle, self.context.stream(command_buffer), g.pointer, len(g), t.pointer, len(t), C.byref(p)))
+
+    _weight_record = np.dtype([("weights", "u8"), ("positions", "u8"), ("fresh_rows", "u4"), ("end_position", "u4")])
+
+    def encode_accumulate(self, sessions, weights, head_dim, num_q_heads, num_kv_heads, positions=None, fresh_rows=0,
+                          end_positions=None, kv_token_stride_elements=None, q_row_stride_elements=None,
+                          out_row_stride_elements=None, scale=None, io_dtype=None, command_buffer=None):
+        """Decode / few-token attention that adds every key's attention weight to `weights`
+        (tt_attn_decode_accumulate). weights: fp32 [n, n_kv_heads, rows]; positions: int32 like it, or None;
+        fresh_rows, end_positions: one per session or one for all (end_positions default: the sessions' seq_len)."""
+        t = self._table(sessions)
+        t.check_capacity()
+        n = len(t)
+        head_stride = _statistic("weights", weights, "torch.float32", n, num_kv_heads, self.context)
+        if positions is not None:
+            if (_statistic("positions", positions, "torch.int32", n, num_kv_heads, self.context) != head_stride or
+                    positions.shape[2] != weights.shape[2]):
+                raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "positions must be laid out like weights")
+        if n and int(t.records["seq_len"].max()) > weights.shape[2]:
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a session is longer than a weight row of {weights.shape[2]}")
+        w = np.zeros(n, dtype=self._weight_record)
+        w["weights"] = _batch_addresses(weights)[:n]
+        if positions is not None:
+            w["positions"] = _batch_addresses(positions)[:n]
+        w["fresh_rows"] = _counts("fresh_rows", fresh_rows, n)
+        w["end_position"] = t.records["seq_len"] if end_positions is None else _counts("end_positions", end_positions, n)
+        p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
+                     out_row_stride_elements, scale, io_dtype)
+        self.context.check(L.lib().tt_attn_decode_accumulate(
+            self.context.handle, self.context.stream(command_buffer), t.pointer, w.ctypes.data, n, C.byref(p),
+            head_stride))
+
     def encode_pre(self, q_packed, q_out, gate_out, k_rows, q_norm_weight, k_norm_weight, head_dim, num_q_heads,
                    num_kv_heads, rotary_dim, theta, eps, position, rows=1, k_row_stride_elements=None,
                    command_buffer=None):
@@ -343,6 +575,66 @@ def quantize_kv_rows(context: Context, source, destination, element_count: int, 
         group_size, tokens))
 
 
+def _statistic(name: str, t, dtype: str, n: int, num_kv_heads: int, context: Context):
+    if str(t.dtype) != dtype or t.dim() != 3 or t.shape[0] < n or t.shape[1] != num_kv_heads or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must be {dtype} [{n}, {num_kv_heads}, rows], rows contiguous")
+    context.check_device(t)
+    return int(t.stride(1)) if num_kv_heads > 1 else int(t.shape[2])      # elements between the heads
+
+
+_evict_record = np.dtype([(n, "u8") for n in ("k", "v", "k_out", "v_out", "weights", "weights_out", "positions",
+                                              "positions_out")] + [("rows", "u4"), ("end_position", "u4")])
+
+
+def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_tokens=0, recent_tokens=0, positions=None,
+                  end_positions=None, k_out=None, v_out=None, weights_out=None, positions_out=None, command_buffer=None):
+    """Keeps `budget` rows per KV head of every session's cache and compacts them (tt_kv_evict).
+
+    k, v: [n, capacity, n_kv_heads, head_dim], the first rows[i] of slot i in use; weights: fp32 [n, n_kv_heads, *];
+    positions: int32 like weights, None = row j holds position j; end_positions: position of the next token (default:
+    rows). *_out: None for in place, or tensors of the same kind with room for min(rows, budget) rows. Afterwards
+    session i has min(rows[i], budget) rows per head."""
+    n, num_kv_heads, head_dim = k.shape[0], k.shape[2], k.shape[3]
+    tensors = [t for t in (k, v, k_out, v_out) if t is not None]
+    _same_kind("K and V", *tensors)
+    context.check_device(*tensors)
+    rows = _counts("rows", rows, n)
+    kept = np.minimum(rows, budget)
+    in_stride = _row_stride("k", k, 4)
+    out_stride = in_stride if k_out is None else _row_stride("k_out", k_out, 4)
+    if v.shape != k.shape or _row_stride("v", v, 4) != in_stride:
+        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "v must be laid out like k")
+    if n and int(rows.max()) > k.shape[1]:
+        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a session has more rows than the {k.shape[1]} of its slot")
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is not None and (t.shape[0] < n or tuple(t.shape[2:]) != tuple(k.shape[2:]) or _row_stride(name, t, 4) != out_stride or
+                              (n and int(kept.max()) > t.shape[1])):
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must hold the kept rows of {n} sessions, laid out like k_out")
+    stat_stride, stat_out_stride = None, None
+    for name, t, dtype, is_out in (("weights", weights, "torch.float32", False), ("positions", positions, "torch.int32", False),
+                                   ("weights_out", weights_out, "torch.float32", True), ("positions_out", positions_out, "torch.int32", True)):
+        if t is None:
+            continue
+        have = _statistic(name, t, dtype, n, num_kv_heads, context)
+        want = stat_out_stride if is_out else stat_stride
+        if (want is not None and have != want) or (n and int((kept if is_out else rows).max()) > t.shape[2]):
+            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must hold the rows and be laid out like its weights")
+        if is_out:
+            stat_out_stride = have
+        else:
+            stat_stride = have
+    r = np.zeros(n, dtype=_evict_record)
+    for name, t in (("k", k), ("v", v), ("k_out", k_out), ("v_out", v_out), ("weights", weights), ("weights_out", weights_out),
+                    ("positions", positions), ("positions_out", positions_out)):
+        if t is not None:
+            r[name] = _batch_addresses(t)[:n]
+    r["rows"] = rows
+    r["end_position"] = rows if end_positions is None else _counts("end_positions", end_positions, n)
+    p = L.KVEvictParams(head_dim, num_kv_heads, budget, sink_tokens, recent_tokens, in_stride, out_stride, stat_stride,
+                        stat_out_stride or stat_stride, 0)
+    context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), r.ctypes.data, n, C.byref(p)))
+
+
 @dataclass
 class PrefillAttentionParams:
     """PrefillAttentionParams (PrefillAttention.swift:5-55), same fields and defaults."""
@@ -391,6 +683,22 @@ class PrefillAttention:
             self.context.handle, _stream(command_buffer), _addr(q, q_offset), _addr(k, k_offset),
             _addr(v, v_offset), _addr(out, out_offset), C.byref(cp), kv_ring_capacity,
             io_dtype if io_dtype is not None else _dtype_of(q)))
+
+    def encode_sink_window(self, q, k, v, out, params: PrefillAttentionParams, sink_tokens, kv_ring_capacity=0,
+                           io_dtype=None, command_buffer=None, q_offset=0, k_offset=0, v_offset=0, out_offset=0):
+        """Causal prefill over the first `sink_tokens` keys and a sliding window of params.sliding_window
+        (tt_attn_prefill_sink_window); a ring lies behind the sinks' rows as in Attention.encode_sink_window."""
+        self.context.check_device(q, k, v, out)
+        self.context.check(L.lib().tt_attn_prefill_sink_window(
+            self.context.handle, self.context.stream(command_buffer), _addr(q, q_offset), _addr(k, k_offset),
+            _addr(v, v_offset), _addr(out, out_offset), C.byref(params.to_c()), sink_tokens, kv_ring_capacity,
+            io_dtype if io_dtype is not None else _dtype_of(q)))
+
+    @staticmethod
+    def sink_window_path(q, k, v, out, params: PrefillAttentionParams, kv_ring_capacity=0) -> str:
+        path = L.lib().tt_attn_prefill_sink_path(_addr(q), _addr(k), _addr(v), _addr(out), C.byref(params.to_c()),
+                                                 kv_ring_capacity)
+        return "tcgen05" if path == 1 else "generic"
 
     @staticmethod
     def selected_path(q, k, v, out, params: PrefillAttentionParams, kv_ring_capacity=0, q_offset=0, k_offset=0,
