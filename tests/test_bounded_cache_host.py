@@ -153,5 +153,7 @@ def test_wrappers_refuse_before_the_library():
         tt.PrefixTable.over_cache(k, v, 21, 1)
     with pytest.raises(tt.InvalidArgument):
         tt.evict_kv_rows(_Context(), k, v, torch.zeros(3, 2, 20), 20, 8)          # CPU tensors
-    assert C.sizeof(L.KVEvictSession) == tt.operators._evict_record.itemsize
-    assert C.sizeof(L.AttnWeightRows) == tt.Attention._weight_record.itemsize
+    # the blocks of 64-bit words the wrappers build are the C structures
+    assert C.sizeof(L.KVEvictSession) == 9 * 8 and C.sizeof(L.AttnWeightRows) == 3 * 8
+    assert [getattr(L.KVEvictSession, n).offset for n in ("k_out", "weights", "positions_out", "rows", "end_position")] == [16, 32, 56, 64, 68]
+    assert [getattr(L.AttnWeightRows, n).offset for n in ("positions", "fresh_rows", "end_position")] == [8, 16, 20]

@@ -9,7 +9,9 @@
 #include "tt_common.h"
 
 int tt_launch_prefill_tc(tt_context *ctx, cudaStream_t stream, const void *q, const void *k, const void *v,
-                         void *out, const tt_prefill_params *p, uint32_t io_dtype, const TTPrefillSink *sink = nullptr);
+                         void *out, const tt_prefill_params *p, uint32_t io_dtype);
+int tt_launch_prefill_sink(tt_context *ctx, cudaStream_t stream, const void *q, const void *k, const void *v, void *out,
+                           const tt_prefill_params *p, uint32_t io_dtype, uint32_t sink_tokens, uint32_t ring);
 
 namespace {
 
@@ -290,10 +292,8 @@ TT_API int tt_attn_prefill_sink_window(tt_context *ctx, tt_stream stream, const 
         (params->sliding_window == 0 || (uint64_t)ring_capacity < (uint64_t)params->sliding_window + newest - 1))
         return tt_set_error(ctx, TT_ERR_INVALID_ARG, "a ring of %u rows cannot hold a window of %u for %u new rows", ring_capacity,
                             params->sliding_window, (uint32_t)newest);
-    if (tt_attn_prefill_sink_path(q, k, v, out, params, ring_capacity) == 1 && getenv("TT_PREFILL_FORCE_GENERIC") == nullptr) {
-        const TTPrefillSink sink = {sink_tokens, ring_capacity};
-        return tt_launch_prefill_tc(ctx, (cudaStream_t)stream, q, k, v, out, params, io_dtype, &sink);
-    }
+    if (tt_attn_prefill_sink_path(q, k, v, out, params, ring_capacity) == 1 && getenv("TT_PREFILL_FORCE_GENERIC") == nullptr)
+        return tt_launch_prefill_sink(ctx, (cudaStream_t)stream, q, k, v, out, params, io_dtype, sink_tokens, ring_capacity);
     const PrefillSelection sel = {0, nullptr, 0, nullptr, nullptr, 0, nullptr, sink_tokens};
     return launch_generic(ctx, (cudaStream_t)stream, q, k, v, out, params, ring_capacity, io_dtype, sel);
 }

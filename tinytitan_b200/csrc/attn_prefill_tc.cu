@@ -90,22 +90,11 @@ struct PrefillTcParams {
     uint32_t idesc_qk, idesc_pv;
 };
 
-// What the form with sinks needs beyond the plain kernel: its own maps over the first `sink` rows alone, so that
-// the rows behind them in the cache (no query of the tile may see them) read as zeros and may hold anything.
-template <bool SINK>
-struct PrefillSink {};
-template <>
-struct PrefillSink<true> {
-    CUtensorMap k_map, v_map;
-    uint32_t sink;
-    uint32_t ring;      // rows of the ring behind the sinks, a multiple of the 64-key box; 0: plain rows
-};
-
-template <typename T, bool SINK>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_prefill_tc_kernel(const T *__restrict__ q, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map, T *__restrict__ out, PrefillTcParams p,
-                       uint32_t *__restrict__ status, const __grid_constant__ PrefillSink<SINK> sk) {
+                       uint32_t *__restrict__ status) {
     // every byte of the 227 KB is spoken for, so there is no slack to align the tiles by hand: the
     // dynamic window of a kernel without static shared memory starts 1024-byte aligned, and a launch
     // where it does not is refused rather than run with broken swizzles
@@ -133,29 +122,8 @@ attn_prefill_tc_kernel(const T *__restrict__ q, const __grid_constant__ CUtensor
     uint32_t key_lo = 0;
     if (p.sliding_window != 0 && abs_lo + 1 > p.sliding_window) key_lo = abs_lo + 1 - p.sliding_window;
     const uint32_t key_hi = min(p.kv_valid_count, abs_hi + 1);       // exclusive
-    // Key tiles. Plain: the multiples of 128 that cover [key_lo, key_hi). With sinks and a window that starts behind
-    // them: tiles over [0, sink) first, then tiles from the window's first key on (in a ring: from the last 64-key
-    // box boundary before it, so that no box runs over the ring's end).
-    uint32_t sink_tiles = 0, base = key_lo / kBN * kBN;
-    if constexpr (SINK) {
-        base = 0;
-        if (key_lo > sk.sink) {
-            sink_tiles = (sk.sink + kBN - 1) / kBN;
-            base = sk.ring ? sk.sink + (key_lo - sk.sink) / kBox * kBox : key_lo;
-        }
-    }
-    const uint32_t n_tiles = sink_tiles + (key_hi - base + kBN - 1) / kBN;     // >= 1
-    // first key of tile j, and where 64-key box `half` of tile j starts: the map it is read through and its row
-    auto tile_key = [&](uint32_t j) { return SINK && j < sink_tiles ? j * kBN : base + (j - sink_tiles) * kBN; };
-    auto box = [&](uint32_t j, int half, const CUtensorMap *plain, const CUtensorMap *sinks, int &row) {
-        const uint32_t key = tile_key(j) + half * kBox;
-        row = (int)key;
-        if constexpr (SINK) {
-            if (j < sink_tiles) return sinks;
-            if (sk.ring && key >= sk.sink) row = (int)(sk.sink + (key - sk.sink) % sk.ring);
-        }
-        return plain;
-    };
+    const uint32_t tile_lo = key_lo / kBN;
+    const uint32_t n_tiles = (key_hi + kBN - 1) / kBN - tile_lo;     // >= 1
 
     if (threadIdx.x == 0) {
         mbar_init(&bars->q_ready, 256);
@@ -192,15 +160,11 @@ attn_prefill_tc_kernel(const T *__restrict__ q, const __grid_constant__ CUtensor
                 if (kc >= (uint32_t)kKSlots) ok = mbar_wait(&bars->k_empty[slot], ((kc / kKSlots) - 1) & 1);
                 if (!ok) break;
                 mbar_expect_tx(&bars->k_full[slot], kKChunk);
-                for (int half = 0; half < 2; ++half) {
-                    int row;
-                    const CUtensorMap *map = &k_map;
-                    if constexpr (SINK) map = box(kc >> 1, half, &k_map, &sk.k_map, row);
-                    else row = (int)(tile_key(kc >> 1) + half * kBox);
-                    for (int sub = 0; sub < 2; ++sub)
-                        tma_load_2d(k_s + slot * kKChunk + sub * kKVSub + half * kBoxBytes, map,
-                                    (int)(kv_head * kHD + (kc & 1) * 128 + sub * 64), row, &bars->k_full[slot]);
-                }
+                for (int sub = 0; sub < 2; ++sub)
+                    for (int half = 0; half < 2; ++half)
+                        tma_load_2d(k_s + slot * kKChunk + sub * kKVSub + half * kBoxBytes, &k_map,
+                                    (int)(kv_head * kHD + (kc & 1) * 128 + sub * 64),
+                                    (int)((tile_lo + (kc >> 1)) * kBN + half * kBox), &bars->k_full[slot]);
             }
             failed = !ok;
         } else if (lane == 1) {
@@ -210,13 +174,9 @@ attn_prefill_tc_kernel(const T *__restrict__ q, const __grid_constant__ CUtensor
                     if (j >= 1) ok = mbar_wait(&bars->v_empty[half], (j - 1) & 1);
                     if (!ok) break;
                     mbar_expect_tx(&bars->v_full[half], kKVTile / 2);
-                    int row;
-                    const CUtensorMap *map = &v_map;
-                    if constexpr (SINK) map = box(j, half, &v_map, &sk.v_map, row);
-                    else row = (int)(tile_key(j) + half * kBox);
                     for (int sub = 0; sub < 4; ++sub)
-                        tma_load_2d(v_s + sub * kKVSub + half * kBoxBytes, map, (int)(kv_head * kHD + sub * 64), row,
-                                    &bars->v_full[half]);
+                        tma_load_2d(v_s + sub * kKVSub + half * kBoxBytes, &v_map, (int)(kv_head * kHD + sub * 64),
+                                    (int)((tile_lo + j) * kBN + half * kBox), &bars->v_full[half]);
                 }
             failed = !ok;
         }
@@ -331,13 +291,8 @@ attn_prefill_tc_kernel(const T *__restrict__ q, const __grid_constant__ CUtensor
             tc_fence_before();
             mbar_arrive(&bars->s_read);        // this half of the score tile is in registers
 
-            const uint32_t key0 = tile_key(j) + wg * 64;           // first key of this thread's half
-            bool need_mask = (key0 + 64 > abs_lo + 1) || (key0 < first) || (key0 + 64 > p.kv_valid_count);
-            uint32_t lo = first, hi = last;
-            if constexpr (SINK) {
-                // a sink tile counts its keys below `sink` alone (the window's tiles count the others)
-                if (j < sink_tiles) { lo = 0; hi = min(sk.sink, last); need_mask = key0 + 64 > hi; }
-            }
+            const uint32_t key0 = (tile_lo + j) * kBN + wg * 64;   // first key of this thread's half
+            const bool need_mask = (key0 + 64 > abs_lo + 1) || (key0 < first) || (key0 + 64 > p.kv_valid_count);
             // masked keys become -inf before the scale (which is positive, so they stay -inf and the row
             // maximum can be taken on the unscaled scores, in four independent chains)
             if (need_mask) {
@@ -346,11 +301,7 @@ attn_prefill_tc_kernel(const T *__restrict__ q, const __grid_constant__ CUtensor
 #pragma unroll
                     for (int c = 0; c < 32; ++c) {
                         const uint32_t key = key0 + h * 32 + c;
-                        if constexpr (SINK) {
-                            if ((key < lo && key >= sk.sink) || key >= hi) raw[h][c] = 0xff800000u;
-                        } else {
-                            if (key < lo || key >= hi) raw[h][c] = 0xff800000u;
-                        }
+                        if (key < first || key >= last) raw[h][c] = 0xff800000u;
                     }
             }
             float mx4[4];
@@ -509,39 +460,13 @@ bool tt_make_tensor_map_2d_f32(CUtensorMap *map, const void *base, uint64_t widt
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-namespace {
-
-template <typename T, bool SINK>
-cudaError_t launch_tc(tt_context *ctx, cudaStream_t stream, const void *q, const CUtensorMap &k_map, const CUtensorMap &v_map,
-                      void *out, const PrefillTcParams &kp, const PrefillSink<SINK> &sk) {
-    auto kernel = attn_prefill_tc_kernel<T, SINK>;
-    cudaError_t e = tt_set_smem_once(kernel, kSmemBytes);
-    if (e != cudaSuccess) return e;
-    kernel<<<kp.n_q_tiles * kp.n_q_heads, kThreads, kSmemBytes, stream>>>(reinterpret_cast<const T *>(q), k_map, v_map,
-                                                                          reinterpret_cast<T *>(out), kp, ctx->status, sk);
-    return cudaGetLastError();
-}
-
-}  // namespace
-
-// `sink` null: the plain call. Otherwise the keys below sink->tokens stay visible beside the window and the rows behind
-// them form a ring of sink->ring rows (0: plain rows).
 int tt_launch_prefill_tc(tt_context *ctx, cudaStream_t stream, const void *q, const void *k, const void *v,
-                         void *out, const tt_prefill_params *p, uint32_t io_dtype, const TTPrefillSink *sink) {
-    const uint64_t width = (uint64_t)p->n_kv_heads * kHD;
-    uint64_t rows = p->kv_valid_count;
-    if (sink != nullptr && sink->ring != 0 && rows > (uint64_t)sink->tokens + sink->ring) rows = (uint64_t)sink->tokens + sink->ring;
+                         void *out, const tt_prefill_params *p, uint32_t io_dtype) {
     CUtensorMap k_map, v_map;
-    bool ok = tt_make_tensor_map_2d(&k_map, k, io_dtype, width, rows, p->kv_token_stride_elements, kBox) &&
-              tt_make_tensor_map_2d(&v_map, v, io_dtype, width, rows, p->kv_token_stride_elements, kBox);
-    PrefillSink<true> sk;
-    if (ok && sink != nullptr) {
-        const uint64_t sink_rows = sink->tokens == 0 ? 1 : sink->tokens < rows ? sink->tokens : rows;
-        ok = tt_make_tensor_map_2d(&sk.k_map, k, io_dtype, width, sink_rows, p->kv_token_stride_elements, kBox) &&
-             tt_make_tensor_map_2d(&sk.v_map, v, io_dtype, width, sink_rows, p->kv_token_stride_elements, kBox);
-        sk.sink = sink->tokens;
-        sk.ring = sink->ring;
-    }
+    const bool ok = tt_make_tensor_map_2d(&k_map, k, io_dtype, (uint64_t)p->n_kv_heads * kHD, p->kv_valid_count,
+                             p->kv_token_stride_elements, kBox) &&
+                    tt_make_tensor_map_2d(&v_map, v, io_dtype, (uint64_t)p->n_kv_heads * kHD, p->kv_valid_count,
+                             p->kv_token_stride_elements, kBox);
     if (!ok) return tt_set_error(ctx, TT_ERR_CUDA, "cuTensorMapEncodeTiled failed for the prefill operands");
     PrefillTcParams kp;
     kp.start_position = p->start_position; kp.query_count = p->query_count; kp.n_q_heads = p->n_q_heads;
@@ -552,13 +477,20 @@ int tt_launch_prefill_tc(tt_context *ctx, cudaStream_t stream, const void *q, co
     kp.scale_log2 = p->scale * kLog2e;
     kp.idesc_qk = tt_make_idesc_f16(io_dtype, kBN, false);
     kp.idesc_pv = tt_make_idesc_f16(io_dtype, kHD, true);
+    const uint32_t grid = kp.n_q_tiles * p->n_q_heads;
     cudaError_t e;
-    if (sink == nullptr)
-        e = io_dtype == TT_F16 ? launch_tc<__half, false>(ctx, stream, q, k_map, v_map, out, kp, PrefillSink<false>())
-                               : launch_tc<__nv_bfloat16, false>(ctx, stream, q, k_map, v_map, out, kp, PrefillSink<false>());
-    else
-        e = io_dtype == TT_F16 ? launch_tc<__half, true>(ctx, stream, q, k_map, v_map, out, kp, sk)
-                               : launch_tc<__nv_bfloat16, true>(ctx, stream, q, k_map, v_map, out, kp, sk);
+    if (io_dtype == TT_F16) {
+        auto kernel = attn_prefill_tc_kernel<__half>;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) return tt_check_cuda(ctx, e, "prefill smem attribute");
+        kernel<<<grid, kThreads, kSmemBytes, stream>>>(reinterpret_cast<const __half *>(q), k_map, v_map, reinterpret_cast<__half *>(out), kp, ctx->status);
+    } else {
+        auto kernel = attn_prefill_tc_kernel<__nv_bfloat16>;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) return tt_check_cuda(ctx, e, "prefill smem attribute");
+        kernel<<<grid, kThreads, kSmemBytes, stream>>>(reinterpret_cast<const __nv_bfloat16 *>(q), k_map, v_map, reinterpret_cast<__nv_bfloat16 *>(out), kp, ctx->status);
+    }
+    e = cudaGetLastError();
     if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_prefill_tc launch");
     ctx->launches++;
     return TT_OK;

@@ -205,13 +205,6 @@ struct TTDecodeForm {
     float *part_m2 = nullptr, *part_l2 = nullptr;   // kPassScores
 };
 
-// Prefill over the first `tokens` keys and a sliding window: cache rows [0, tokens) hold the sinks, the rows behind
-// them a ring of `ring` rows (0: one row per key).
-struct TTPrefillSink {
-    uint32_t tokens;
-    uint32_t ring;
-};
-
 // Calls whose tables do not fit the kernel parameters upload them from host memory that the next call
 // rewrites: inside a stream capture the graph would replay whatever stands there by then, so the entry points
 // that take a TTDecodeForm refuse it.

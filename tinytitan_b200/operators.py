@@ -163,36 +163,66 @@ class PrefixGroup:
     v_offset: int = 0
 
 
-def _row_stride(name: str, t, dims: int) -> int:
+def _refuse(message: str):
+    raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, message)
+
+
+def _cache_stride(name: str, t) -> int:
     """Elements between the rows (dimension 1) of a [batch, rows, heads, head_dim] tensor with tight rows."""
-    if t.dim() != dims or t.stride(-1) != 1 or t.stride(-2) != t.shape[-1]:
-        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must be [batch, rows, heads, head_dim] with tight rows")
-    return int(t.stride(1))
+    stride = t.stride()
+    if len(stride) != 4 or stride[3] != 1 or stride[2] != t.shape[3]:
+        _refuse(f"{name} must be [batch, rows, heads, head_dim] with tight rows")
+    return stride[1]
 
 
-def _batch_addresses(t, index=None):
-    """Device addresses of t[i] (or t[index[i]]) for every i of the first dimension."""
-    i = np.arange(t.shape[0], dtype=np.uint64) if index is None else np.asarray(index, dtype=np.uint64)
-    return np.uint64(t.data_ptr()) + i * np.uint64(t.stride(0) * t.element_size())
+def _half_dtype(what: str, first, *others) -> int:
+    """The tt_dtype of tensors that must share one 16-bit type and one device."""
+    dtype, device = first.dtype, first.device
+    for t in others:
+        if t.dtype != dtype or t.device != device:
+            _refuse(f"{what} must share one dtype and one device")
+    name = str(dtype)
+    if name == "torch.float16":
+        return L.TT_F16
+    if name != "torch.bfloat16":
+        _refuse(f"{what} must be fp16 or bf16, not {name}")
+    return L.TT_BF16
 
 
-def _same_kind(what: str, *tensors):
-    first = tensors[0]
-    for t in tensors[1:]:
-        if t.dtype != first.dtype or t.device != first.device:
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{what} must share one dtype and one device")
-    if str(first.dtype) not in ("torch.float16", "torch.bfloat16"):
-        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{what} must be fp16 or bf16, not {first.dtype}")
+_indices = np.arange(64, dtype=np.uint64)[:, None]
+
+
+def _addresses(n: int, *tensors, index=None):
+    """[n, len(tensors)] device addresses of t[i] (or t[index[i]]) for i < n; None gives zeros."""
+    global _indices
+    if index is not None:
+        i = np.asarray(index, dtype=np.uint64)[:, None]
+    else:
+        if n > len(_indices):
+            _indices = np.arange(2 * n, dtype=np.uint64)[:, None]
+        i = _indices[:n]
+    base = np.array([0 if t is None else t.data_ptr() for t in tensors], dtype=np.uint64)
+    step = np.array([0 if t is None else t.stride(0) * t.element_size() for t in tensors], dtype=np.uint64)
+    return i * step + base
 
 
 def _counts(name: str, values, n: int):
-    """One non-negative 32-bit number per session from a sequence, or the same for all from an int."""
-    a = np.asarray(values, dtype=np.int64)
-    if a.ndim == 0:
-        a = np.full(n, int(a), dtype=np.int64)
-    if a.shape != (n,) or (n and (int(a.min()) < 0 or int(a.max()) > 0xFFFFFFFF)):
-        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must be {n} numbers in 0..2^32-1")
-    return a.astype(np.uint32)
+    """n numbers in 0..2^32-1 from a sequence, or from one int for all."""
+    try:
+        if isinstance(values, int):
+            a = np.full(n, values, dtype=np.uint32)
+        elif isinstance(values, (list, tuple)):
+            a = np.array(values, dtype=np.uint32)
+        else:
+            wide = np.asarray(values)
+            a = wide.astype(np.uint32)
+            if (wide != a).any():
+                raise OverflowError
+    except (OverflowError, TypeError, ValueError):
+        a = None
+    if a is None or a.shape != (n,):
+        _refuse(f"{name} must be {n} numbers in 0..2^32-1")
+    return a
 
 
 class SessionTable:
@@ -204,46 +234,56 @@ class SessionTable:
     record = np.dtype([("q", "u8"), ("out", "u8"), ("k", "u8"), ("v", "u8"), ("seq_len", "u4"), ("q_rows", "u4"),
                        ("kv_start", "u4"), ("reserved", "u4")])
 
-    def __init__(self, records, kv_stride=None, q_stride=None, out_stride=None, io_dtype=None, capacity=None, device=None):
-        self.records, self.kv_stride, self.q_stride, self.out_stride = records, kv_stride, q_stride, out_stride
+    def __init__(self, words, longest=0, kv_stride=None, q_stride=None, out_stride=None, io_dtype=None, capacity=None, device=None):
+        self.words, self.longest, self.kv_stride, self.q_stride, self.out_stride = words, longest, kv_stride, q_stride, out_stride
         self.io_dtype, self.capacity, self.device = io_dtype, capacity, device
 
     def __len__(self):
-        return len(self.records)
+        return len(self.words)
+
+    @property
+    def records(self):
+        return self.words.view(self.record)[:, 0]
 
     @property
     def pointer(self) -> int:
-        return self.records.ctypes.data
+        return self.words.__array_interface__["data"][0]
 
     @classmethod
     def over_cache(cls, q, out, k, v, seq_lens, slots=None) -> "SessionTable":
         """q, out: [n, q_rows, n_q_heads, head_dim]; k, v: [slots, capacity, n_kv_heads, head_dim], session i in
         slot i or slots[i]; seq_lens[i] keys are visible to the last of its rows."""
-        _same_kind("q, out, k and v", q, out, k, v)
-        q_stride, out_stride = _row_stride("q", q, 4), _row_stride("out", out, 4)
-        kv_stride = _row_stride("k", k, 4)
-        n = q.shape[0]
-        if out.shape != q.shape or v.shape != k.shape or _row_stride("v", v, 4) != kv_stride:
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "out must be shaped like q, and v laid out like k")
-        if slots is None and k.shape[0] < n:
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{n} sessions, but the cache has {k.shape[0]} slots")
-        if slots is not None and (len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k.shape[0]))):
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"slots must name {n} of the cache's {k.shape[0]} slots")
-        r = np.zeros(n, dtype=cls.record)
-        r["q"], r["out"] = _batch_addresses(q), _batch_addresses(out)
-        r["k"], r["v"] = _batch_addresses(k, slots if slots is not None else range(n)), _batch_addresses(v, slots if slots is not None else range(n))
-        r["seq_len"], r["q_rows"] = _counts("seq_lens", seq_lens, n), q.shape[1]
-        return cls(r, kv_stride, q_stride, out_stride, _dtype_of(q), int(k.shape[1]), k.device)
+        io_dtype = _half_dtype("q, out, k and v", q, out, k, v)
+        q_stride, out_stride, kv_stride = _cache_stride("q", q), _cache_stride("out", out), _cache_stride("k", k)
+        n, q_rows = q.shape[:2]
+        if out.shape != q.shape or v.shape != k.shape or _cache_stride("v", v) != kv_stride:
+            _refuse("out must be shaped like q, and v laid out like k")
+        if slots is None:
+            if k.shape[0] < n:
+                _refuse(f"{n} sessions, but the cache has {k.shape[0]} slots")
+        elif len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k.shape[0])):
+            _refuse(f"slots must name {n} of the cache's {k.shape[0]} slots")
+        lens = _counts("seq_lens", seq_lens, n)
+        words = np.empty((n, 6), dtype=np.uint64)
+        if slots is None:
+            words[:, :4] = _addresses(n, q, out, k, v)
+        else:
+            words[:, :2], words[:, 2:4] = _addresses(n, q, out), _addresses(n, k, v, index=slots)
+        words[:, 4] = lens + np.uint64(q_rows << 32)
+        words[:, 5] = 0
+        return cls(words, int(lens.max()) if n else 0, kv_stride, q_stride, out_stride, io_dtype, k.shape[1], k.device)
 
     @classmethod
     def of(cls, sessions) -> "SessionTable":
         if isinstance(sessions, cls):
             return sessions
-        r = np.zeros(len(sessions), dtype=cls.record)
+        words = np.zeros((len(sessions), 6), dtype=np.uint64)
+        r = words.view(cls.record)[:, 0]
         for i, s in enumerate(sessions):
             r[i] = (_addr(s.q, s.q_offset), _addr(s.out, s.out_offset), _addr(s.k, s.k_offset), _addr(s.v, s.v_offset),
                     s.seq_len, s.q_rows, s.kv_start, 0)
-        return cls(r, io_dtype=_dtype_of(sessions[0].q) if len(sessions) else None)
+        return cls(words, max((s.seq_len for s in sessions), default=0),
+                   io_dtype=_dtype_of(sessions[0].q) if len(sessions) else None)
 
     def params(self, attention, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                out_row_stride_elements, scale, io_dtype) -> "L.AttnBatchParams":
@@ -258,12 +298,9 @@ class SessionTable:
 
     def check_capacity(self, rows=None):
         """Refuses sessions that reach past their slot; `rows`: the rows a ring cache has."""
-        if self.capacity is None or not len(self.records):
-            return
-        need = int(self.records["seq_len"].max())
-        need = need if rows is None else min(need, rows)
-        if need > self.capacity:
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a session needs {need} rows, its slot has {self.capacity}")
+        need = self.longest if rows is None else min(self.longest, rows)
+        if self.capacity is not None and need > self.capacity:
+            _refuse(f"a session needs {need} rows, its slot has {self.capacity}")
 
 
 class PrefixTable:
@@ -271,38 +308,44 @@ class PrefixTable:
 
     record = np.dtype([("k", "u8"), ("v", "u8"), ("prefix_len", "u4"), ("n_sessions", "u4")])
 
-    def __init__(self, records, device=None):
-        self.records, self.device = records, device
+    def __init__(self, words, device=None):
+        self.words, self.device = words, device
 
     def __len__(self):
-        return len(self.records)
+        return len(self.words)
+
+    @property
+    def records(self):
+        return self.words.view(self.record)[:, 0]
 
     @property
     def pointer(self) -> int:
-        return self.records.ctypes.data
+        return self.words.__array_interface__["data"][0]
 
     @classmethod
     def over_cache(cls, k, v, prefix_lens, n_sessions) -> "PrefixTable":
         """k, v: [groups, capacity, n_kv_heads, head_dim]; n_sessions: per group, or one number for all."""
-        _same_kind("k and v", k, v)
-        if v.shape != k.shape or _row_stride("v", v, 4) != _row_stride("k", k, 4):
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "v must be laid out like k")
+        _half_dtype("k and v", k, v)
+        if v.shape != k.shape or _cache_stride("v", v) != _cache_stride("k", k):
+            _refuse("v must be laid out like k")
         g = k.shape[0]
-        r = np.zeros(g, dtype=cls.record)
-        r["k"], r["v"] = _batch_addresses(k), _batch_addresses(v)
-        r["prefix_len"], r["n_sessions"] = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
-        if g and int(r["prefix_len"].max()) > k.shape[1]:
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a prefix is longer than the {k.shape[1]} rows of its slot")
-        return cls(r, k.device)
+        lens, counts = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
+        if g and int(lens.max()) > k.shape[1]:
+            _refuse(f"a prefix is longer than the {k.shape[1]} rows of its slot")
+        words = np.empty((g, 3), dtype=np.uint64)
+        words[:, :2] = _addresses(g, k, v)
+        words[:, 2] = lens + (counts.astype(np.uint64) << np.uint64(32))
+        return cls(words, k.device)
 
     @classmethod
     def of(cls, groups) -> "PrefixTable":
         if isinstance(groups, cls):
             return groups
-        r = np.zeros(len(groups), dtype=cls.record)
+        words = np.zeros((len(groups), 3), dtype=np.uint64)
+        r = words.view(cls.record)[:, 0]
         for i, g in enumerate(groups):
             r[i] = (_addr(g.k, g.k_offset), _addr(g.v, g.v_offset), g.prefix_len, g.n_sessions)
-        return cls(r)
+        return cls(words)
 
 
 class Attention:
@@ -442,8 +485,6 @@ class Attention:
         self.context.check(L.lib().tt_attn_decode_shared_prefix(
             self.context.handle, self.context.stream(command_buffer), g.pointer, len(g), t.pointer, len(t), C.byref(p)))
 
-    _weight_record = np.dtype([("weights", "u8"), ("positions", "u8"), ("fresh_rows", "u4"), ("end_position", "u4")])
-
     def encode_accumulate(self, sessions, weights, head_dim, num_q_heads, num_kv_heads, positions=None, fresh_rows=0,
                           end_positions=None, kv_token_stride_elements=None, q_row_stride_elements=None,
                           out_row_stride_elements=None, scale=None, io_dtype=None, command_buffer=None):
@@ -454,23 +495,20 @@ class Attention:
         t.check_capacity()
         n = len(t)
         head_stride = _statistic("weights", weights, "torch.float32", n, num_kv_heads, self.context)
-        if positions is not None:
-            if (_statistic("positions", positions, "torch.int32", n, num_kv_heads, self.context) != head_stride or
-                    positions.shape[2] != weights.shape[2]):
-                raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "positions must be laid out like weights")
-        if n and int(t.records["seq_len"].max()) > weights.shape[2]:
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a session is longer than a weight row of {weights.shape[2]}")
-        w = np.zeros(n, dtype=self._weight_record)
-        w["weights"] = _batch_addresses(weights)[:n]
-        if positions is not None:
-            w["positions"] = _batch_addresses(positions)[:n]
-        w["fresh_rows"] = _counts("fresh_rows", fresh_rows, n)
-        w["end_position"] = t.records["seq_len"] if end_positions is None else _counts("end_positions", end_positions, n)
+        if positions is not None and (positions.shape != weights.shape or head_stride != _statistic(
+                "positions", positions, "torch.int32", n, num_kv_heads, self.context)):
+            _refuse("positions must be laid out like weights")
+        if t.longest > weights.shape[2]:
+            _refuse(f"a session is longer than a weight row of {weights.shape[2]}")
+        words = np.empty((n, 3), dtype=np.uint64)          # tt_attn_weight_rows
+        words[:, :2] = _addresses(n, weights, positions)
+        ends = (t.words[:, 4] & np.uint64(0xFFFFFFFF)) if end_positions is None else _counts("end_positions", end_positions, n).astype(np.uint64)
+        words[:, 2] = _counts("fresh_rows", fresh_rows, n) + (ends << np.uint64(32))
         p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                      out_row_stride_elements, scale, io_dtype)
         self.context.check(L.lib().tt_attn_decode_accumulate(
-            self.context.handle, self.context.stream(command_buffer), t.pointer, w.ctypes.data, n, C.byref(p),
-            head_stride))
+            self.context.handle, self.context.stream(command_buffer), t.pointer, words.__array_interface__["data"][0], n,
+            C.byref(p), head_stride))
 
     def encode_pre(self, q_packed, q_out, gate_out, k_rows, q_norm_weight, k_norm_weight, head_dim, num_q_heads,
                    num_kv_heads, rotary_dim, theta, eps, position, rows=1, k_row_stride_elements=None,
@@ -575,15 +613,13 @@ def quantize_kv_rows(context: Context, source, destination, element_count: int, 
         group_size, tokens))
 
 
-def _statistic(name: str, t, dtype: str, n: int, num_kv_heads: int, context: Context):
-    if str(t.dtype) != dtype or t.dim() != 3 or t.shape[0] < n or t.shape[1] != num_kv_heads or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must be {dtype} [{n}, {num_kv_heads}, rows], rows contiguous")
+def _statistic(name: str, t, dtype: str, n: int, num_kv_heads: int, context: Context) -> int:
+    """Elements between the heads of a [sessions, n_kv_heads, rows] tensor that holds one number per cache row."""
+    shape, stride = t.shape, t.stride()
+    if str(t.dtype) != dtype or len(shape) != 3 or shape[0] < n or shape[1] != num_kv_heads or (shape[2] > 1 and stride[2] != 1):
+        _refuse(f"{name} must be {dtype} [{n}, {num_kv_heads}, rows], rows contiguous")
     context.check_device(t)
-    return int(t.stride(1)) if num_kv_heads > 1 else int(t.shape[2])      # elements between the heads
-
-
-_evict_record = np.dtype([(n, "u8") for n in ("k", "v", "k_out", "v_out", "weights", "weights_out", "positions",
-                                              "positions_out")] + [("rows", "u4"), ("end_position", "u4")])
+    return stride[1] if num_kv_heads > 1 else shape[2]
 
 
 def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_tokens=0, recent_tokens=0, positions=None,
@@ -594,45 +630,44 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
     positions: int32 like weights, None = row j holds position j; end_positions: position of the next token (default:
     rows). *_out: None for in place, or tensors of the same kind with room for min(rows, budget) rows. Afterwards
     session i has min(rows[i], budget) rows per head."""
-    n, num_kv_heads, head_dim = k.shape[0], k.shape[2], k.shape[3]
-    tensors = [t for t in (k, v, k_out, v_out) if t is not None]
-    _same_kind("K and V", *tensors)
-    context.check_device(*tensors)
-    rows = _counts("rows", rows, n)
-    kept = np.minimum(rows, budget)
-    in_stride = _row_stride("k", k, 4)
-    out_stride = in_stride if k_out is None else _row_stride("k_out", k_out, 4)
-    if v.shape != k.shape or _row_stride("v", v, 4) != in_stride:
-        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, "v must be laid out like k")
-    if n and int(rows.max()) > k.shape[1]:
-        raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a session has more rows than the {k.shape[1]} of its slot")
+    _half_dtype("K and V", k, *(t for t in (v, k_out, v_out) if t is not None))
+    context.check_device(k)
+    in_stride = _cache_stride("k", k)
+    if v.shape != k.shape or _cache_stride("v", v) != in_stride:
+        _refuse("v must be laid out like k")
+    n, capacity, num_kv_heads, head_dim = k.shape
+    used = _counts("rows", rows, n)
+    most = int(used.max()) if n else 0
+    kept = min(most, budget)
+    if most > capacity:
+        _refuse(f"a session has more rows than the {capacity} of its slot")
+    out_stride = in_stride
     for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is not None and (t.shape[0] < n or tuple(t.shape[2:]) != tuple(k.shape[2:]) or _row_stride(name, t, 4) != out_stride or
-                              (n and int(kept.max()) > t.shape[1])):
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must hold the kept rows of {n} sessions, laid out like k_out")
-    stat_stride, stat_out_stride = None, None
-    for name, t, dtype, is_out in (("weights", weights, "torch.float32", False), ("positions", positions, "torch.int32", False),
-                                   ("weights_out", weights_out, "torch.float32", True), ("positions_out", positions_out, "torch.int32", True)):
         if t is None:
             continue
-        have = _statistic(name, t, dtype, n, num_kv_heads, context)
-        want = stat_out_stride if is_out else stat_stride
-        if (want is not None and have != want) or (n and int((kept if is_out else rows).max()) > t.shape[2]):
-            raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"{name} must hold the rows and be laid out like its weights")
-        if is_out:
-            stat_out_stride = have
-        else:
-            stat_stride = have
-    r = np.zeros(n, dtype=_evict_record)
-    for name, t in (("k", k), ("v", v), ("k_out", k_out), ("v_out", v_out), ("weights", weights), ("weights_out", weights_out),
-                    ("positions", positions), ("positions_out", positions_out)):
-        if t is not None:
-            r[name] = _batch_addresses(t)[:n]
-    r["rows"] = rows
-    r["end_position"] = rows if end_positions is None else _counts("end_positions", end_positions, n)
-    p = L.KVEvictParams(head_dim, num_kv_heads, budget, sink_tokens, recent_tokens, in_stride, out_stride, stat_stride,
-                        stat_out_stride or stat_stride, 0)
-    context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), r.ctypes.data, n, C.byref(p)))
+        stride = _cache_stride(name, t)
+        if t.shape[0] < n or t.shape[1] < kept or t.shape[2:] != k.shape[2:] or (name == "v_out" and k_out is not None and stride != out_stride):
+            _refuse(f"{name} must hold the kept rows of {n} sessions, and v_out be laid out like k_out")
+        out_stride = stride
+    stat = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context)
+    if positions is not None and _statistic("positions", positions, "torch.int32", n, num_kv_heads, context) != stat:
+        _refuse("positions must be laid out like weights")
+    if weights.shape[2] < most or (positions is not None and positions.shape[2] < most):
+        _refuse(f"weights and positions must hold {most} rows")
+    stat_out = None
+    for name, t, dtype in (("weights_out", weights_out, "torch.float32"), ("positions_out", positions_out, "torch.int32")):
+        if t is None:
+            continue
+        stride = _statistic(name, t, dtype, n, num_kv_heads, context)
+        if t.shape[2] < kept or stat_out not in (None, stride):
+            _refuse(f"{name} must hold {kept} rows, and positions_out be laid out like weights_out")
+        stat_out = stride
+    words = np.empty((n, 9), dtype=np.uint64)              # tt_kv_evict_session
+    words[:, :8] = _addresses(n, k, v, k_out, v_out, weights, weights_out, positions, positions_out)
+    ends = used if end_positions is None else _counts("end_positions", end_positions, n)
+    words[:, 8] = used + (ends.astype(np.uint64) << np.uint64(32))
+    p = L.KVEvictParams(head_dim, num_kv_heads, budget, sink_tokens, recent_tokens, in_stride, out_stride, stat, stat_out or stat, 0)
+    context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), words.__array_interface__["data"][0], n, C.byref(p)))
 
 
 @dataclass
