@@ -542,7 +542,7 @@ static uint32_t tt_decode_heads_per_cta(uint32_t n_kv_heads, bool quantised) {
 static int plan_splits(const uint32_t *keys_per_session, const uint32_t *q_rows_per_session,
                        uint32_t n_sessions, uint32_t head_dim, uint32_t n_q_heads,
                        uint32_t n_kv_heads, uint32_t sm_count, size_t workspace_bytes, uint32_t heads_per_cta,
-                       uint32_t *out_keys_per_item, uint32_t *out_n_items);
+                       uint32_t *out_keys_per_item, uint32_t *out_n_items, uint32_t max_waves = 3);
 
 TT_API int tt_attn_plan_splits(const uint32_t *keys_per_session, const uint32_t *q_rows_per_session,
                                uint32_t n_sessions, uint32_t head_dim, uint32_t n_q_heads,
@@ -556,7 +556,7 @@ TT_API int tt_attn_plan_splits(const uint32_t *keys_per_session, const uint32_t 
 static int plan_splits(const uint32_t *keys_per_session, const uint32_t *q_rows_per_session,
                        uint32_t n_sessions, uint32_t head_dim, uint32_t n_q_heads,
                        uint32_t n_kv_heads, uint32_t sm_count, size_t workspace_bytes, uint32_t heads_per_cta,
-                       uint32_t *out_keys_per_item, uint32_t *out_n_items) {
+                       uint32_t *out_keys_per_item, uint32_t *out_n_items, uint32_t max_waves) {
     if (keys_per_session == nullptr || n_sessions == 0 || n_kv_heads == 0 || n_q_heads % n_kv_heads != 0 ||
         head_dim == 0 || sm_count == 0)
         return TT_ERR_INVALID_ARG;
@@ -591,7 +591,7 @@ static int plan_splits(const uint32_t *keys_per_session, const uint32_t *q_rows_
         streams += (uint64_t)units_per_part * ceil_div_u32((uint64_t)qr * group, rows_per_item);
         if (keys_per_session[i] > max_keys) max_keys = keys_per_session[i];
     }
-    uint32_t waves = waves_env ? waves_env : (streams * 8 <= slots ? 1u : 3u);
+    uint32_t waves = waves_env ? waves_env : (streams * 8 <= slots ? 1u : max_waves);
     uint32_t keys = 64;
     if (streams >= waves * slots) {
         keys = 1u << 30;                    // more streams than slots: one item per stream, nothing to split
@@ -886,7 +886,9 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     }
     // Verify batches (17..128 packed rows per KV head, head_dim 256, plain 16-bit rows) take the
     // tensor-core pass 1: one item serves all packed rows of a (session, kv head, key range).
-    bool wide = !quantised && form == nullptr && p->head_dim == 256 && getenv("TT_VERIFY_FORCE_MMA_SYNC") == nullptr;
+    // (also for the sessions behind a shared prefix, while their tables travel in the parameters: this form uploads maps)
+    const bool wide_form = form == nullptr || (form->partials_only && form->form == kPassPlain && n_sessions <= kVerifyParamSessions);
+    bool wide = !quantised && wide_form && p->head_dim == 256 && getenv("TT_VERIFY_FORCE_MMA_SYNC") == nullptr;
     bool wide128 = false;       // some session has more than 64 packed rows: the 128-row form of the kernel
     for (uint32_t i = 0; wide && i < n_sessions; ++i) {
         const TTDecodeSession &s = in_sessions[i];
@@ -920,7 +922,11 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     }
     if (!wide) {
         int rc = plan_splits(keys, rows, n_sessions, p->head_dim, p->n_q_heads, p->n_kv_heads, (uint32_t)ctx->sm_count,
-                             partial_bytes, hpc, &keys_per_item, &n_items);
+                             partial_bytes, hpc, &keys_per_item, &n_items,
+                             // sessions of some hundred keys (what follows a shared prefix): three waves would be items of
+                             // 64 keys, whose start-up and partials cost more than the balance is worth (64 sessions of
+                             // 1..1024 keys behind 32768 shared ones: 63.5 us a call, 60.2 us with one wave)
+                             form != nullptr && form->short_sessions ? 1u : 3u);
         if (rc != TT_OK) return tt_set_error(ctx, rc, "split-KV partials do not fit the context workspace");
         if (!in_params && n_items > ctx->max_items)
             return tt_set_error(ctx, TT_ERR_OOM, "%u work items exceed the context's item table (%u)", n_items,
@@ -995,7 +1001,7 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
 
     TTLaunchTimer timer(ctx, stream, TT_PROFILE_DECODE_PARTIAL);
     // a verify batch whose sessions are all one part needs no merge: pass 1 stores the output rows
-    bool direct = wide && mode == 0;
+    bool direct = wide && mode == 0 && form == nullptr;
     for (uint32_t i = 0; direct && i < n_sessions; ++i) direct = ctx->h_sessions[i].n_parts == 1;
     if (wide) {
         const int rc = tt_launch_verify_tc(ctx, stream, n_sessions, n_items, part_o, part_m, part_l, p, direct, in_params, wide128);

@@ -50,10 +50,7 @@ struct PairShared {
     // within a CTA
     uint64_t published[2][4];
     uint64_t pair[4];
-    union {
-        const void *row_q[128];
-        float l_sum[2][128];
-    };
+    float l_sum[2][128];
     float m_ref[2][128];
     uint32_t tmem_base;
     uint32_t pad;
@@ -160,7 +157,12 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
         for (int w = 0; w < 4; ++w) mbar_init(&sh->pair[w], 2);
         mbar_fence_init();
     }
-    if (threadIdx.x < 128) sh->row_q[threadIdx.x] = form.query(item, my_row0 + threadIdx.x, HD, ROWS);
+    if (warp < 8)
+        // whole rows of Q by asynchronous copies into the P buffers, 16-byte chunk c of row r at c ^ (r & 7); in flight
+        // while the barriers and TMEM are set up
+        load_query_rows<HD, ROWS, 16>(form, item, my_row0, warp, 8, lane, [&](uint32_t r, uint32_t chunk) {
+            return p_s + r * (HD * 2) + ((chunk ^ (r & 7)) << 4);
+        });
     if (warp == 8) {
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(kTmemCols) : "memory");
@@ -168,7 +170,7 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
     }
     __syncwarp();
     tc_fence_before();
-    cluster_sync_all();            // the barriers of both CTAs exist, and within the CTA row_q and the TMEM base are visible
+    cluster_sync_all();            // the barriers of both CTAs exist, and within the CTA the TMEM base is visible
     tc_fence_after();
     const uint32_t tmem = sh->tmem_base;
     bool failed = false;
@@ -282,17 +284,6 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
         const uint32_t wg = warp >> 2, quarter = warp & 3;
         const uint32_t row = quarter * 32 + lane;                // row of this CTA == TMEM lane
         const uint32_t lane_addr = (quarter * 32) << 16;
-        // whole rows by asynchronous copies into the P buffers, 16-byte chunk c of row r at c ^ (r & 7)
-        for (uint32_t c = threadIdx.x; c < 128 * (HD / 8); c += 256) {
-            const uint32_t r = c / (HD / 8), chunk = c % (HD / 8);
-            unsigned char *dst = p_s + r * (HD * 2) + ((chunk ^ (r & 7)) << 4);
-            const T *src = reinterpret_cast<const T *>(sh->row_q[r]);
-            if (src != nullptr)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src + chunk * 8) : "memory");
-            else
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         asm volatile("bar.sync 1, 256;" ::: "memory");           // the eight softmax warps
 #pragma unroll

@@ -33,6 +33,7 @@ struct alignas(64) SinkForm {
         uint32_t queries;
         uint32_t sink_tiles;             // tiles over [0, sink) before the window's
         uint32_t base;                   // first key of the window's tiles
+        uint32_t base_row;               // ... and its cache row behind the sinks, in a ring
         bool windowed;                   // some query's window starts behind the sinks
     };
     __device__ __forceinline__ Item item(uint32_t block, int hd, int rows) const {
@@ -53,6 +54,7 @@ struct alignas(64) SinkForm {
             it.base = max(sink, from);
             if (ring) it.base = sink + (it.base - sink) / kBoxKeys * kBoxKeys;
         }
+        it.base_row = ring && it.windowed ? (it.base - sink) % ring : 0u;
         it.n_tiles = it.sink_tiles + (key_end - it.base + kBK - 1) / kBK;
         return it;
     }
@@ -66,9 +68,14 @@ struct alignas(64) SinkForm {
             row = (int)(tile * kBK + half * kBoxKeys);
             return is_k ? &k_sink : &v_sink;
         }
-        uint32_t key = it.base + (tile - it.sink_tiles) * kBK + half * kBoxKeys;
-        if (ring && key >= sink) key = sink + (key - sink) % ring;
-        row = (int)key;
+        uint32_t off = (tile - it.sink_tiles) * kBK + half * kBoxKeys;
+        if (ring && it.windowed) {
+            off += it.base_row;
+            while (off >= ring) off -= ring;
+            row = (int)(sink + off);
+        } else {
+            row = (int)(it.base + off);
+        }
         return is_k ? &k_map : &v_map;
     }
     __device__ __forceinline__ bool masked(const Item &it, uint32_t tile) const {

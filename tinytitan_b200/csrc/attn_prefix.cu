@@ -33,6 +33,12 @@ struct PrefixGroup {
     uint32_t partial_base;               // first partial row
     uint32_t item_begin;
     uint32_t row_tiles;
+    // sessions of q_rows query rows each whose queries lie q_step bytes apart (the slots of one tensor): a row's address is
+    // arithmetic. q_rows 0: anything else, found by a search over the sessions -- divergent reads of the parameter bank,
+    // 3000 clocks at the start of every CTA for 64 sessions.
+    uint32_t q_rows;
+    const void *q;
+    long long q_step;
 };
 struct alignas(64) PrefixMaps { unsigned char m[2][128]; };    // K and V tensor maps of a group
 
@@ -40,10 +46,12 @@ struct alignas(64) PrefixMaps { unsigned char m[2][128]; };    // K and V tensor
 // parameters; larger ones read the copies the host uploaded.
 struct alignas(64) PrefixTable {
     PrefixMaps maps[kParamGroups];
-    PrefixGroup g[kParamGroups];
-    PrefixSession s[kParamSessions];
+    // a CTA's first reads, next to each other: every line of the parameters it touches costs a miss
     uint32_t n_groups, n_sessions;
     uint32_t in_params;
+    uint32_t item_begin[kParamGroups];
+    PrefixGroup g[kParamGroups];
+    PrefixSession s[kParamSessions];
 };
 
 // The prefix pass's items for attn_rows_kernel.
@@ -60,17 +68,24 @@ struct PrefixForm {
         const CUtensorMap *maps;
         uint32_t key_begin, n_keys;
         uint32_t row0, n_rows;           // first packed row, packed rows in use
-        uint32_t row_begin, session_begin, session_count;
+        uint32_t row_begin, session_begin, session_count, q_rows;
+        const void *q;
+        long long q_step;
         size_t partial_base;             // of packed row 0's query row in this part
     };
     __device__ __forceinline__ Item item(uint32_t block, int hd, int rows) const {
-        const PrefixGroup *g = table.in_params ? table.g : groups;
         uint32_t lo = 0, hi = table.n_groups;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (g[mid].item_begin <= block) lo = mid; else hi = mid;
+        if (table.in_params) {
+#pragma unroll
+            for (uint32_t i = 1; i < kParamGroups; ++i)
+                if (i < hi && table.item_begin[i] <= block) lo = i;
+        } else {
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (groups[mid].item_begin <= block) lo = mid; else hi = mid;
+            }
         }
-        const PrefixGroup grp = g[lo];
+        const PrefixGroup grp = table.in_params ? table.g[lo] : groups[lo];
         const uint32_t local = block - grp.item_begin, group = n_q_heads / n_kv_heads;
         const uint32_t part = local / (grp.row_tiles * n_kv_heads);
         Item it;
@@ -82,14 +97,20 @@ struct PrefixForm {
         it.row0 = local % grp.row_tiles * rows;
         it.n_rows = min((uint32_t)rows, grp.n_rows * group - it.row0);
         it.row_begin = grp.row_begin; it.session_begin = grp.session_begin; it.session_count = grp.session_count;
+        it.q_rows = grp.q_rows; it.q = grp.q; it.q_step = grp.q_step;
         it.partial_base = (size_t)grp.partial_base + (size_t)part * grp.n_rows * n_q_heads;
         return it;
     }
-    // a search over the group's sessions
     __device__ __forceinline__ const void *query(const Item &it, uint32_t r, int hd, int rows) const {
         if (r >= it.n_rows) return nullptr;
+        const uint32_t group = n_q_heads / n_kv_heads, packed = it.row0 + r;
+        if (it.q_rows != 0) {
+            const uint32_t t = packed / group;
+            return reinterpret_cast<const unsigned char *>(it.q) + (long long)(t / it.q_rows) * it.q_step +
+                   ((size_t)(t % it.q_rows) * q_row_stride + (size_t)(it.kv_head * group + packed % group) * hd) * 2;
+        }
         const PrefixSession *s = table.in_params ? table.s : sessions;
-        const uint32_t group = n_q_heads / n_kv_heads, packed = it.row0 + r, qrow = it.row_begin + packed / group;
+        const uint32_t qrow = it.row_begin + packed / group;
         uint32_t lo = it.session_begin, hi = it.session_begin + it.session_count;
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) >> 1;
@@ -121,100 +142,133 @@ struct PrefixForm {
 };
 
 // ---------------------------------------------------------------------------------------
-// Merge: one CTA per output row (session, query row, head); 256 threads are groups of HD / 4 column threads that walk
-// the row's partials, the prefix's first, then the session's own, with an online (max, sum, output) triple each.
+// Merge: a warp takes 128 (at head_dim 64: 64) columns of an output row (session, query row, head) and walks the row's
+// partials, the prefix's first, then the session's own, 32 at a time: every lane forms the weight of one partial, and the
+// columns are summed with the weights handed round by shuffles, so that a partial costs a lane one load and four FMAs.
+// (With every thread forming every weight the kernel was bound by instructions: 12.7 us for 1024 rows of 21 partials.)
+// `groups` (a power of two) sets of warps share a row where there are few rows.
 // ---------------------------------------------------------------------------------------
 struct MergeSession {
     void *out;
-    uint32_t first_row, q_rows;          // query rows of the call before this session, and its own
+    uint32_t q_rows;                     // this session's query rows
     uint32_t prefix_base, prefix_parts;  // partial rows of this session's first query row in its group's prefix pass
     uint32_t prefix_stride;              // partial rows between two parts of the prefix
     uint32_t own_base, own_parts;        // the session's own split partials
-    uint32_t pad;
 };
 struct MergeTable {
-    MergeSession s[kParamSessions];
     uint32_t n;                          // 0: the device copy
+    uint32_t q_rows;                     // of every session; 0: they differ
+    uint32_t first_row[kParamSessions];  // query rows of the call before each session
+    MergeSession s[kParamSessions];
 };
+
+template <int VEC>
+struct Columns { float v[VEC]; };
+__device__ __forceinline__ Columns<4> load_columns(const float *p, Columns<4> *) {
+    const float4 x = *reinterpret_cast<const float4 *>(p);
+    return Columns<4>{{x.x, x.y, x.z, x.w}};
+}
+__device__ __forceinline__ Columns<2> load_columns(const float *p, Columns<2> *) {
+    const float2 x = *reinterpret_cast<const float2 *>(p);
+    return Columns<2>{{x.x, x.y}};
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
-attn_prefix_merge_kernel(const __grid_constant__ MergeTable table, const MergeSession *__restrict__ dev, uint32_t n_sessions,
+attn_prefix_merge_kernel(const __grid_constant__ MergeTable table, const MergeSession *__restrict__ dev,
+                         const uint32_t *__restrict__ dev_first_row, uint32_t n_sessions,
                          const float *__restrict__ pre_o, const float *__restrict__ pre_m, const float *__restrict__ pre_l,
                          const float *__restrict__ own_o, const float *__restrict__ own_m, const float *__restrict__ own_l,
-                         uint32_t n_q_heads, uint32_t out_row_stride) {
-    constexpr uint32_t kCols = HD / 4, kGroups = 256 / kCols;
-    __shared__ float grp_m[kGroups], grp_d[kGroups];
-    __shared__ float4 accs[256];
+                         uint32_t n_q_heads, uint32_t out_row_stride, uint32_t n_rows, uint32_t groups) {
+    constexpr int kVec = HD >= 128 ? 4 : 2;
+    constexpr uint32_t kRowWarps = HD / (32 * kVec), kSets = 8 / kRowWarps;
+    using Cols = Columns<kVec>;
+    __shared__ float set_m[8], set_d[8];
+    __shared__ Cols accs[256];
     pdl_launch_dependents();
     pdl_wait();
-    const MergeSession *sessions = table.n != 0 ? table.s : dev;
-    const uint32_t qrow = blockIdx.x / n_q_heads, head = blockIdx.x % n_q_heads;
-    uint32_t lo = 0, hi = n_sessions;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (sessions[mid].first_row <= qrow) lo = mid; else hi = mid;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t set = warp / kRowWarps, grp = set & (groups - 1);
+    const uint32_t out_row = blockIdx.x * (kSets / groups) + set / groups, col = (warp % kRowWarps * 32 + lane) * kVec;
+    const bool live = out_row < n_rows;
+    const uint32_t qrow = out_row / n_q_heads, head = out_row - qrow * n_q_heads;
+    uint32_t lo = 0;
+    const uint32_t *first_row = table.n != 0 ? table.first_row : dev_first_row;
+    if (table.q_rows != 0) {
+        lo = min(qrow / table.q_rows, n_sessions - 1);
+    } else {
+        uint32_t hi = n_sessions;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (first_row[mid] <= qrow) lo = mid; else hi = mid;
+        }
     }
-    const MergeSession ses = sessions[lo];
-    const uint32_t w = qrow - ses.first_row;
-    const uint32_t grp = threadIdx.x / kCols, ct = threadIdx.x % kCols;
-    const uint32_t n_parts = ses.prefix_parts + ses.own_parts;
-    const size_t pre = (size_t)ses.prefix_base + w * n_q_heads + head, own = (size_t)ses.own_base + w * n_q_heads + head;
-    const size_t own_stride = (size_t)ses.q_rows * n_q_heads;
+    const uint32_t w = table.q_rows != 0 ? qrow - lo * table.q_rows : qrow - first_row[lo];
+    const MergeSession ses = table.n != 0 ? table.s[lo] : dev[lo];
 
     float m_run = -INFINITY, d_run = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kBatch = 4;                             // independent loads in flight per thread
-    for (uint32_t c0 = grp; c0 < n_parts; c0 += kBatch * kGroups) {
-        float e[kBatch], l[kBatch]; float4 o[kBatch];
+    Cols acc;
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            const uint32_t c = c0 + x * kGroups;
-            e[x] = -INFINITY; l[x] = 0.f; o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (c < n_parts) {
-                const bool shared = c < ses.prefix_parts;
-                const size_t row = shared ? pre + (size_t)c * ses.prefix_stride : own + (c - ses.prefix_parts) * own_stride;
-                e[x] = (shared ? pre_m : own_m)[row];
-                l[x] = (shared ? pre_l : own_l)[row];
-                o[x] = *reinterpret_cast<const float4 *>((shared ? pre_o : own_o) + row * HD + ct * 4);
+    for (int x = 0; x < kVec; ++x) acc.v[x] = 0.f;
+    auto walk = [&](const float *po, const float *pm, const float *pl, size_t base, size_t stride, uint32_t n) {
+        for (uint32_t c0 = grp; c0 < n; c0 += 32 * groups) {
+            const uint32_t count = min(32u, (n - c0 + groups - 1) / groups);       // partials of this round
+            const size_t row0 = base + (size_t)c0 * stride, step = stride * groups;
+            float e = -INFINITY, l = 0.f;
+            if (lane < count) { e = pm[row0 + lane * step]; l = pl[row0 + lane * step]; }
+            float mx = e;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float m_new = fmaxf(m_run, mx);
+            if (m_new == -INFINITY) continue;                          // nothing visible so far: exp(-inf - -inf) would be NaN
+            const float sc = __expf(m_run - m_new), wgt = __expf(e - m_new);
+            float d = l * wgt;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+            d_run = d_run * sc + d;
+            m_run = m_new;
+#pragma unroll
+            for (int x = 0; x < kVec; ++x) acc.v[x] *= sc;
+            const float *p = po + row0 * HD + col;
+#pragma unroll 8
+            for (uint32_t i = 0; i < count; ++i, p += step * HD) {
+                const float wi = __shfl_sync(0xffffffffu, wgt, i);
+                const Cols o = load_columns(p, (Cols *)nullptr);
+#pragma unroll
+                for (int x = 0; x < kVec; ++x) acc.v[x] = fmaf(o.v[x], wi, acc.v[x]);
             }
         }
-        const float m_new = fmaxf(m_run, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
-        if (m_new != -INFINITY) {
-            const float sc = __expf(m_run - m_new);
-            acc.x *= sc; acc.y *= sc; acc.z *= sc; acc.w *= sc; d_run *= sc;
+    };
+    if (live) {
+        walk(pre_o, pre_m, pre_l, (size_t)ses.prefix_base + w * n_q_heads + head, ses.prefix_stride, ses.prefix_parts);
+        walk(own_o, own_m, own_l, (size_t)ses.own_base + w * n_q_heads + head, (size_t)ses.q_rows * n_q_heads, ses.own_parts);
+    }
+    if (groups > 1) {
+        accs[threadIdx.x] = acc;
+        if (lane == 0) { set_m[warp] = m_run; set_d[warp] = d_run; }
+        __syncthreads();
+        if (grp != 0) return;
+        float mg = m_run;
+        for (uint32_t g = 1; g < groups; ++g) mg = fmaxf(mg, set_m[warp + g * kRowWarps]);
+        if (mg != -INFINITY) {
+            const float sc = __expf(m_run - mg);
+            d_run *= sc;
 #pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-                const float wgt = __expf(e[x] - m_new);
-                acc.x += o[x].x * wgt; acc.y += o[x].y * wgt; acc.z += o[x].z * wgt; acc.w += o[x].w * wgt;
-                d_run += l[x] * wgt;
+            for (int x = 0; x < kVec; ++x) acc.v[x] *= sc;
+            for (uint32_t g = 1; g < groups; ++g) {
+                const float wgt = __expf(set_m[warp + g * kRowWarps] - mg);
+                const Cols o = accs[threadIdx.x + g * kRowWarps * 32];
+#pragma unroll
+                for (int x = 0; x < kVec; ++x) acc.v[x] = fmaf(o.v[x], wgt, acc.v[x]);
+                d_run += set_d[warp + g * kRowWarps] * wgt;
             }
-            m_run = m_new;
         }
     }
-    accs[threadIdx.x] = acc;
-    if (ct == 0) { grp_m[grp] = m_run; grp_d[grp] = d_run; }
-    __syncthreads();
-    if (grp != 0) return;
-    float mg = grp_m[0];
+    if (!live) return;
+    const float inv = d_run > 0.f ? 1.f / d_run : 0.f;    // a row that sees nothing: zeros
+    T *dst = reinterpret_cast<T *>(ses.out) + (size_t)w * out_row_stride + (size_t)head * HD + col;
 #pragma unroll
-    for (uint32_t g = 1; g < kGroups; ++g) mg = fmaxf(mg, grp_m[g]);
-    float D = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mg != -INFINITY)
-#pragma unroll
-        for (uint32_t g = 0; g < kGroups; ++g) {
-            const float wgt = __expf(grp_m[g] - mg);
-            const float4 o = accs[g * kCols + ct];
-            acc.x += o.x * wgt; acc.y += o.y * wgt; acc.z += o.z * wgt; acc.w += o.w * wgt;
-            D += grp_d[g] * wgt;
-        }
-    const float inv = D > 0.f ? 1.f / D : 0.f;            // a row that sees nothing: zeros
-    T *dst = reinterpret_cast<T *>(ses.out) + (size_t)w * out_row_stride + (size_t)head * HD + ct * 4;
-    uint2 packed;
-    packed.x = pack2<T>(acc.x * inv, acc.y * inv);
-    packed.y = pack2<T>(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2 *>(dst) = packed;
+    for (int x = 0; x < kVec; x += 2) *reinterpret_cast<uint32_t *>(dst + x) = pack2<T>(acc.v[x] * inv, acc.v[x + 1] * inv);
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
@@ -238,9 +292,15 @@ cudaError_t launch_prefix(cudaStream_t stream, uint32_t head_dim, uint32_t rows,
 
 template <typename T>
 cudaError_t launch_merge(cudaStream_t stream, uint32_t head_dim, uint32_t rows, const MergeTable &table, const MergeSession *dev,
-                         uint32_t n_sessions, const PrefixForm &kp, const TTDecodeForm &own, uint32_t n_q_heads, uint32_t out_row_stride) {
-#define TT_X(HD) tt_launch_pdl(attn_prefix_merge_kernel<T, HD>, dim3(rows), dim3(256), 0, stream, table, dev, n_sessions, kp.part_o, \
-                               kp.part_m, kp.part_l, own.part_o, own.part_m, own.part_l, n_q_heads, out_row_stride)
+                         const uint32_t *dev_first_row, uint32_t n_sessions, const PrefixForm &kp, const TTDecodeForm &own,
+                         uint32_t n_q_heads, uint32_t out_row_stride, uint32_t sm_count) {
+    // sets of warps per row: as many as keep two CTAs an SM busy
+    const uint32_t sets = head_dim == 256 ? 4 : 8;
+    uint32_t groups = 1;
+    while (groups < sets && (uint64_t)rows * groups * 2 <= (uint64_t)sets * 2 * sm_count) groups *= 2;
+    const uint32_t grid = (rows * groups + sets - 1) / sets;
+#define TT_X(HD) tt_launch_pdl(attn_prefix_merge_kernel<T, HD>, dim3(grid), dim3(256), 0, stream, table, dev, dev_first_row, n_sessions, \
+                               kp.part_o, kp.part_m, kp.part_l, own.part_o, own.part_m, own.part_l, n_q_heads, out_row_stride, rows, groups)
     return head_dim == 64 ? TT_X(64) : head_dim == 128 ? TT_X(128) : TT_X(256);
 #undef TT_X
 }
@@ -326,12 +386,15 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
     static thread_local MergeTable merge;
     const size_t off_groups = sizeof(PrefixMaps) * (size_t)n_groups, off_sessions = off_groups + sizeof(PrefixGroup) * (size_t)n_groups;
     const size_t off_merge = (off_sessions + sizeof(PrefixSession) * (size_t)n_sessions + 15) / 16 * 16;
-    const size_t table_bytes = off_merge + sizeof(MergeSession) * (size_t)n_sessions;
+    const size_t off_first = off_merge + sizeof(MergeSession) * (size_t)n_sessions;
+    const size_t table_bytes = off_first + sizeof(uint32_t) * (size_t)n_sessions;
     unsigned char *host = ctx->h_prefix_tables;
     PrefixMaps *h_maps = in_params ? table.maps : reinterpret_cast<PrefixMaps *>(host);
     PrefixGroup *h_groups = in_params ? table.g : reinterpret_cast<PrefixGroup *>(host + off_groups);
     PrefixSession *h_sessions = in_params ? table.s : reinterpret_cast<PrefixSession *>(host + off_sessions);
     MergeSession *h_merge = in_params ? merge.s : reinterpret_cast<MergeSession *>(host + off_merge);
+    uint32_t *h_first = in_params ? merge.first_row : reinterpret_cast<uint32_t *>(host + off_first);
+    merge.q_rows = sessions[0].q_rows;
     if (!in_params && table_bytes > ctx->prefix_table_bytes) return tt_set_error(ctx, TT_ERR_OOM, "the prefix tables do not fit the context");
 
     // ---- sessions, query rows per group ----
@@ -347,7 +410,8 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
         if (((uintptr_t)s.q | (uintptr_t)s.out) & 15)
             return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "session %u: buffers must be 16-byte aligned", i);
         h_sessions[i].q = s.q; h_sessions[i].first_row = total_rows; h_sessions[i].q_rows = s.q_rows;
-        h_merge[i].out = s.out; h_merge[i].first_row = total_rows; h_merge[i].q_rows = s.q_rows; h_merge[i].pad = 0;
+        h_merge[i].out = s.out; h_merge[i].q_rows = s.q_rows; h_first[i] = total_rows;
+        if (s.q_rows != merge.q_rows) merge.q_rows = 0;
         TTDecodeSession &d = tmp[i];
         d.q = s.q; d.out = s.out; d.k = s.k; d.v = s.v; d.seq_len = s.seq_len; d.q_rows = s.q_rows; d.kv_start = 0;
         d.n_parts = 0; d.partial_base = 0; d.ring_capacity = 0; d.keep = nullptr; d.row_index = nullptr;
@@ -379,10 +443,16 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
         d.session_begin = session; d.session_count = groups[g].n_sessions;
         d.row_begin = row; d.n_rows = rows[g];
         d.partial_base = partial; d.item_begin = item;
+        if (in_params) table.item_begin[g] = item;
         d.row_tiles = ceil_div((uint64_t)rows[g] * group, tile_rows);
+        d.q = sessions[session].q; d.q_rows = sessions[session].q_rows; d.q_step = 0;
+        if (groups[g].n_sessions > 1) d.q_step = (long long)((uintptr_t)sessions[session + 1].q - (uintptr_t)sessions[session].q);
+        for (uint32_t i = 1; i < groups[g].n_sessions; ++i)
+            if (sessions[session + i].q_rows != d.q_rows ||
+                (long long)((uintptr_t)sessions[session + i].q - (uintptr_t)sessions[session + i - 1].q) != d.q_step) d.q_rows = 0;
         for (uint32_t i = 0; i < groups[g].n_sessions; ++i) {
             MergeSession &m = h_merge[session + i];
-            m.prefix_base = partial + (m.first_row - row) * q.n_q_heads;
+            m.prefix_base = partial + (h_first[session + i] - row) * q.n_q_heads;
             m.prefix_parts = d.n_parts;
             m.prefix_stride = rows[g] * q.n_q_heads;
         }
@@ -404,6 +474,7 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
     TTDecodeForm own;
     own.reserved_bytes = partial_bytes + 256;
     own.partials_only = true;
+    own.short_sessions = true;
     int rc = tt_launch_decode(ctx, (cudaStream_t)stream, tmp, n_sessions, params, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &own);
     if (rc != TT_OK) return rc;
     for (uint32_t i = 0; i < n_sessions; ++i) {
@@ -434,9 +505,10 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
     }
     // ---- merge ----
     const MergeSession *dev = reinterpret_cast<const MergeSession *>(ctx->prefix_tables + off_merge);
+    const uint32_t *dev_first = reinterpret_cast<const uint32_t *>(ctx->prefix_tables + off_first);
     e = q.io_dtype == TT_F16
-            ? launch_merge<__half>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, merge, dev, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements)
-            : launch_merge<__nv_bfloat16>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, merge, dev, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements);
+            ? launch_merge<__half>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, merge, dev, dev_first, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements, (uint32_t)ctx->sm_count)
+            : launch_merge<__nv_bfloat16>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, merge, dev, dev_first, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements, (uint32_t)ctx->sm_count);
     if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_prefix_merge launch");
     ctx->launches++;
     return TT_OK;

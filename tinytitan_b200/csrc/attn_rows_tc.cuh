@@ -85,10 +85,7 @@ struct RowsShared {
     uint64_t o_ready[2];        // [tile parity]: P.V of the tile has retired
     uint64_t published[2][4];   // [tile parity][lane quarter]: m of the tile is in m_ref
     uint64_t pair[4];           // the two warps of a lane quarter, at the end
-    union {
-        const void *row_q[128]; // where each row's query starts (null: no such row), until Q is in shared memory
-        float l_sum[2][128];    // the groups' row sums, at the end
-    };
+    float l_sum[2][128];        // the groups' row sums, at the end
     float m_ref[2][128];
     uint32_t tmem_base;
     uint32_t pad;
@@ -137,6 +134,28 @@ __device__ __forceinline__ float add_pair<__nv_bfloat16>(float sum, uint32_t pac
     return sum;
 }
 
+// Issues the asynchronous copies of query rows row0 + first, row0 + first + step, ... (N of them) of a CTA by one warp, 16
+// bytes a lane; `at(r, chunk)` is where chunk `chunk` of the CTA's row r goes. Rows that do not exist become zeros.
+template <int HD, int ROWS, int N, class Form, class At>
+__device__ __forceinline__ void load_query_rows(const Form &form, const typename Form::Item &item, uint32_t row0, uint32_t first,
+                                                uint32_t step, uint32_t lane, At at) {
+    static_assert(N <= 32, "one lane looks a row up");
+    constexpr uint32_t kLanes = HD / 8, kAtOnce = 32 / kLanes;       // lanes a row takes, rows per round
+    // the rows' addresses, one per lane: a lookup may be a search
+    const unsigned long long mine = lane < (uint32_t)N ? (unsigned long long)form.query(item, row0 + first + lane * step, HD, ROWS) : 0ull;
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)N; i += kAtOnce) {
+        const uint32_t nth = i + lane / kLanes, r = first + nth * step, chunk = lane % kLanes;
+        const unsigned char *src = (const unsigned char *)__shfl_sync(0xffffffffu, mine, nth);
+        unsigned char *dst = at(r, chunk);
+        if (src != nullptr)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src + chunk * 16) : "memory");
+        else
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
 // A Form says what the items are. It provides
 //   struct Item : RowsItem
 //   Item item(block, HD, ROWS)                 from the block index
@@ -153,7 +172,7 @@ template <typename T, int HD, int ROWS, class Form>
 __global__ void __launch_bounds__(RowsGeom<HD, ROWS>::kThreads, 1)
 attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_constant__ Form form) {
     using G = RowsGeom<HD, ROWS>;
-    constexpr int kSlots = G::kSlots, kThreads = G::kThreads, kQSub = G::kQSub, kChunks = G::kChunks;
+    constexpr int kSlots = G::kSlots, kQSub = G::kQSub, kChunks = G::kChunks;
     // nearly every byte is spoken for, so there is no slack to align the tiles by hand: the dynamic window of a kernel
     // without static shared memory starts 1024-byte aligned, and a launch where it does not is refused rather than run
     // with broken swizzles
@@ -224,7 +243,12 @@ attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
         mbar_init(&sh->q_ready, 2 * G::kGroupWarps);
         mbar_fence_init();
     }
-    for (uint32_t r = threadIdx.x; r < (uint32_t)ROWS; r += kThreads) sh->row_q[r] = form.query(item, r, HD, ROWS);
+    if (warp != G::kProducerWarp && warp != G::kMmaWarp && warp != G::kVProducerWarp)
+        // Q: K-major, 128-byte swizzle, 64-wide sub-tiles; in flight while the barriers and TMEM are set up
+        load_query_rows<HD, ROWS, ROWS / (2 * G::kGroupWarps)>(form, item, 0, (warp >> 2) * G::kGroupWarps + (warp & 3), 2 * G::kGroupWarps, lane,
+                                                               [&](uint32_t r, uint32_t chunk) {
+            return q_s + (chunk >> 3) * kQSub + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+        });
     if (warp == G::kProducerWarp) {
         __syncwarp();
         tmem_alloc(&sh->tmem_base, kTmemCols);
@@ -300,18 +324,6 @@ attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
         const uint32_t row = quarter * 32 + lane;                // row of the item == TMEM lane
         const uint32_t lane_addr = (quarter * 32) << 16;
         const uint32_t s_addr = tmem + lane_addr + kColS + wg * kBK;
-        // ---- Q: K-major, 128-byte swizzle, 64-wide sub-tiles; whole rows per warp ----
-        constexpr uint32_t kSoftmaxThreads = 64 * G::kGroupWarps;
-        for (uint32_t c = (wg * G::kGroupWarps + quarter) * 32 + lane; c < ROWS * (HD / 8); c += kSoftmaxThreads) {
-            const uint32_t r = c / (HD / 8), chunk = c % (HD / 8);          // 16-byte chunk of the row
-            unsigned char *dst = q_s + (chunk >> 3) * kQSub + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
-            const T *src = reinterpret_cast<const T *>(sh->row_q[r]);
-            if (src != nullptr)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src + chunk * 8) : "memory");
-            else
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
