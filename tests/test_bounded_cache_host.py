@@ -52,9 +52,15 @@ def _prefix_plan(lens, rows, hd=256, hq=16, hkv=2, sms=148, ws=128 << 20):
 
 
 def test_prefix_plan():
-    # one long prefix, 64 sessions x 8 heads = 512 packed rows: 4 row tiles x 2 KV heads = 8 streams cut into one wave
+    # one long prefix, 64 sessions x 8 heads = 512 packed rows: two items of 256 rows (a pair of SMs each) x 2 KV heads = 4
+    # streams, cut so that one wave fills the 74 pairs
     rc, per, items = _prefix_plan([32768], [64])
-    assert rc == 0 and per % 128 == 0 and items == 8 * -(-32768 // per) and 100 <= items <= 148
+    assert rc == 0 and per % 128 == 0 and items == 4 * -(-32768 // per) and 50 <= items <= 74
+    # 128 packed rows fit one SM: 2 streams over 148 of them; at head_dim 128 512 rows are four items of 128
+    rc, per, items = _prefix_plan([32768], [16])
+    assert rc == 0 and items == 2 * -(-32768 // per) and 100 <= items <= 148
+    rc, per, items = _prefix_plan([32768], [64], hd=128)
+    assert rc == 0 and items == 8 * -(-32768 // per) and 100 <= items <= 148
     # a short prefix of a few sessions: one tile per item
     rc, per, items = _prefix_plan([2000], [4], hq=8)
     assert rc == 0 and per == 128 and items == 2 * 16

@@ -8,14 +8,16 @@
 // move, one when a full cache takes in one token; sources lie at or above `budget` and destinations below it, so the
 // moves are free of order and the same in place and into other buffers.
 //
-// kv_evict_select_kernel: one thread-block cluster per (session, KV head). The selection key of a row is 32 bits whose
+// kv_evict_select_kernel: one CTA or thread-block cluster per (session, KV head). The selection key of a row is 32 bits whose
 //   unsigned order is the order above; a CTA keeps its slice of keys in shared memory, so the statistic and the
-//   positions are read once. The budget-th largest key is found by three histogram rounds (11 + 11 + 10 bits, counts
-//   of the cluster's CTAs added through distributed shared memory), then one pass gives ties their rank in row order
-//   and one numbers holes and fills. A thread owns consecutive rows, an odd number of them, so that ranks need one
-//   block scan and the strided shared-memory reads meet no bank twice. Bound: latency of about a dozen block or
-//   cluster barriers for the usual few thousand rows.
-// kv_evict_move_kernel: a warp per 32 destination rows copies what changes, 16 bytes a lane; bound by HBM.
+//   positions are read once, 16 bytes a thread where they are aligned. The budget-th largest key is found by three
+//   histogram rounds (11 + 11 + 10 bits, counts of the cluster's CTAs added through distributed shared memory; a warp
+//   whose keys all fall into one bin -- protected rows, rows that nothing has looked at -- adds once), then one pass gives
+//   ties their rank in row order and one numbers holes and fills. A thread owns consecutive rows, an odd number of them,
+//   so that ranks need one block scan and the strided shared-memory reads meet no bank twice. Bound: the latency of about
+//   a dozen block or cluster barriers.
+// kv_evict_move_kernel: a warp per 32 destination rows copies what changes, 16 bytes a lane; bound by HBM. A session that
+//   gives up a handful of rows in place (one per step at the budget) is compacted by the selecting CTA itself: one launch.
 #include "tt_sm100.h"
 
 #include <cooperative_groups.h>
@@ -27,7 +29,8 @@ namespace {
 constexpr uint32_t kSelThreads = 512;
 constexpr uint32_t kSelWarps = kSelThreads / 32;
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kMaxCluster = 16;               // above 8: the non-portable size, allowed for this kernel
+constexpr uint32_t kFusedMoves = 64;               // rows a selecting CTA moves itself
 constexpr uint32_t kSelSliceKeys = 50000;          // keys a CTA holds: 200,000 bytes beside the histogram and the counters
 constexpr uint32_t kHoleFlag = 0x80000000u;
 
@@ -93,35 +96,65 @@ struct __align__(16) SelShared {
     uint32_t warp_sums[kSelWarps];
     uint32_t counts[4];          // this CTA's ties, holes, fills (read by the cluster)
     uint32_t pick[2];            // the bin that holds the budget-th key, keys above it
+    uint32_t hole_rows[kFusedMoves], fill_rows[kFusedMoves];
 };
 
+// One row of one head, 16 bytes a lane.
+__device__ __forceinline__ void copy_row(unsigned char *dst, const unsigned char *src, uint32_t bytes, uint32_t lane) {
+    if (lane * 16 < bytes) *reinterpret_cast<uint4 *>(dst + lane * 16) = *reinterpret_cast<const uint4 *>(src + lane * 16);
+}
+
+// CLUSTER: several CTAs per (session, head). FUSED (one CTA, in place, at most kFusedMoves rows given up): the moves too.
+template <bool CLUSTER, bool FUSED>
 __global__ void __launch_bounds__(kSelThreads)
 kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, uint32_t *__restrict__ maps) {
-    extern __shared__ uint32_t keys[];
+    extern __shared__ __align__(16) uint32_t keys[];
     __shared__ SelShared sh;
     const cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t size = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t size = CLUSTER ? cluster.num_blocks() : 1u, rank = CLUSTER ? cluster.block_rank() : 0u;
+    auto sync_all = [&]() { if constexpr (CLUSTER) cluster.sync(); else __syncthreads(); };
     const uint32_t pair = blockIdx.x / size;
-    const EvictSession &ses = table.s[pair / p.n_kv_heads];
+    const EvictSession ses = table.s[pair / p.n_kv_heads];
     const uint32_t head = pair % p.n_kv_heads;
     pdl_launch_dependents();
     pdl_wait();
-    if (ses.rows <= p.budget) return;                      // nothing is given up (the whole cluster leaves)
-
     const float *weights = ses.weights + (size_t)head * p.weight_stride;
     const uint32_t *positions = ses.positions ? ses.positions + (size_t)head * p.weight_stride : nullptr;
+    if (ses.rows <= p.budget) {                            // nothing is given up (the whole cluster leaves)
+        if constexpr (FUSED) {
+            for (uint32_t j = threadIdx.x; j < ses.rows; j += kSelThreads) {
+                const size_t to = (size_t)head * p.weight_out_stride + j;
+                if (ses.weights_out != ses.weights) ses.weights_out[to] = weights[j];
+                if (ses.positions_out != nullptr && ses.positions_out != ses.positions) ses.positions_out[to] = positions ? positions[j] : j;
+            }
+        }
+        return;
+    }
+
     uint32_t *map = maps + ses.map_begin + (size_t)head * ses.map_pitch;
     uint32_t *fills = map + p.budget;
-    const uint32_t slice = (ses.rows + size - 1) / size;
+    const uint32_t slice = ((ses.rows + size - 1) / size + 3) / 4 * 4;
     const uint32_t begin = min(ses.rows, rank * slice), n = min(ses.rows, begin + slice) - begin;
     const bool held = slice <= p.held_keys;                // else every round reads the statistic again
-    auto key_at = [&](uint32_t i) {
-        const uint32_t row = begin + i;
-        const uint32_t pos = positions ? positions[row] : row;
-        return evict_key(weights[row], pos < p.sink || (uint64_t)pos + p.recent >= ses.end_position);
+    auto key_from = [&](float w, uint32_t pos) {
+        return evict_key(w, pos < p.sink || (uint64_t)pos + p.recent >= ses.end_position);
     };
+    auto key_at = [&](uint32_t i) { return key_from(weights[begin + i], positions ? positions[begin + i] : begin + i); };
     if (held) {
-        for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) keys[i] = key_at(i);
+        uint32_t i = threadIdx.x;
+        if ((((uintptr_t)weights | (uintptr_t)positions) & 15) == 0) {
+            const uint32_t quads = n / 4;
+#pragma unroll 4
+            for (uint32_t c = threadIdx.x; c < quads; c += kSelThreads) {
+                const float4 w = *reinterpret_cast<const float4 *>(weights + begin + 4 * c);
+                uint4 q = make_uint4(begin + 4 * c, begin + 4 * c + 1, begin + 4 * c + 2, begin + 4 * c + 3);
+                if (positions) q = *reinterpret_cast<const uint4 *>(positions + begin + 4 * c);
+                *reinterpret_cast<uint4 *>(keys + 4 * c) = make_uint4(key_from(w.x, q.x), key_from(w.y, q.y), key_from(w.z, q.z), key_from(w.w, q.w));
+            }
+            i = quads * 4 + threadIdx.x;
+        }
+#pragma unroll 4
+        for (; i < n; i += kSelThreads) keys[i] = key_at(i);
     }
     auto key_of = [&](uint32_t i) { return held ? keys[i] : key_at(i); };
 
@@ -132,16 +165,31 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
         const uint32_t bits = round < 2 ? 11u : 10u, shift = round == 0 ? 21u : round == 1 ? 10u : 0u;
         for (uint32_t b = threadIdx.x; b < kBins; b += kSelThreads) sh.hist[b] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) {
-            const uint32_t key = key_of(i);
-            if (round == 0 || key >> (shift + bits) == prefix) atomicAdd(&sh.hist[(key >> shift) & ((1u << bits) - 1)], 1u);
+        for (uint32_t i0 = 0; i0 < n; i0 += kSelThreads) {
+            const uint32_t i = i0 + threadIdx.x;
+            uint32_t bin = 0xffffffffu;
+            if (i < n) {
+                const uint32_t key = key_of(i);
+                if (round == 0 || key >> (shift + bits) == prefix) bin = (key >> shift) & ((1u << bits) - 1);
+            }
+            const uint32_t counted = __ballot_sync(0xffffffffu, bin != 0xffffffffu);
+            if (counted == 0) continue;
+            const int first = __ffs(counted) - 1;
+            const uint32_t same = __shfl_sync(0xffffffffu, bin, first);
+            if (__ballot_sync(0xffffffffu, bin == same) == counted) {
+                if ((threadIdx.x & 31) == (uint32_t)first) atomicAdd(&sh.hist[same], (uint32_t)__popc(counted));
+            } else if (bin != 0xffffffffu) {
+                atomicAdd(&sh.hist[bin], 1u);
+            }
         }
-        cluster.sync();
+        sync_all();
         // thread t adds up bins 4t .. 4t+3 counted from the top, over the CTAs of the cluster
         uint32_t c[4] = {0u, 0u, 0u, 0u};
         const uint32_t top = kBins - 4 * (threadIdx.x + 1);
+#pragma unroll 4
         for (uint32_t r = 0; r < size; ++r) {
-            const uint4 h = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(sh.hist, r) + top);
+            const uint32_t *hist = CLUSTER ? cluster.map_shared_rank(sh.hist, r) : sh.hist;
+            const uint4 h = *reinterpret_cast<const uint4 *>(hist + top);
             c[0] += h.w; c[1] += h.z; c[2] += h.y; c[3] += h.x;
         }
         uint32_t total;
@@ -153,7 +201,7 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
             sh.pick[0] = top + 3 - j;
             sh.pick[1] = seen;
         }
-        cluster.sync();                                    // the picked bin is known here, and no CTA still reads these counts
+        sync_all();                                        // the picked bin is known here, and no CTA still reads these counts
         prefix = (prefix << bits) | sh.pick[0];
         want -= sh.pick[1];
         __syncthreads();
@@ -167,9 +215,12 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
     for (uint32_t i = i0; i < i1; ++i) ties += key_of(i) == threshold;
     uint32_t total;
     uint32_t tie_rank = block_scan(ties, sh.warp_sums, &total);
-    if (threadIdx.x == 0) sh.counts[0] = total;
-    cluster.sync();
-    for (uint32_t r = 0; r < rank; ++r) tie_rank += *cluster.map_shared_rank(&sh.counts[0], r);
+    if constexpr (CLUSTER) {
+        if (threadIdx.x == 0) sh.counts[0] = total;
+        cluster.sync();
+#pragma unroll 4
+        for (uint32_t r = 0; r < rank; ++r) tie_rank += *cluster.map_shared_rank(&sh.counts[0], r);
+    }
 
     uint32_t holes = 0, kept_above = 0, t = tie_rank;
     for (uint32_t i = i0; i < i1; ++i) {
@@ -181,22 +232,56 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
     uint32_t total_holes, total_fills;
     uint32_t hole = block_scan(holes, sh.warp_sums, &total_holes);
     uint32_t fill = block_scan(kept_above, sh.warp_sums, &total_fills);
-    if (threadIdx.x == 0) { sh.counts[1] = total_holes; sh.counts[2] = total_fills; }
-    cluster.sync();
-    for (uint32_t r = 0; r < rank; ++r) {
-        const uint32_t *other = cluster.map_shared_rank(sh.counts, r);
-        hole += other[1];
-        fill += other[2];
+    if constexpr (CLUSTER) {
+        if (threadIdx.x == 0) { sh.counts[1] = total_holes; sh.counts[2] = total_fills; }
+        cluster.sync();
+#pragma unroll 4
+        for (uint32_t r = 0; r < rank; ++r) {
+            const uint32_t *other = cluster.map_shared_rank(sh.counts, r);
+            hole += other[1];
+            fill += other[2];
+        }
     }
     t = tie_rank;
     for (uint32_t i = i0; i < i1; ++i) {
         const uint32_t key = key_of(i), row = begin + i;
         const bool keep = key > threshold || (key == threshold && t < ties_kept);
         t += key == threshold;
-        if (row < p.budget) map[row] = keep ? row : kHoleFlag | hole++;
-        else if (keep) fills[fill++] = row;
+        if constexpr (FUSED) {
+            if (row < p.budget) {
+                if (!keep) sh.hole_rows[hole++] = row;
+            } else if (keep) {
+                sh.fill_rows[fill++] = row;
+            }
+        } else {
+            if (row < p.budget) map[row] = keep ? row : kHoleFlag | hole++;
+            else if (keep) fills[fill++] = row;
+        }
     }
-    cluster.sync();                                        // a CTA's counters outlive their readers
+    if constexpr (CLUSTER) cluster.sync();                 // a CTA's counters outlive their readers
+    if constexpr (FUSED) {
+        __syncthreads();
+        const size_t out0 = (size_t)head * p.weight_out_stride;
+        // statistics of other buffers: the rows that stay (holes get theirs below, in order behind a barrier)
+        if (ses.weights_out != ses.weights || (ses.positions_out != nullptr && ses.positions_out != ses.positions)) {
+            for (uint32_t j = threadIdx.x; j < p.budget; j += kSelThreads) {
+                if (ses.weights_out != ses.weights) ses.weights_out[out0 + j] = weights[j];
+                if (ses.positions_out != nullptr && ses.positions_out != ses.positions) ses.positions_out[out0 + j] = positions ? positions[j] : j;
+            }
+            __syncthreads();
+        }
+        const uint32_t lane = threadIdx.x & 31;
+        for (uint32_t m = threadIdx.x >> 5; m < total_holes; m += kSelWarps) {
+            const uint32_t to = sh.hole_rows[m], from = sh.fill_rows[m];
+            const size_t dst = (size_t)to * p.out_stride + (size_t)head * p.row_bytes, src = (size_t)from * p.in_stride + (size_t)head * p.row_bytes;
+            copy_row(ses.k_out + dst, ses.k + src, p.row_bytes, lane);
+            copy_row(ses.v_out + dst, ses.v + src, p.row_bytes, lane);
+            if (lane == 0) {
+                ses.weights_out[out0 + to] = weights[from];
+                if (ses.positions_out != nullptr) ses.positions_out[out0 + to] = positions ? positions[from] : from;
+            }
+        }
+    }
 }
 
 // grid = (blocks of 256 destination rows, sessions x KV heads), a warp per 32 of them.
@@ -255,7 +340,7 @@ kv_evict_move_kernel(const __grid_constant__ EvictTable table, EvictParams p, co
 // shared memory.
 uint32_t cluster_size(uint32_t max_rows, uint32_t pairs, uint32_t sm_count) {
     uint32_t c = 1;
-    while (c < kMaxCluster && ((max_rows > c * 4096u && pairs * c * 2 <= sm_count) || (uint64_t)c * kSelSliceKeys < max_rows)) c *= 2;
+    while (c < kMaxCluster && ((max_rows > c * 4096u && (uint64_t)pairs * c * 2 <= sm_count) || (uint64_t)c * kSelSliceKeys < max_rows)) c *= 2;
     return c;
 }
 
@@ -264,29 +349,43 @@ bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
     return x < y + b_bytes && y < x + a_bytes;
 }
 
+template <bool CLUSTER, bool FUSED>
+cudaError_t launch_select(cudaStream_t stream, const EvictTable &table, const EvictParams &p, uint32_t ctas, uint32_t cluster, uint32_t *maps) {
+    auto kernel = kv_evict_select_kernel<CLUSTER, FUSED>;
+    cudaError_t e = tt_set_smem_once(kernel, (int)(kSelSliceKeys * sizeof(uint32_t)));
+    if (e != cudaSuccess) return e;
+    if (CLUSTER && cluster > 8) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = sizeof(uint32_t) * p.held_keys; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = tt_pdl_enabled() ? attr : attr + 1;
+    cfg.numAttrs = (tt_pdl_enabled() ? 1 : 0) + (CLUSTER ? 1 : 0);
+    return cudaLaunchKernelEx(&cfg, kernel, table, p, maps);
+}
+
+// `given_up`: most rows a session gives up; `in_place`: K and V of every session
 cudaError_t launch_evict(tt_context *ctx, cudaStream_t stream, const EvictTable &table, EvictParams p, uint32_t max_rows,
-                         bool select, uint32_t *maps) {
+                         uint32_t given_up, bool in_place, uint32_t *maps) {
     const uint32_t pairs = table.n * p.n_kv_heads;
     cudaError_t e = cudaSuccess;
-    if (select) {
+    if (given_up != 0) {
         const uint32_t c = cluster_size(max_rows, pairs, (uint32_t)ctx->sm_count);
-        const uint32_t slice = (max_rows + c - 1) / c;
+        const uint32_t slice = ((max_rows + c - 1) / c + 3) / 4 * 4;
         p.held_keys = slice <= kSelSliceKeys ? slice : kSelSliceKeys;
-        const size_t smem = sizeof(uint32_t) * p.held_keys;
-        e = tt_set_smem_once(kv_evict_select_kernel, (int)(kSelSliceKeys * sizeof(uint32_t)));
-        if (e != cudaSuccess) return e;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(pairs * c); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
-        cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[1].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = tt_pdl_enabled() ? 2 : 1;
-        e = cudaLaunchKernelEx(&cfg, kv_evict_select_kernel, table, p, maps);
+        const bool fused = c == 1 && in_place && given_up <= kFusedMoves;
+        e = fused ? launch_select<false, true>(stream, table, p, pairs, 1, maps)
+                  : c == 1 ? launch_select<false, false>(stream, table, p, pairs, 1, maps)
+                           : launch_select<true, false>(stream, table, p, pairs * c, c, maps);
         if (e != cudaSuccess) return e;
         ctx->launches++;
+        if (fused) return cudaSuccess;
     }
     const uint32_t kept = max_rows < p.budget ? max_rows : p.budget;
     if (kept == 0) return cudaSuccess;
@@ -360,8 +459,8 @@ TT_API int tt_kv_evict(tt_context *ctx, tt_stream stream, const tt_kv_evict_sess
     uint32_t i = 0;
     while (i < n_sessions) {
         uint64_t used = 0;
-        uint32_t max_rows = 0;
-        bool select = false;
+        uint32_t max_rows = 0, given_up = 0;
+        bool in_place = true;
         table.n = 0;
         for (; i < n_sessions && table.n < kParamSessions; ++i) {
             const tt_kv_evict_session &s = sessions[i];
@@ -379,10 +478,11 @@ TT_API int tt_kv_evict(tt_context *ctx, tt_stream stream, const tt_kv_evict_sess
             d.rows = s.rows; d.end_position = s.end_position;
             d.map_begin = (uint32_t)used; d.map_pitch = (uint32_t)pitch;
             used += pitch * q.n_kv_heads;
-            select |= pitch != 0;
+            in_place = in_place && d.k_out == d.k && d.v_out == d.v;
+            if (s.rows > q.budget && s.rows - q.budget > given_up) given_up = s.rows - q.budget;
             if (s.rows > max_rows) max_rows = s.rows;
         }
-        const cudaError_t e = launch_evict(ctx, (cudaStream_t)stream, table, p, max_rows, select, reinterpret_cast<uint32_t *>(ctx->partials));
+        const cudaError_t e = launch_evict(ctx, (cudaStream_t)stream, table, p, max_rows, given_up, in_place, reinterpret_cast<uint32_t *>(ctx->partials));
         if (e != cudaSuccess) return tt_check_cuda(ctx, e, "kv_evict launch");
     }
     return TT_OK;

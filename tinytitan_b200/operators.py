@@ -105,14 +105,14 @@ class Context:
         if command_buffer is not None:
             return int(getattr(command_buffer, "cuda_stream", command_buffer))
         import torch
-        return int(torch.cuda.current_stream(self.device).cuda_stream)
+        return torch.cuda.current_stream(self.device).cuda_stream
 
     def check_device(self, *holders):
         """Refuses tensors (or tables over tensors) that are not on this context's device."""
         for t in holders:
             device = getattr(t, "device", None)
-            if device is not None and (device.type != "cuda" or device.index != self.device):
-                raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, f"a buffer is on {device}, the context on cuda:{self.device}")
+            if device is not None and (device.index != self.device or device.type != "cuda"):
+                _refuse(f"a buffer is on {device}, the context on cuda:{self.device}")
 
     @property
     def launch_count(self) -> int:
@@ -189,40 +189,42 @@ def _half_dtype(what: str, first, *others) -> int:
     return L.TT_BF16
 
 
-_indices = np.arange(64, dtype=np.uint64)[:, None]
-
-
-def _addresses(n: int, *tensors, index=None):
-    """[n, len(tensors)] device addresses of t[i] (or t[index[i]]) for i < n; None gives zeros."""
-    global _indices
-    if index is not None:
-        i = np.asarray(index, dtype=np.uint64)[:, None]
-    else:
-        if n > len(_indices):
-            _indices = np.arange(2 * n, dtype=np.uint64)[:, None]
-        i = _indices[:n]
-    base = np.array([0 if t is None else t.data_ptr() for t in tensors], dtype=np.uint64)
-    step = np.array([0 if t is None else t.stride(0) * t.element_size() for t in tensors], dtype=np.uint64)
-    return i * step + base
-
-
-def _counts(name: str, values, n: int):
+def _counts(name: str, values, n: int) -> list:
     """n numbers in 0..2^32-1 from a sequence, or from one int for all."""
-    try:
-        if isinstance(values, int):
-            a = np.full(n, values, dtype=np.uint32)
-        elif isinstance(values, (list, tuple)):
-            a = np.array(values, dtype=np.uint32)
-        else:
-            wide = np.asarray(values)
-            a = wide.astype(np.uint32)
-            if (wide != a).any():
-                raise OverflowError
-    except (OverflowError, TypeError, ValueError):
-        a = None
-    if a is None or a.shape != (n,):
+    if isinstance(values, int):
+        values = [values] * n
+    elif not isinstance(values, list):
+        values = [int(x) for x in values]
+    if len(values) != n or (n and (min(values) < 0 or max(values) > 0xFFFFFFFF)):
         _refuse(f"{name} must be {n} numbers in 0..2^32-1")
-    return a
+    return values
+
+
+def _block(n: int, tensors, lows, highs, spare=0, indices=None):
+    """n records of 64-bit words as the C structures lay them out: the addresses of t[i] (or t[indices[i]]; None gives 0),
+    one word of two 32-bit numbers, `spare` zero words."""
+    base = [0 if t is None else t.data_ptr() for t in tensors]
+    step = [0 if t is None else t.stride(0) * t.element_size() for t in tensors]
+    width = len(base)
+    if n <= 4 and indices is None:      # a handful of sessions: cheaper without numpy's fixed costs
+        tail = [0] * spare
+        rows = [[b + i * s for b, s in zip(base, step)] + [lows[i] | highs[i] << 32] + tail for i in range(n)]
+        return np.array(rows, dtype=np.uint64).reshape(n, width + 1 + spare)
+    words = np.zeros((n, width + 1 + spare), dtype=np.uint64)
+    i = np.arange(n, dtype=np.uint64)[:, None]
+    if indices is None:
+        words[:, :width] = i * np.array(step, dtype=np.uint64) + np.array(base, dtype=np.uint64)
+    else:                               # indices: per tensor, None for i itself
+        for c, which in enumerate(indices):
+            at = i[:, 0] if which is None else np.asarray(which, dtype=np.uint64)
+            words[:, c] = at * np.uint64(step[c]) + np.uint64(base[c])
+    halves = words.view(np.uint32)
+    halves[:, 2 * width], halves[:, 2 * width + 1] = lows, highs
+    return words
+
+
+def _pointer(words) -> int:
+    return words.__array_interface__["data"][0]
 
 
 class SessionTable:
@@ -247,7 +249,7 @@ class SessionTable:
 
     @property
     def pointer(self) -> int:
-        return self.words.__array_interface__["data"][0]
+        return _pointer(self.words)
 
     @classmethod
     def over_cache(cls, q, out, k, v, seq_lens, slots=None) -> "SessionTable":
@@ -255,23 +257,18 @@ class SessionTable:
         slot i or slots[i]; seq_lens[i] keys are visible to the last of its rows."""
         io_dtype = _half_dtype("q, out, k and v", q, out, k, v)
         q_stride, out_stride, kv_stride = _cache_stride("q", q), _cache_stride("out", out), _cache_stride("k", k)
-        n, q_rows = q.shape[:2]
-        if out.shape != q.shape or v.shape != k.shape or _cache_stride("v", v) != kv_stride:
+        q_shape, k_shape = q.shape, k.shape
+        n, q_rows = q_shape[0], q_shape[1]
+        if out.shape != q_shape or v.shape != k_shape or _cache_stride("v", v) != kv_stride:
             _refuse("out must be shaped like q, and v laid out like k")
         if slots is None:
-            if k.shape[0] < n:
-                _refuse(f"{n} sessions, but the cache has {k.shape[0]} slots")
-        elif len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k.shape[0])):
-            _refuse(f"slots must name {n} of the cache's {k.shape[0]} slots")
+            if k_shape[0] < n:
+                _refuse(f"{n} sessions, but the cache has {k_shape[0]} slots")
+        elif len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k_shape[0])):
+            _refuse(f"slots must name {n} of the cache's {k_shape[0]} slots")
         lens = _counts("seq_lens", seq_lens, n)
-        words = np.empty((n, 6), dtype=np.uint64)
-        if slots is None:
-            words[:, :4] = _addresses(n, q, out, k, v)
-        else:
-            words[:, :2], words[:, 2:4] = _addresses(n, q, out), _addresses(n, k, v, index=slots)
-        words[:, 4] = lens + np.uint64(q_rows << 32)
-        words[:, 5] = 0
-        return cls(words, int(lens.max()) if n else 0, kv_stride, q_stride, out_stride, io_dtype, k.shape[1], k.device)
+        words = _block(n, (q, out, k, v), lens, [q_rows] * n, 1, None if slots is None else (None, None, slots, slots))
+        return cls(words, max(lens, default=0), kv_stride, q_stride, out_stride, io_dtype, k_shape[1], k.device)
 
     @classmethod
     def of(cls, sessions) -> "SessionTable":
@@ -320,7 +317,7 @@ class PrefixTable:
 
     @property
     def pointer(self) -> int:
-        return self.words.__array_interface__["data"][0]
+        return _pointer(self.words)
 
     @classmethod
     def over_cache(cls, k, v, prefix_lens, n_sessions) -> "PrefixTable":
@@ -330,12 +327,9 @@ class PrefixTable:
             _refuse("v must be laid out like k")
         g = k.shape[0]
         lens, counts = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
-        if g and int(lens.max()) > k.shape[1]:
+        if max(lens, default=0) > k.shape[1]:
             _refuse(f"a prefix is longer than the {k.shape[1]} rows of its slot")
-        words = np.empty((g, 3), dtype=np.uint64)
-        words[:, :2] = _addresses(g, k, v)
-        words[:, 2] = lens + (counts.astype(np.uint64) << np.uint64(32))
-        return cls(words, k.device)
+        return cls(_block(g, (k, v), lens, counts), k.device)
 
     @classmethod
     def of(cls, groups) -> "PrefixTable":
@@ -500,14 +494,12 @@ class Attention:
             _refuse("positions must be laid out like weights")
         if t.longest > weights.shape[2]:
             _refuse(f"a session is longer than a weight row of {weights.shape[2]}")
-        words = np.empty((n, 3), dtype=np.uint64)          # tt_attn_weight_rows
-        words[:, :2] = _addresses(n, weights, positions)
-        ends = (t.words[:, 4] & np.uint64(0xFFFFFFFF)) if end_positions is None else _counts("end_positions", end_positions, n).astype(np.uint64)
-        words[:, 2] = _counts("fresh_rows", fresh_rows, n) + (ends << np.uint64(32))
+        ends = t.records["seq_len"].tolist() if end_positions is None else _counts("end_positions", end_positions, n)
+        words = _block(n, (weights, positions), _counts("fresh_rows", fresh_rows, n), ends)      # tt_attn_weight_rows
         p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                      out_row_stride_elements, scale, io_dtype)
         self.context.check(L.lib().tt_attn_decode_accumulate(
-            self.context.handle, self.context.stream(command_buffer), t.pointer, words.__array_interface__["data"][0], n,
+            self.context.handle, self.context.stream(command_buffer), t.pointer, _pointer(words), n,
             C.byref(p), head_stride))
 
     def encode_pre(self, q_packed, q_out, gate_out, k_rows, q_norm_weight, k_norm_weight, head_dim, num_q_heads,
@@ -637,7 +629,7 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
         _refuse("v must be laid out like k")
     n, capacity, num_kv_heads, head_dim = k.shape
     used = _counts("rows", rows, n)
-    most = int(used.max()) if n else 0
+    most = max(used, default=0)
     kept = min(most, budget)
     if most > capacity:
         _refuse(f"a session has more rows than the {capacity} of its slot")
@@ -662,12 +654,10 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
         if t.shape[2] < kept or stat_out not in (None, stride):
             _refuse(f"{name} must hold {kept} rows, and positions_out be laid out like weights_out")
         stat_out = stride
-    words = np.empty((n, 9), dtype=np.uint64)              # tt_kv_evict_session
-    words[:, :8] = _addresses(n, k, v, k_out, v_out, weights, weights_out, positions, positions_out)
     ends = used if end_positions is None else _counts("end_positions", end_positions, n)
-    words[:, 8] = used + (ends.astype(np.uint64) << np.uint64(32))
+    words = _block(n, (k, v, k_out, v_out, weights, weights_out, positions, positions_out), used, ends)  # tt_kv_evict_session
     p = L.KVEvictParams(head_dim, num_kv_heads, budget, sink_tokens, recent_tokens, in_stride, out_stride, stat, stat_out or stat, 0)
-    context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), words.__array_interface__["data"][0], n, C.byref(p)))
+    context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), _pointer(words), n, C.byref(p)))
 
 
 @dataclass
