@@ -26,11 +26,10 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr uint32_t kSelThreads = 512;
-constexpr uint32_t kSelWarps = kSelThreads / 32;
+constexpr uint32_t kMaxSelWarps = 32;
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kMaxCluster = 16;               // above 8: the non-portable size, allowed for this kernel
-constexpr uint32_t kFusedMoves = 64;               // rows a selecting CTA moves itself
+constexpr uint32_t kFusedMoves = 256;              // rows a selecting CTA moves itself
 constexpr uint32_t kSelSliceKeys = 50000;          // keys a CTA holds: 200,000 bytes beside the histogram and the counters
 constexpr uint32_t kHoleFlag = 0x80000000u;
 
@@ -69,6 +68,7 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool is_protected) {
 }
 
 // Exclusive block scan of one value per thread; *total gets the sum. Two barriers.
+template <uint32_t WARPS>
 __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *warp_sums, uint32_t *total) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t inc = x;
@@ -82,7 +82,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *warp_sums, 
     __syncthreads();
     uint32_t before = 0, all = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kSelWarps; ++w) {
+    for (uint32_t w = 0; w < WARPS; ++w) {
         const uint32_t s = warp_sums[w];
         before += w < warp ? s : 0u;
         all += s;
@@ -93,23 +93,24 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *warp_sums, 
 
 struct __align__(16) SelShared {
     uint32_t hist[kBins];
-    uint32_t warp_sums[kSelWarps];
+    uint32_t sum[2][kBins / 2];  // [round parity]: counts of this CTA's share of the bins over the cluster (read by the cluster)
+    uint32_t warp_sums[kMaxSelWarps];
+    uint32_t total[2];           // ... and their total
     uint32_t counts[4];          // this CTA's ties, holes, fills (read by the cluster)
-    uint32_t pick[2];            // the bin that holds the budget-th key, keys above it
+    uint32_t before[4];          // ... of the CTAs before this one
+    uint32_t owner[2];           // the CTA whose bins hold the wanted rank, keys above its bins
+    uint32_t pick[2];            // the bin that holds it, keys above it
     uint32_t hole_rows[kFusedMoves], fill_rows[kFusedMoves];
 };
 
-// One row of one head, 16 bytes a lane.
-__device__ __forceinline__ void copy_row(unsigned char *dst, const unsigned char *src, uint32_t bytes, uint32_t lane) {
-    if (lane * 16 < bytes) *reinterpret_cast<uint4 *>(dst + lane * 16) = *reinterpret_cast<const uint4 *>(src + lane * 16);
-}
-
 // CLUSTER: several CTAs per (session, head). FUSED (one CTA, in place, at most kFusedMoves rows given up): the moves too.
+// 512 threads alone (a few thousand rows: barriers dominate), 1024 in a cluster.
 template <bool CLUSTER, bool FUSED>
-__global__ void __launch_bounds__(kSelThreads)
+__global__ void __launch_bounds__(CLUSTER ? 1024 : 512)
 kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, uint32_t *__restrict__ maps) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ SelShared sh;
+    constexpr uint32_t kSelThreads = CLUSTER ? 1024 : 512, kSelWarps = kSelThreads / 32;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t size = CLUSTER ? cluster.num_blocks() : 1u, rank = CLUSTER ? cluster.block_rank() : 0u;
     auto sync_all = [&]() { if constexpr (CLUSTER) cluster.sync(); else __syncthreads(); };
@@ -141,67 +142,118 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
     };
     auto key_at = [&](uint32_t i) { return key_from(weights[begin + i], positions ? positions[begin + i] : begin + i); };
     if (held) {
-        uint32_t i = threadIdx.x;
-        if ((((uintptr_t)weights | (uintptr_t)positions) & 15) == 0) {
-            const uint32_t quads = n / 4;
-#pragma unroll 4
-            for (uint32_t c = threadIdx.x; c < quads; c += kSelThreads) {
-                const float4 w = *reinterpret_cast<const float4 *>(weights + begin + 4 * c);
-                uint4 q = make_uint4(begin + 4 * c, begin + 4 * c + 1, begin + 4 * c + 2, begin + 4 * c + 3);
-                if (positions) q = *reinterpret_cast<const uint4 *>(positions + begin + 4 * c);
-                *reinterpret_cast<uint4 *>(keys + 4 * c) = make_uint4(key_from(w.x, q.x), key_from(w.y, q.y), key_from(w.z, q.z), key_from(w.w, q.w));
-            }
-            i = quads * 4 + threadIdx.x;
+        // 16 bytes a thread behind the first aligned row, where the statistic and the positions share their alignment
+        uint32_t head_rows = 0, quads = 0;
+        if (((uintptr_t)weights ^ (positions ? (uintptr_t)positions : (uintptr_t)weights)) % 16 == 0) {
+            head_rows = min(n, (uint32_t)((16 - (uintptr_t)(weights + begin) % 16) % 16 / 4));
+            quads = (n - head_rows) / 4;
         }
+        const float *w0 = weights + begin + head_rows;
+        const uint32_t *p0 = positions + begin + head_rows;
 #pragma unroll 4
-        for (; i < n; i += kSelThreads) keys[i] = key_at(i);
+        for (uint32_t c = threadIdx.x; c < quads; c += kSelThreads) {
+            const float4 w = *reinterpret_cast<const float4 *>(w0 + 4 * c);
+            const uint32_t i = head_rows + 4 * c;
+            uint4 q = make_uint4(begin + i, begin + i + 1, begin + i + 2, begin + i + 3);
+            if (positions) q = *reinterpret_cast<const uint4 *>(p0 + 4 * c);
+            keys[i] = key_from(w.x, q.x); keys[i + 1] = key_from(w.y, q.y); keys[i + 2] = key_from(w.z, q.z); keys[i + 3] = key_from(w.w, q.w);
+        }
+        for (uint32_t i = threadIdx.x; i < head_rows; i += kSelThreads) keys[i] = key_at(i);
+#pragma unroll 4
+        for (uint32_t i = head_rows + quads * 4 + threadIdx.x; i < n; i += kSelThreads) keys[i] = key_at(i);
     }
     auto key_of = [&](uint32_t i) { return held ? keys[i] : key_at(i); };
 
     // ---- the budget-th largest key: three rounds over its bits from the top ----
     uint32_t prefix = 0, want = p.budget;                  // key bits fixed so far; rank wanted among the keys that share them
+    const uint32_t share = CLUSTER ? kBins / size : kBins;      // bins whose counts a CTA adds up
 #pragma unroll 1
     for (int round = 0; round < 3; ++round) {
         const uint32_t bits = round < 2 ? 11u : 10u, shift = round == 0 ? 21u : round == 1 ? 10u : 0u;
+        uint32_t *sum = sh.sum[round & 1];
         for (uint32_t b = threadIdx.x; b < kBins; b += kSelThreads) sh.hist[b] = 0;
+        if constexpr (CLUSTER)
+            if (threadIdx.x < share) sum[threadIdx.x] = 0;
         __syncthreads();
+#pragma unroll 4
         for (uint32_t i0 = 0; i0 < n; i0 += kSelThreads) {
             const uint32_t i = i0 + threadIdx.x;
-            uint32_t bin = 0xffffffffu;
-            if (i < n) {
-                const uint32_t key = key_of(i);
-                if (round == 0 || key >> (shift + bits) == prefix) bin = (key >> shift) & ((1u << bits) - 1);
-            }
-            const uint32_t counted = __ballot_sync(0xffffffffu, bin != 0xffffffffu);
-            if (counted == 0) continue;
+            const uint32_t key = i < n ? key_of(i) : 0u;
+            const bool counts = i < n && (round == 0 || key >> (shift + bits) == prefix);
+            const uint32_t counted = __ballot_sync(0xffffffffu, counts);
+            if (counted == 0) continue;                    // after the first round: nearly always
+            // a warp of one bin adds once; else every lane adds its own
+            const uint32_t bin = (key >> shift) & ((1u << bits) - 1);
             const int first = __ffs(counted) - 1;
             const uint32_t same = __shfl_sync(0xffffffffu, bin, first);
-            if (__ballot_sync(0xffffffffu, bin == same) == counted) {
-                if ((threadIdx.x & 31) == (uint32_t)first) atomicAdd(&sh.hist[same], (uint32_t)__popc(counted));
-            } else if (bin != 0xffffffffu) {
+            if (__all_sync(0xffffffffu, !counts || bin == same)) {
+                if ((threadIdx.x & 31) == (uint32_t)first) atomicAdd(&sh.hist[bin], (uint32_t)__popc(counted));
+            } else if (counts) {
                 atomicAdd(&sh.hist[bin], 1u);
             }
         }
         sync_all();
-        // thread t adds up bins 4t .. 4t+3 counted from the top, over the CTAs of the cluster
-        uint32_t c[4] = {0u, 0u, 0u, 0u};
-        const uint32_t top = kBins - 4 * (threadIdx.x + 1);
+        const uint32_t *bins = sh.hist;
+        uint32_t first_bin = 0, above0 = 0;
+        if constexpr (CLUSTER) {
+            // every CTA adds up its share of the bins, then the share that holds the wanted rank is found from the shares'
+            // totals, and its bins are read from its owner (adding up all bins in every CTA took 15,000 clocks a round)
+            const uint32_t b = threadIdx.x & (share - 1), q = threadIdx.x / share, step = kSelThreads / share;
+            uint32_t v = 0;
 #pragma unroll 4
-        for (uint32_t r = 0; r < size; ++r) {
-            const uint32_t *hist = CLUSTER ? cluster.map_shared_rank(sh.hist, r) : sh.hist;
-            const uint4 h = *reinterpret_cast<const uint4 *>(hist + top);
-            c[0] += h.w; c[1] += h.z; c[2] += h.y; c[3] += h.x;
+            for (uint32_t r = q; r < size; r += step) v += cluster.map_shared_rank(sh.hist, r)[rank * share + b];
+            if (v) atomicAdd(&sum[b], v);
+            __syncthreads();
+            if (threadIdx.x < 32) {
+                uint32_t all = 0;
+                for (uint32_t x = threadIdx.x; x < share; x += 32) all += sum[x];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+                if (threadIdx.x == 0) sh.total[round & 1] = all;
+            }
+            cluster.sync();
+            if (threadIdx.x < 32) {
+                const uint32_t lane = threadIdx.x;                                   // lane i: the i-th share from the top
+                const uint32_t x = lane < size ? cluster.map_shared_rank(sh.total, size - 1 - lane)[round & 1] : 0u;
+                uint32_t inc = x;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= (uint32_t)o) inc += up;
+                }
+                if (lane < size && inc - x < want && want <= inc) { sh.owner[0] = size - 1 - lane; sh.owner[1] = inc - x; }
+            }
+            __syncthreads();
+            bins = cluster.map_shared_rank(sum, sh.owner[0]);
+            first_bin = sh.owner[0] * share;
+            above0 = sh.owner[1];
+        }
+        // thread t takes bins kPer t .. counted from the top
+        constexpr uint32_t kPer = CLUSTER ? 2 : kBins / kSelThreads;
+        uint32_t c[kPer], mine = 0;
+#pragma unroll
+        for (uint32_t x = 0; x < kPer; ++x) c[x] = 0;
+        if (kPer * threadIdx.x < share) {
+            const uint32_t *from = bins + (share - kPer - kPer * threadIdx.x);
+            if constexpr (kPer == 4) {
+                const uint4 h = *reinterpret_cast<const uint4 *>(from);
+                c[0] = h.w; c[1] = h.z; c[2] = h.y; c[3] = h.x;
+            } else {
+                const uint2 h = *reinterpret_cast<const uint2 *>(from);
+                c[0] = h.y; c[1] = h.x;
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < kPer; ++x) mine += c[x];
         }
         uint32_t total;
-        const uint32_t above = block_scan(c[0] + c[1] + c[2] + c[3], sh.warp_sums, &total);
-        if (above < want && want <= above + c[0] + c[1] + c[2] + c[3]) {
-            uint32_t seen = above;
-            int j = 0;
-            while (j < 3 && seen + c[j] < want) seen += c[j++];
-            sh.pick[0] = top + 3 - j;
+        const uint32_t above = above0 + block_scan<kSelWarps>(mine, sh.warp_sums, &total);
+        if (above < want && want <= above + mine) {
+            uint32_t seen = above, x = 0;
+            while (x + 1 < kPer && seen + c[x] < want) seen += c[x++];
+            sh.pick[0] = first_bin + share - 1 - kPer * threadIdx.x - x;
             sh.pick[1] = seen;
         }
-        sync_all();                                        // the picked bin is known here, and no CTA still reads these counts
+        __syncthreads();
         prefix = (prefix << bits) | sh.pick[0];
         want -= sh.pick[1];
         __syncthreads();
@@ -214,12 +266,22 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
     uint32_t ties = 0;
     for (uint32_t i = i0; i < i1; ++i) ties += key_of(i) == threshold;
     uint32_t total;
-    uint32_t tie_rank = block_scan(ties, sh.warp_sums, &total);
+    uint32_t tie_rank = block_scan<kSelWarps>(ties, sh.warp_sums, &total);
+    // what the CTAs before this one have of counts[k], one read each
+    auto before = [&](int k) {
+        if (threadIdx.x < 32) {
+            uint32_t x = threadIdx.x < rank ? cluster.map_shared_rank(sh.counts, threadIdx.x)[k] : 0u;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            if (threadIdx.x == 0) sh.before[k] = x;
+        }
+    };
     if constexpr (CLUSTER) {
         if (threadIdx.x == 0) sh.counts[0] = total;
         cluster.sync();
-#pragma unroll 4
-        for (uint32_t r = 0; r < rank; ++r) tie_rank += *cluster.map_shared_rank(&sh.counts[0], r);
+        before(0);
+        __syncthreads();
+        tie_rank += sh.before[0];
     }
 
     uint32_t holes = 0, kept_above = 0, t = tie_rank;
@@ -230,17 +292,16 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
         if (begin + i < p.budget) holes += !keep; else kept_above += keep;
     }
     uint32_t total_holes, total_fills;
-    uint32_t hole = block_scan(holes, sh.warp_sums, &total_holes);
-    uint32_t fill = block_scan(kept_above, sh.warp_sums, &total_fills);
+    uint32_t hole = block_scan<kSelWarps>(holes, sh.warp_sums, &total_holes);
+    uint32_t fill = block_scan<kSelWarps>(kept_above, sh.warp_sums, &total_fills);
     if constexpr (CLUSTER) {
         if (threadIdx.x == 0) { sh.counts[1] = total_holes; sh.counts[2] = total_fills; }
         cluster.sync();
-#pragma unroll 4
-        for (uint32_t r = 0; r < rank; ++r) {
-            const uint32_t *other = cluster.map_shared_rank(sh.counts, r);
-            hole += other[1];
-            fill += other[2];
-        }
+        before(1);
+        before(2);
+        __syncthreads();
+        hole += sh.before[1];
+        fill += sh.before[2];
     }
     t = tie_rank;
     for (uint32_t i = i0; i < i1; ++i) {
@@ -254,9 +315,18 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
                 sh.fill_rows[fill++] = row;
             }
         } else {
-            if (row < p.budget) map[row] = keep ? row : kHoleFlag | hole++;
-            else if (keep) fills[fill++] = row;
+            if (row < p.budget) {
+                const uint32_t entry = keep ? row : kHoleFlag | hole++;
+                if (held) keys[i] = entry; else map[row] = entry;      // a thread's rows lie apart: through shared memory
+            } else if (keep) {
+                fills[fill++] = row;
+            }
         }
+    }
+    if (!FUSED && held) {
+        __syncthreads();
+        const uint32_t below = begin < p.budget ? min(n, p.budget - begin) : 0u;
+        for (uint32_t i = threadIdx.x; i < below; i += kSelThreads) map[begin + i] = keys[i];
     }
     if constexpr (CLUSTER) cluster.sync();                 // a CTA's counters outlive their readers
     if constexpr (FUSED) {
@@ -270,77 +340,97 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
             }
             __syncthreads();
         }
-        const uint32_t lane = threadIdx.x & 31;
-        for (uint32_t m = threadIdx.x >> 5; m < total_holes; m += kSelWarps) {
+        // the moves: a group of row_bytes / 16 lanes per row, four rows' K and V in flight
+        const uint32_t lanes = p.row_bytes / 16, unit = threadIdx.x / lanes, units = kSelThreads / lanes;
+        const size_t off = (size_t)head * p.row_bytes + threadIdx.x % lanes * 16;
+        for (uint32_t m0 = unit; m0 < total_holes; m0 += 4 * units) {
+            uint4 k[4], v[4];
+#pragma unroll
+            for (uint32_t x = 0; x < 4; ++x)
+                if (m0 + x * units < total_holes) {
+                    const size_t src = (size_t)sh.fill_rows[m0 + x * units] * p.in_stride + off;
+                    k[x] = *reinterpret_cast<const uint4 *>(ses.k + src);
+                    v[x] = *reinterpret_cast<const uint4 *>(ses.v + src);
+                }
+#pragma unroll
+            for (uint32_t x = 0; x < 4; ++x)
+                if (m0 + x * units < total_holes) {
+                    const size_t dst = (size_t)sh.hole_rows[m0 + x * units] * p.out_stride + off;
+                    *reinterpret_cast<uint4 *>(ses.k_out + dst) = k[x];
+                    *reinterpret_cast<uint4 *>(ses.v_out + dst) = v[x];
+                }
+        }
+        for (uint32_t m = threadIdx.x; m < total_holes; m += kSelThreads) {
             const uint32_t to = sh.hole_rows[m], from = sh.fill_rows[m];
-            const size_t dst = (size_t)to * p.out_stride + (size_t)head * p.row_bytes, src = (size_t)from * p.in_stride + (size_t)head * p.row_bytes;
-            copy_row(ses.k_out + dst, ses.k + src, p.row_bytes, lane);
-            copy_row(ses.v_out + dst, ses.v + src, p.row_bytes, lane);
-            if (lane == 0) {
-                ses.weights_out[out0 + to] = weights[from];
-                if (ses.positions_out != nullptr) ses.positions_out[out0 + to] = positions ? positions[from] : from;
-            }
+            ses.weights_out[out0 + to] = weights[from];
+            if (ses.positions_out != nullptr) ses.positions_out[out0 + to] = positions ? positions[from] : from;
         }
     }
 }
 
-// grid = (blocks of 256 destination rows, sessions x KV heads), a warp per 32 of them.
-template <int ROW_BYTES>
+// grid = (blocks of 8 * ROWS destination rows, sessions x KV heads), a warp per ROWS of them: 32 in place, where few of them
+// change, 8 into other buffers. Up to eight rows' loads are in flight before their stores.
+template <int ROW_BYTES, int ROWS>
 __global__ void __launch_bounds__(256)
 kv_evict_move_kernel(const __grid_constant__ EvictTable table, EvictParams p, const uint32_t *__restrict__ maps) {
-    constexpr uint32_t kLanes = ROW_BYTES / 16, kRowsAtOnce = 32 / kLanes;
-    __shared__ uint8_t todo_list[8][32];            // the lanes whose row is copied, packed
+    constexpr uint32_t kLanes = ROW_BYTES / 16, kAtOnce = 32 / kLanes, kRounds = 8 / kAtOnce;
+    __shared__ uint8_t lists[8][32];
     const EvictSession &ses = table.s[blockIdx.y / p.n_kv_heads];
     const uint32_t head = blockIdx.y % p.n_kv_heads;
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 32;
+    const uint32_t j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * ROWS;
     const uint32_t kept = min(ses.rows, p.budget);
     if (j0 >= kept) return;
-    const bool selected = ses.rows > p.budget;
-    const uint32_t *map = maps + ses.map_begin + (size_t)head * ses.map_pitch;
     const uint32_t j = j0 + lane;
+    const bool mine = lane < ROWS && j < kept;
     uint32_t src = j;
     bool hole = false;
-    if (selected && j < kept) {
+    if (ses.rows > p.budget && mine) {
+        const uint32_t *map = maps + ses.map_begin + (size_t)head * ses.map_pitch;
         const uint32_t e = map[j];
         hole = (e & kHoleFlag) != 0;
         if (hole) src = map[p.budget + (e & ~kHoleFlag)];
     }
-    if (j < kept) {
+    // rows to copy: the holes, and every row where the destination is another buffer
+    const uint32_t live = __ballot_sync(0xffffffffu, mine), holes = __ballot_sync(0xffffffffu, hole);
+    const uint32_t todo_k = ses.k_out != ses.k ? live : holes, todo_v = ses.v_out != ses.v ? live : holes, todo = todo_k | todo_v;
+    uint8_t *list = lists[threadIdx.x >> 5];
+    if ((todo >> lane) & 1u) list[__popc(todo & ((1u << lane) - 1))] = (uint8_t)lane;
+    __syncwarp();
+    const uint32_t n = __popc(todo);
+    const size_t head_off = (size_t)head * ROW_BYTES + (lane % kLanes) * 16;
+    for (uint32_t i0 = 0; i0 < n; i0 += 8) {
+        uint4 k[kRounds], v[kRounds];
+#pragma unroll
+        for (uint32_t i = 0; i < kRounds; ++i) {
+            const uint32_t nth = i0 + i * kAtOnce + lane / kLanes, at = list[min(nth, n - 1)];
+            const size_t in = (size_t)__shfl_sync(0xffffffffu, src, at) * p.in_stride + head_off;
+            if (nth < n && ((todo_k >> at) & 1u)) k[i] = *reinterpret_cast<const uint4 *>(ses.k + in);
+            if (nth < n && ((todo_v >> at) & 1u)) v[i] = *reinterpret_cast<const uint4 *>(ses.v + in);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kRounds; ++i) {
+            const uint32_t nth = i0 + i * kAtOnce + lane / kLanes, at = list[min(nth, n - 1)];
+            const size_t out = (size_t)(j0 + at) * p.out_stride + head_off;
+            if (nth < n && ((todo_k >> at) & 1u)) *reinterpret_cast<uint4 *>(ses.k_out + out) = k[i];
+            if (nth < n && ((todo_v >> at) & 1u)) *reinterpret_cast<uint4 *>(ses.v_out + out) = v[i];
+        }
+    }
+    if (mine) {
         const size_t at = (size_t)head * p.weight_stride + src, to = (size_t)head * p.weight_out_stride + j;
         if (hole || ses.weights_out != ses.weights) ses.weights_out[to] = ses.weights[at];
         if (ses.positions_out != nullptr && (hole || ses.positions_out != ses.positions))
             ses.positions_out[to] = ses.positions ? ses.positions[at] : src;
     }
-    // rows to copy: the holes, and every row where the destination is another buffer
-    const bool all_k = ses.k_out != ses.k, all_v = ses.v_out != ses.v;
-    const uint32_t live = __ballot_sync(0xffffffffu, j < kept), holes = __ballot_sync(0xffffffffu, hole);
-    const uint32_t todo = (all_k || all_v) ? live : holes;
-    const size_t head_off = (size_t)head * ROW_BYTES + (lane % kLanes) * 16;
-    const uint32_t n = __popc(todo);
-    uint8_t *list = todo_list[threadIdx.x >> 5];
-    if ((todo >> lane) & 1u) list[__popc(todo & ((1u << lane) - 1))] = (uint8_t)lane;
-    __syncwarp();
-#pragma unroll 4
-    for (uint32_t i = 0; i < n; i += kRowsAtOnce) {
-        const uint32_t nth = i + lane / kLanes;
-        const uint32_t at = nth < n ? list[nth] : 0u;
-        const uint32_t from = __shfl_sync(0xffffffffu, src, at);
-        if (nth >= n) continue;
-        const bool moved = (holes >> at) & 1u;
-        const size_t in = (size_t)from * p.in_stride + head_off, out = (size_t)(j0 + at) * p.out_stride + head_off;
-        if (moved || all_k) *reinterpret_cast<uint4 *>(ses.k_out + out) = *reinterpret_cast<const uint4 *>(ses.k + in);
-        if (moved || all_v) *reinterpret_cast<uint4 *>(ses.v_out + out) = *reinterpret_cast<const uint4 *>(ses.v + in);
-    }
 }
 
-// CTAs per (session, KV head): one per 4096 rows while the machine has SMs for them, and enough that the slices fit
+// CTAs per (session, KV head): one per 8192 rows while the machine has SMs for them, and enough that the slices fit
 // shared memory.
 uint32_t cluster_size(uint32_t max_rows, uint32_t pairs, uint32_t sm_count) {
     uint32_t c = 1;
-    while (c < kMaxCluster && ((max_rows > c * 4096u && (uint64_t)pairs * c * 2 <= sm_count) || (uint64_t)c * kSelSliceKeys < max_rows)) c *= 2;
+    while (c < kMaxCluster && ((max_rows > c * 8192u && (uint64_t)pairs * c * 2 <= sm_count) || (uint64_t)c * kSelSliceKeys < max_rows)) c *= 2;
     return c;
 }
 
@@ -359,7 +449,7 @@ cudaError_t launch_select(cudaStream_t stream, const EvictTable &table, const Ev
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = sizeof(uint32_t) * p.held_keys; cfg.stream = stream;
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(CLUSTER ? 1024 : 512); cfg.dynamicSmemBytes = sizeof(uint32_t) * p.held_keys; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -389,12 +479,14 @@ cudaError_t launch_evict(tt_context *ctx, cudaStream_t stream, const EvictTable 
     }
     const uint32_t kept = max_rows < p.budget ? max_rows : p.budget;
     if (kept == 0) return cudaSuccess;
-    const dim3 grid((kept + 255) / 256, pairs);
-    switch (p.row_bytes) {
-        case 128: e = tt_launch_pdl(kv_evict_move_kernel<128>, grid, dim3(256), 0, stream, table, p, maps); break;
-        case 256: e = tt_launch_pdl(kv_evict_move_kernel<256>, grid, dim3(256), 0, stream, table, p, maps); break;
-        default: e = tt_launch_pdl(kv_evict_move_kernel<512>, grid, dim3(256), 0, stream, table, p, maps); break;
-    }
+    const uint32_t rows = in_place ? 32 : 8;
+    const dim3 grid((kept + 8 * rows - 1) / (8 * rows), pairs);
+#define TT_X(BYTES) e = in_place ? tt_launch_pdl(kv_evict_move_kernel<BYTES, 32>, grid, dim3(256), 0, stream, table, p, maps) \
+                                 : tt_launch_pdl(kv_evict_move_kernel<BYTES, 8>, grid, dim3(256), 0, stream, table, p, maps)
+    if (p.row_bytes == 128) TT_X(128);
+    else if (p.row_bytes == 256) TT_X(256);
+    else TT_X(512);
+#undef TT_X
     if (e == cudaSuccess) ctx->launches++;
     return e;
 }
