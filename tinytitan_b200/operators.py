@@ -108,11 +108,11 @@ class Context:
         return torch.cuda.current_stream(self.device).cuda_stream
 
     def check_device(self, *holders):
-        """Refuses tensors (or tables over tensors) that are not on this context's device."""
+        """Refuses tensors (or tables over tensors) that are not on this context's device. Raw addresses pass."""
         for t in holders:
-            device = getattr(t, "device", None)
-            if device is not None and (device.index != self.device or device.type != "cuda"):
-                _refuse(f"a buffer is on {device}, the context on cuda:{self.device}")
+            get = getattr(t, "get_device", None)            # CUDA index, -1 on the host
+            if get is not None and get() not in (self.device, None):
+                _refuse(f"a buffer is on device {get()}, the context on cuda:{self.device}")
 
     @property
     def launch_count(self) -> int:
@@ -177,9 +177,9 @@ def _cache_stride(name: str, t) -> int:
 
 def _half_dtype(what: str, first, *others) -> int:
     """The tt_dtype of tensors that must share one 16-bit type and one device."""
-    dtype, device = first.dtype, first.device
+    dtype, device = first.dtype, first.get_device()
     for t in others:
-        if t.dtype != dtype or t.device != device:
+        if t.dtype != dtype or t.get_device() != device:
             _refuse(f"{what} must share one dtype and one device")
     name = str(dtype)
     if name == "torch.float16":
@@ -192,6 +192,8 @@ def _half_dtype(what: str, first, *others) -> int:
 def _counts(name: str, values, n: int) -> list:
     """n numbers in 0..2^32-1 from a sequence, or from one int for all."""
     if isinstance(values, int):
+        if n and 0 <= values <= 0xFFFFFFFF:
+            return [values] * n
         values = [values] * n
     elif not isinstance(values, list):
         values = [int(x) for x in values]
@@ -200,27 +202,44 @@ def _counts(name: str, values, n: int) -> list:
     return values
 
 
-def _block(n: int, tensors, lows, highs, spare=0, indices=None):
-    """n records of 64-bit words as the C structures lay them out: the addresses of t[i] (or t[indices[i]]; None gives 0),
-    one word of two 32-bit numbers, `spare` zero words."""
-    base = [0 if t is None else t.data_ptr() for t in tensors]
-    step = [0 if t is None else t.stride(0) * t.element_size() for t in tensors]
-    width = len(base)
-    if n <= 4 and indices is None:      # a handful of sessions: cheaper without numpy's fixed costs
-        tail = [0] * spare
-        rows = [[b + i * s for b, s in zip(base, step)] + [lows[i] | highs[i] << 32] + tail for i in range(n)]
-        return np.array(rows, dtype=np.uint64).reshape(n, width + 1 + spare)
-    words = np.zeros((n, width + 1 + spare), dtype=np.uint64)
-    i = np.arange(n, dtype=np.uint64)[:, None]
+def _block(n: int, places, lows, highs, spare=0, indices=None):
+    """n records of 64-bit words as the C structures lay them out: for every (address, step) of `places` address + i * step (or
+    + indices[i] * step), one word of two 32-bit numbers, `spare` zero words."""
+    width = len(places)
+    if n == 1 and indices is None:      # one session: cheaper without numpy's fixed costs
+        high = highs if isinstance(highs, int) else highs[0]
+        return np.array([[p[0] for p in places] + [lows[0] | high << 32] + [0] * spare], dtype=np.uint64)
+    words = np.empty((n, width + 1 + spare), dtype=np.uint64)
+    base, step = [p[0] for p in places], [p[1] for p in places]
+    i = _numbers(n)
     if indices is None:
-        words[:, :width] = i * np.array(step, dtype=np.uint64) + np.array(base, dtype=np.uint64)
-    else:                               # indices: per tensor, None for i itself
+        np.add(i * np.array(step, dtype=np.uint64), np.array(base, dtype=np.uint64), out=words[:, :width])
+    else:                               # indices: per place, None for i itself
         for c, which in enumerate(indices):
             at = i[:, 0] if which is None else np.asarray(which, dtype=np.uint64)
             words[:, c] = at * np.uint64(step[c]) + np.uint64(base[c])
     halves = words.view(np.uint32)
-    halves[:, 2 * width], halves[:, 2 * width + 1] = lows, highs
+    halves[:, 2 * width] = np.array(lows, dtype=np.uint32)
+    halves[:, 2 * width + 1] = highs if isinstance(highs, int) else np.array(highs, dtype=np.uint32)
+    if spare:
+        words[:, width + 1:] = 0
     return words
+
+
+_number_column = np.arange(64, dtype=np.uint64)[:, None]
+
+
+def _numbers(n: int):
+    """The column 0 .. n-1."""
+    global _number_column
+    if n > len(_number_column):
+        _number_column = np.arange(2 * n, dtype=np.uint64)[:, None]
+    return _number_column[:n]
+
+
+def _halves_place(t):
+    """(address, bytes between the batch entries) of a 16-bit tensor."""
+    return t.data_ptr(), 2 * t.stride()[0]
 
 
 def _pointer(words) -> int:
@@ -242,6 +261,9 @@ class SessionTable:
 
     def __len__(self):
         return len(self.words)
+
+    def get_device(self):
+        return self.device
 
     @property
     def records(self):
@@ -267,8 +289,9 @@ class SessionTable:
         elif len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k_shape[0])):
             _refuse(f"slots must name {n} of the cache's {k_shape[0]} slots")
         lens = _counts("seq_lens", seq_lens, n)
-        words = _block(n, (q, out, k, v), lens, [q_rows] * n, 1, None if slots is None else (None, None, slots, slots))
-        return cls(words, max(lens, default=0), kv_stride, q_stride, out_stride, io_dtype, k_shape[1], k.device)
+        words = _block(n, (_halves_place(q), _halves_place(out), _halves_place(k), _halves_place(v)), lens, q_rows, 1,
+                       None if slots is None else (None, None, slots, slots))
+        return cls(words, max(lens, default=0), kv_stride, q_stride, out_stride, io_dtype, k_shape[1], k.get_device())
 
     @classmethod
     def of(cls, sessions) -> "SessionTable":
@@ -311,6 +334,9 @@ class PrefixTable:
     def __len__(self):
         return len(self.words)
 
+    def get_device(self):
+        return self.device
+
     @property
     def records(self):
         return self.words.view(self.record)[:, 0]
@@ -329,7 +355,7 @@ class PrefixTable:
         lens, counts = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
         if max(lens, default=0) > k.shape[1]:
             _refuse(f"a prefix is longer than the {k.shape[1]} rows of its slot")
-        return cls(_block(g, (k, v), lens, counts), k.device)
+        return cls(_block(g, (_halves_place(k), _halves_place(v)), lens, counts), k.get_device())
 
     @classmethod
     def of(cls, groups) -> "PrefixTable":
@@ -488,14 +514,16 @@ class Attention:
         t = self._table(sessions)
         t.check_capacity()
         n = len(t)
-        head_stride = _statistic("weights", weights, "torch.float32", n, num_kv_heads, self.context)
-        if positions is not None and (positions.shape != weights.shape or head_stride != _statistic(
-                "positions", positions, "torch.int32", n, num_kv_heads, self.context)):
-            _refuse("positions must be laid out like weights")
+        head_stride, at = _statistic("weights", weights, "torch.float32", n, num_kv_heads, self.context)
+        at_positions = (0, 0)
+        if positions is not None:
+            stride, at_positions = _statistic("positions", positions, "torch.int32", n, num_kv_heads, self.context)
+            if stride != head_stride or positions.shape != weights.shape:
+                _refuse("positions must be laid out like weights")
         if t.longest > weights.shape[2]:
             _refuse(f"a session is longer than a weight row of {weights.shape[2]}")
         ends = t.records["seq_len"].tolist() if end_positions is None else _counts("end_positions", end_positions, n)
-        words = _block(n, (weights, positions), _counts("fresh_rows", fresh_rows, n), ends)      # tt_attn_weight_rows
+        words = _block(n, (at, at_positions), _counts("fresh_rows", fresh_rows, n), ends)      # tt_attn_weight_rows
         p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                      out_row_stride_elements, scale, io_dtype)
         self.context.check(L.lib().tt_attn_decode_accumulate(
@@ -605,13 +633,18 @@ def quantize_kv_rows(context: Context, source, destination, element_count: int, 
         group_size, tokens))
 
 
-def _statistic(name: str, t, dtype: str, n: int, num_kv_heads: int, context: Context) -> int:
-    """Elements between the heads of a [sessions, n_kv_heads, rows] tensor that holds one number per cache row."""
+def _statistic(name: str, t, dtype: str, n: int, num_kv_heads: int, context: Context):
+    """A [sessions, n_kv_heads, rows] tensor of one 32-bit number per cache row: elements between its heads, and
+    (address, bytes between sessions)."""
     shape, stride = t.shape, t.stride()
     if str(t.dtype) != dtype or len(shape) != 3 or shape[0] < n or shape[1] != num_kv_heads or (shape[2] > 1 and stride[2] != 1):
         _refuse(f"{name} must be {dtype} [{n}, {num_kv_heads}, rows], rows contiguous")
-    context.check_device(t)
-    return stride[1] if num_kv_heads > 1 else shape[2]
+    if t.get_device() != context.device:
+        context.check_device(t)
+    return stride[1] if num_kv_heads > 1 else shape[2], (t.data_ptr(), 4 * stride[0])
+
+
+_nowhere = (0, 0)
 
 
 def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_tokens=0, recent_tokens=0, positions=None,
@@ -622,40 +655,52 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
     positions: int32 like weights, None = row j holds position j; end_positions: position of the next token (default:
     rows). *_out: None for in place, or tensors of the same kind with room for min(rows, budget) rows. Afterwards
     session i has min(rows[i], budget) rows per head."""
-    _half_dtype("K and V", k, *(t for t in (v, k_out, v_out) if t is not None))
+    _half_dtype("K and V", k, v)
     context.check_device(k)
     in_stride = _cache_stride("k", k)
-    if v.shape != k.shape or _cache_stride("v", v) != in_stride:
+    shape = k.shape
+    if v.shape != shape or _cache_stride("v", v) != in_stride:
         _refuse("v must be laid out like k")
-    n, capacity, num_kv_heads, head_dim = k.shape
+    n, capacity, num_kv_heads, head_dim = shape
     used = _counts("rows", rows, n)
     most = max(used, default=0)
     kept = min(most, budget)
     if most > capacity:
         _refuse(f"a session has more rows than the {capacity} of its slot")
-    out_stride = in_stride
+    # destinations of K and V
+    out_stride, at_k, at_v = in_stride, _nowhere, _nowhere
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is None:
             continue
-        stride = _cache_stride(name, t)
-        if t.shape[0] < n or t.shape[1] < kept or t.shape[2:] != k.shape[2:] or (name == "v_out" and k_out is not None and stride != out_stride):
+        _half_dtype("K and V", k, t)
+        stride, s = _cache_stride(name, t), t.shape
+        if s[0] < n or s[1] < kept or s[2] != num_kv_heads or s[3] != head_dim or (t is v_out and k_out is not None and stride != out_stride):
             _refuse(f"{name} must hold the kept rows of {n} sessions, and v_out be laid out like k_out")
         out_stride = stride
-    stat = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context)
-    if positions is not None and _statistic("positions", positions, "torch.int32", n, num_kv_heads, context) != stat:
-        _refuse("positions must be laid out like weights")
-    if weights.shape[2] < most or (positions is not None and positions.shape[2] < most):
-        _refuse(f"weights and positions must hold {most} rows")
-    stat_out = None
-    for name, t, dtype in (("weights_out", weights_out, "torch.float32"), ("positions_out", positions_out, "torch.int32")):
-        if t is None:
-            continue
-        stride = _statistic(name, t, dtype, n, num_kv_heads, context)
-        if t.shape[2] < kept or stat_out not in (None, stride):
-            _refuse(f"{name} must hold {kept} rows, and positions_out be laid out like weights_out")
+        if t is k_out:
+            at_k = _halves_place(t)
+        if t is v_out:
+            at_v = _halves_place(t)
+    # the statistic and the positions, then where they go
+    stat, at_w = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context)
+    at_p, at_wo, at_po, stat_out = _nowhere, _nowhere, _nowhere, None
+    if positions is not None:
+        stride, at_p = _statistic("positions", positions, "torch.int32", n, num_kv_heads, context)
+        if stride != stat or positions.shape[2] < most:
+            _refuse(f"positions must be laid out like weights and hold {most} rows")
+    if weights.shape[2] < most:
+        _refuse(f"weights must hold {most} rows")
+    if weights_out is not None:
+        stat_out, at_wo = _statistic("weights_out", weights_out, "torch.float32", n, num_kv_heads, context)
+        if weights_out.shape[2] < kept:
+            _refuse(f"weights_out must hold {kept} rows")
+    if positions_out is not None:
+        stride, at_po = _statistic("positions_out", positions_out, "torch.int32", n, num_kv_heads, context)
+        if positions_out.shape[2] < kept or stat_out not in (None, stride):
+            _refuse(f"positions_out must hold {kept} rows and be laid out like weights_out")
         stat_out = stride
     ends = used if end_positions is None else _counts("end_positions", end_positions, n)
-    words = _block(n, (k, v, k_out, v_out, weights, weights_out, positions, positions_out), used, ends)  # tt_kv_evict_session
+    words = _block(n, (_halves_place(k), _halves_place(v), at_k, at_v, at_w, at_wo, at_p, at_po), used, ends)  # tt_kv_evict_session
     p = L.KVEvictParams(head_dim, num_kv_heads, budget, sink_tokens, recent_tokens, in_stride, out_stride, stat, stat_out or stat, 0)
     context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), _pointer(words), n, C.byref(p)))
 
