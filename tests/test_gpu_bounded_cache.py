@@ -395,7 +395,7 @@ def test_accumulate_in_a_small_workspace():
     ctx.close(), tiny.close()
 
 
-def test_accumulate_is_deterministic_and_its_output_is_plain_decode():
+def test_accumulate_is_deterministic_and_its_output_is_that_of_decode():
     n, hq, hkv, hd, s = 4, 16, 2, 256, 3000
     q, k, v = (normal(i, *x).cuda() for i, x in enumerate([(n, 1, hq, hd), (n, s, hkv, hd), (n, s, hkv, hd)]))
     a = tt.Attention(context())
@@ -405,7 +405,10 @@ def test_accumulate_is_deterministic_and_its_output_is_plain_decode():
         a.encode_accumulate(tt.SessionTable.over_cache(q, o, k, v, lens), w, hd, hq, hkv)
     a.encode_batched([tt.DecodeSession(q[i], outs[2][i], k[i], v[i], m) for i, m in enumerate(lens)], hd, hq, hkv)
     done()
-    assert torch.equal(stats[0], stats[1]) and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    assert torch.equal(stats[0], stats[1]) and torch.equal(outs[0], outs[1])
+    # the same partials merged in another order: 32-bit sums of a few dozen terms, then one rounding (half a step each)
+    a, b = outs[0].double(), outs[2].double()
+    assert ((a - b).abs() <= 2 * 2.0 ** -11 * b.abs() + 1e-6).all()
     # every row of the softmax weighs one: the statistic of a KV head grows by its number of query heads
     total = stats[0].double().sum(-1)
     assert ((total - hq // hkv).abs() <= 2e-5 * hq // hkv + 1e-4).all()

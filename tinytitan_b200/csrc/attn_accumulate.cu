@@ -4,94 +4,157 @@
 // A[j] += sum over the session's query rows r and the head's query heads g of softmax(q_rg . K^T * scale)[j].
 // A weight needs the maximum and the sum of its whole row, which exist only after all splits of the key range are
 // done. Instead of reading K a second time, pass 1 (attn_pass1.cuh) leaves the raw scores behind (4 bytes per key and
-// query head next to the 4 * head_dim bytes of K and V it reads per key and KV head; they mostly stay in L2), the
-// usual merge writes the output rows, and the kernel below forms the weights from the scores. The sums it divides by
-// are those of the unrounded weights: the output divides by the sum of the ROUNDED ones its P.V product used, whose
-// error (2^-9 with bf16 weights) the statistic, in 32 bits, would otherwise collect step after step.
-// Every statistic is written by one thread in a fixed order, so results do not depend on the schedule.
+// query head next to the 4 * head_dim bytes of K and V it reads per key and KV head; stored to stay in L2), and one
+// launch behind it merges the output rows in its first CTAs and forms the weights from the scores in the others. The
+// sums the weights divide by are those of the unrounded weights: the output divides by the sum of the ROUNDED ones its
+// P.V product used, whose error (2^-9 with bf16 weights) the statistic, in 32 bits, would otherwise collect step after
+// step. Every statistic is written by one thread in a fixed order, so results do not depend on the schedule.
+#include "attn_merge.cuh"
 #include "attn_pass1.cuh"
 
 namespace {
 
 constexpr uint32_t kAccThreads = 256;
-constexpr uint32_t kAccKeys = 512;        // keys of one CTA
+constexpr uint32_t kAccPerThread = 4;                            // keys of one thread
+constexpr uint32_t kAccKeys = kAccThreads * kAccPerThread;       // ... and of one CTA
 
 struct AccSession {
     const float *scores;
     float *weights;              // row 0 of KV head 0
     uint32_t *positions;         // nullable
+    void *out;
     uint32_t seq_len;            // keys the scores cover
     uint32_t total_len;          // keys of the whole session (>= seq_len when its rows are taken in several passes)
     uint32_t q_rows;
     uint32_t n_parts, partial_base;
     uint32_t fresh_begin;        // rows from here on start at zero (total_len: none)
     uint32_t end_position;
-    uint32_t block_begin;        // CTAs of the sessions before this one
 };
 
 struct AccTable {
+    uint32_t n, merge_ctas, merge_groups, merge_rows;
+    uint32_t first_cta[kParamSessions];      // CTAs (behind the merge's) of the sessions before each one
+    uint32_t first_row[kParamSessions];      // query rows of the sessions before each one
     AccSession s[kParamSessions];
-    uint32_t n;
 };
 
-// grid = sum over sessions of (KV heads x key chunks). One thread per key; the rows' normalisers are merged from the
-// parts' (max, sum) by one warp per row first.
-__global__ void __launch_bounds__(kAccThreads)
-attn_accumulate_kernel(const __grid_constant__ AccTable table, const float *__restrict__ part_m2,
-                       const float *__restrict__ part_l2, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t row_pad,
-                       uint32_t head_stride, float scale_log2) {
-    extern __shared__ float norm[];           // log2 of the softmax denominator of every packed row
-    pdl_launch_dependents();
-    pdl_wait();
-    uint32_t lo = 0, hi = table.n;
+struct AccParams {
+    const float *part_o, *part_m, *part_l;
+    const float *part_m2, *part_l2;
+    uint32_t n_q_heads, n_kv_heads, row_pad, head_stride, out_row_stride;
+    float scale_log2;
+};
+
+__device__ __forceinline__ uint32_t last_not_above(const uint32_t *first, uint32_t n, uint32_t x) {
+    uint32_t lo = 0, hi = n;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (table.s[mid].block_begin <= blockIdx.x) lo = mid; else hi = mid;
+        if (first[mid] <= x) lo = mid; else hi = mid;
     }
-    const AccSession &ses = table.s[lo];
-    const uint32_t local = blockIdx.x - ses.block_begin;
-    const uint32_t kv_head = local % n_kv_heads, chunk = local / n_kv_heads;
-    const uint32_t group = n_q_heads / n_kv_heads;
-    const uint32_t rows = ses.q_rows * group, rows_padded = (rows + row_pad - 1) / row_pad * row_pad;
-    const uint32_t rows_total = ses.q_rows * n_q_heads;
+    return lo;
+}
+
+// grid = merge CTAs, then per session (key chunks x KV heads). In the latter a thread has four keys; the scores of its
+// first eight rows are on their way while the rows' normalisers are merged from the parts' (max, sum), a warp per row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kAccThreads)
+attn_accumulate_kernel(const __grid_constant__ AccTable table, AccParams p) {
+    extern __shared__ float norm[];           // log2 of the softmax denominator of every packed row
+    __shared__ typename RowMerge<HD>::Shared shared;
+    pdl_launch_dependents();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (uint32_t r = warp; r < rows; r += kAccThreads / 32) {
-        const size_t base = (size_t)ses.partial_base + (r / group) * n_q_heads + kv_head * group + r % group;
-        float m = -INFINITY;
-        for (uint32_t c = lane; c < ses.n_parts; c += 32) m = fmaxf(m, part_m2[base + (size_t)c * rows_total]);
+    if (blockIdx.x < table.merge_ctas) {
+        const uint32_t out_row = RowMerge<HD>::row(blockIdx.x, warp, table.merge_groups);
+        const bool live = out_row < table.merge_rows;
+        const uint32_t qrow = out_row / p.n_q_heads, head = out_row - qrow * p.n_q_heads;
+        const uint32_t i = last_not_above(table.first_row, table.n, qrow);
+        const AccSession &ses = table.s[i];
+        const uint32_t w = qrow - table.first_row[i];
+        RowMerge<HD> merge(warp, lane, table.merge_groups);
+        pdl_wait();                           // pass 1 is done
+        if (live)
+            merge.walk(p.part_o, p.part_m, p.part_l, (size_t)ses.partial_base + w * p.n_q_heads + head, (size_t)ses.q_rows * p.n_q_heads, ses.n_parts);
+        if (!merge.join(shared) || !live) return;
+        merge.template store<T>(reinterpret_cast<T *>(ses.out) + (size_t)w * p.out_row_stride + (size_t)head * HD);
+        return;
+    }
+    const uint32_t cta = blockIdx.x - table.merge_ctas, i = last_not_above(table.first_cta, table.n, cta);
+    const AccSession &ses = table.s[i];
+    const uint32_t local = cta - table.first_cta[i];
+    const uint32_t kv_head = local % p.n_kv_heads, chunk = local / p.n_kv_heads;
+    const uint32_t group = p.n_q_heads / p.n_kv_heads;
+    const uint32_t rows = ses.q_rows * group, rows_padded = (rows + p.row_pad - 1) / p.row_pad * p.row_pad;
+    const uint32_t rows_total = ses.q_rows * p.n_q_heads;
+    const uint32_t seq_len = ses.seq_len, total_len = ses.total_len;
+    const float *scores = ses.scores + (size_t)kv_head * seq_len * rows_padded;
+
+    uint32_t key[kAccPerThread];
+    float s[kAccPerThread][8], sum[kAccPerThread], old[kAccPerThread];
+    auto load_rows = [&](uint32_t r0) {       // eight rows' scores of every key (the padding reaches a multiple of eight)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float l = 0.f;
-        if (m != -INFINITY)
-            for (uint32_t c = lane; c < ses.n_parts; c += 32) {
-                const size_t at = base + (size_t)c * rows_total;
-                l += part_l2[at] * exp2f(part_m2[at] - m);
+        for (uint32_t x = 0; x < kAccPerThread; ++x)
+            if (key[x] < seq_len) {
+                const float4 *row = reinterpret_cast<const float4 *>(scores + (size_t)key[x] * rows_padded + r0);
+                const float4 a = row[0], b = row[1];
+                s[x][0] = a.x; s[x][1] = a.y; s[x][2] = a.z; s[x][3] = a.w;
+                s[x][4] = b.x; s[x][5] = b.y; s[x][6] = b.z; s[x][7] = b.w;
             }
+    };
+    float *weights = ses.weights + (size_t)kv_head * p.head_stride;
+    pdl_wait();                               // pass 1 is done
+#pragma unroll
+    for (uint32_t x = 0; x < kAccPerThread; ++x) {
+        key[x] = chunk * kAccKeys + x * kAccThreads + threadIdx.x;
+        sum[x] = 0.f;
+        old[x] = key[x] < min(total_len, ses.fresh_begin) ? weights[key[x]] : 0.f;
+    }
+    load_rows(0);
+    for (uint32_t r = warp; r < rows; r += kAccThreads / 32) {
+        const size_t base = (size_t)ses.partial_base + (r / group) * p.n_q_heads + kv_head * group + r % group;
+        float m = -INFINITY, l = 0.f;
+        for (uint32_t c = lane; c < ses.n_parts; c += 32) {
+            const size_t at = base + (size_t)c * rows_total;
+            const float m2 = p.part_m2[at], l2 = p.part_l2[at];
+            const float m_new = fmaxf(m, m2);
+            if (m_new != -INFINITY) l = l * exp2f(m - m_new) + l2 * exp2f(m2 - m_new);
+            m = m_new;
+        }
+        float mx = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        l = mx != -INFINITY ? l * exp2f(m - mx) : 0.f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) norm[r] = l > 0.f ? m + log2f(l) : INFINITY;      // a row that sees nothing weighs nothing
+        if (lane == 0) norm[r] = l > 0.f ? mx + log2f(l) : INFINITY;      // a row that sees nothing weighs nothing
     }
     __syncthreads();
-    const float *scores = ses.scores + (size_t)kv_head * ses.seq_len * rows_padded;
-    const uint32_t key_end = min(ses.total_len, (chunk + 1) * kAccKeys);
-    for (uint32_t key = chunk * kAccKeys + threadIdx.x; key < key_end; key += kAccThreads) {
-        float sum = 0.f;
-        if (key < ses.seq_len) {
-            const float *row = scores + (size_t)key * rows_padded;
-            // query row w of q_rows sees keys below seq_len - (q_rows - 1 - w)
-            const uint32_t hidden = key + ses.q_rows > ses.seq_len ? key + ses.q_rows - ses.seq_len : 0u;   // first rows that do not see it
-            for (uint32_t r = hidden * group / 4 * 4; r < rows; r += 4) {
-                const float4 s = *reinterpret_cast<const float4 *>(row + r);
-                const float v[4] = {s.x, s.y, s.z, s.w};
+    for (uint32_t r0 = 0; r0 < rows; r0 += 8) {
+        if (r0 != 0) load_rows(r0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (r + j < rows && r + j >= hidden * group) sum += exp2f(fmaf(v[j], scale_log2, -norm[r + j]));
-            }
+        for (uint32_t x = 0; x < kAccPerThread; ++x) {
+            if (key[x] >= seq_len) continue;
+            // query row w of q_rows sees keys below seq_len - (q_rows - 1 - w): the first rows do not see the last keys
+            const uint32_t hidden = key[x] + ses.q_rows > seq_len ? (key[x] + ses.q_rows - seq_len) * group : 0u;
+#pragma unroll
+            for (uint32_t y = 0; y < 8; ++y)
+                if (r0 + y < rows && r0 + y >= hidden) sum[x] += exp2f(fmaf(s[x][y], p.scale_log2, -norm[r0 + y]));
         }
-        const size_t at = (size_t)kv_head * head_stride + key;
-        const bool fresh = key >= ses.fresh_begin;
-        if (fresh && ses.positions != nullptr) ses.positions[at] = ses.end_position - (ses.total_len - key);
-        ses.weights[at] = fresh ? sum : ses.weights[at] + sum;
+    }
+#pragma unroll
+    for (uint32_t x = 0; x < kAccPerThread; ++x) {
+        if (key[x] >= total_len) continue;
+        weights[key[x]] = old[x] + sum[x];
+        if (key[x] >= ses.fresh_begin && ses.positions != nullptr)
+            ses.positions[(size_t)kv_head * p.head_stride + key[x]] = ses.end_position - (total_len - key[x]);
+    }
+}
+
+template <typename T>
+cudaError_t launch_accumulate(cudaStream_t stream, uint32_t head_dim, uint32_t ctas, size_t smem, const AccTable &table, const AccParams &p) {
+    switch (head_dim) {
+        case 64: return tt_launch_pdl(attn_accumulate_kernel<T, 64>, dim3(ctas), dim3(kAccThreads), smem, stream, table, p);
+        case 128: return tt_launch_pdl(attn_accumulate_kernel<T, 128>, dim3(ctas), dim3(kAccThreads), smem, stream, table, p);
+        default: return tt_launch_pdl(attn_accumulate_kernel<T, 256>, dim3(ctas), dim3(kAccThreads), smem, stream, table, p);
     }
 }
 
@@ -175,7 +238,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
         const uint32_t pad = wide_rows ? 16u : 8u;
         float *scores = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->partials) + (ctx->workspace_bytes / 16 * 16 - (bytes + 255) / 256 * 256));
         table.n = count;
-        uint32_t blocks = 0, max_rows = 0;
+        uint32_t blocks = 0, max_rows = 0, query_rows = 0;
         for (uint32_t c = 0; c < count; ++c) {
             const tt_attn_session &s = sessions[i + c];
             const uint32_t skip = c == 0 ? row_done : 0u, rows = c == 0 ? rows_of_first : s.q_rows;
@@ -192,7 +255,10 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
             a.seq_len = d.seq_len; a.total_len = s.seq_len; a.q_rows = rows;
             a.fresh_begin = skip == 0 ? s.seq_len - weight_rows[i + c].fresh_rows : s.seq_len;
             a.end_position = weight_rows[i + c].end_position;
-            a.block_begin = blocks;
+            a.out = d.out;
+            table.first_cta[c] = blocks;
+            table.first_row[c] = query_rows;
+            query_rows += rows;
             blocks += ceil_div(s.seq_len, kAccKeys) * params->n_kv_heads;
             const uint32_t padded = (rows * group + pad - 1) / pad * pad;
             scores += ((size_t)params->n_kv_heads * d.seq_len * padded + 3) / 4 * 4;
@@ -200,6 +266,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
         }
         TTDecodeForm form;
         form.form = kPassScores;
+        form.partials_only = true;
         form.reserved_bytes = (bytes + 255) / 256 * 256 + 16;
         int rc = tt_launch_decode(ctx, (cudaStream_t)stream, tmp, count, params, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &form);
         if (rc != TT_OK) return rc;
@@ -207,13 +274,18 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
             table.s[c].n_parts = ctx->h_sessions[c].n_parts;
             table.s[c].partial_base = ctx->h_sessions[c].partial_base;
         }
-        if (blocks != 0) {
-            const cudaError_t e = tt_launch_pdl(attn_accumulate_kernel, dim3(blocks), dim3(kAccThreads), max_rows * sizeof(float),
-                                                (cudaStream_t)stream, table, form.part_m2, form.part_l2, params->n_q_heads,
-                                                params->n_kv_heads, pad, head_stride, params->scale * kLog2e);
-            if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_accumulate launch");
-            ctx->launches++;
-        }
+        table.merge_rows = query_rows * params->n_q_heads;
+        table.merge_groups = merge_groups(table.merge_rows, params->head_dim, (uint32_t)ctx->sm_count, &table.merge_ctas);
+        AccParams p;
+        p.part_o = form.part_o; p.part_m = form.part_m; p.part_l = form.part_l; p.part_m2 = form.part_m2; p.part_l2 = form.part_l2;
+        p.n_q_heads = params->n_q_heads; p.n_kv_heads = params->n_kv_heads; p.row_pad = pad; p.head_stride = head_stride;
+        p.out_row_stride = params->out_row_stride_elements; p.scale_log2 = params->scale * kLog2e;
+        const uint32_t ctas = table.merge_ctas + blocks;
+        const size_t smem = max_rows * sizeof(float);
+        const cudaError_t e = params->io_dtype == TT_F16 ? launch_accumulate<__half>((cudaStream_t)stream, params->head_dim, ctas, smem, table, p)
+                                                         : launch_accumulate<__nv_bfloat16>((cudaStream_t)stream, params->head_dim, ctas, smem, table, p);
+        if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_accumulate launch");
+        ctx->launches++;
         // the next pass: the rest of a cut session, or the sessions behind it
         if (count == 1 && row_done + rows_of_first < sessions[i].q_rows) {
             row_done += rows_of_first;

@@ -139,8 +139,8 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
     const uint32_t rank = cluster_rank();
 
     pdl_launch_dependents();
+    const typename Form::Item item = form.item(blockIdx.x >> 1, HD, ROWS);   // from the parameters alone
     pdl_wait();       // the kernel before this one may have produced the query or cache rows
-    const typename Form::Item item = form.item(blockIdx.x >> 1, HD, ROWS);
     const uint32_t n_tiles = item.n_tiles;                                   // >= 1
     const uint32_t my_row0 = rank * 128;
 

@@ -46,6 +46,14 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A store whose lines are the last to leave L2: read back by the next launch, next to a stream of K and V that is not
+// (scores of 435,000 keys: 216.5 -> 212.7 us a call).
+__device__ __forceinline__ void store_keep(float *dst, float x, float y) {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
+    asm volatile("st.global.L2::cache_hint.v2.f32 [%0], {%1, %2}, %3;" ::"l"(dst), "f"(x), "f"(y), "l"(policy) : "memory");
+}
+
 // Shared memory of the fp16/bf16 pass-1 kernel for HPC KV heads per CTA.
 template <int HD, int HPC>
 struct DecodeSmem {
@@ -274,8 +282,8 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t key = item.key_begin + i * kKeysPerBlock + g + 8 * h;
                         if (key < item.key_end)
-                            *reinterpret_cast<float2 *>(ses.scores + ((size_t)kv_head * ses.seq_len + key) * rows_pad + item.row_begin + nt * 8 + 2 * t) =
-                                make_float2(s0[nt][2 * h] + s1[nt][2 * h], s0[nt][2 * h + 1] + s1[nt][2 * h + 1]);
+                            store_keep(ses.scores + ((size_t)kv_head * ses.seq_len + key) * rows_pad + item.row_begin + nt * 8 + 2 * t,
+                                       s0[nt][2 * h] + s1[nt][2 * h], s0[nt][2 * h + 1] + s1[nt][2 * h + 1]);
                     }
                 }
             }

@@ -13,6 +13,7 @@
 // after session. Every row of an item sees every key of its range: only the last tile of a prefix is masked. What
 // bounds the pass depends on the rows: with up to about 256 packed rows per KV head the bytes of the prefix, beyond
 // that the tensor pipe and the exponentials.
+#include "attn_merge.cuh"
 #include "attn_pair_tc.cuh"
 
 namespace {
@@ -45,24 +46,25 @@ struct alignas(64) PrefixMaps { unsigned char m[2][128]; };    // K and V tensor
 // Calls of up to kParamGroups groups and kParamSessions sessions carry their tables and tensor maps in the kernel
 // parameters; larger ones read the copies the host uploaded.
 struct alignas(64) PrefixTable {
-    PrefixMaps maps[kParamGroups];
-    // a CTA's first reads, next to each other: every line of the parameters it touches costs a miss
     uint32_t n_groups, n_sessions;
     uint32_t in_params;
     uint32_t item_begin[kParamGroups];
     PrefixGroup g[kParamGroups];
+    PrefixMaps maps[kParamGroups];
     PrefixSession s[kParamSessions];
 };
 
 // The prefix pass's items for attn_rows_kernel.
 struct PrefixForm {
     static constexpr bool kPartials = true;
-    PrefixTable table;
+    // what every CTA reads first stands first and together: every line of the parameters it touches costs a miss, some 600
+    // clocks each and one after the other
+    uint32_t n_q_heads, n_kv_heads, q_row_stride;
     const PrefixGroup *groups;           // device copies, when !table.in_params
     const PrefixSession *sessions;
     const PrefixMaps *maps;
     float *part_o, *part_m, *part_l;
-    uint32_t n_q_heads, n_kv_heads, q_row_stride;
+    PrefixTable table;
 
     struct Item : RowsItem {
         const CUtensorMap *maps;
@@ -142,11 +144,7 @@ struct PrefixForm {
 };
 
 // ---------------------------------------------------------------------------------------
-// Merge: a warp takes 128 (at head_dim 64: 64) columns of an output row (session, query row, head) and walks the row's
-// partials, the prefix's first, then the session's own, 32 at a time: every lane forms the weight of one partial, and the
-// columns are summed with the weights handed round by shuffles, so that a partial costs a lane one load and four FMAs.
-// (With every thread forming every weight the kernel was bound by instructions: 12.7 us for 1024 rows of 21 partials.)
-// `groups` (a power of two) sets of warps share a row where there are few rows.
+// Merge (attn_merge.cuh): the row's partials of its group's prefix, then the session's own.
 // ---------------------------------------------------------------------------------------
 struct MergeSession {
     void *out;
@@ -162,17 +160,6 @@ struct MergeTable {
     MergeSession s[kParamSessions];
 };
 
-template <int VEC>
-struct Columns { float v[VEC]; };
-__device__ __forceinline__ Columns<4> load_columns(const float *p, Columns<4> *) {
-    const float4 x = *reinterpret_cast<const float4 *>(p);
-    return Columns<4>{{x.x, x.y, x.z, x.w}};
-}
-__device__ __forceinline__ Columns<2> load_columns(const float *p, Columns<2> *) {
-    const float2 x = *reinterpret_cast<const float2 *>(p);
-    return Columns<2>{{x.x, x.y}};
-}
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
 attn_prefix_merge_kernel(const __grid_constant__ MergeTable table, const MergeSession *__restrict__ dev,
@@ -180,16 +167,11 @@ attn_prefix_merge_kernel(const __grid_constant__ MergeTable table, const MergeSe
                          const float *__restrict__ pre_o, const float *__restrict__ pre_m, const float *__restrict__ pre_l,
                          const float *__restrict__ own_o, const float *__restrict__ own_m, const float *__restrict__ own_l,
                          uint32_t n_q_heads, uint32_t out_row_stride, uint32_t n_rows, uint32_t groups) {
-    constexpr int kVec = HD >= 128 ? 4 : 2;
-    constexpr uint32_t kRowWarps = HD / (32 * kVec), kSets = 8 / kRowWarps;
-    using Cols = Columns<kVec>;
-    __shared__ float set_m[8], set_d[8];
-    __shared__ Cols accs[256];
+    using M = RowMerge<HD>;
+    __shared__ typename M::Shared shared;
     pdl_launch_dependents();
-    pdl_wait();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t set = warp / kRowWarps, grp = set & (groups - 1);
-    const uint32_t out_row = blockIdx.x * (kSets / groups) + set / groups, col = (warp % kRowWarps * 32 + lane) * kVec;
+    const uint32_t out_row = M::row(blockIdx.x, warp, groups);
     const bool live = out_row < n_rows;
     const uint32_t qrow = out_row / n_q_heads, head = out_row - qrow * n_q_heads;
     uint32_t lo = 0;
@@ -206,69 +188,14 @@ attn_prefix_merge_kernel(const __grid_constant__ MergeTable table, const MergeSe
     const uint32_t w = table.q_rows != 0 ? qrow - lo * table.q_rows : qrow - first_row[lo];
     const MergeSession ses = table.n != 0 ? table.s[lo] : dev[lo];
 
-    float m_run = -INFINITY, d_run = 0.f;
-    Cols acc;
-#pragma unroll
-    for (int x = 0; x < kVec; ++x) acc.v[x] = 0.f;
-    auto walk = [&](const float *po, const float *pm, const float *pl, size_t base, size_t stride, uint32_t n) {
-        for (uint32_t c0 = grp; c0 < n; c0 += 32 * groups) {
-            const uint32_t count = min(32u, (n - c0 + groups - 1) / groups);       // partials of this round
-            const size_t row0 = base + (size_t)c0 * stride, step = stride * groups;
-            float e = -INFINITY, l = 0.f;
-            if (lane < count) { e = pm[row0 + lane * step]; l = pl[row0 + lane * step]; }
-            float mx = e;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float m_new = fmaxf(m_run, mx);
-            if (m_new == -INFINITY) continue;                          // nothing visible so far: exp(-inf - -inf) would be NaN
-            const float sc = __expf(m_run - m_new), wgt = __expf(e - m_new);
-            float d = l * wgt;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-            d_run = d_run * sc + d;
-            m_run = m_new;
-#pragma unroll
-            for (int x = 0; x < kVec; ++x) acc.v[x] *= sc;
-            const float *p = po + row0 * HD + col;
-#pragma unroll 8
-            for (uint32_t i = 0; i < count; ++i, p += step * HD) {
-                const float wi = __shfl_sync(0xffffffffu, wgt, i);
-                const Cols o = load_columns(p, (Cols *)nullptr);
-#pragma unroll
-                for (int x = 0; x < kVec; ++x) acc.v[x] = fmaf(o.v[x], wi, acc.v[x]);
-            }
-        }
-    };
+    pdl_wait();       // the partials are there
+    M merge(warp, lane, groups);
     if (live) {
-        walk(pre_o, pre_m, pre_l, (size_t)ses.prefix_base + w * n_q_heads + head, ses.prefix_stride, ses.prefix_parts);
-        walk(own_o, own_m, own_l, (size_t)ses.own_base + w * n_q_heads + head, (size_t)ses.q_rows * n_q_heads, ses.own_parts);
+        merge.walk(pre_o, pre_m, pre_l, (size_t)ses.prefix_base + w * n_q_heads + head, ses.prefix_stride, ses.prefix_parts);
+        merge.walk(own_o, own_m, own_l, (size_t)ses.own_base + w * n_q_heads + head, (size_t)ses.q_rows * n_q_heads, ses.own_parts);
     }
-    if (groups > 1) {
-        accs[threadIdx.x] = acc;
-        if (lane == 0) { set_m[warp] = m_run; set_d[warp] = d_run; }
-        __syncthreads();
-        if (grp != 0) return;
-        float mg = m_run;
-        for (uint32_t g = 1; g < groups; ++g) mg = fmaxf(mg, set_m[warp + g * kRowWarps]);
-        if (mg != -INFINITY) {
-            const float sc = __expf(m_run - mg);
-            d_run *= sc;
-#pragma unroll
-            for (int x = 0; x < kVec; ++x) acc.v[x] *= sc;
-            for (uint32_t g = 1; g < groups; ++g) {
-                const float wgt = __expf(set_m[warp + g * kRowWarps] - mg);
-                const Cols o = accs[threadIdx.x + g * kRowWarps * 32];
-#pragma unroll
-                for (int x = 0; x < kVec; ++x) acc.v[x] = fmaf(o.v[x], wgt, acc.v[x]);
-                d_run += set_d[warp + g * kRowWarps] * wgt;
-            }
-        }
-    }
-    if (!live) return;
-    const float inv = d_run > 0.f ? 1.f / d_run : 0.f;    // a row that sees nothing: zeros
-    T *dst = reinterpret_cast<T *>(ses.out) + (size_t)w * out_row_stride + (size_t)head * HD + col;
-#pragma unroll
-    for (int x = 0; x < kVec; x += 2) *reinterpret_cast<uint32_t *>(dst + x) = pack2<T>(acc.v[x] * inv, acc.v[x + 1] * inv);
+    if (!merge.join(shared) || !live) return;
+    merge.template store<T>(reinterpret_cast<T *>(ses.out) + (size_t)w * out_row_stride + (size_t)head * HD);
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
@@ -294,11 +221,8 @@ template <typename T>
 cudaError_t launch_merge(cudaStream_t stream, uint32_t head_dim, uint32_t rows, const MergeTable &table, const MergeSession *dev,
                          const uint32_t *dev_first_row, uint32_t n_sessions, const PrefixForm &kp, const TTDecodeForm &own,
                          uint32_t n_q_heads, uint32_t out_row_stride, uint32_t sm_count) {
-    // sets of warps per row: as many as keep two CTAs an SM busy
-    const uint32_t sets = head_dim == 256 ? 4 : 8;
-    uint32_t groups = 1;
-    while (groups < sets && (uint64_t)rows * groups * 2 <= (uint64_t)sets * 2 * sm_count) groups *= 2;
-    const uint32_t grid = (rows * groups + sets - 1) / sets;
+    uint32_t grid = 0;
+    const uint32_t groups = merge_groups(rows, head_dim, sm_count, &grid);
 #define TT_X(HD) tt_launch_pdl(attn_prefix_merge_kernel<T, HD>, dim3(grid), dim3(256), 0, stream, table, dev, dev_first_row, n_sessions, \
                                kp.part_o, kp.part_m, kp.part_l, own.part_o, own.part_m, own.part_l, n_q_heads, out_row_stride, rows, groups)
     return head_dim == 64 ? TT_X(64) : head_dim == 128 ? TT_X(128) : TT_X(256);

@@ -158,7 +158,8 @@ __device__ __forceinline__ void load_query_rows(const Form &form, const typename
 
 // A Form says what the items are. It provides
 //   struct Item : RowsItem
-//   Item item(block, HD, ROWS)                 from the block index
+//   Item item(block, HD, ROWS)                 from the block index and the parameters (or tables that a copy, not a kernel,
+//                                              brought: it runs ahead of the wait for the kernel before)
 //   const void *query(item, row, HD, ROWS)     start of a row's query (null: no such row)
 //   void acquire(item)                         one thread, before its first load: fences the tensor maps if they need it
 //   const CUtensorMap *box(item, tile, half, is_k, row)   keys 64 half .. of a tile: the map (boxes [64 rows][64]), the row
@@ -187,8 +188,8 @@ attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_launch_dependents();
+    const typename Form::Item item = form.item(blockIdx.x, HD, ROWS);        // from the parameters alone
     pdl_wait();       // the kernel before this one may have produced the query or cache rows
-    const typename Form::Item item = form.item(blockIdx.x, HD, ROWS);
     const uint32_t n_tiles = item.n_tiles;                                   // >= 1
 
     // the producers: block after block of K's (or V's) units, each into its place of the ring once that is free
