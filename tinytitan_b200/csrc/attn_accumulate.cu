@@ -128,16 +128,22 @@ attn_accumulate_kernel(const __grid_constant__ AccTable table, AccParams p) {
         if (lane == 0) norm[r] = l > 0.f ? mx + log2f(l) : INFINITY;      // a row that sees nothing weighs nothing
     }
     __syncthreads();
+    // query row w of q_rows sees keys below seq_len - (q_rows - 1 - w): the first `hidden` packed rows do not see a last key
+    uint32_t hidden[kAccPerThread];
+#pragma unroll
+    for (uint32_t x = 0; x < kAccPerThread; ++x)
+        hidden[x] = key[x] >= seq_len ? 0xffffffffu : key[x] + ses.q_rows > seq_len ? (key[x] + ses.q_rows - seq_len) * group : 0u;
     for (uint32_t r0 = 0; r0 < rows; r0 += 8) {
         if (r0 != 0) load_rows(r0);
 #pragma unroll
-        for (uint32_t x = 0; x < kAccPerThread; ++x) {
-            if (key[x] >= seq_len) continue;
-            // query row w of q_rows sees keys below seq_len - (q_rows - 1 - w): the first rows do not see the last keys
-            const uint32_t hidden = key[x] + ses.q_rows > seq_len ? (key[x] + ses.q_rows - seq_len) * group : 0u;
+        for (uint32_t y = 0; y < 8; ++y) {
+            if (r0 + y >= rows) break;
+            const float n = norm[r0 + y];
 #pragma unroll
-            for (uint32_t y = 0; y < 8; ++y)
-                if (r0 + y < rows && r0 + y >= hidden) sum[x] += exp2f(fmaf(s[x][y], p.scale_log2, -norm[r0 + y]));
+            for (uint32_t x = 0; x < kAccPerThread; ++x) {
+                const float w = fast_exp2(fmaf(s[x][y], p.scale_log2, -n));      // 2^-22 relative
+                sum[x] += r0 + y >= hidden[x] ? w : 0.f;
+            }
         }
     }
 #pragma unroll

@@ -272,8 +272,13 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_full[i & 1]);
+            if (head == 0 && issued < n_blocks) {           // block i + kStages goes into the stage block i just left
+                if (!warp_all(mbar_wait(&k_empty[i % kStages], (i / kStages) & 1))) { timed_out = true; break; }
+                issue(issued, k_ring, kbase, k_full, false);
+                ++issued;
+            }
             if constexpr (FORM == kPassScores) {
-                // 8 keys x 8 rows per store: 256 contiguous bytes of the warp when the row count is padded to 8
+                // behind the refill, which must not wait for them; 8 keys x 8 rows per store: 256 contiguous bytes of the warp when the row count is padded to 8
                 const uint32_t rows_pad = (ses.q_rows * group + 8 * NT - 1) / (8 * NT) * (8 * NT);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -286,11 +291,6 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
                                        s0[nt][2 * h] + s1[nt][2 * h], s0[nt][2 * h + 1] + s1[nt][2 * h + 1]);
                     }
                 }
-            }
-            if (head == 0 && issued < n_blocks) {           // block i + kStages goes into the stage block i just left
-                if (!warp_all(mbar_wait(&k_empty[i % kStages], (i / kStages) & 1))) { timed_out = true; break; }
-                issue(issued, k_ring, kbase, k_full, false);
-                ++issued;
             }
         }
         if (timed_out) {
