@@ -266,6 +266,16 @@ def test_prefix_groups_and_ragged_rows():
     run_prefix(64, 32, 2, F16, [3, 129, 2], [3, 3, 1], rows, lens)
 
 
+@pytest.mark.parametrize("sessions", [1, 5, 16, 17])                    # up to 16 the sessions' own rows are items of the prefix pass
+@pytest.mark.parametrize("hd,hq,hkv", [(64, 8, 2), (128, 4, 1), (256, 8, 2)])
+def test_prefix_long_suffixes(hd, hq, hkv, sessions):
+    # query rows whose last keys lie on both sides of a tile's edge, a last part that only the last rows see, rows without keys
+    rows = ([4, 64, 9, 1, 33] * 4)[:sessions]
+    lens = ([129, 63, 515, 1000, 256, 130, 127, 8, 0, 161, 385, 700, 10, 128, 32, 3, 65, 12, 260, 40])[:sessions]
+    run_prefix(hd, hq, hkv, BF16, [5], [sessions], rows, lens, pad=8)
+    run_prefix(hd, hq, hkv, F16, [0] * (sessions > 1) + [130], [1] * (sessions > 1) + [sessions - (sessions > 1)], rows, lens)
+
+
 def test_prefix_large_tables():
     n = 70
     run_prefix(128, 4, 2, F16, [200], [n], [1] * n, [i % 9 for i in range(n)])

@@ -886,9 +886,7 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     }
     // Verify batches (17..128 packed rows per KV head, head_dim 256, plain 16-bit rows) take the
     // tensor-core pass 1: one item serves all packed rows of a (session, kv head, key range).
-    // (also for the sessions behind a shared prefix, while their tables travel in the parameters: this form uploads maps)
-    const bool wide_form = form == nullptr || (form->partials_only && form->form == kPassPlain && n_sessions <= kVerifyParamSessions);
-    bool wide = !quantised && wide_form && p->head_dim == 256 && getenv("TT_VERIFY_FORCE_MMA_SYNC") == nullptr;
+    bool wide = !quantised && form == nullptr && p->head_dim == 256 && getenv("TT_VERIFY_FORCE_MMA_SYNC") == nullptr;
     bool wide128 = false;       // some session has more than 64 packed rows: the 128-row form of the kernel
     for (uint32_t i = 0; wide && i < n_sessions; ++i) {
         const TTDecodeSession &s = in_sessions[i];
@@ -1001,7 +999,7 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
 
     TTLaunchTimer timer(ctx, stream, TT_PROFILE_DECODE_PARTIAL);
     // a verify batch whose sessions are all one part needs no merge: pass 1 stores the output rows
-    bool direct = wide && mode == 0 && form == nullptr;
+    bool direct = wide && mode == 0;
     for (uint32_t i = 0; direct && i < n_sessions; ++i) direct = ctx->h_sessions[i].n_parts == 1;
     if (wide) {
         const int rc = tt_launch_verify_tc(ctx, stream, n_sessions, n_items, part_o, part_m, part_l, p, direct, in_params, wide128);

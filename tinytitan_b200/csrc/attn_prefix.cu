@@ -9,6 +9,8 @@
 //   suffix pass   the split-KV decode kernel over every session's own rows                            -> (m, l, o) partials
 //   merge         attn_prefix_merge_kernel: log-sum-exp over both kinds of partials of an output row
 //
+// In a batch of up to 16 sessions the suffixes are items of the prefix pass and there is no suffix pass.
+//
 // The prefix pass (attn_rows_tc.cuh) packs row = (query row of the group) * G + g with G query heads per KV head, session
 // after session. Every row of an item sees every key of its range: only the last tile of a prefix is masked. What
 // bounds the pass depends on the rows: with up to about 256 packed rows per KV head the bytes of the prefix, beyond
@@ -19,6 +21,8 @@
 namespace {
 
 constexpr uint32_t kParamGroups = 8;
+constexpr uint32_t kFusedSessions = 16;                            // sessions whose own rows join the prefix pass
+constexpr uint32_t kTableGroups = kParamGroups + kFusedSessions;
 
 // Query rows of one session, in call order.
 struct PrefixSession {
@@ -40,6 +44,8 @@ struct PrefixGroup {
     uint32_t q_rows;
     const void *q;
     long long q_step;
+    uint32_t causal_rows;                // of a session's own rows: its query rows, of which row r sees prefix_len - (rows - 1 - r) keys
+    uint32_t pad;
 };
 struct alignas(64) PrefixMaps { unsigned char m[2][128]; };    // K and V tensor maps of a group
 
@@ -48,9 +54,9 @@ struct alignas(64) PrefixMaps { unsigned char m[2][128]; };    // K and V tensor
 struct alignas(64) PrefixTable {
     uint32_t n_groups, n_sessions;
     uint32_t in_params;
-    uint32_t item_begin[kParamGroups];
-    PrefixGroup g[kParamGroups];
-    PrefixMaps maps[kParamGroups];
+    uint32_t item_begin[kTableGroups];
+    PrefixGroup g[kTableGroups];
+    PrefixMaps maps[kTableGroups];
     PrefixSession s[kParamSessions];
 };
 
@@ -69,6 +75,7 @@ struct PrefixForm {
     struct Item : RowsItem {
         const CUtensorMap *maps;
         uint32_t key_begin, n_keys;
+        uint32_t causal_rows, causal_end;    // PrefixGroup.causal_rows, and the last of those rows' end behind key_begin
         uint32_t row0, n_rows;           // first packed row, packed rows in use
         uint32_t row_begin, session_begin, session_count, q_rows;
         const void *q;
@@ -81,6 +88,11 @@ struct PrefixForm {
 #pragma unroll
             for (uint32_t i = 1; i < kParamGroups; ++i)
                 if (i < hi && table.item_begin[i] <= block) lo = i;
+            if (hi > kParamGroups) {
+#pragma unroll
+                for (uint32_t i = kParamGroups; i < kTableGroups; ++i)
+                    if (i < hi && table.item_begin[i] <= block) lo = i;
+            }
         } else {
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) >> 1;
@@ -96,6 +108,7 @@ struct PrefixForm {
         it.key_begin = min(grp.prefix_len, part * grp.part_len);
         it.n_keys = min(grp.prefix_len, it.key_begin + grp.part_len) - it.key_begin;
         it.n_tiles = (it.n_keys + kBK - 1) / kBK;
+        it.causal_rows = grp.causal_rows; it.causal_end = grp.prefix_len - it.key_begin;
         it.row0 = local % grp.row_tiles * rows;
         it.n_rows = min((uint32_t)rows, grp.n_rows * group - it.row0);
         it.row_begin = grp.row_begin; it.session_begin = grp.session_begin; it.session_count = grp.session_count;
@@ -131,10 +144,17 @@ struct PrefixForm {
         row = (int)(it.key_begin + tile * kBK + half * 64);
         return is_k ? it.maps : it.maps + 1;
     }
-    __device__ __forceinline__ bool masked(const Item &it, uint32_t tile) const { return (tile + 1) * kBK > it.n_keys; }
+    __device__ __forceinline__ bool masked(const Item &it, uint32_t tile) const {
+        return (tile + 1) * kBK > it.n_keys || (it.causal_rows > 1 && (tile + 1) * kBK + it.causal_rows - 1 > it.causal_end);
+    }
     __device__ __forceinline__ void visible(const Item &it, uint32_t row, uint32_t tile, uint32_t &lo, uint32_t &hi) const {
+        uint32_t end = it.n_keys;
+        if (it.causal_rows > 1) {
+            const uint32_t w = min((it.row0 + row) / (n_q_heads / n_kv_heads), it.causal_rows - 1), later = it.causal_rows - 1 - w;
+            end = min(end, it.causal_end > later ? it.causal_end - later : 0u);
+        }
         lo = 0;
-        hi = min((uint32_t)kBK, it.n_keys - tile * kBK);
+        hi = end > tile * kBK ? min((uint32_t)kBK, end - tile * kBK) : 0u;
     }
     __device__ __forceinline__ bool exists(const Item &it, uint32_t r) const { return r < it.n_rows; }
     __device__ __forceinline__ size_t partial(const Item &it, uint32_t r, int rows) const {
@@ -231,10 +251,10 @@ cudaError_t launch_merge(cudaStream_t stream, uint32_t head_dim, uint32_t rows, 
 
 }  // namespace
 
-// The items of all groups are nearly equal slices and one CTA is resident per SM (an item of 256 rows takes two), so a launch takes about
-// waves x (tiles per item + what an item costs besides its tiles), which `kItemTiles` puts at three tiles of streaming.
-// The shortest such time over the part counts of the longest prefix wins; equal times go to the longer item (fewer
-// partials to merge).
+// One CTA is resident per SM (an item of 256 rows takes two), and an item costs about kItemTiles tiles besides its own. The
+// length of the items is the one for which the launch takes the least time: the waves of the full-size items, or all items'
+// tiles over the SMs where shorter ones (short groups, a session's own rows) fill the gaps. Equal times go to the longer
+// items (fewer partials to merge).
 TT_API int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_t *query_rows, uint32_t n_groups, uint32_t head_dim,
                                       uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t sm_count, size_t workspace_bytes,
                                       uint32_t *out_keys_per_item, uint32_t *out_n_items) {
@@ -252,14 +272,19 @@ TT_API int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_
     for (uint32_t parts = 1; parts <= 512 && parts <= max_tiles; ++parts) {
         const uint32_t tiles = ceil_div(max_tiles, parts);
         if (parts > 1 && tiles == ceil_div(max_tiles, parts - 1)) continue;      // the same item length again
-        uint64_t items = 0, prows = 0;
+        uint64_t items = 0, full = 0, cost = 0, prows = 0;
         for (uint32_t g = 0; g < n_groups; ++g) {
-            const uint64_t p = ceil_div(prefix_lens[g], (uint64_t)tiles * kBK);
-            items += p * n_kv_heads * ceil_div((uint64_t)query_rows[g] * group, tile_rows);
+            const uint64_t own_tiles = ceil_div(prefix_lens[g], kBK), p = ceil_div(own_tiles, tiles);
+            if (p == 0) continue;
+            const uint64_t n = p * n_kv_heads * ceil_div((uint64_t)query_rows[g] * group, tile_rows), each = ceil_div(own_tiles, p) + kItemTiles;
+            items += n;
+            cost += n * each;
+            if (2 * each > tiles + kItemTiles) full += n;
             prows += p * query_rows[g] * n_q_heads;
         }
         if (workspace_bytes != 0 && prows * ((uint64_t)head_dim + 2) * sizeof(float) > workspace_bytes) break;    // more parts need more
-        const uint64_t time = (items + slots - 1) / slots * (tiles + kItemTiles);
+        const uint64_t waves = (full + slots - 1) / slots * (tiles + kItemTiles), spread = (cost + slots - 1) / slots;
+        const uint64_t time = waves > spread ? waves : spread;
         if (time < best) { best = time; best_tiles = tiles; best_items = items; }
     }
     if (best_tiles == 0) return TT_ERR_OOM;
@@ -341,69 +366,107 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
         d.n_parts = 0; d.partial_base = 0; d.ring_capacity = 0; d.keep = nullptr; d.row_index = nullptr;
         total_rows += s.q_rows;
     }
-    uint32_t *lens = ctx->h_prefix_lens, *rows = ctx->h_prefix_rows;
+    // A small batch's own rows join the prefix pass as groups of one session each: one launch less, and no second pass
+    // that starts when the first one ends (4 sessions of short keys: 20 -> 13 us, 16 sessions of 4 draft rows: 58 -> 47 us). Larger batches keep the split-KV
+    // pass, which needs no tensor maps: 64 sessions' maps would make the parameters 24 KB.
+    const bool fused = in_params && n_sessions <= kFusedSessions;
+    const uint32_t n_table = fused ? n_groups + n_sessions : n_groups;
+    uint32_t fused_lens[kTableGroups], fused_rows[kTableGroups];
+    uint32_t *lens = fused ? fused_lens : ctx->h_prefix_lens, *rows = fused ? fused_rows : ctx->h_prefix_rows;
     for (uint32_t g = 0, first = 0; g < n_groups; ++g) {
         lens[g] = groups[g].prefix_len;
         rows[g] = 0;
         for (uint32_t i = 0; i < groups[g].n_sessions; ++i) rows[g] += sessions[first + i].q_rows;
         first += groups[g].n_sessions;
     }
+    if (fused) {
+        if (q.io_dtype != TT_F16 && q.io_dtype != TT_BF16) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "io_dtype must be TT_F16 or TT_BF16");
+        if (q.q_row_stride_elements < q.n_q_heads * q.head_dim || q.out_row_stride_elements < q.n_q_heads * q.head_dim)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "a row stride is smaller than its tight width");
+        if (q.q_row_stride_elements % 8 || q.out_row_stride_elements % 4)
+            return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "row strides must keep rows 16-byte aligned");
+        for (uint32_t i = 0; i < n_sessions; ++i) {
+            if (sessions[i].k == nullptr || sessions[i].v == nullptr) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has a null buffer", i);
+            if (((uintptr_t)sessions[i].k | (uintptr_t)sessions[i].v) & 15)
+                return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "session %u: buffers must be 16-byte aligned", i);
+            lens[n_groups + i] = sessions[i].seq_len;
+            rows[n_groups + i] = sessions[i].q_rows;
+        }
+    }
     // ---- plan: the prefix pass may take half of the workspace, at its end ----
     uint32_t keys_per_item = 0, n_items = 0;
     const size_t room = ctx->workspace_bytes / 2;
-    if (tt_attn_plan_prefix_splits(lens, rows, n_groups, q.head_dim, q.n_q_heads, q.n_kv_heads, (uint32_t)ctx->sm_count, room,
+    if (tt_attn_plan_prefix_splits(lens, rows, n_table, q.head_dim, q.n_q_heads, q.n_kv_heads, (uint32_t)ctx->sm_count, room,
                                    &keys_per_item, &n_items) != TT_OK)
         return tt_set_error(ctx, TT_ERR_OOM, "the prefix partials do not fit the context workspace");
-    const uint32_t group = q.n_q_heads / q.n_kv_heads, tile_rows = rows_per_tile(rows, n_groups, group, q.head_dim);
-    uint32_t item = 0, partial = 0, session = 0, row = 0;
-    for (uint32_t g = 0; g < n_groups; ++g) {
+    const uint32_t group = q.n_q_heads / q.n_kv_heads, tile_rows = rows_per_tile(rows, n_table, group, q.head_dim);
+    uint32_t item = 0, partial = 0;
+    // group g of the table: `len` keys at k, v for the query rows of sessions first .. first + count - 1
+    auto add_group = [&](uint32_t g, const void *k, const void *v, uint32_t first, uint32_t count, bool own) {
         PrefixGroup &d = h_groups[g];
         d.prefix_len = lens[g];
         d.n_parts = ceil_div(lens[g], keys_per_item);
         d.part_len = keys_per_item;
-        if (d.n_parts != 0)               // parts of equal length
+        if (d.n_parts != 0) {               // parts of equal length
             d.part_len = ceil_div(ceil_div(lens[g], d.n_parts), kBK) * kBK;
-        if (d.n_parts != 0) d.n_parts = ceil_div(lens[g], d.part_len);
-        d.session_begin = session; d.session_count = groups[g].n_sessions;
-        d.row_begin = row; d.n_rows = rows[g];
+            d.n_parts = ceil_div(lens[g], d.part_len);
+        }
+        d.session_begin = first; d.session_count = count;
+        d.row_begin = h_first[first]; d.n_rows = rows[g];
         d.partial_base = partial; d.item_begin = item;
         if (in_params) table.item_begin[g] = item;
         d.row_tiles = ceil_div((uint64_t)rows[g] * group, tile_rows);
-        d.q = sessions[session].q; d.q_rows = sessions[session].q_rows; d.q_step = 0;
-        if (groups[g].n_sessions > 1) d.q_step = (long long)((uintptr_t)sessions[session + 1].q - (uintptr_t)sessions[session].q);
-        for (uint32_t i = 1; i < groups[g].n_sessions; ++i)
-            if (sessions[session + i].q_rows != d.q_rows ||
-                (long long)((uintptr_t)sessions[session + i].q - (uintptr_t)sessions[session + i - 1].q) != d.q_step) d.q_rows = 0;
-        for (uint32_t i = 0; i < groups[g].n_sessions; ++i) {
-            MergeSession &m = h_merge[session + i];
-            m.prefix_base = partial + (h_first[session + i] - row) * q.n_q_heads;
-            m.prefix_parts = d.n_parts;
-            m.prefix_stride = rows[g] * q.n_q_heads;
+        d.q = sessions[first].q; d.q_rows = sessions[first].q_rows; d.q_step = 0;
+        if (count > 1) d.q_step = (long long)((uintptr_t)sessions[first + 1].q - (uintptr_t)sessions[first].q);
+        for (uint32_t i = 1; i < count; ++i)
+            if (sessions[first + i].q_rows != d.q_rows ||
+                (long long)((uintptr_t)sessions[first + i].q - (uintptr_t)sessions[first + i - 1].q) != d.q_step) d.q_rows = 0;
+        d.causal_rows = own ? rows[g] : 0u;
+        d.pad = 0;
+        for (uint32_t i = 0; i < count; ++i) {
+            MergeSession &m = h_merge[first + i];
+            if (own) {
+                m.own_base = partial;
+                m.own_parts = d.n_parts;
+            } else {
+                m.prefix_base = partial + (h_first[first + i] - d.row_begin) * q.n_q_heads;
+                m.prefix_parts = d.n_parts;
+                m.prefix_stride = rows[g] * q.n_q_heads;
+            }
         }
         item += d.n_parts * q.n_kv_heads * d.row_tiles;
         partial += d.n_parts * rows[g] * q.n_q_heads;
-        session += groups[g].n_sessions;
-        row += rows[g];
-        const uint64_t map_rows = lens[g] ? lens[g] : 1;
-        if (lens[g] != 0 &&
-            !(tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(h_maps[g].m[0]), groups[g].k, q.io_dtype, (uint64_t)q.n_kv_heads * q.head_dim,
-                                    map_rows, q.kv_token_stride_elements, 64) &&
-              tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(h_maps[g].m[1]), groups[g].v, q.io_dtype, (uint64_t)q.n_kv_heads * q.head_dim,
-                                    map_rows, q.kv_token_stride_elements, 64)))
-            return tt_set_error(ctx, TT_ERR_CUDA, "cuTensorMapEncodeTiled failed for group %u", g);
+        const uint64_t width = (uint64_t)q.n_kv_heads * q.head_dim;
+        return lens[g] == 0 ||
+               (tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(h_maps[g].m[0]), k, q.io_dtype, width, lens[g], q.kv_token_stride_elements, 64) &&
+                tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(h_maps[g].m[1]), v, q.io_dtype, width, lens[g], q.kv_token_stride_elements, 64));
+    };
+    bool encoded = true;
+    for (uint32_t g = 0, first = 0; g < n_groups; ++g) {
+        encoded = encoded && add_group(g, groups[g].k, groups[g].v, first, groups[g].n_sessions, false);
+        first += groups[g].n_sessions;
     }
+    for (uint32_t i = 0; fused && i < n_sessions; ++i) encoded = encoded && add_group(n_groups + i, sessions[i].k, sessions[i].v, i, 1, true);
+    if (!encoded) return tt_set_error(ctx, TT_ERR_CUDA, "cuTensorMapEncodeTiled failed for the prefix operands");
     const size_t partial_bytes = ((size_t)partial * (q.head_dim + 2) * sizeof(float) + 255) / 256 * 256;
+    kp.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->partials) + (ctx->workspace_bytes / 256 * 256 - partial_bytes));
+    kp.part_m = kp.part_o + (size_t)partial * q.head_dim;
+    kp.part_l = kp.part_m + partial;
 
     // ---- suffix pass (it also checks the rest of the arguments) ----
     TTDecodeForm own;
-    own.reserved_bytes = partial_bytes + 256;
-    own.partials_only = true;
-    own.short_sessions = true;
-    int rc = tt_launch_decode(ctx, (cudaStream_t)stream, tmp, n_sessions, params, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &own);
-    if (rc != TT_OK) return rc;
-    for (uint32_t i = 0; i < n_sessions; ++i) {
-        h_merge[i].own_base = ctx->h_sessions[i].partial_base;
-        h_merge[i].own_parts = ctx->h_sessions[i].n_parts;
+    if (fused) {
+        own.part_o = kp.part_o; own.part_m = kp.part_m; own.part_l = kp.part_l;
+    } else {
+        own.reserved_bytes = partial_bytes + 256;
+        own.partials_only = true;
+        own.short_sessions = true;
+        const int rc = tt_launch_decode(ctx, (cudaStream_t)stream, tmp, n_sessions, params, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &own);
+        if (rc != TT_OK) return rc;
+        for (uint32_t i = 0; i < n_sessions; ++i) {
+            h_merge[i].own_base = ctx->h_sessions[i].partial_base;
+            h_merge[i].own_parts = ctx->h_sessions[i].n_parts;
+        }
     }
     cudaError_t e = cudaSuccess;
     if (!in_params) {
@@ -414,11 +477,8 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
     kp.maps = reinterpret_cast<const PrefixMaps *>(ctx->prefix_tables);
     kp.groups = reinterpret_cast<const PrefixGroup *>(ctx->prefix_tables + off_groups);
     kp.sessions = reinterpret_cast<const PrefixSession *>(ctx->prefix_tables + off_sessions);
-    kp.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->partials) + (ctx->workspace_bytes / 256 * 256 - partial_bytes));
-    kp.part_m = kp.part_o + (size_t)partial * q.head_dim;
-    kp.part_l = kp.part_m + partial;
     kp.n_q_heads = q.n_q_heads; kp.n_kv_heads = q.n_kv_heads; kp.q_row_stride = q.q_row_stride_elements;
-    table.n_groups = n_groups; table.n_sessions = n_sessions; table.in_params = in_params ? 1u : 0u;
+    table.n_groups = n_table; table.n_sessions = n_sessions; table.in_params = in_params ? 1u : 0u;
     merge.n = in_params ? n_sessions : 0u;
     if (item != 0) {
         const RowsParams rp = tile_rows == 256 ? pair_params(q.scale, q.io_dtype) : rows_params(q.scale, q.io_dtype, q.head_dim);

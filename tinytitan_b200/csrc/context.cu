@@ -132,7 +132,7 @@ TT_API tt_context *tt_context_create(int device, const tt_context_options *optio
     ctx->table_bytes = (sizeof(TTDecodeSession) * ctx->max_sessions + 127) / 128 * 128 + (size_t)256 * ctx->max_sessions +
                        sizeof(TTDecodeItem) * ctx->max_items;
     ok = ok && cudaMalloc(&ctx->tables, ctx->table_bytes) == cudaSuccess;
-    ctx->prefix_table_bytes = (size_t)512 * ctx->max_sessions + 256;   // at most 400 bytes a session (one group each)
+    ctx->prefix_table_bytes = (size_t)512 * ctx->max_sessions + 256;   // at most 408 bytes a session (one group each)
     ok = ok && cudaMalloc(&ctx->prefix_tables, ctx->prefix_table_bytes) == cudaSuccess;
     ok = ok && cudaMalloc(&ctx->gdn_sessions, sizeof(tt_gdn_session) * ctx->max_sessions) == cudaSuccess;
     ok = ok && cudaMalloc(&ctx->status, sizeof(uint32_t)) == cudaSuccess;
