@@ -126,6 +126,20 @@ def test_session_table_addresses():
     assert list(p.records["v"]) == [v[i].data_ptr() for i in range(5)] and list(p.records["prefix_len"]) == [3, 0, 20, 1, 5]
 
 
+@pytest.mark.parametrize("n", [0, 1, 2, 6, 7, 65])
+@pytest.mark.parametrize("kind", [list, tuple, np.array, lambda x: list(np.array(x, dtype=np.int32)), torch.tensor])
+def test_session_table_sizes(n, kind):
+    q, k = torch.zeros(n, 3, 4, 64, dtype=torch.bfloat16), torch.zeros(n + 2, 9, 2, 64, dtype=torch.bfloat16)
+    lens, slots = [i % 10 for i in range(n)], [n + 1 - i for i in range(n)]
+    for t, where in ((tt.SessionTable.over_cache(q, q, k, k, kind(lens)), range(n)),
+                     (tt.SessionTable.over_cache(q, q, k, k, kind(lens), slots=kind(slots)), slots)):
+        assert len(t) == len(t.records) == n and t.longest == max(lens, default=0)
+        for i, r in enumerate(t.records):
+            assert r.tolist() == (q[i].data_ptr(), q[i].data_ptr(), k[where[i]].data_ptr(), k[where[i]].data_ptr(), lens[i], 3, 0, 0)
+    p = tt.PrefixTable.over_cache(k[:n], k[:n], kind(lens), kind([1 + i for i in range(n)]))
+    assert len(p) == n and [r.tolist() for r in p.records] == [(k[i].data_ptr(), k[i].data_ptr(), lens[i], 1 + i) for i in range(n)]
+
+
 def test_wrappers_refuse_before_the_library():
     h = torch.float16
     q, out = torch.zeros(3, 1, 8, 64, dtype=h), torch.zeros(3, 1, 8, 64, dtype=h)

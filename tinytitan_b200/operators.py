@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -167,12 +168,13 @@ def _refuse(message: str):
     raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, message)
 
 
-def _cache_stride(name: str, t) -> int:
-    """Elements between the rows (dimension 1) of a [batch, rows, heads, head_dim] tensor with tight rows."""
+def _cache_place(name: str, t):
+    """Of a 16-bit [batch, rows, heads, head_dim] tensor with tight rows: elements between the rows, and
+    (address, bytes between the batch entries)."""
     stride = t.stride()
     if len(stride) != 4 or stride[3] != 1 or stride[2] != t.shape[3]:
         _refuse(f"{name} must be [batch, rows, heads, head_dim] with tight rows")
-    return stride[1]
+    return stride[1], (t.data_ptr(), 2 * stride[0])
 
 
 def _half_dtype(what: str, first, *others) -> int:
@@ -202,14 +204,22 @@ def _counts(name: str, values, n: int) -> list:
     return values
 
 
-def _block(n: int, places, lows, highs, spare=0, indices=None):
+def _block(n: int, places, lows, highs, spare=0, indices=None) -> array:
     """n records of 64-bit words as the C structures lay them out: for every (address, step) of `places` address + i * step (or
     + indices[i] * step), one word of two 32-bit numbers, `spare` zero words."""
+    if n <= 6:          # numpy's fixed costs are those of six records: 7 us
+        flat, rest = [], [0] * spare
+        for i in range(n):
+            if indices is None:
+                flat += [address + i * step for address, step in places]
+            else:
+                flat += [p[0] + int(i if which is None else which[i]) * p[1] for p, which in zip(places, indices)]
+            flat.append(int(lows[i]) | int(highs if isinstance(highs, int) else highs[i]) << 32)
+            flat += rest
+        return array("Q", flat)
     width = len(places)
-    if n == 1 and indices is None:      # one session: cheaper without numpy's fixed costs
-        high = highs if isinstance(highs, int) else highs[0]
-        return np.array([[p[0] for p in places] + [lows[0] | high << 32] + [0] * spare], dtype=np.uint64)
-    words = np.empty((n, width + 1 + spare), dtype=np.uint64)
+    block = array("Q", bytes(8 * n * (width + 1 + spare)))
+    words = np.frombuffer(block, dtype=np.uint64).reshape(n, -1)
     base, step = [p[0] for p in places], [p[1] for p in places]
     i = _numbers(n)
     if indices is None:
@@ -221,9 +231,7 @@ def _block(n: int, places, lows, highs, spare=0, indices=None):
     halves = words.view(np.uint32)
     halves[:, 2 * width] = np.array(lows, dtype=np.uint32)
     halves[:, 2 * width + 1] = highs if isinstance(highs, int) else np.array(highs, dtype=np.uint32)
-    if spare:
-        words[:, width + 1:] = 0
-    return words
+    return block
 
 
 _number_column = np.arange(64, dtype=np.uint64)[:, None]
@@ -237,13 +245,8 @@ def _numbers(n: int):
     return _number_column[:n]
 
 
-def _halves_place(t):
-    """(address, bytes between the batch entries) of a 16-bit tensor."""
-    return t.data_ptr(), 2 * t.stride()[0]
-
-
-def _pointer(words) -> int:
-    return words.__array_interface__["data"][0]
+def _pointer(words: array) -> int:
+    return words.buffer_info()[0]
 
 
 class SessionTable:
@@ -260,28 +263,29 @@ class SessionTable:
         self.io_dtype, self.capacity, self.device = io_dtype, capacity, device
 
     def __len__(self):
-        return len(self.words)
+        return len(self.words) // 6
 
     def get_device(self):
         return self.device
 
     @property
     def records(self):
-        return self.words.view(self.record)[:, 0]
+        return np.frombuffer(self.words, dtype=self.record)
 
     @property
     def pointer(self) -> int:
-        return _pointer(self.words)
+        return self.words.buffer_info()[0]
 
     @classmethod
     def over_cache(cls, q, out, k, v, seq_lens, slots=None) -> "SessionTable":
         """q, out: [n, q_rows, n_q_heads, head_dim]; k, v: [slots, capacity, n_kv_heads, head_dim], session i in
         slot i or slots[i]; seq_lens[i] keys are visible to the last of its rows."""
         io_dtype = _half_dtype("q, out, k and v", q, out, k, v)
-        q_stride, out_stride, kv_stride = _cache_stride("q", q), _cache_stride("out", out), _cache_stride("k", k)
+        (q_stride, at_q), (out_stride, at_out) = _cache_place("q", q), _cache_place("out", out)
+        (kv_stride, at_k), (v_stride, at_v) = _cache_place("k", k), _cache_place("v", v)
         q_shape, k_shape = q.shape, k.shape
         n, q_rows = q_shape[0], q_shape[1]
-        if out.shape != q_shape or v.shape != k_shape or _cache_stride("v", v) != kv_stride:
+        if out.shape != q_shape or v.shape != k_shape or v_stride != kv_stride:
             _refuse("out must be shaped like q, and v laid out like k")
         if slots is None:
             if k_shape[0] < n:
@@ -289,16 +293,15 @@ class SessionTable:
         elif len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k_shape[0])):
             _refuse(f"slots must name {n} of the cache's {k_shape[0]} slots")
         lens = _counts("seq_lens", seq_lens, n)
-        words = _block(n, (_halves_place(q), _halves_place(out), _halves_place(k), _halves_place(v)), lens, q_rows, 1,
-                       None if slots is None else (None, None, slots, slots))
+        words = _block(n, (at_q, at_out, at_k, at_v), lens, q_rows, 1, None if slots is None else (None, None, slots, slots))
         return cls(words, max(lens, default=0), kv_stride, q_stride, out_stride, io_dtype, k_shape[1], k.get_device())
 
     @classmethod
     def of(cls, sessions) -> "SessionTable":
         if isinstance(sessions, cls):
             return sessions
-        words = np.zeros((len(sessions), 6), dtype=np.uint64)
-        r = words.view(cls.record)[:, 0]
+        words = array("Q", bytes(48 * len(sessions)))
+        r = np.frombuffer(words, dtype=cls.record)
         for i, s in enumerate(sessions):
             r[i] = (_addr(s.q, s.q_offset), _addr(s.out, s.out_offset), _addr(s.k, s.k_offset), _addr(s.v, s.v_offset),
                     s.seq_len, s.q_rows, s.kv_start, 0)
@@ -332,37 +335,38 @@ class PrefixTable:
         self.words, self.device = words, device
 
     def __len__(self):
-        return len(self.words)
+        return len(self.words) // 3
 
     def get_device(self):
         return self.device
 
     @property
     def records(self):
-        return self.words.view(self.record)[:, 0]
+        return np.frombuffer(self.words, dtype=self.record)
 
     @property
     def pointer(self) -> int:
-        return _pointer(self.words)
+        return self.words.buffer_info()[0]
 
     @classmethod
     def over_cache(cls, k, v, prefix_lens, n_sessions) -> "PrefixTable":
         """k, v: [groups, capacity, n_kv_heads, head_dim]; n_sessions: per group, or one number for all."""
         _half_dtype("k and v", k, v)
-        if v.shape != k.shape or _cache_stride("v", v) != _cache_stride("k", k):
+        (stride, at_k), (v_stride, at_v), shape = _cache_place("k", k), _cache_place("v", v), k.shape
+        if v.shape != shape or v_stride != stride:
             _refuse("v must be laid out like k")
-        g = k.shape[0]
+        g = shape[0]
         lens, counts = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
-        if max(lens, default=0) > k.shape[1]:
-            _refuse(f"a prefix is longer than the {k.shape[1]} rows of its slot")
-        return cls(_block(g, (_halves_place(k), _halves_place(v)), lens, counts), k.get_device())
+        if max(lens, default=0) > shape[1]:
+            _refuse(f"a prefix is longer than the {shape[1]} rows of its slot")
+        return cls(_block(g, (at_k, at_v), lens, counts), k.get_device())
 
     @classmethod
     def of(cls, groups) -> "PrefixTable":
         if isinstance(groups, cls):
             return groups
-        words = np.zeros((len(groups), 3), dtype=np.uint64)
-        r = words.view(cls.record)[:, 0]
+        words = array("Q", bytes(24 * len(groups)))
+        r = np.frombuffer(words, dtype=cls.record)
         for i, g in enumerate(groups):
             r[i] = (_addr(g.k, g.k_offset), _addr(g.v, g.v_offset), g.prefix_len, g.n_sessions)
         return cls(words)
@@ -657,9 +661,8 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
     session i has min(rows[i], budget) rows per head."""
     _half_dtype("K and V", k, v)
     context.check_device(k)
-    in_stride = _cache_stride("k", k)
-    shape = k.shape
-    if v.shape != shape or _cache_stride("v", v) != in_stride:
+    (in_stride, from_k), (v_stride, from_v), shape = _cache_place("k", k), _cache_place("v", v), k.shape
+    if v.shape != shape or v_stride != in_stride:
         _refuse("v must be laid out like k")
     n, capacity, num_kv_heads, head_dim = shape
     used = _counts("rows", rows, n)
@@ -673,14 +676,14 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
         if t is None:
             continue
         _half_dtype("K and V", k, t)
-        stride, s = _cache_stride(name, t), t.shape
+        (stride, at), s = _cache_place(name, t), t.shape
         if s[0] < n or s[1] < kept or s[2] != num_kv_heads or s[3] != head_dim or (t is v_out and k_out is not None and stride != out_stride):
             _refuse(f"{name} must hold the kept rows of {n} sessions, and v_out be laid out like k_out")
         out_stride = stride
         if t is k_out:
-            at_k = _halves_place(t)
+            at_k = at
         if t is v_out:
-            at_v = _halves_place(t)
+            at_v = at
     # the statistic and the positions, then where they go
     stat, at_w = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context)
     at_p, at_wo, at_po, stat_out = _nowhere, _nowhere, _nowhere, None
@@ -700,7 +703,7 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
             _refuse(f"positions_out must hold {kept} rows and be laid out like weights_out")
         stat_out = stride
     ends = used if end_positions is None else _counts("end_positions", end_positions, n)
-    words = _block(n, (_halves_place(k), _halves_place(v), at_k, at_v, at_w, at_wo, at_p, at_po), used, ends)  # tt_kv_evict_session
+    words = _block(n, (from_k, from_v, at_k, at_v, at_w, at_wo, at_p, at_po), used, ends)  # tt_kv_evict_session
     p = L.KVEvictParams(head_dim, num_kv_heads, budget, sink_tokens, recent_tokens, in_stride, out_stride, stat, stat_out or stat, 0)
     context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), _pointer(words), n, C.byref(p)))
 
