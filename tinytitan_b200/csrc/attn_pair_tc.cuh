@@ -194,6 +194,7 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
                 if (is_k) map = form.box(item, j, rank, true, row);
 #pragma unroll 1
                 for (half = 0; half < 2; ++half) {
+                    if (!is_k && half == 1 && 2 * j + 1 >= item.n_halves) break;     // every key of it is hidden
                     if (!is_k) map = form.box(item, j, half, false, row);
                     const uint32_t slot = ring0 + pos.slot;
                     if (pos.lap > 0) ok = mbar_wait(&sh->empty[slot], (pos.lap - 1) & 1);
@@ -254,16 +255,18 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
             RingPos<kPairRing> pos(0);
             bool ok = true;
             for (uint32_t j = 0; ok && j < n_tiles; ++j) {
+                const uint32_t halves = 2 * j + 1 < item.n_halves ? 2 : 1;       // 1: the last tile's second half is hidden from all rows
                 const uint32_t slot0 = kPairRing + pos.slot, lap0 = pos.lap;
                 pos.advance(1);
                 const uint32_t slot1 = kPairRing + pos.slot, lap1 = pos.lap;
                 pos.advance(1);
-                ok = mbar_wait(&sh->full[slot0], lap0 & 1) && mbar_wait(&sh->full[slot1], lap1 & 1);
+                ok = mbar_wait(&sh->full[slot0], lap0 & 1) && (halves == 1 || mbar_wait(&sh->full[slot1], lap1 & 1));
                 if (ok) ok = mbar_poll(&sh->p_ready[j & 1], (j >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
+                    if (half == halves) break;
                     const uint32_t slot = half ? slot1 : slot0;
                     // P: K-major, sub-tile `half` = keys 64 half .., 16 keys (32 B) per step. V: MN-major, 64-wide
                     // head-dim atoms 8 KB apart (LBO), 8-key groups 1024 B apart (SBO), 16 keys (2048 B) per step
@@ -318,14 +321,14 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_even(&sh->s_read);        // the score tile may take the next product
-            uint32_t lo = 0, hi = kBK;
-            if (form.masked(item, j)) form.visible(item, my_row0 + row, j, lo, hi);
-            if (__any_sync(0xffffffffu, lo > 0 || hi < (uint32_t)kBK)) {      // hidden keys become -inf before the (positive) scale
+            uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (form.masked(item, j)) form.visible(item, my_row0 + row, j, bits);
+            if (__any_sync(0xffffffffu, (bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu)) {      // hidden keys become -inf before the (positive) scale
 #pragma unroll
                 for (int c4 = 0; c4 < 4; ++c4)
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
-                        if ((uint32_t)(c4 * 32 + c) < lo || (uint32_t)(c4 * 32 + c) >= hi) raw[c4][c] = 0xff800000u;
+                        if (!(bits[c4] >> c & 1)) raw[c4][c] = 0xff800000u;
             }
             float mx4[4];
 #pragma unroll
@@ -460,7 +463,7 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
             constexpr uint32_t kRowBytes = Form::kPartials ? HD * 4 : HD * 2;
             for (uint32_t i = 0; i < 16; ++i) {
                 const uint32_t r = quarter * 32 + wg * 16 + i;
-                if (!form.exists(item, my_row0 + r)) break;
+                if (!form.exists(item, my_row0 + r)) continue;
                 unsigned char *dst;
                 if constexpr (Form::kPartials) dst = reinterpret_cast<unsigned char *>(form.part_o + form.partial(item, my_row0 + r, ROWS) * HD);
                 else dst = reinterpret_cast<unsigned char *>(form.output(item, my_row0 + r, HD));

@@ -108,6 +108,7 @@ struct PrefixForm {
         it.key_begin = min(grp.prefix_len, part * grp.part_len);
         it.n_keys = min(grp.prefix_len, it.key_begin + grp.part_len) - it.key_begin;
         it.n_tiles = (it.n_keys + kBK - 1) / kBK;
+        it.n_halves = (it.n_keys + 63) / 64;
         it.causal_rows = grp.causal_rows; it.causal_end = grp.prefix_len - it.key_begin;
         it.row0 = local % grp.row_tiles * rows;
         it.n_rows = min((uint32_t)rows, grp.n_rows * group - it.row0);
@@ -147,14 +148,14 @@ struct PrefixForm {
     __device__ __forceinline__ bool masked(const Item &it, uint32_t tile) const {
         return (tile + 1) * kBK > it.n_keys || (it.causal_rows > 1 && (tile + 1) * kBK + it.causal_rows - 1 > it.causal_end);
     }
-    __device__ __forceinline__ void visible(const Item &it, uint32_t row, uint32_t tile, uint32_t &lo, uint32_t &hi) const {
+    __device__ __forceinline__ void visible(const Item &it, uint32_t row, uint32_t tile, uint32_t (&bits)[4]) const {
         uint32_t end = it.n_keys;
         if (it.causal_rows > 1) {
             const uint32_t w = min((it.row0 + row) / (n_q_heads / n_kv_heads), it.causal_rows - 1), later = it.causal_rows - 1 - w;
             end = min(end, it.causal_end > later ? it.causal_end - later : 0u);
         }
-        lo = 0;
-        hi = end > tile * kBK ? min((uint32_t)kBK, end - tile * kBK) : 0u;
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) bits[c4] = bits_between(0, (int)end - (int)(tile * kBK) - c4 * 32);
     }
     __device__ __forceinline__ bool exists(const Item &it, uint32_t r) const { return r < it.n_rows; }
     __device__ __forceinline__ size_t partial(const Item &it, uint32_t r, int rows) const {

@@ -98,7 +98,15 @@ static_assert(rows_smem_bytes<256, 128>() <= 232448 && rows_smem_bytes<256, 64>(
 // What an item is, the same for every form.
 struct RowsItem {
     uint32_t kv_head, n_tiles;
+    uint32_t n_halves;                   // halves of 64 keys in use: the last tile may have one
 };
+
+// bits lo .. hi-1 of a word's 32, for any lo and hi
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+    const uint32_t below_hi = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u;
+    const uint32_t below_lo = lo >= 32 ? 0xffffffffu : lo <= 0 ? 0u : (1u << lo) - 1u;
+    return below_hi & ~below_lo;
+}
 
 struct RowsParams {
     float scale_log2;
@@ -164,7 +172,7 @@ __device__ __forceinline__ void load_query_rows(const Form &form, const typename
 //   void acquire(item)                         one thread, before its first load: fences the tensor maps if they need it
 //   const CUtensorMap *box(item, tile, half, is_k, row)   keys 64 half .. of a tile: the map (boxes [64 rows][64]), the row
 //   bool masked(item, tile)                    whether some row of the item does not see all 128 keys of the tile
-//   void visible(item, row, tile, lo, hi)      keys [lo, hi) of the tile are visible to the row
+//   void visible(item, row, tile, bits)        bit c % 32 of bits[c / 32]: key c of the tile is visible to the row
 //   bool exists(item, row)
 //   kPartials                                  true: (m, l, o) partial rows; false: normalised rows of T
 //   partial(item, row, HD) / output(item, row, HD)     partial row number / where the row goes
@@ -340,14 +348,14 @@ attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
 #pragma unroll
             for (int c4 = 0; c4 < 4; ++c4) tmem_ld32(s_addr + c4 * 32, raw[c4]);
             tmem_wait_ld();
-            uint32_t lo = 0, hi = kBK;
-            if (form.masked(item, j)) form.visible(item, row, j, lo, hi);
-            if (__any_sync(0xffffffffu, lo > 0 || hi < (uint32_t)kBK)) {      // hidden keys become -inf before the (positive) scale
+            uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (form.masked(item, j)) form.visible(item, row, j, bits);
+            if (__any_sync(0xffffffffu, (bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu)) {      // hidden keys become -inf before the (positive) scale
 #pragma unroll
                 for (int c4 = 0; c4 < 4; ++c4)
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
-                        if ((uint32_t)(c4 * 32 + c) < lo || (uint32_t)(c4 * 32 + c) >= hi) raw[c4][c] = 0xff800000u;
+                        if (!(bits[c4] >> c & 1)) raw[c4][c] = 0xff800000u;
             }
             float mx4[4];
 #pragma unroll
