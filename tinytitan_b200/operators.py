@@ -105,8 +105,13 @@ class Context:
         """The stream handle of a call: `command_buffer`, else torch's current stream of THIS context's device."""
         if command_buffer is not None:
             return int(getattr(command_buffer, "cuda_stream", command_buffer))
+        raw = self.__dict__.get("_raw_stream")      # the handle without a Stream object: 0.2 us instead of 1.4
+        if raw is not None:
+            return raw(self.device)
         import torch
-        return torch.cuda.current_stream(self.device).cuda_stream
+        now = torch.cuda.current_stream(self.device).cuda_stream
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return now
 
     def check_device(self, *holders):
         """Refuses tensors (or tables over tensors) that are not on this context's device. Raw addresses pass."""
