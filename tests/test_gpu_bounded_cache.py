@@ -98,16 +98,30 @@ def test_sink_decode_many_sessions_uses_the_uploaded_tables():
 
 
 def test_sink_decode_window_covering_everything_is_plain_decode():
-    # the same keys in the same order through the same arithmetic: bit for bit
+    # too many keys for clusters of parts: the same keys in the same order through the same arithmetic, bit for bit
     n, hq, hkv, hd = 3, 16, 2, 256
-    q, k, v = (normal(i, *s).cuda() for i, s in enumerate([(n, 1, hq, hd), (n, 700, hkv, hd), (n, 700, hkv, hd)]))
+    q, k, v = (normal(i, *s).cuda() for i, s in enumerate([(n, 1, hq, hd), (n, 1700, hkv, hd), (n, 1700, hkv, hd)]))
     a = tt.Attention(context())
     outs = [torch.empty_like(q) for _ in range(2)]
-    t = [tt.SessionTable.over_cache(q, o, k, v, [700, 256, 3]) for o in outs]
-    a.encode_sink_window(t[0], hd, hq, hkv, 0, 700)
-    a.encode_batched([tt.DecodeSession(q[i], outs[1][i], k[i], v[i], s) for i, s in enumerate([700, 256, 3])], hd, hq, hkv)
+    t = [tt.SessionTable.over_cache(q, o, k, v, [1700, 256, 3]) for o in outs]
+    a.encode_sink_window(t[0], hd, hq, hkv, 0, 1700)
+    a.encode_batched([tt.DecodeSession(q[i], outs[1][i], k[i], v[i], s) for i, s in enumerate([1700, 256, 3])], hd, hq, hkv)
     done()
     assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("longest", [1, 16, 17, 33, 65, 129, 257, 1000, 1024])       # clusters of 1 .. 16 CTAs, down to parts without keys
+@pytest.mark.parametrize("hd,hq,hkv,rows", [(64, 8, 2, 1), (128, 5, 5, 1), (256, 8, 2, 1), (256, 16, 2, 3), (128, 24, 3, 2), (64, 40, 1, 1)])
+def test_sink_decode_clusters(hd, hq, hkv, rows, longest):
+    least = rows - 1
+    lens = [max(least, x) for x in (longest, least, longest // 3, min(longest, 20))]
+    run_sink_decode(hd, hq, hkv, F16 if longest % 2 else BF16, rows, lens, 2, max(1, longest - 2), 0)
+    run_sink_decode(hd, hq, hkv, BF16, rows, [x * 5 for x in lens], 3, max(1, longest - 3), longest + 40)
+
+
+@pytest.mark.parametrize("hd,hq,hkv,n,rows,longest", [(64, 8, 8, 64, 1, 300), (256, 8, 2, 64, 1, 270), (128, 4, 1, 64, 1, 1100), (64, 16, 2, 64, 4, 300)])
+def test_sink_decode_clusters_that_fill_the_machine(hd, hq, hkv, n, rows, longest):
+    run_sink_decode(hd, hq, hkv, F16, rows, [longest + i % 7 for i in range(n)], 1, longest + 3, 0)
 
 
 def test_sink_decode_refusals():

@@ -884,6 +884,11 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
         if (form != nullptr && form->form == kPassSink) keys[i] += s.seq_len < form->sink ? s.seq_len : form->sink;
         rows[i] = s.q_rows;
     }
+    if (form != nullptr && form->form == kPassSink) {
+        bool taken = false;
+        const int rc = tt_launch_sink_cluster(ctx, stream, in_sessions, keys, n_sessions, *form, p, tt_decode_heads_per_cta(p->n_kv_heads, false), &taken);
+        if (rc != TT_OK || taken) return rc;
+    }
     // Verify batches (17..128 packed rows per KV head, head_dim 256, plain 16-bit rows) take the
     // tensor-core pass 1: one item serves all packed rows of a (session, kv head, key range).
     bool wide = !quantised && form == nullptr && p->head_dim == 256 && getenv("TT_VERIFY_FORCE_MMA_SYNC") == nullptr;

@@ -78,11 +78,20 @@ struct DecodeSmem {
 //   kPassScores  besides the partials, the raw scores q.k go to ses.scores[kv head][key][packed row] and
 //                each row's (max, sum) of the item in log2 units with UNROUNDED weights to part_m2 / part_l2,
 //                from which the weights of the whole softmax are formed once every part is done.
-enum : int { kPassPlain = 0, kPassSink = 1, kPassScores = 2 };
+//   kPassSinkCluster   kPassSink whose parts of a (session, KV heads, row tile) are the CTAs of one cluster: they
+//                leave (m, l, O) in their shared memory, and each forms a slice of the output columns from all
+//                of them. No partials, no second launch.
+enum : int { kPassPlain = 0, kPassSink = 1, kPassScores = 2, kPassSinkCluster = 3 };
+constexpr uint32_t kMaxSinkCluster = 16;
 template <int FORM>
 struct PassExtra {};
 template <>
 struct PassExtra<kPassSink> { uint32_t sink, window; };
+template <>
+struct PassExtra<kPassSinkCluster> {
+    uint32_t sink, window, cluster, out_row_stride;
+    int *resident;               // host: launch nothing, store how many clusters run at once
+};
 template <>
 struct PassExtra<kPassScores> { float *part_m2, *part_l2; };
 
@@ -119,6 +128,7 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
                            const __grid_constant__ TTSessionTable table, uint32_t table_keys_per_item,
                            PassExtra<FORM> extra) {
     using S = DecodeSmem<HD, HPC>;
+    constexpr bool SINK = FORM == kPassSink || FORM == kPassSinkCluster;
     constexpr int KS = HD / 16;         // k-steps of K.Q^T and m-tiles of V^T.P^T
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -144,13 +154,20 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
         const uint32_t local = blockIdx.x - table.item_prefix[lo];
         const uint32_t packed_rows = ses.q_rows * group;
         const uint32_t row_tiles = (packed_rows + 15) / 16;
-        const uint32_t rt = local % row_tiles, kvg = (local / row_tiles) % n_kv_groups;
-        const uint32_t part = local / (row_tiles * n_kv_groups);
+        uint32_t unit = local, part = 0;
+        if constexpr (FORM == kPassSinkCluster) { part = local % extra.cluster; unit = local / extra.cluster; }
+        const uint32_t rt = unit % row_tiles, kvg = (unit / row_tiles) % n_kv_groups;
+        if constexpr (FORM != kPassSinkCluster) part = local / (row_tiles * n_kv_groups);
         item.session = lo; item.kv_head = kvg * HPC; item.part_index = part; item.partial_base = ses.partial_base;
-        if constexpr (FORM == kPassSink) {
+        if constexpr (SINK) {
             const uint32_t visible = min(extra.sink, ses.seq_len) + (ses.seq_len > ses.kv_start ? ses.seq_len - ses.kv_start : 0u);
-            item.key_begin = min(visible, part * table_keys_per_item);
-            item.key_end = min(visible, item.key_begin + table_keys_per_item);
+            uint32_t keys = table_keys_per_item;
+            if constexpr (FORM == kPassSinkCluster) {      // a cluster's own keys, in whole blocks
+                keys = (visible + extra.cluster - 1) / extra.cluster;
+                keys = (keys + kKeysPerBlock - 1) / kKeysPerBlock * kKeysPerBlock;
+            }
+            item.key_begin = min(visible, part * keys);
+            item.key_end = min(visible, item.key_begin + keys);
         } else {
             item.key_begin = min(ses.seq_len, ses.kv_start + part * table_keys_per_item);
             item.key_end = min(ses.seq_len, item.key_begin + table_keys_per_item);
@@ -193,7 +210,7 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
             unsigned char *dst = ring + stage * S::kTileBytes + lane * S::kRowBytes;
             if ((uint32_t)lane < valid) {
                 uint32_t p = item.key_begin + i * kKeysPerBlock + lane;
-                if constexpr (FORM == kPassSink) {
+                if constexpr (SINK) {
                     if (p >= extra.sink) {
                         p = ses.kv_start + (p - extra.sink);
                         if (ses.ring_capacity) p = extra.sink + (p - extra.sink) % ses.ring_capacity;
@@ -342,7 +359,7 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
         // ---- mask + online softmax of row 8 nt + g over this lane's four keys ----
         const uint32_t blk_key0 = item.key_begin + i * kKeysPerBlock;
         bool plain = blk_key0 + kKeysPerBlock <= item.key_end;
-        if constexpr (FORM == kPassSink)
+        if constexpr (SINK)
             plain = plain && ses.q_rows == 1;        // one row: the union of the windows is its window
         else
             plain = plain && blk_key0 + kKeysPerBlock <= limit_min && (FORM != kPassPlain || ses.keep == nullptr);
@@ -357,7 +374,7 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
                 if (!plain) {
                     const uint32_t key = blk_key0 + 2 * t + (j >> 1) * 8 + (j & 1);
                     bool ok = key < item.key_end;
-                    if constexpr (FORM == kPassSink) {
+                    if constexpr (SINK) {
                         const uint32_t at = key < extra.sink ? key : ses.kv_start + (key - extra.sink);
                         ok = ok && at < limit[nt] && (at < extra.sink || at + extra.window >= limit[nt]);
                     } else {
@@ -428,6 +445,72 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
         if (lane == 0) atomicOr(status, TT_DEV_WAIT_TIMEOUT);
     }
 
+    if constexpr (FORM == kPassSinkCluster) {
+        // ---- (m, l, O) of this part in shared memory, then the cluster's parts of this CTA's columns ----
+        constexpr uint32_t kRows = 8 * NT, kPitch = HD + 4;                    // floats per row
+        static_assert((HPC * kRows * (kPitch + 2)) * 4 <= S::kRingBytes, "the parts must fit the rings");
+        float *mine_o = reinterpret_cast<float *>(smem), *mine_m = mine_o + HPC * kRows * kPitch, *mine_l = mine_m + HPC * kRows;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * HPC) : "memory");            // no P.V warp, hence no K.Q^T warp, reads the rings any more
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float l = l_run[nt];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (t == 0) { mine_m[head * kRows + nt * 8 + g] = m_run[nt]; mine_l[head * kRows + nt * 8 + g] = l; }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float *dst = mine_o + (head * kRows + nt * 8 + 2 * t + h) * kPitch + g;
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) { dst[mt * 16] = acc[nt][mt][h]; dst[mt * 16 + 8] = acc[nt][mt][2 + h]; }
+            }
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+        uint32_t rank;
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        const uint32_t vecs = HD / 4 / extra.cluster, tasks = HPC * item.row_count * vecs;
+        const uint32_t o_addr = smem_u32(mine_o), m_addr = smem_u32(mine_m), l_addr = smem_u32(mine_l);
+        for (uint32_t task = threadIdx.x - 32 * HPC; task < tasks; task += 32 * HPC) {
+            const uint32_t row = task / vecs, col = (rank * vecs + task % vecs) * 4;
+            const uint32_t hh = row / item.row_count, r = row % item.row_count, at = hh * kRows + r;
+            float m[kMaxSinkCluster], l[kMaxSinkCluster];
+            float4 o[kMaxSinkCluster];
+#pragma unroll
+            for (uint32_t i = 0; i < kMaxSinkCluster; ++i) {
+                m[i] = -INFINITY; l[i] = 0.f; o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i >= extra.cluster) continue;
+                uint32_t a;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(m_addr + at * 4), "r"(i));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m[i]) : "r"(a) : "memory");
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(l_addr + at * 4), "r"(i));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l[i]) : "r"(a) : "memory");
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(o_addr + (at * kPitch + col) * 4), "r"(i));
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[i].x), "=f"(o[i].y), "=f"(o[i].z), "=f"(o[i].w) : "r"(a) : "memory");
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (uint32_t i = 0; i < kMaxSinkCluster; ++i) mx = fmaxf(mx, m[i]);
+            const float m_use = mx == -INFINITY ? 0.f : mx;                    // a row that sees nothing: all weights 0
+            float d = 0.f;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (uint32_t i = 0; i < kMaxSinkCluster; ++i) {
+                const float w = fast_exp2(m[i] - m_use);
+                d = fmaf(l[i], w, d);
+                sum.x = fmaf(o[i].x, w, sum.x); sum.y = fmaf(o[i].y, w, sum.y);
+                sum.z = fmaf(o[i].z, w, sum.z); sum.w = fmaf(o[i].w, w, sum.w);
+            }
+            const float inv = d > 0.f ? 1.f / d : 0.f;
+            const uint32_t packed = item.row_begin + r;
+            T *dst = reinterpret_cast<T *>(ses.out) + (size_t)(packed / group) * extra.out_row_stride +
+                     (size_t)((item.kv_head + hh) * group + packed % group) * HD + col;
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(sum.x * inv, sum.y * inv), pack2<T>(sum.z * inv, sum.w * inv));
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");      // this CTA's part has been read
+        return;
+    }
+
     // ---- write the partial: (m, l) of row 8 nt + g by the quad's first lane, O^T by everyone ----
     const uint32_t rows_total = ses.q_rows * n_q_heads;
     auto partial_row = [&](uint32_t r) {
@@ -478,6 +561,24 @@ cudaError_t launch_partial_nt(cudaStream_t stream, uint32_t n_items, const TTDec
     const int smem = DecodeSmem<HD, HPC>::kTotal;
     cudaError_t e = tt_set_smem_once(kernel, smem);
     if (e != cudaSuccess) return e;
+    if constexpr (FORM == kPassSinkCluster) {
+        if (extra.cluster > 8) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) return e;
+        }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(n_items); cfg.blockDim = dim3(64 * HPC); cfg.dynamicSmemBytes = (size_t)smem; cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = extra.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = tt_pdl_enabled() ? 2 : 1;
+        if (extra.resident != nullptr) return cudaOccupancyMaxActiveClusters(extra.resident, kernel, &cfg);
+        return cudaLaunchKernelEx(&cfg, kernel, items, sessions, part_o, part_m, part_l, p->n_q_heads, p->n_kv_heads,
+                                  p->kv_token_stride_elements * 2u, p->q_row_stride_elements, p->scale * kLog2e, status, table, table_keys, extra);
+    }
     return tt_launch_pdl(kernel, dim3(n_items), dim3(64 * HPC), (size_t)smem, stream, items, sessions, part_o, part_m, part_l,
                          p->n_q_heads, p->n_kv_heads, p->kv_token_stride_elements * 2u, p->q_row_stride_elements,
                          p->scale * kLog2e, status, table, table_keys, extra);

@@ -103,6 +103,7 @@ struct tt_context {
     uint32_t *h_prefix_lens = nullptr;  // [max_sessions]
     uint32_t *h_prefix_rows = nullptr;
     TTSessionTable session_table;       // the parameter form of the current decode call's sessions
+    int sink_clusters[24][5] = {};      // attn_sink.cu: clusters of 1 << [second index] CTAs that run at once, per kernel; -1 none, 0 not asked yet
     TTVerifyMaps verify_maps;           // ... and of a verify batch's tensor maps
     uint64_t launches = 0;
     uint32_t exchange_poll_limit = 0;   // 0: the exchange kernels' default (about a second)
@@ -212,6 +213,8 @@ struct TTDecodeForm {
 bool tt_stream_is_capturing(cudaStream_t stream);
 
 // Launchers implemented in the .cu files.
+int tt_launch_sink_cluster(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, const uint32_t *keys, uint32_t n_sessions,
+                           const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t hpc, bool *taken);
 cudaError_t tt_launch_pass1_sink(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items, const TTDecodeSession *sessions,
                                  const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t *status,
                                  const TTSessionTable &table, uint32_t table_keys, bool wide_rows, uint32_t hpc);
