@@ -225,17 +225,16 @@ def _block(n: int, places, lows, highs, spare=0, indices=None) -> array:
     width = len(places)
     block = array("Q", bytes(8 * n * (width + 1 + spare)))
     words = np.frombuffer(block, dtype=np.uint64).reshape(n, -1)
-    base, step = [p[0] for p in places], [p[1] for p in places]
+    at = np.frombuffer(array("Q", [p[0] for p in places] + [p[1] for p in places]), dtype=np.uint64)     # addresses, steps
     i = _numbers(n)
     if indices is None:
-        np.add(i * np.array(step, dtype=np.uint64), np.array(base, dtype=np.uint64), out=words[:, :width])
+        np.add(i * at[width:], at[:width], out=words[:, :width])
     else:                               # indices: per place, None for i itself
         for c, which in enumerate(indices):
-            at = i[:, 0] if which is None else np.asarray(which, dtype=np.uint64)
-            words[:, c] = at * np.uint64(step[c]) + np.uint64(base[c])
+            words[:, c] = (i[:, 0] if which is None else np.asarray(which, dtype=np.uint64)) * at[width + c] + at[c]
     halves = words.view(np.uint32)
-    halves[:, 2 * width] = np.array(lows, dtype=np.uint32)
-    halves[:, 2 * width + 1] = highs if isinstance(highs, int) else np.array(highs, dtype=np.uint32)
+    halves[:, 2 * width] = np.frombuffer(array("I", lows), dtype=np.uint32)
+    halves[:, 2 * width + 1] = highs if isinstance(highs, int) else np.frombuffer(array("I", highs), dtype=np.uint32)
     return block
 
 
