@@ -373,6 +373,13 @@ int tt_attn_prefill_causal_selected(tt_context *ctx, tt_stream stream, const voi
  * are refused with TT_ERR_UNSUPPORTED_SHAPE; accumulate and evict take any). Captured calls use the
  * context's workspace when replayed: like calls, graphs of one context must not overlap on the GPU. */
 
+/* The tables of these calls (tt_attn_session, tt_attn_prefix, tt_attn_weight_rows, tt_kv_evict_session)
+ * when everything lies in equal slots of a few tensors (host arithmetic, no context): record i is
+ * `width` addresses places[j] + i * places[width + j], then lows[i] in the lower and highs[i] (highs NULL: high) in
+ * the upper half of one 64-bit word, then `spare` zero words. */
+void tt_table_fill(uint64_t *words, uint32_t n, uint32_t width, uint32_t spare, const uint64_t *places,
+                   const uint32_t *lows, const uint32_t *highs, uint32_t high);
+
 /* Sinks: row r of a session (causal end e = seq_len - (q_rows - 1 - r)) sees key j when j < e and
  * (j < sink_tokens or j >= e - window); window 0 = no window. A row without visible keys gives
  * zeros. Key j is cache row j, or with ring_capacity R > 0 (window > 0 then) row
@@ -402,8 +409,8 @@ int tt_attn_prefill_sink_path(const void *q, const void *k, const void *v, const
  * once. Every query row sees the whole prefix of its group and the keys of its own session as in
  * tt_attn_decode_batched (session k, v, seq_len describe the rows behind the prefix; seq_len may be
  * q_rows - 1, kv_start must be 0). groups[g] owns the next n_sessions entries of `sessions`; the
- * counts add up to the batch. The prefix is streamed once per 128 packed query rows of a KV head
- * (sessions x q_rows x n_q_heads / n_kv_heads), not once per session. */
+ * counts add up to the batch. The prefix is streamed once per 128 (at head_dim 256: 256) packed query
+ * rows of a KV head (sessions x q_rows x n_q_heads / n_kv_heads), not once per session. */
 typedef struct tt_attn_prefix {
     const void *k; /* row 0 of the prefix, params->kv_token_stride_elements apart */
     const void *v;
@@ -414,7 +421,8 @@ int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const tt_att
                                  uint32_t n_groups, const tt_attn_session *sessions,
                                  uint32_t n_sessions, const tt_attn_batch_params *params);
 /* The split of the prefix pass (host arithmetic): keys per work item (a multiple of 128) for groups
- * of the given prefix lengths and query rows (sessions x q_rows), and the number of items.
+ * of the given prefix lengths and query rows (sessions x q_rows), and the number of items. In a batch of
+ * up to 16 sessions each session's own keys are one more group.
  * TT_ERR_OOM when the partials do not fit workspace_bytes (0 = no limit). */
 int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_t *query_rows,
                                uint32_t n_groups, uint32_t head_dim, uint32_t n_q_heads,

@@ -197,6 +197,7 @@ SIGNATURES = {
     "tt_gdn_step": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(GdnShape), _u32, _u32, _vp]),
     "tt_gdn_step_batched": (C.c_int, [_vp, _vp, C.POINTER(GdnSession), _u32, _vp, _vp, C.POINTER(GdnShape), _u32,
                                       _u32]),
+    "tt_table_fill": (None, [_vp, _u32, _u32, _u32, _vp, _vp, _vp, _u32]),
     "tt_attn_decode_sink_window": (C.c_int, [_vp, _vp, _vp, _u32, C.POINTER(AttnBatchParams), _u32, _u32, _u32]),
     "tt_attn_sink_keys": (C.c_int, [_u32, _u32, _u32, _u32, C.POINTER(_u32), C.POINTER(_u32)]),
     "tt_attn_prefill_sink_window": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(PrefillParams), _u32, _u32,

@@ -196,57 +196,40 @@ def _half_dtype(what: str, first, *others) -> int:
     return L.TT_BF16
 
 
-def _counts(name: str, values, n: int) -> list:
+def _counts(name: str, values, n: int) -> array:
     """n numbers in 0..2^32-1 from a sequence, or from one int for all."""
-    if isinstance(values, int):
-        if n and 0 <= values <= 0xFFFFFFFF:
-            return [values] * n
-        values = [values] * n
-    elif not isinstance(values, list):
-        values = [int(x) for x in values]
-    if len(values) != n or (n and (min(values) < 0 or max(values) > 0xFFFFFFFF)):
+    try:
+        if isinstance(values, int):
+            found = array("I", (values,)) * n
+        else:
+            found = array("I", values if isinstance(values, list) else [int(x) for x in values])
+    except (OverflowError, TypeError):
+        found = None
+    if found is None or len(found) != n:
         _refuse(f"{name} must be {n} numbers in 0..2^32-1")
-    return values
+    return found
 
 
-def _block(n: int, places, lows, highs, spare=0, indices=None) -> array:
+def _block(n: int, places, lows: array, highs, spare=0, indices=None) -> array:
     """n records of 64-bit words as the C structures lay them out: for every (address, step) of `places` address + i * step (or
-    + indices[i] * step), one word of two 32-bit numbers, `spare` zero words."""
-    if n <= 6:          # numpy's fixed costs are those of six records: 7 us
+    + indices[i] * step), one word of two 32-bit numbers (`highs`: an array too, or one int), `spare` zero words."""
+    one = isinstance(highs, int)
+    if n <= 3 or indices is not None:   # up to three records Python is as fast as the call below
         flat, rest = [], [0] * spare
         for i in range(n):
             if indices is None:
                 flat += [address + i * step for address, step in places]
-            else:
+            else:                       # per place, None for i itself
                 flat += [p[0] + int(i if which is None else which[i]) * p[1] for p, which in zip(places, indices)]
-            flat.append(int(lows[i]) | int(highs if isinstance(highs, int) else highs[i]) << 32)
+            flat.append(lows[i] | (highs if one else highs[i]) << 32)
             flat += rest
         return array("Q", flat)
     width = len(places)
     block = array("Q", bytes(8 * n * (width + 1 + spare)))
-    words = np.frombuffer(block, dtype=np.uint64).reshape(n, -1)
-    at = np.frombuffer(array("Q", [p[0] for p in places] + [p[1] for p in places]), dtype=np.uint64)     # addresses, steps
-    i = _numbers(n)
-    if indices is None:
-        np.add(i * at[width:], at[:width], out=words[:, :width])
-    else:                               # indices: per place, None for i itself
-        for c, which in enumerate(indices):
-            words[:, c] = (i[:, 0] if which is None else np.asarray(which, dtype=np.uint64)) * at[width + c] + at[c]
-    halves = words.view(np.uint32)
-    halves[:, 2 * width] = np.frombuffer(array("I", lows), dtype=np.uint32)
-    halves[:, 2 * width + 1] = highs if isinstance(highs, int) else np.frombuffer(array("I", highs), dtype=np.uint32)
+    at = array("Q", [p[0] for p in places] + [p[1] for p in places])
+    L.lib().tt_table_fill(block.buffer_info()[0], n, width, spare, at.buffer_info()[0], lows.buffer_info()[0],
+                          None if one else highs.buffer_info()[0], highs if one else 0)
     return block
-
-
-_number_column = np.arange(64, dtype=np.uint64)[:, None]
-
-
-def _numbers(n: int):
-    """The column 0 .. n-1."""
-    global _number_column
-    if n > len(_number_column):
-        _number_column = np.arange(2 * n, dtype=np.uint64)[:, None]
-    return _number_column[:n]
 
 
 def _pointer(words: array) -> int:
@@ -530,7 +513,7 @@ class Attention:
                 _refuse("positions must be laid out like weights")
         if t.longest > weights.shape[2]:
             _refuse(f"a session is longer than a weight row of {weights.shape[2]}")
-        ends = t.records["seq_len"].tolist() if end_positions is None else _counts("end_positions", end_positions, n)
+        ends = array("I", t.records["seq_len"].tolist()) if end_positions is None else _counts("end_positions", end_positions, n)
         words = _block(n, (at, at_positions), _counts("fresh_rows", fresh_rows, n), ends)      # tt_attn_weight_rows
         p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                      out_row_stride_elements, scale, io_dtype)
