@@ -270,7 +270,9 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
     // what the CTAs before this one have of counts[k], one read each
     auto before = [&](int k) {
         if (threadIdx.x < 32) {
-            uint32_t x = threadIdx.x < rank ? cluster.map_shared_rank(sh.counts, threadIdx.x)[k] : 0u;
+            uint32_t x = 0;
+            if constexpr (CLUSTER)
+                if (threadIdx.x < rank) x = cluster.map_shared_rank(sh.counts, threadIdx.x)[k];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
             if (threadIdx.x == 0) sh.before[k] = x;
@@ -426,11 +428,14 @@ kv_evict_move_kernel(const __grid_constant__ EvictTable table, EvictParams p, co
     }
 }
 
-// CTAs per (session, KV head): one per 8192 rows while the machine has SMs for them, and enough that the slices fit
-// shared memory.
+// CTAs per (session, KV head). The rounds of a cluster cost three times those of a CTA alone, so up to 10000 rows stay with
+// one (9000 rows of 16 sessions x 2 heads: 23 us, 32 with two); beyond, slices of some 2048 rows while half of the SMs
+// have room for them (16000 rows of 4 sessions: 21.7 us, 25.5 with slices of 8192), and enough CTAs that the slices
+// fit shared memory.
 uint32_t cluster_size(uint32_t max_rows, uint32_t pairs, uint32_t sm_count) {
     uint32_t c = 1;
-    while (c < kMaxCluster && ((max_rows > c * 8192u && (uint64_t)pairs * c * 2 <= sm_count) || (uint64_t)c * kSelSliceKeys < max_rows)) c *= 2;
+    while (c < kMaxCluster && ((max_rows > (c == 1 ? 10000u : c * 2048u) && (uint64_t)pairs * c * 4 <= sm_count) || (uint64_t)c * kSelSliceKeys < max_rows))
+        c *= 2;
     return c;
 }
 
