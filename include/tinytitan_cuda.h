@@ -435,7 +435,8 @@ int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_t *quer
  * call: their sums start from zero whatever stood there, and positions (when given) records their
  * token positions, end_position - fresh_rows .. end_position - 1. A decode step has
  * fresh_rows = q_rows; the first call after a prompt has fresh_rows = seq_len, with the prompt's
- * last queries as its rows. Entries at seq_len and beyond are left alone. Sums are deterministic. */
+ * last queries as its rows. Entries at seq_len and beyond are left alone. Sums are deterministic.
+ * Sessions must not share weights or positions. */
 typedef struct tt_attn_weight_rows {
     float *weights;      /* KV head 0; the heads are head_stride elements apart */
     uint32_t *positions; /* nullable, same layout */

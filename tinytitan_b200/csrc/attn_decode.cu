@@ -13,7 +13,7 @@
 // mma.sync m16n8k16 with fp32 accumulation, the softmax is done on the accumulator fragments
 // with quad shuffles. Pass 2 merges the items of a session by log-sum-exp. A call with one
 // session carries it in the kernel parameters (no table upload), which also makes that call
-// capturable in a CUDA graph.
+// capturable in a CUDA graph. The kernel of pass 1 is in attn_pass1.cuh.
 #include "attn_pass1.cuh"
 
 #include <algorithm>

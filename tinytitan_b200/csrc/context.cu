@@ -213,6 +213,7 @@ TT_API int tt_ctx_profile_collect(tt_context *ctx, float *out_ms, uint32_t capac
 
 TT_API void tt_table_fill(uint64_t *words, uint32_t n, uint32_t width, uint32_t spare, const uint64_t *places, const uint32_t *lows,
                           const uint32_t *highs, uint32_t high) {
+    if (words == nullptr || lows == nullptr || (places == nullptr && width != 0)) return;
     for (uint32_t i = 0; i < n; ++i) {
         for (uint32_t j = 0; j < width; ++j) *words++ = places[j] + (uint64_t)i * places[width + j];
         *words++ = lows[i] | (uint64_t)(highs != nullptr ? highs[i] : high) << 32;
