@@ -547,6 +547,13 @@ def test_evict_clusters_and_long_caches():
     run_evict([100 + 7 * i for i in range(70)], 150, 1, 9, hkv=2, hd=64)                      # more sessions than one launch takes
 
 
+@pytest.mark.parametrize("sessions", [1, 16, 32, 40])                   # clusters of 8, 4, 2 and 1 beyond 10000 rows
+def test_evict_around_one_cta(sessions):
+    lens = [10000 + 7 * i for i in range(sessions)]
+    run_evict(lens, 9990, 4, 100, hkv=1, hd=64)
+    run_evict(lens, 300, 0, 0, hkv=1, hd=64, in_place=False, mix=True)
+
+
 def test_evict_refusals():
     k, v = torch.zeros(2, 64, 2, 64, dtype=F16, device="cuda"), torch.zeros(2, 64, 2, 64, dtype=F16, device="cuda")
     w, pos = torch.zeros(2, 2, 64, device="cuda"), torch.zeros(2, 2, 64, dtype=torch.int32, device="cuda")
