@@ -1003,6 +1003,8 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     }
 
     TTLaunchTimer timer(ctx, stream, TT_PROFILE_DECODE_PARTIAL);
+    PassExtra<kPassPlain> plain;
+    plain.dependents_late = form != nullptr && form->partials_only ? 1u : 0u;
     // a verify batch whose sessions are all one part needs no merge: pass 1 stores the output rows
     bool direct = wide && mode == 0;
     for (uint32_t i = 0; direct && i < n_sessions; ++i) direct = ctx->h_sessions[i].n_parts == 1;
@@ -1018,10 +1020,10 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
         e = tt_launch_pass1_scores(stream, n_items, ctx->items, ctx->sessions, *form, p, ctx->status, table, table_keys, wide_rows, hpc);
     else if (p->io_dtype == TT_F16)
         e = launch_partial_hd<__half>(stream, n_items, ctx->items, ctx->sessions, part_o, part_m, part_l, p, ctx->status,
-                                      table, table_keys, wide_rows, hpc, PassExtra<kPassPlain>());
+                                      table, table_keys, wide_rows, hpc, plain);
     else
         e = launch_partial_hd<__nv_bfloat16>(stream, n_items, ctx->items, ctx->sessions, part_o, part_m, part_l, p,
-                                             ctx->status, table, table_keys, wide_rows, hpc, PassExtra<kPassPlain>());
+                                             ctx->status, table, table_keys, wide_rows, hpc, plain);
     if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_decode_partial launch");
     timer.stop();
     ctx->launches++;

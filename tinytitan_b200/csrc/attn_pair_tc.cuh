@@ -145,7 +145,7 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
 
     pdl_launch_dependents();
     const typename Form::Item item = form.item(blockIdx.x >> 1, HD, ROWS);   // from the parameters alone
-    pdl_wait();       // the kernel before this one may have produced the query or cache rows
+    if (!form.waits_late()) pdl_wait();       // the kernel before this one may have produced the query or cache rows
     const uint32_t n_tiles = item.n_tiles;                                   // >= 1
     const uint32_t my_row0 = rank * 128;
 
@@ -481,6 +481,7 @@ attn_pair_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
     }
 
     if (failed) atomicOr(status, TT_DEV_WAIT_TIMEOUT);
+    if (form.waits_late()) pdl_wait();
     __syncwarp();
     tc_fence_before();
     cluster_sync_all();            // no product reads the other CTA's memory or TMEM any more

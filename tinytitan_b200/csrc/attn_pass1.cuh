@@ -84,7 +84,11 @@ struct DecodeSmem {
 enum : int { kPassPlain = 0, kPassSink = 1, kPassScores = 2, kPassSinkCluster = 3 };
 constexpr uint32_t kMaxSinkCluster = 16;
 template <int FORM>
-struct PassExtra {};
+struct PassExtra {
+    // the next launch may start once every CTA has seen the end of the launches before this one; it then need not wait
+    // for this one's results before it reads what they left
+    uint32_t dependents_late;
+};
 template <>
 struct PassExtra<kPassSink> { uint32_t sink, window; };
 template <>
@@ -141,7 +145,9 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
     // work item from the block index (the items of a session are equal slices, item_prefix says
     // where each session's items start), so no table is copied to the device and a CTA starts
     // without two dependent global loads.
-    pdl_launch_dependents();
+    bool dependents_late = false;
+    if constexpr (FORM == kPassPlain) dependents_late = extra.dependents_late != 0;
+    if (!dependents_late) pdl_launch_dependents();
     TTDecodeItem item;
     TTDecodeSession ses;
     if (table.n != 0) {
@@ -197,6 +203,7 @@ attn_decode_partial_kernel(const TTDecodeItem *__restrict__ items,
     // everything above overlapped the tail of the kernel before this one in the stream; its
     // results (the query rows, the newest K/V rows, partials being merged) are read from here on
     pdl_wait();
+    if (dependents_late) pdl_launch_dependents();
 
     const uint32_t n_keys = item.key_end - item.key_begin;
     const uint32_t n_blocks = (n_keys + kKeysPerBlock - 1) / kKeysPerBlock;

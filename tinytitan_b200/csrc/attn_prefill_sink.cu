@@ -72,6 +72,7 @@ struct alignas(64) SinkForm {
         return t < it.queries ? q + ((size_t)(it.row0 + t) * q_stride + (size_t)head_of(it, r) * hd) * 2 : nullptr;
     }
     __device__ __forceinline__ void acquire(const Item &) const {}
+    __device__ __forceinline__ bool waits_late() const { return false; }
     __device__ __forceinline__ const CUtensorMap *box(const Item &it, uint32_t tile, uint32_t half, bool is_k, int &row) const {
         const uint32_t u = 2 * tile + half;
         if (u < it.sink_halves) {

@@ -71,6 +71,7 @@ struct PrefixForm {
     // what every CTA reads first stands first and together: every line of the parameters it touches costs a miss, some 600
     // clocks each and one after the other
     uint32_t n_q_heads, n_kv_heads, q_row_stride;
+    uint32_t behind_own_rows;            // the launch before this one is the pass over the sessions' own rows
     const PrefixGroup *groups;           // device copies, when !table.in_params
     const PrefixSession *sessions;
     const PrefixMaps *maps;
@@ -140,6 +141,7 @@ struct PrefixForm {
         return reinterpret_cast<const unsigned char *>(s[lo].q) +
                ((size_t)(qrow - s[lo].first_row) * q_row_stride + (size_t)(it.kv_head * group + packed % group) * hd) * 2;
     }
+    __device__ __forceinline__ bool waits_late() const { return behind_own_rows != 0; }
     __device__ __forceinline__ void acquire(const Item &it) const {
         if (table.in_params) return;
         // the maps were rewritten by a host copy since the last launch that used these addresses
@@ -484,6 +486,7 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
     kp.groups = reinterpret_cast<const PrefixGroup *>(ctx->prefix_tables + off_groups);
     kp.sessions = reinterpret_cast<const PrefixSession *>(ctx->prefix_tables + off_sessions);
     kp.n_q_heads = q.n_q_heads; kp.n_kv_heads = q.n_kv_heads; kp.q_row_stride = q.q_row_stride_elements;
+    kp.behind_own_rows = fused ? 0u : 1u;
     table.n_groups = n_table; table.n_sessions = n_sessions; table.in_params = in_params ? 1u : 0u;
     merge.n = in_params ? n_sessions : 0u;
     if (item != 0) {

@@ -177,6 +177,8 @@ __device__ __forceinline__ void load_query_rows(const Form &form, const typename
 //   kPartials                                  true: (m, l, o) partial rows; false: normalised rows of T
 //   partial(item, row, HD) / output(item, row, HD)     partial row number / where the row goes
 //   float *part_o, *part_m, *part_l            (kPartials)
+//   bool waits_late()                          the launch before this one produces nothing it reads and has waited for those
+//                                              that do: a CTA waits for its end only before it ends itself
 template <typename T, int HD, int ROWS, class Form>
 __global__ void __launch_bounds__(RowsGeom<HD, ROWS>::kThreads, 1)
 attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_constant__ Form form) {
@@ -197,7 +199,7 @@ attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
 
     pdl_launch_dependents();
     const typename Form::Item item = form.item(blockIdx.x, HD, ROWS);        // from the parameters alone
-    pdl_wait();       // the kernel before this one may have produced the query or cache rows
+    if (!form.waits_late()) pdl_wait();       // the kernel before this one may have produced the query or cache rows
     const uint32_t n_tiles = item.n_tiles;                                   // >= 1
 
     // the producers: block after block of K's (or V's) units, each into its place of the ring once that is free
@@ -496,6 +498,7 @@ attn_rows_kernel(RowsParams p, uint32_t *__restrict__ status, const __grid_const
     }
 
     if (failed) atomicOr(status, TT_DEV_WAIT_TIMEOUT);
+    if (form.waits_late()) pdl_wait();
     tc_fence_before();
     __syncthreads();
     if (warp == G::kProducerWarp) {
