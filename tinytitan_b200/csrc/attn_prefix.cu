@@ -259,19 +259,21 @@ cudaError_t launch_merge(cudaStream_t stream, uint32_t head_dim, uint32_t rows, 
 
 }  // namespace
 
-// One CTA is resident per SM (an item of 256 rows takes two), and an item costs about kItemTiles tiles besides its own. The
-// length of the items is the one for which the launch takes the least time: the waves of the full-size items, or all items'
-// tiles over the SMs where shorter ones (short groups, a session's own rows) fill the gaps. Equal times go to the longer
-// items (fewer partials to merge).
+// One CTA is resident per SM (an item of 256 rows takes two), and an item costs some tiles besides its own: 3 on one SM, 6
+// on a pair. The length of the items is the one for which the launch takes the least time: the waves of the full-size
+// items, whose last one leaves places for the short ones (short groups, a session's own rows), and what of these does not
+// fit behind it. (16 sessions of 4 rows behind four prefixes of 12,000 to 16,000 keys: items of 18 tiles 41.8 us, of 15,
+// whose waves are shorter but leave no room, 48.1.) Equal times go to the longer items (fewer partials to merge).
 TT_API int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_t *query_rows, uint32_t n_groups, uint32_t head_dim,
                                       uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t sm_count, size_t workspace_bytes,
                                       uint32_t *out_keys_per_item, uint32_t *out_n_items) {
     if (prefix_lens == nullptr || query_rows == nullptr || n_groups == 0 || n_kv_heads == 0 || n_q_heads == 0 ||
         n_q_heads % n_kv_heads != 0 || head_dim == 0 || sm_count == 0)
         return TT_ERR_INVALID_ARG;
-    constexpr uint32_t kItemTiles = 3;
     const uint32_t group = n_q_heads / n_kv_heads, tile_rows = rows_per_tile(query_rows, n_groups, group, head_dim);
-    const uint32_t slots = tile_rows == 256 ? sm_count / 2 : sm_count;          // items that run at once
+    const uint64_t slots = tile_rows == 256 ? sm_count / 2 : sm_count;          // items that run at once
+    const uint64_t item_tiles = tile_rows == 256 ? 6 : 3;
+    if (slots == 0) return TT_ERR_INVALID_ARG;
     uint32_t longest = 0;
     for (uint32_t g = 0; g < n_groups; ++g) longest = prefix_lens[g] > longest ? prefix_lens[g] : longest;
     const uint32_t max_tiles = longest == 0 ? 1 : ceil_div(longest, kBK);
@@ -280,19 +282,24 @@ TT_API int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_
     for (uint32_t parts = 1; parts <= 512 && parts <= max_tiles; ++parts) {
         const uint32_t tiles = ceil_div(max_tiles, parts);
         if (parts > 1 && tiles == ceil_div(max_tiles, parts - 1)) continue;      // the same item length again
-        uint64_t items = 0, full = 0, cost = 0, prows = 0;
+        uint64_t full = 0, longest_item = 0, few = 0, few_cost = 0, prows = 0;
         for (uint32_t g = 0; g < n_groups; ++g) {
             const uint64_t own_tiles = ceil_div(prefix_lens[g], kBK), p = ceil_div(own_tiles, tiles);
             if (p == 0) continue;
-            const uint64_t n = p * n_kv_heads * ceil_div((uint64_t)query_rows[g] * group, tile_rows), each = ceil_div(own_tiles, p) + kItemTiles;
-            items += n;
-            cost += n * each;
-            if (2 * each > tiles + kItemTiles) full += n;
+            const uint64_t n = p * n_kv_heads * ceil_div((uint64_t)query_rows[g] * group, tile_rows), each = ceil_div(own_tiles, p) + item_tiles;
+            if (2 * each > tiles + item_tiles) {
+                full += n;
+                if (each > longest_item) longest_item = each;
+            } else {
+                few += n;
+                few_cost += n * each;
+            }
             prows += p * query_rows[g] * n_q_heads;
         }
         if (workspace_bytes != 0 && prows * ((uint64_t)head_dim + 2) * sizeof(float) > workspace_bytes) break;    // more parts need more
-        const uint64_t waves = (full + slots - 1) / slots * (tiles + kItemTiles), spread = (cost + slots - 1) / slots;
-        const uint64_t time = waves > spread ? waves : spread;
+        const uint64_t items = full + few, waves = (full + slots - 1) / slots, mean = few != 0 ? (few_cost + few - 1) / few : 1;
+        const uint64_t beside = (waves * slots - full) * (longest_item / mean), left = few > beside ? few - beside : 0;
+        const uint64_t time = waves * longest_item + (left + slots - 1) / slots * mean;
         if (time < best) { best = time; best_tiles = tiles; best_items = items; }
     }
     if (best_tiles == 0) return TT_ERR_OOM;
@@ -454,7 +461,20 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
         encoded = encoded && add_group(g, groups[g].k, groups[g].v, first, groups[g].n_sessions, false);
         first += groups[g].n_sessions;
     }
-    for (uint32_t i = 0; fused && i < n_sessions; ++i) encoded = encoded && add_group(n_groups + i, sessions[i].k, sessions[i].v, i, 1, true);
+    if (fused) {        // the longest sessions first: what starts last is short
+        uint32_t order[kFusedSessions];
+        for (uint32_t i = 0; i < n_sessions; ++i) {
+            uint32_t at = i;
+            for (; at > 0 && sessions[order[at - 1]].seq_len < sessions[i].seq_len; --at) order[at] = order[at - 1];
+            order[at] = i;
+        }
+        for (uint32_t i = 0; i < n_sessions; ++i) {
+            const uint32_t x = order[i];
+            lens[n_groups + i] = sessions[x].seq_len;
+            rows[n_groups + i] = sessions[x].q_rows;
+            encoded = encoded && add_group(n_groups + i, sessions[x].k, sessions[x].v, x, 1, true);
+        }
+    }
     if (!encoded) return tt_set_error(ctx, TT_ERR_CUDA, "cuTensorMapEncodeTiled failed for the prefix operands");
     const size_t partial_bytes = ((size_t)partial * (q.head_dim + 2) * sizeof(float) + 255) / 256 * 256;
     kp.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->partials) + (ctx->workspace_bytes / 256 * 256 - partial_bytes));
