@@ -286,7 +286,7 @@ def test_prefix_groups_and_ragged_rows():
     run_prefix(64, 32, 2, F16, [3, 129, 2], [3, 3, 1], rows, lens)
 
 
-@pytest.mark.parametrize("sessions", [1, 5, 16, 17])                    # up to 16 the sessions' own rows are items of the prefix pass
+@pytest.mark.parametrize("sessions", [1, 5, 16, 17, 20])                # their own rows as items of the prefix pass
 @pytest.mark.parametrize("hd,hq,hkv", [(64, 8, 2), (128, 4, 1), (256, 8, 2)])
 def test_prefix_long_suffixes(hd, hq, hkv, sessions):
     # query rows whose last keys lie on both sides of a tile's edge, a last part that only the last rows see, rows without keys
@@ -294,6 +294,15 @@ def test_prefix_long_suffixes(hd, hq, hkv, sessions):
     lens = ([129, 63, 515, 1000, 256, 130, 127, 8, 0, 161, 385, 700, 10, 128, 32, 3, 65, 12, 260, 40])[:sessions]
     run_prefix(hd, hq, hkv, BF16, [5], [sessions], rows, lens, pad=8)
     run_prefix(hd, hq, hkv, F16, [0] * (sessions > 1) + [130], [1] * (sessions > 1) + [sessions - (sessions > 1)], rows, lens)
+
+
+@pytest.mark.parametrize("hd,hq,hkv,rows,sessions", [
+    (256, 16, 2, 1, 17), (256, 16, 2, 1, 64), (256, 16, 2, 3, 40),           # a pass of their own; a pair's items
+    (128, 16, 2, 1, 32), (128, 16, 2, 1, 33), (64, 8, 8, 1, 32), (128, 16, 1, 2, 64), (64, 18, 2, 2, 50)])
+def test_prefix_many_sessions(hd, hq, hkv, rows, sessions):
+    lens = [rows - 1 + (37 * i) % 290 for i in range(sessions)]
+    run_prefix(hd, hq, hkv, F16, [260, 0, 131], [sessions - 3, 1, 2], [rows] * sessions, lens, pad=8)
+    run_prefix(hd, hq, hkv, BF16, [140], [sessions], [1 + i % rows for i in range(sessions)], lens)
 
 
 def test_prefix_large_tables():

@@ -10,7 +10,7 @@
 //   suffix pass   the split-KV decode kernel over every session's own rows                            -> (m, l, o) partials
 //   merge         attn_prefix_merge_kernel: log-sum-exp over both kinds of partials of an output row
 //
-// In a batch of up to 16 sessions the suffixes are items of the prefix pass and there is no suffix pass.
+// Where that is faster (tt_attn_decode_shared_prefix) the suffixes are items of the prefix pass and there is no suffix pass.
 //
 // The prefix pass (attn_rows_tc.cuh) packs row = (query row of the group) * G + g with G query heads per KV head, session
 // after session. Every row of an item sees every key of its range: only the last tile of a prefix is masked. What
@@ -26,7 +26,7 @@
 namespace {
 
 constexpr uint32_t kParamGroups = 8;
-constexpr uint32_t kFusedSessions = 16;                            // sessions whose own rows join the prefix pass
+constexpr uint32_t kFusedSessions = kParamSessions;                // sessions whose own rows may join the prefix pass
 constexpr uint32_t kTableGroups = kParamGroups + kFusedSessions;
 
 // Query rows of one session, in call order.
@@ -94,10 +94,12 @@ struct PrefixForm {
 #pragma unroll
             for (uint32_t i = 1; i < kParamGroups; ++i)
                 if (i < hi && table.item_begin[i] <= block) lo = i;
-            if (hi > kParamGroups) {
-#pragma unroll
-                for (uint32_t i = kParamGroups; i < kTableGroups; ++i)
-                    if (i < hi && table.item_begin[i] <= block) lo = i;
+            if (hi > kParamGroups && table.item_begin[kParamGroups] <= block) {
+                lo = kParamGroups;
+                while (hi - lo > 1) {
+                    const uint32_t mid = (lo + hi) >> 1;
+                    if (table.item_begin[mid] <= block) lo = mid; else hi = mid;
+                }
             }
         } else {
             while (hi - lo > 1) {
@@ -381,10 +383,24 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
         d.n_parts = 0; d.partial_base = 0; d.ring_capacity = 0; d.keep = nullptr; d.row_index = nullptr;
         total_rows += s.q_rows;
     }
-    // A small batch's own rows join the prefix pass as groups of one session each: one launch less, and no second pass
-    // that starts when the first one ends (4 sessions of short keys: 20 -> 13 us, 16 sessions of 4 draft rows: 58 -> 47 us). Larger batches keep the split-KV
-    // pass, which needs no tensor maps: 64 sessions' maps would make the parameters 24 KB.
-    const bool fused = in_params && n_sessions <= kFusedSessions;
+    // The sessions' own rows as groups of one session each in the prefix pass: one launch less, no second pass that starts
+    // when the first one ends, and the tensor cores for draft rows. Up to 16 sessions always: 4 of short keys 18.5 -> 13 us,
+    // 16 of 4000 to 8000 keys 52 -> 48, of 4 rows of 16 heads 176 -> 82. Up to 64, whose maps and groups make the parameters
+    // 26 KB (10 us more of host time), with more than the 16 packed rows a split-KV item takes: 64 sessions of 4 rows and 800
+    // to 1600 keys 220 -> 123 us, of 4 to 300 98 -> 94. Up to 32 otherwise unless a few rows would have items of 256:
+    // head_dim 128, 32 sessions of 800 to 1600 keys 29 -> 23; head_dim 256, 16/2 heads, 4000 to 8000 keys 79 -> 115.
+    bool fused = in_params && n_sessions <= 16;
+    if (in_params && !fused) {
+        uint32_t group_rows = 0, most_rows = 0, most_own = 0;
+        for (uint32_t g = 0, i = 0; g < n_groups; ++g, group_rows = 0)
+            for (uint32_t x = 0; x < groups[g].n_sessions; ++x, ++i) {
+                group_rows += sessions[i].q_rows;
+                most_rows = std::max(most_rows, group_rows);
+                most_own = std::max(most_own, sessions[i].q_rows);
+            }
+        const uint32_t heads = q.n_q_heads / q.n_kv_heads, rows_tile = rows_per_tile(&most_rows, 1, heads, q.head_dim);
+        fused = most_own * heads > 16 || (n_sessions <= 32 && rows_tile < 256);
+    }
     const uint32_t n_table = fused ? n_groups + n_sessions : n_groups;
     uint32_t fused_lens[kTableGroups], fused_rows[kTableGroups];
     uint32_t *lens = fused ? fused_lens : ctx->h_prefix_lens, *rows = fused ? fused_rows : ctx->h_prefix_rows;
