@@ -173,21 +173,18 @@ def _refuse(message: str):
     raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, message)
 
 
-def _cache_place(name: str, t):
-    """Of a 16-bit [batch, rows, heads, head_dim] tensor with tight rows: elements between the rows, and
-    (address, bytes between the batch entries)."""
-    stride = t.stride()
-    if len(stride) != 4 or stride[3] != 1 or stride[2] != t.shape[3]:
-        _refuse(f"{name} must be [batch, rows, heads, head_dim] with tight rows")
-    return stride[1], (t.data_ptr(), 2 * stride[0])
+def _pair(what: str, a, b):
+    """Of two [batch, rows, heads, head_dim] tensors of one shape, type and device with tight rows: the shape and their
+    strides."""
+    shape, s, t = a.shape, a.stride(), b.stride()
+    if b.shape != shape or len(shape) != 4 or s[3] != 1 or t[3] != 1 or s[2] != shape[3] or t[2] != shape[3]:
+        _refuse(f"{what} must be [batch, rows, heads, head_dim] of one shape with tight rows")
+    if b.dtype is not a.dtype or a.get_device() != b.get_device():
+        _refuse(f"{what} must share one dtype and one device")
+    return shape, s, t
 
 
-def _half_dtype(what: str, first, *others) -> int:
-    """The tt_dtype of tensors that must share one 16-bit type and one device."""
-    dtype, device = first.dtype, first.get_device()
-    for t in others:
-        if t.dtype != dtype or t.get_device() != device:
-            _refuse(f"{what} must share one dtype and one device")
+def _half_dtype(what: str, dtype) -> int:
     name = str(dtype)
     if name == "torch.float16":
         return L.TT_F16
@@ -267,21 +264,22 @@ class SessionTable:
     def over_cache(cls, q, out, k, v, seq_lens, slots=None) -> "SessionTable":
         """q, out: [n, q_rows, n_q_heads, head_dim]; k, v: [slots, capacity, n_kv_heads, head_dim], session i in
         slot i or slots[i]; seq_lens[i] keys are visible to the last of its rows."""
-        io_dtype = _half_dtype("q, out, k and v", q, out, k, v)
-        (q_stride, at_q), (out_stride, at_out) = _cache_place("q", q), _cache_place("out", out)
-        (kv_stride, at_k), (v_stride, at_v) = _cache_place("k", k), _cache_place("v", v)
-        q_shape, k_shape = q.shape, k.shape
+        q_shape, q_strides, out_strides = _pair("q and out", q, out)
+        k_shape, k_strides, v_strides = _pair("k and v", k, v)
+        device, io_dtype = k.get_device(), _half_dtype("q, out, k and v", q.dtype)
+        if k.dtype is not q.dtype or q.get_device() != device or v_strides[1] != k_strides[1]:
+            _refuse("q and k must share one dtype and one device, and v be laid out like k")
         n, q_rows = q_shape[0], q_shape[1]
-        if out.shape != q_shape or v.shape != k_shape or v_stride != kv_stride:
-            _refuse("out must be shaped like q, and v laid out like k")
         if slots is None:
             if k_shape[0] < n:
                 _refuse(f"{n} sessions, but the cache has {k_shape[0]} slots")
         elif len(slots) != n or (n and not (0 <= min(slots) and max(slots) < k_shape[0])):
             _refuse(f"slots must name {n} of the cache's {k_shape[0]} slots")
         lens = _counts("seq_lens", seq_lens, n)
-        words = _block(n, (at_q, at_out, at_k, at_v), lens, q_rows, 1, None if slots is None else (None, None, slots, slots))
-        return cls(words, max(lens, default=0), kv_stride, q_stride, out_stride, io_dtype, k_shape[1], k.get_device())
+        places = ((q.data_ptr(), 2 * q_strides[0]), (out.data_ptr(), 2 * out_strides[0]),
+                  (k.data_ptr(), 2 * k_strides[0]), (v.data_ptr(), 2 * v_strides[0]))
+        words = _block(n, places, lens, q_rows, 1, None if slots is None else (None, None, slots, slots))
+        return cls(words, max(lens, default=0), k_strides[1], q_strides[1], out_strides[1], io_dtype, k_shape[1], device)
 
     @classmethod
     def of(cls, sessions) -> "SessionTable":
@@ -338,15 +336,15 @@ class PrefixTable:
     @classmethod
     def over_cache(cls, k, v, prefix_lens, n_sessions) -> "PrefixTable":
         """k, v: [groups, capacity, n_kv_heads, head_dim]; n_sessions: per group, or one number for all."""
-        _half_dtype("k and v", k, v)
-        (stride, at_k), (v_stride, at_v), shape = _cache_place("k", k), _cache_place("v", v), k.shape
-        if v.shape != shape or v_stride != stride:
+        shape, k_strides, v_strides = _pair("k and v", k, v)
+        _half_dtype("k and v", k.dtype)
+        if v_strides[1] != k_strides[1]:
             _refuse("v must be laid out like k")
         g = shape[0]
         lens, counts = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
         if max(lens, default=0) > shape[1]:
             _refuse(f"a prefix is longer than the {shape[1]} rows of its slot")
-        return cls(_block(g, (at_k, at_v), lens, counts), k.get_device())
+        return cls(_block(g, ((k.data_ptr(), 2 * k_strides[0]), (v.data_ptr(), 2 * v_strides[0])), lens, counts), k.get_device())
 
     @classmethod
     def of(cls, groups) -> "PrefixTable":
@@ -646,10 +644,11 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
     positions: int32 like weights, None = row j holds position j; end_positions: position of the next token (default:
     rows). *_out: None for in place, or tensors of the same kind with room for min(rows, budget) rows. Afterwards
     session i has min(rows[i], budget) rows per head."""
-    _half_dtype("K and V", k, v)
+    shape, k_strides, v_strides = _pair("k and v", k, v)
+    _half_dtype("k and v", k.dtype)
     context.check_device(k)
-    (in_stride, from_k), (v_stride, from_v), shape = _cache_place("k", k), _cache_place("v", v), k.shape
-    if v.shape != shape or v_stride != in_stride:
+    in_stride = k_strides[1]
+    if v_strides[1] != in_stride:
         _refuse("v must be laid out like k")
     n, capacity, num_kv_heads, head_dim = shape
     used = _counts("rows", rows, n)
@@ -659,18 +658,17 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
         _refuse(f"a session has more rows than the {capacity} of its slot")
     # destinations of K and V
     out_stride, at_k, at_v = in_stride, _nowhere, _nowhere
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is None:
-            continue
-        _half_dtype("K and V", k, t)
-        (stride, at), s = _cache_place(name, t), t.shape
-        if s[0] < n or s[1] < kept or s[2] != num_kv_heads or s[3] != head_dim or (t is v_out and k_out is not None and stride != out_stride):
-            _refuse(f"{name} must hold the kept rows of {n} sessions, and v_out be laid out like k_out")
-        out_stride = stride
-        if t is k_out:
-            at_k = at
-        if t is v_out:
-            at_v = at
+    if k_out is not None or v_out is not None:
+        a, b = (v_out if k_out is None else k_out), (k_out if v_out is None else v_out)
+        room, a_strides, b_strides = _pair("k_out and v_out", a, b)
+        out_stride = a_strides[1]
+        if (a.dtype is not k.dtype or a.get_device() != k.get_device() or room[0] < n or room[1] < kept or room[2] != num_kv_heads or
+                room[3] != head_dim or b_strides[1] != out_stride):
+            _refuse(f"k_out and v_out must hold the kept rows of {n} sessions, in the layout of k and v")
+        if k_out is not None:
+            at_k = (k_out.data_ptr(), 2 * a_strides[0])
+        if v_out is not None:
+            at_v = (v_out.data_ptr(), 2 * b_strides[0])
     # the statistic and the positions, then where they go
     stat, at_w = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context)
     at_p, at_wo, at_po, stat_out = _nowhere, _nowhere, _nowhere, None
@@ -690,7 +688,7 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
             _refuse(f"positions_out must hold {kept} rows and be laid out like weights_out")
         stat_out = stride
     ends = used if end_positions is None else _counts("end_positions", end_positions, n)
-    words = _block(n, (from_k, from_v, at_k, at_v, at_w, at_wo, at_p, at_po), used, ends)  # tt_kv_evict_session
+    words = _block(n, ((k.data_ptr(), 2 * k_strides[0]), (v.data_ptr(), 2 * v_strides[0]), at_k, at_v, at_w, at_wo, at_p, at_po), used, ends)  # tt_kv_evict_session
     p = L.KVEvictParams(head_dim, num_kv_heads, budget, sink_tokens, recent_tokens, in_stride, out_stride, stat, stat_out or stat, 0)
     context.check(L.lib().tt_kv_evict(context.handle, context.stream(command_buffer), _pointer(words), n, C.byref(p)))
 
