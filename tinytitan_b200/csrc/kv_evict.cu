@@ -17,7 +17,7 @@
 //   so that ranks need one block scan and the strided shared-memory reads meet no bank twice. Bound: the latency of about
 //   a dozen block or cluster barriers. Clocks for 4200 rows (one CTA of 512 threads) and 131071 (16 of 1024): loads 3700 and
 //   4200, the three rounds 10,000 and 30,000, ties 1400 and 4700, holes and fills 4000 and 11,000; a call 15 and 34 us.
-// kv_evict_move_kernel: a warp per 32 destination rows copies what changes, 16 bytes a lane; bound by HBM and, at 17 MB (10 us),
+// kv_evict_move_kernel: a warp per 8 to 32 destination rows copies what changes, 16 bytes a lane; bound by HBM and, at 17 MB (10 us),
 //   by its start. A session that gives up a handful of rows in place (one per step at the budget) is compacted by the selecting CTA itself: one launch.
 #include "tt_sm100.h"
 
@@ -371,8 +371,9 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
     }
 }
 
-// grid = (blocks of 8 * ROWS destination rows, sessions x KV heads), a warp per ROWS of them: 32 in place, where few of them
-// change, 8 into other buffers. Up to eight rows' loads are in flight before their stores.
+// grid = (blocks of 8 * ROWS destination rows, sessions x KV heads), a warp per ROWS of them: 8 into other buffers, 32 in place,
+// where few of them change, but 16 of 512 bytes (32 sessions of 4096 rows give up a quarter: head_dim 256 46.9 us with 32, 41.8
+// with 16; head_dim 128 and 8 KV heads 57.6 and 64.3). Up to eight rows' loads are in flight before their stores.
 template <int ROW_BYTES, int ROWS>
 __global__ void __launch_bounds__(256)
 kv_evict_move_kernel(const __grid_constant__ EvictTable table, EvictParams p, const uint32_t *__restrict__ maps) {
@@ -485,9 +486,9 @@ cudaError_t launch_evict(tt_context *ctx, cudaStream_t stream, const EvictTable 
     }
     const uint32_t kept = max_rows < p.budget ? max_rows : p.budget;
     if (kept == 0) return cudaSuccess;
-    const uint32_t rows = in_place ? 32 : 8;
+    const uint32_t rows = !in_place ? 8 : p.row_bytes == 512 ? 16 : 32;
     const dim3 grid((kept + 8 * rows - 1) / (8 * rows), pairs);
-#define TT_X(BYTES) e = in_place ? tt_launch_pdl(kv_evict_move_kernel<BYTES, 32>, grid, dim3(256), 0, stream, table, p, maps) \
+#define TT_X(BYTES) e = in_place ? tt_launch_pdl(kv_evict_move_kernel<BYTES, BYTES == 512 ? 16 : 32>, grid, dim3(256), 0, stream, table, p, maps) \
                                  : tt_launch_pdl(kv_evict_move_kernel<BYTES, 8>, grid, dim3(256), 0, stream, table, p, maps)
     if (p.row_bytes == 128) TT_X(128);
     else if (p.row_bytes == 256) TT_X(256);
