@@ -563,6 +563,14 @@ def test_evict_around_one_cta(sessions):
     run_evict(lens, 300, 0, 0, hkv=1, hd=64, in_place=False, mix=True)
 
 
+@pytest.mark.parametrize("sessions,given_up", [(15, 256), (15, 257), (16, 512), (16, 513), (32, 1024), (32, 1025)])
+def test_evict_moves_by_the_selecting_cta(sessions, given_up):
+    # the most rows one launch moves, and one more
+    lens = [2500 - (i % 3) * 400 for i in range(sessions)]
+    run_evict(lens, 2500 - given_up, 3, 50, hkv=2, hd=64)
+    run_evict(lens, 2500 - given_up, 0, 0, hkv=2, hd=128, dtype=BF16, mix=True)
+
+
 def test_evict_refusals():
     k, v = torch.zeros(2, 64, 2, 64, dtype=F16, device="cuda"), torch.zeros(2, 64, 2, 64, dtype=F16, device="cuda")
     w, pos = torch.zeros(2, 2, 64, device="cuda"), torch.zeros(2, 2, 64, dtype=torch.int32, device="cuda")

@@ -30,7 +30,7 @@ namespace {
 constexpr uint32_t kMaxSelWarps = 32;
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kMaxCluster = 16;               // above 8: the non-portable size, allowed for this kernel
-constexpr uint32_t kFusedMoves = 256;              // rows a selecting CTA moves itself
+constexpr uint32_t kFusedMoves = 1024;             // most rows a selecting CTA moves itself
 constexpr uint32_t kSelSliceKeys = 50000;          // keys a CTA holds: 200,000 bytes beside the histogram and the counters
 constexpr uint32_t kHoleFlag = 0x80000000u;
 
@@ -441,6 +441,11 @@ uint32_t cluster_size(uint32_t max_rows, uint32_t pairs, uint32_t sm_count) {
     return c;
 }
 
+// Rows the selecting CTA moves itself rather than a second launch: a CTA moves some 73 GB/s, so it pays with few rows or many
+// CTAs (4096 rows of 512 bytes a head, 410 given up: 2 CTAs 17.1 us against 13.7, 32 17.2 against 20.6, 128 24.4 against 53.5;
+// 614 given up: 32 CTAs 21.9 both ways, 64 25.3 against 39.1; 1024: 33.9 against 42.4).
+uint32_t fused_moves(uint32_t pairs) { return pairs >= 64 ? kFusedMoves : pairs >= 32 ? kFusedMoves / 2 : kFusedMoves / 4; }
+
 bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return x < y + b_bytes && y < x + a_bytes;
@@ -476,7 +481,7 @@ cudaError_t launch_evict(tt_context *ctx, cudaStream_t stream, const EvictTable 
         const uint32_t c = cluster_size(max_rows, pairs, (uint32_t)ctx->sm_count);
         const uint32_t slice = ((max_rows + c - 1) / c + 3) / 4 * 4;
         p.held_keys = slice <= kSelSliceKeys ? slice : kSelSliceKeys;
-        const bool fused = c == 1 && in_place && given_up <= kFusedMoves;
+        const bool fused = c == 1 && in_place && given_up <= fused_moves(pairs);
         e = fused ? launch_select<false, true>(stream, table, p, pairs, 1, maps)
                   : c == 1 ? launch_select<false, false>(stream, table, p, pairs, 1, maps)
                            : launch_select<true, false>(stream, table, p, pairs * c, c, maps);
