@@ -16,7 +16,7 @@
 // after session. Every row of an item sees every key of its range: only the last tile of a prefix is masked. What
 // bounds the pass depends on the rows: with up to about 256 packed rows per KV head the bytes of the prefix, beyond
 // that the tensor pipe and the exponentials. 64 sessions of 16/2 heads behind 32768 keys (512 packed rows per KV head):
-// own rows 16 us (67 MB, 4.2 TB/s), prefix pass 36 us (954 TFLOP/s), merge 8 us (24 MB of partials), a call 59-61 us;
+// own rows 16 us (67 MB, 4.2 TB/s), prefix pass 36 us (954 TFLOP/s), merge 7 us (24 MB of partials), a call 56 to 60 us;
 // as 64 sessions of 33,000 keys each the same batch would read 4.3 GB, 660 us.
 #include "attn_merge.cuh"
 #include "attn_pair_tc.cuh"
