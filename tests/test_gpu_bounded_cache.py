@@ -124,6 +124,24 @@ def test_sink_decode_clusters_that_fill_the_machine(hd, hq, hkv, n, rows, longes
     run_sink_decode(hd, hq, hkv, F16, rows, [longest + i % 7 for i in range(n)], 1, longest + 3, 0)
 
 
+@pytest.mark.parametrize("hd,hq,hkv,rows", [(64, 40, 2, 1), (128, 16, 2, 4), (256, 16, 2, 3), (256, 32, 2, 9), (128, 9, 3, 64), (256, 24, 1, 6)])
+@pytest.mark.parametrize("sink,window", [(0, 130), (4, 700), (70, 64), (200, 1), (3, 0)])
+def test_sink_decode_draft_rows(hd, hq, hkv, rows, sink, window):
+    # items of 64, 128 and 256 packed rows and several of them, halves of sinks and window, rows without keys
+    lens = [max(rows - 1, x) for x in (900, 0, 131, 64, sink, sink + window, sink + window + 1, 1500)]
+    run_sink_decode(hd, hq, hkv, F16, rows, lens, sink, window, 0, pad=8)
+    if window:
+        run_sink_decode(hd, hq, hkv, BF16, rows, lens[1:5], sink, window, 1000)          # a ring that has not wrapped
+        run_sink_decode(hd, hq, hkv, BF16, rows, lens, sink, window, window + rows + 60)    # ... and one that has
+
+
+@pytest.mark.parametrize("sessions", [40, 41, 90])
+def test_sink_decode_draft_rows_of_many_sessions(sessions):
+    lens = [5 + (41 * i) % 300 for i in range(sessions)]
+    run_sink_decode(256, 16, 2, F16, 3, lens, 4, 100, 0)
+    run_sink_decode(64, 20, 1, BF16, 2, lens, 0, 64, 0)
+
+
 def test_sink_decode_refusals():
     n, hq, hkv, hd = 1, 8, 2, 256
     q, k, v = (torch.zeros(*s, dtype=F16, device="cuda") for s in [(n, 2, hq, hd), (n, 64, hkv, hd), (n, 64, hkv, hd)])

@@ -173,6 +173,62 @@ struct PrefixForm {
     }
 };
 
+// Draft rows over sinks and a window (tt_attn_decode_sink_window with more than the 16 packed rows of a split-KV item):
+// every session is a group, and its keys are numbered as the rows of the prompt kernel's tiles are (attn_prefill_sink.cu):
+// whole halves of 64 over [0, sink), then those from `base`, the first key of the windows, on. Nothing that no row sees is
+// multiplied: V's maps end with the sinks and with the session. A ring that has wrapped has no such end and stays with the
+// split-KV kernel, which fetches single rows.
+constexpr uint32_t kSinkRowSessions = 40;          // what the parameters have room for
+struct SinkRowsForm : PrefixForm {
+    uint32_t sink, window;
+    struct Session { uint32_t seq_len, q_rows, base, windowed; } session[kSinkRowSessions];
+    // V rows [0, sink) alone: a hidden key's weight is 0, which its row must not turn into NaN. (K's hidden scores are replaced.)
+    struct alignas(64) { unsigned char m[128]; } v_sink[kSinkRowSessions];
+
+    struct Item : PrefixForm::Item {
+        Session s;
+        uint32_t sink_keys;              // key numbers that stand for the sinks
+        const CUtensorMap *v_sink;
+    };
+    __device__ __forceinline__ Item item(uint32_t block, int hd, int rows) const {
+        Item it;
+        static_cast<PrefixForm::Item &>(it) = PrefixForm::item(block, hd, rows);
+        it.s = session[it.session_begin];
+        it.sink_keys = it.s.windowed ? (sink + 63) / 64 * 64 : 0u;
+        it.v_sink = reinterpret_cast<const CUtensorMap *>(v_sink[it.session_begin].m);
+        return it;
+    }
+    __device__ __forceinline__ const CUtensorMap *box(const Item &it, uint32_t tile, uint32_t half, bool is_k, int &row) const {
+        const uint32_t c = it.key_begin + tile * kBK + half * 64;
+        if (c < it.sink_keys) {
+            row = (int)c;
+            return is_k ? it.maps : it.v_sink;
+        }
+        row = (int)(it.s.base + (c - it.sink_keys));
+        return is_k ? it.maps : it.maps + 1;
+    }
+    __device__ __forceinline__ bool masked(const Item &it, uint32_t tile) const {
+        const uint32_t c = it.key_begin + tile * kBK;
+        if (c < it.sink_keys) return true;
+        const uint32_t key = it.s.base + (c - it.sink_keys);
+        return key + kBK + it.s.q_rows - 1 > it.s.seq_len || (it.s.windowed && key < max(sink, it.s.seq_len - window));
+    }
+    __device__ __forceinline__ void visible(const Item &it, uint32_t row, uint32_t tile, uint32_t (&bits)[4]) const {
+        const uint32_t w = min((it.row0 + row) / (n_q_heads / n_kv_heads), it.s.q_rows - 1);
+        const uint32_t end = it.s.seq_len - (it.s.q_rows - 1 - w);
+        const uint32_t from = it.s.windowed ? max(sink, end > window ? end - window : 0u) : 0u;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t c = it.key_begin + tile * kBK + half * 64;
+            const bool of_sink = c < it.sink_keys;
+            const int key0 = (int)(of_sink ? c : it.s.base + (c - it.sink_keys));
+            const int lo = of_sink ? 0 : (int)from - key0, hi = (int)(of_sink ? min(end, sink) : end) - key0;
+            bits[2 * half] = bits_between(lo, hi);
+            bits[2 * half + 1] = bits_between(lo - 32, hi - 32);
+        }
+    }
+};
+
 // ---------------------------------------------------------------------------------------
 // Merge (attn_merge.cuh): the row's partials of its group's prefix, then the session's own.
 // ---------------------------------------------------------------------------------------
@@ -238,9 +294,9 @@ uint32_t rows_per_tile(const uint32_t *query_rows, uint32_t n_groups, uint32_t g
     return most <= 64 ? 64 : most > 128 && head_dim == 256 ? 256 : 128;
 }
 
-template <typename T>
+template <typename T, class Form>
 cudaError_t launch_prefix(cudaStream_t stream, uint32_t head_dim, uint32_t rows, uint32_t n_items, const RowsParams &p, uint32_t *status,
-                          const PrefixForm &form) {
+                          const Form &form) {
 #define TT_X(HD) (rows == 64 ? launch_rows<T, HD, 64>(stream, n_items, p, status, form) : launch_rows<T, HD, 128>(stream, n_items, p, status, form))
     if (rows == 256) return launch_pair<T>(stream, n_items, p, status, form);
     return head_dim == 64 ? TT_X(64) : head_dim == 128 ? TT_X(128) : TT_X(256);
@@ -542,5 +598,118 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
             : launch_merge<__nv_bfloat16>((cudaStream_t)stream, q.head_dim, total_rows * q.n_q_heads, parts, merge, dev, dev_first, n_sessions, kp, own, q.n_q_heads, q.out_row_stride_elements, (uint32_t)ctx->sm_count);
     if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_prefix_merge launch");
     ctx->launches++;
+    return TT_OK;
+}
+
+// Whether the tensor cores take a sink call: more packed rows than a split-KV item has (which reads K and V again for every
+// 16 of them; 16 sessions of 4 rows of 8 heads, 1024 keys: 25.2 us against 14.9, 4096 keys 70 against 34; of 16 heads 143 against 35),
+// and no ring that has wrapped. Sessions beyond one launch's tables need more than a tile or two of keys (64 sessions of 64 keys,
+// head_dim 128: 13.9 us in clusters, 20.5 here; of 1024 62 and 31).
+bool tt_sink_rows_form(const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form, const tt_attn_batch_params *p) {
+    if (!(p->scale > 0.f)) return false;
+    uint32_t most_rows = 0, most_keys = 0;
+    for (uint32_t i = 0; i < n_sessions; ++i) {
+        if (sessions[i].ring_capacity != 0 && sessions[i].seq_len > (uint64_t)form.sink + sessions[i].ring_capacity) return false;
+        most_rows = std::max(most_rows, sessions[i].q_rows);
+        most_keys = std::max(most_keys, sessions[i].seq_len - std::min(sessions[i].seq_len, sessions[i].kv_start));
+    }
+    return most_rows * (p->n_q_heads / p->n_kv_heads) > 16 && (n_sessions <= kSinkRowSessions || most_keys > 2 * kBK);
+}
+
+// One launch and merge of that form.
+static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form,
+                            const tt_attn_batch_params *p) {
+    const tt_attn_batch_params &q = *p;
+    const uint32_t group = q.n_q_heads / q.n_kv_heads;
+    static thread_local SinkRowsForm f;
+    static thread_local MergeTable merge;
+    f.n_q_heads = q.n_q_heads; f.n_kv_heads = q.n_kv_heads; f.q_row_stride = q.q_row_stride_elements; f.behind_own_rows = 0;
+    f.groups = nullptr; f.sessions = nullptr; f.maps = nullptr;
+    f.sink = form.sink; f.window = form.window;
+    f.table.n_groups = n_sessions; f.table.n_sessions = n_sessions; f.table.in_params = 1;
+    merge.n = n_sessions; merge.q_rows = sessions[0].q_rows;
+    // the longest first
+    uint32_t order[kSinkRowSessions] = {}, keys[kSinkRowSessions] = {}, lens[kSinkRowSessions] = {}, rows[kSinkRowSessions] = {}, total_rows = 0;
+    for (uint32_t i = 0; i < n_sessions; ++i) {
+        const TTDecodeSession &s = sessions[i];
+        SinkRowsForm::Session &d = f.session[i];
+        d.seq_len = s.seq_len; d.q_rows = s.q_rows;
+        d.windowed = s.seq_len > form.window && s.seq_len - form.window > form.sink ? 1u : 0u;
+        d.base = d.windowed ? s.kv_start : 0u;
+        keys[i] = (d.windowed ? (form.sink + 63) / 64 * 64 : 0u) + (s.seq_len - d.base);
+        f.table.s[i].q = s.q; f.table.s[i].first_row = total_rows; f.table.s[i].q_rows = s.q_rows;
+        merge.first_row[i] = total_rows;
+        MergeSession &m = merge.s[i];
+        m.out = s.out; m.q_rows = s.q_rows; m.prefix_base = 0; m.prefix_parts = 0; m.prefix_stride = 0;
+        if (s.q_rows != merge.q_rows) merge.q_rows = 0;
+        total_rows += s.q_rows;
+        uint32_t at = i;
+        for (; at > 0 && keys[order[at - 1]] < keys[i]; --at) order[at] = order[at - 1];
+        order[at] = i;
+    }
+    for (uint32_t g = 0; g < n_sessions; ++g) { lens[g] = keys[order[g]]; rows[g] = sessions[order[g]].q_rows; }
+    uint32_t keys_per_item = 0, n_items = 0, item = 0, partial = 0, parts = 0;
+    if (tt_attn_plan_prefix_splits(lens, rows, n_sessions, q.head_dim, q.n_q_heads, q.n_kv_heads, (uint32_t)ctx->sm_count, ctx->workspace_bytes,
+                                   &keys_per_item, &n_items) != TT_OK)
+        return tt_set_error(ctx, TT_ERR_OOM, "the partials do not fit the context workspace");
+    const uint32_t tile_rows = rows_per_tile(rows, n_sessions, group, q.head_dim);
+    const uint64_t width = (uint64_t)q.n_kv_heads * q.head_dim;
+    for (uint32_t g = 0; g < n_sessions; ++g) {
+        const uint32_t x = order[g];
+        const TTDecodeSession &s = sessions[x];
+        PrefixGroup &d = f.table.g[g];
+        d.prefix_len = lens[g];
+        d.n_parts = ceil_div(lens[g], keys_per_item);
+        d.part_len = d.n_parts != 0 ? ceil_div(ceil_div(lens[g], d.n_parts), kBK) * kBK : keys_per_item;
+        if (d.n_parts != 0) d.n_parts = ceil_div(lens[g], d.part_len);       // parts of equal length
+        d.session_begin = x; d.session_count = 1;
+        d.row_begin = merge.first_row[x]; d.n_rows = s.q_rows;
+        d.partial_base = partial; d.item_begin = item;
+        f.table.item_begin[g] = item;
+        d.row_tiles = ceil_div((uint64_t)s.q_rows * group, tile_rows);
+        d.q = s.q; d.q_rows = s.q_rows; d.q_step = 0; d.causal_rows = s.q_rows; d.pad = 0;
+        merge.s[x].own_base = partial; merge.s[x].own_parts = d.n_parts;
+        item += d.n_parts * q.n_kv_heads * d.row_tiles;
+        partial += d.n_parts * s.q_rows * q.n_q_heads;
+        parts = std::max(parts, d.n_parts);
+        if (lens[g] == 0) continue;
+        const uint64_t cached = s.seq_len, sinks = form.sink == 0 ? 1 : std::min<uint64_t>(form.sink, cached);
+        if (!tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(f.table.maps[g].m[0]), s.k, q.io_dtype, width, cached, q.kv_token_stride_elements, 64) ||
+            !tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(f.table.maps[g].m[1]), s.v, q.io_dtype, width, cached, q.kv_token_stride_elements, 64) ||
+            !tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(f.v_sink[x].m), s.v, q.io_dtype, width, sinks, q.kv_token_stride_elements, 64))
+            return tt_set_error(ctx, TT_ERR_CUDA, "cuTensorMapEncodeTiled failed for the decode operands");
+    }
+    f.part_o = ctx->partials; f.part_m = f.part_o + (size_t)partial * q.head_dim; f.part_l = f.part_m + partial;
+    cudaError_t e = cudaSuccess;
+    if (item != 0) {
+        const RowsParams rp = tile_rows == 256 ? pair_params(q.scale, q.io_dtype) : rows_params(q.scale, q.io_dtype, q.head_dim);
+        TTLaunchTimer timer(ctx, stream, TT_PROFILE_DECODE_PARTIAL);
+        e = q.io_dtype == TT_F16 ? launch_prefix<__half>(stream, q.head_dim, tile_rows, item, rp, ctx->status, f)
+                                 : launch_prefix<__nv_bfloat16>(stream, q.head_dim, tile_rows, item, rp, ctx->status, f);
+        if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_sink launch");
+        timer.stop();
+        ctx->launches++;
+    }
+    TTDecodeForm own;
+    own.part_o = f.part_o; own.part_m = f.part_m; own.part_l = f.part_l;
+    const uint32_t out_rows = total_rows * q.n_q_heads;
+    e = q.io_dtype == TT_F16 ? launch_merge<__half>(stream, q.head_dim, out_rows, parts, merge, nullptr, nullptr, n_sessions, f, own, q.n_q_heads,
+                                                    q.out_row_stride_elements, (uint32_t)ctx->sm_count)
+                             : launch_merge<__nv_bfloat16>(stream, q.head_dim, out_rows, parts, merge, nullptr, nullptr, n_sessions, f, own, q.n_q_heads,
+                                                           q.out_row_stride_elements, (uint32_t)ctx->sm_count);
+    if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_sink merge launch");
+    ctx->launches++;
+    return TT_OK;
+}
+
+// Launches the form for sessions checked by tt_launch_decode, as many at a time as the parameters take; kv_start is the first key
+// of the rows' windows behind the sinks.
+int tt_launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form,
+                        const tt_attn_batch_params *p) {
+    const uint32_t passes = ceil_div(n_sessions, kSinkRowSessions), each = ceil_div(n_sessions, passes);
+    for (uint32_t i = 0; i < n_sessions; i += each) {
+        const int rc = launch_sink_rows(ctx, stream, sessions + i, std::min(each, n_sessions - i), form, p);
+        if (rc != TT_OK) return rc;
+    }
     return TT_OK;
 }

@@ -12,7 +12,7 @@
 // the window and wrapping around a ring cost an address each, no tile is half empty, and its bound stays the bytes of
 // the visible rows. With one row every fetched key is visible and no score is masked. A window bounds the keys of a
 // session, so its parts often fit one cluster of CTAs, which joins them without the partials and the second launch that
-// unbounded decode needs. 32 sessions of up to 4100 keys, 16/2 heads of 256: 46 us, 5.8 TB/s; one of 1024 keys 8.9 us.
+// unbounded decode needs; draft rows beyond a split-KV item's 16 go to the tensor cores (tt_sink_rows_form). 32 sessions of up to 4100 keys, 16/2 heads of 256: 46 us, 5.8 TB/s; one of 1024 keys 8.9 us.
 #include "attn_pass1.cuh"
 
 cudaError_t tt_launch_pass1_sink(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items, const TTDecodeSession *sessions,
@@ -66,9 +66,11 @@ uint32_t resident_clusters(tt_context *ctx, const tt_attn_batch_params *p, bool 
 //   keys 45.7 us against 48.9, 64 of 2048 46.2 against 52.1, at head_dim 128 with 8 KV heads 32 of 1024 26.2 against 38.5.
 //   A half-empty machine is left to finer parts (16 of 4096: 44.1 us against 26.8), and so are more than 1024 keys a CTA (256
 //   with two n-tiles: 16 sessions of 4 rows and 4096 keys 74.7 us against 70.2).
+// Draft rows that the tensor-core form takes (tt_sink_rows_form) are left to it except for the latency of short ones on half a
+// machine (2 sessions of 4 rows of 8 heads, 256 keys: 8.8 us against 11.4).
 // 0: the parts meet through memory in a second launch.
 static uint32_t cluster_size(tt_context *ctx, const uint32_t *keys, uint32_t n_sessions, const tt_attn_batch_params *p, uint64_t streams,
-                             bool wide_rows, uint32_t hpc) {
+                             bool wide_rows, uint32_t hpc, bool rows_form) {
     uint64_t longest = 0, sum = 0;
     for (uint32_t i = 0; i < n_sessions; ++i) {
         longest = keys[i] > longest ? keys[i] : longest;
@@ -81,14 +83,16 @@ static uint32_t cluster_size(tt_context *ctx, const uint32_t *keys, uint32_t n_s
     while (bits > 0 && streams * (bits == 4 ? 2 : 1) > resident) resident = resident_clusters(ctx, p, wide_rows, hpc, --bits);
     if (streams > resident) return 0;
     const uint64_t per_cta = (longest + (1u << bits) - 1) >> bits;
+    const uint64_t ctas = streams << bits, machine = resident_clusters(ctx, p, wide_rows, hpc, 0);
+    if (rows_form) return per_cta <= 32 && ctas * 2 <= machine ? 1u << bits : 0u;
     if (per_cta <= (wide_rows ? 32u : 64u)) return 1u << bits;
-    const bool full = streams << bits >= (uint64_t)resident_clusters(ctx, p, wide_rows, hpc, 0) * 5 / 6;
+    const bool full = ctas * 6 >= machine * 5;
     return full && per_cta <= (wide_rows ? 256u : 1024u) && sum * 128 >= longest * n_sessions * 127 ? 1u << bits : 0u;
 }
 
 // Launches the cluster form when it is the faster one; *taken says whether.
 int tt_launch_sink_cluster(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, const uint32_t *keys, uint32_t n_sessions,
-                           const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t hpc, bool *taken) {
+                           const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t hpc, bool rows_form, bool *taken) {
     const uint32_t group = p->n_q_heads / p->n_kv_heads;
     auto row_tiles = [&](uint32_t i) { return (sessions[i].q_rows * group + 15) / 16; };
     uint64_t streams = 0;
@@ -97,7 +101,7 @@ int tt_launch_sink_cluster(tt_context *ctx, cudaStream_t stream, const TTDecodeS
         streams += (uint64_t)(p->n_kv_heads / hpc) * row_tiles(i);
         wide_rows |= sessions[i].q_rows * group > 8;
     }
-    const uint32_t cluster = n_sessions <= kParamSessions ? cluster_size(ctx, keys, n_sessions, p, streams, wide_rows, hpc) : 0u;
+    const uint32_t cluster = n_sessions <= kParamSessions ? cluster_size(ctx, keys, n_sessions, p, streams, wide_rows, hpc, rows_form) : 0u;
     *taken = cluster != 0;
     if (cluster == 0) return TT_OK;
     TTSessionTable &table = ctx->session_table;

@@ -213,8 +213,11 @@ struct TTDecodeForm {
 bool tt_stream_is_capturing(cudaStream_t stream);
 
 // Launchers implemented in the .cu files.
+bool tt_sink_rows_form(const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form, const tt_attn_batch_params *p);
+int tt_launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form,
+                        const tt_attn_batch_params *p);
 int tt_launch_sink_cluster(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, const uint32_t *keys, uint32_t n_sessions,
-                           const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t hpc, bool *taken);
+                           const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t hpc, bool rows_form, bool *taken);
 cudaError_t tt_launch_pass1_sink(cudaStream_t stream, uint32_t n_items, const TTDecodeItem *items, const TTDecodeSession *sessions,
                                  const TTDecodeForm &form, const tt_attn_batch_params *p, uint32_t *status,
                                  const TTSessionTable &table, uint32_t table_keys, bool wide_rows, uint32_t hpc);
