@@ -886,7 +886,7 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     }
     if (form != nullptr && form->form == kPassSink) {
         bool taken = false;
-        const bool rows_form = tt_sink_rows_form(in_sessions, n_sessions, *form, p);
+        const bool rows_form = tt_sink_rows_form(in_sessions, n_sessions, p);
         const int rc = tt_launch_sink_cluster(ctx, stream, in_sessions, keys, n_sessions, *form, p, tt_decode_heads_per_cta(p->n_kv_heads, false), rows_form, &taken);
         if (rc != TT_OK || taken) return rc;
         if (rows_form) return tt_launch_sink_rows(ctx, stream, in_sessions, n_sessions, *form, p);

@@ -174,43 +174,50 @@ struct PrefixForm {
 };
 
 // Draft rows over sinks and a window (tt_attn_decode_sink_window with more than the 16 packed rows of a split-KV item):
-// every session is a group, and its keys are numbered as the rows of the prompt kernel's tiles are (attn_prefill_sink.cu):
-// whole halves of 64 over [0, sink), then those from `base`, the first key of the windows, on. Nothing that no row sees is
-// multiplied: V's maps end with the sinks and with the session. A ring that has wrapped has no such end and stays with the
-// split-KV kernel, which fetches single rows.
-constexpr uint32_t kSinkRowSessions = 40;          // what the parameters have room for
+// every session is a group, and its keys are numbered in whole halves of 64: those over [0, sink), those of the windows from
+// `base` on up to the ring's end, those behind it. Nothing that no row sees is multiplied: V has a map for each of the three
+// ranges that ends with it. (What K has there makes scores that are replaced.)
+constexpr uint32_t kSinkRowSessions = kTableGroups / 2;      // two groups' maps each
 struct SinkRowsForm : PrefixForm {
     uint32_t sink, window;
-    struct Session { uint32_t seq_len, q_rows, base, windowed; } session[kSinkRowSessions];
-    // V rows [0, sink) alone: a hidden key's weight is 0, which its row must not turn into NaN. (K's hidden scores are replaced.)
-    struct alignas(64) { unsigned char m[128]; } v_sink[kSinkRowSessions];
+    // keys base .. base + straight - 1 are rows first_row on, the later ones rows sink on
+    struct Session { uint32_t seq_len, q_rows, base, windowed, first_row, straight; } session[kSinkRowSessions];
 
     struct Item : PrefixForm::Item {
         Session s;
-        uint32_t sink_keys;              // key numbers that stand for the sinks
-        const CUtensorMap *v_sink;
+        uint32_t sink_keys, straight_keys;      // key numbers that stand for the sinks, for the first range of the window
+        const CUtensorMap *v_ends;              // of the sinks, of the range behind the ring's end
     };
     __device__ __forceinline__ Item item(uint32_t block, int hd, int rows) const {
         Item it;
         static_cast<PrefixForm::Item &>(it) = PrefixForm::item(block, hd, rows);
         it.s = session[it.session_begin];
         it.sink_keys = it.s.windowed ? (sink + 63) / 64 * 64 : 0u;
-        it.v_sink = reinterpret_cast<const CUtensorMap *>(v_sink[it.session_begin].m);
+        it.straight_keys = (it.s.straight + 63) / 64 * 64;
+        it.v_ends = reinterpret_cast<const CUtensorMap *>(table.maps[kSinkRowSessions + it.session_begin].m[0]);
         return it;
     }
     __device__ __forceinline__ const CUtensorMap *box(const Item &it, uint32_t tile, uint32_t half, bool is_k, int &row) const {
-        const uint32_t c = it.key_begin + tile * kBK + half * 64;
+        uint32_t c = it.key_begin + tile * kBK + half * 64;
         if (c < it.sink_keys) {
             row = (int)c;
-            return is_k ? it.maps : it.v_sink;
+            return is_k ? it.maps : it.v_ends;
         }
-        row = (int)(it.s.base + (c - it.sink_keys));
-        return is_k ? it.maps : it.maps + 1;
+        c -= it.sink_keys;
+        if (c < it.straight_keys) {
+            row = (int)(it.s.first_row + c);
+            return is_k ? it.maps : it.maps + 1;
+        }
+        row = (int)(sink + (c - it.straight_keys));
+        return is_k ? it.maps : it.v_ends + 1;
     }
     __device__ __forceinline__ bool masked(const Item &it, uint32_t tile) const {
-        const uint32_t c = it.key_begin + tile * kBK;
+        uint32_t c = it.key_begin + tile * kBK;
         if (c < it.sink_keys) return true;
-        const uint32_t key = it.s.base + (c - it.sink_keys);
+        c -= it.sink_keys;
+        uint32_t key = it.s.base + c;
+        if (c >= it.straight_keys) key = it.s.base + it.s.straight + (c - it.straight_keys);
+        else if (c + kBK > it.s.straight) return true;
         return key + kBK + it.s.q_rows - 1 > it.s.seq_len || (it.s.windowed && key < max(sink, it.s.seq_len - window));
     }
     __device__ __forceinline__ void visible(const Item &it, uint32_t row, uint32_t tile, uint32_t (&bits)[4]) const {
@@ -219,10 +226,20 @@ struct SinkRowsForm : PrefixForm {
         const uint32_t from = it.s.windowed ? max(sink, end > window ? end - window : 0u) : 0u;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const uint32_t c = it.key_begin + tile * kBK + half * 64;
-            const bool of_sink = c < it.sink_keys;
-            const int key0 = (int)(of_sink ? c : it.s.base + (c - it.sink_keys));
-            const int lo = of_sink ? 0 : (int)from - key0, hi = (int)(of_sink ? min(end, sink) : end) - key0;
+            uint32_t c = it.key_begin + tile * kBK + half * 64, first = 0, to = end, key0 = c;
+            if (c < it.sink_keys) {
+                to = min(end, sink);
+            } else {
+                c -= it.sink_keys;
+                first = from;
+                if (c < it.straight_keys) {
+                    key0 = it.s.base + c;
+                    to = min(end, it.s.base + it.s.straight);
+                } else {
+                    key0 = it.s.base + it.s.straight + (c - it.straight_keys);
+                }
+            }
+            const int lo = (int)first - (int)key0, hi = (int)to - (int)key0;
             bits[2 * half] = bits_between(lo, hi);
             bits[2 * half + 1] = bits_between(lo - 32, hi - 32);
         }
@@ -602,14 +619,13 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
 }
 
 // Whether the tensor cores take a sink call: more packed rows than a split-KV item has (which reads K and V again for every
-// 16 of them; 16 sessions of 4 rows of 8 heads, 1024 keys: 25.2 us against 14.9, 4096 keys 70 against 34; of 16 heads 143 against 35),
-// and no ring that has wrapped. Sessions beyond one launch's tables need more than a tile or two of keys (64 sessions of 64 keys,
+// 16 of them; 16 sessions of 4 rows of 8 heads, 1024 keys: 25.2 us against 14.9, 4096 keys 70 against 34; of 16 heads 143 against
+// 35). Sessions beyond one launch's tables need more than a tile or two of keys (64 sessions of 64 keys,
 // head_dim 128: 13.9 us in clusters, 20.5 here; of 1024 62 and 31).
-bool tt_sink_rows_form(const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form, const tt_attn_batch_params *p) {
+bool tt_sink_rows_form(const TTDecodeSession *sessions, uint32_t n_sessions, const tt_attn_batch_params *p) {
     if (!(p->scale > 0.f)) return false;
     uint32_t most_rows = 0, most_keys = 0;
     for (uint32_t i = 0; i < n_sessions; ++i) {
-        if (sessions[i].ring_capacity != 0 && sessions[i].seq_len > (uint64_t)form.sink + sessions[i].ring_capacity) return false;
         most_rows = std::max(most_rows, sessions[i].q_rows);
         most_keys = std::max(most_keys, sessions[i].seq_len - std::min(sessions[i].seq_len, sessions[i].kv_start));
     }
@@ -636,7 +652,14 @@ static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecode
         d.seq_len = s.seq_len; d.q_rows = s.q_rows;
         d.windowed = s.seq_len > form.window && s.seq_len - form.window > form.sink ? 1u : 0u;
         d.base = d.windowed ? s.kv_start : 0u;
-        keys[i] = (d.windowed ? (form.sink + 63) / 64 * 64 : 0u) + (s.seq_len - d.base);
+        d.first_row = d.base;
+        d.straight = s.seq_len - d.base;
+        if (s.ring_capacity != 0 && s.seq_len > (uint64_t)form.sink + s.ring_capacity) {        // wrapped, hence windowed
+            d.first_row = form.sink + (d.base - form.sink) % s.ring_capacity;
+            d.straight = std::min(d.straight, form.sink + s.ring_capacity - d.first_row);
+        }
+        const uint32_t behind = s.seq_len - d.base - d.straight;
+        keys[i] = (d.windowed ? (form.sink + 63) / 64 * 64 : 0u) + (behind != 0 ? (d.straight + 63) / 64 * 64 + behind : d.straight);
         f.table.s[i].q = s.q; f.table.s[i].first_row = total_rows; f.table.s[i].q_rows = s.q_rows;
         merge.first_row[i] = total_rows;
         MergeSession &m = merge.s[i];
@@ -673,10 +696,16 @@ static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecode
         partial += d.n_parts * s.q_rows * q.n_q_heads;
         parts = std::max(parts, d.n_parts);
         if (lens[g] == 0) continue;
-        const uint64_t cached = s.seq_len, sinks = form.sink == 0 ? 1 : std::min<uint64_t>(form.sink, cached);
-        if (!tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(f.table.maps[g].m[0]), s.k, q.io_dtype, width, cached, q.kv_token_stride_elements, 64) ||
-            !tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(f.table.maps[g].m[1]), s.v, q.io_dtype, width, cached, q.kv_token_stride_elements, 64) ||
-            !tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(f.v_sink[x].m), s.v, q.io_dtype, width, sinks, q.kv_token_stride_elements, 64))
+        const SinkRowsForm::Session &e = f.session[x];
+        const uint64_t cached = s.ring_capacity != 0 ? std::min<uint64_t>(s.seq_len, (uint64_t)form.sink + s.ring_capacity) : s.seq_len;
+        const uint64_t sinks = std::max<uint64_t>(1, std::min<uint64_t>(form.sink, cached));
+        const uint64_t behind = form.sink + (uint64_t)(s.seq_len - e.base - e.straight);
+        auto encode = [&](unsigned char *map, const void *from, uint64_t count) {
+            return tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(map), from, q.io_dtype, width, count, q.kv_token_stride_elements, 64);
+        };
+        if (!encode(f.table.maps[g].m[0], s.k, cached) || !encode(f.table.maps[g].m[1], s.v, (uint64_t)e.first_row + e.straight) ||
+            !encode(f.table.maps[kSinkRowSessions + x].m[0], s.v, sinks) ||
+            !encode(f.table.maps[kSinkRowSessions + x].m[1], s.v, std::max<uint64_t>(1, std::min(behind, cached))))
             return tt_set_error(ctx, TT_ERR_CUDA, "cuTensorMapEncodeTiled failed for the decode operands");
     }
     f.part_o = ctx->partials; f.part_m = f.part_o + (size_t)partial * q.head_dim; f.part_l = f.part_m + partial;

@@ -213,7 +213,7 @@ struct TTDecodeForm {
 bool tt_stream_is_capturing(cudaStream_t stream);
 
 // Launchers implemented in the .cu files.
-bool tt_sink_rows_form(const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form, const tt_attn_batch_params *p);
+bool tt_sink_rows_form(const TTDecodeSession *sessions, uint32_t n_sessions, const tt_attn_batch_params *p);
 int tt_launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form,
                         const tt_attn_batch_params *p);
 int tt_launch_sink_cluster(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, const uint32_t *keys, uint32_t n_sessions,
