@@ -370,7 +370,8 @@ int tt_attn_prefill_causal_selected(tt_context *ctx, tt_stream stream, const voi
  * strides, streams, workspace and errors of the calls above, fp16 or bf16 rows, head_dim 64, 128 or
  * 256 for decode. Batches of any size up to max_sessions; during a stream capture, decode batches of
  * up to 64 sessions (8 prefix groups), whose tables travel in the kernel parameters (larger ones
- * are refused with TT_ERR_UNSUPPORTED_SHAPE; accumulate and evict take any). Captured calls use the
+ * are refused with TT_ERR_UNSUPPORTED_SHAPE where their tables would be uploaded; accumulate and
+ * evict take any). Captured calls use the
  * context's workspace when replayed: like calls, graphs of one context must not overlap on the GPU. */
 
 /* The tables of these calls (tt_attn_session, tt_attn_prefix, tt_attn_weight_rows, tt_kv_evict_session)
