@@ -16,7 +16,7 @@
 //   ties their rank in row order and one numbers holes and fills. A thread owns consecutive rows, an odd number of them,
 //   so that ranks need one block scan and the strided shared-memory reads meet no bank twice. Bound: the latency of about
 //   a dozen block or cluster barriers. Clocks for 4200 rows (one CTA of 512 threads) and 131071 (16 of 1024): loads 3700 and
-//   4200, the three rounds 10,000 and 30,000, ties 1400 and 4700, holes and fills 4000 and 11,000; a call 15 and 34 us.
+//   4200, the bits of the threshold 6500 and 30,000, ties 1400 and 4700, holes and fills 4000 and 11,000; a call 13 and 34 us.
 // kv_evict_move_kernel: a warp per 8 to 32 destination rows copies what changes, 16 bytes a lane; bound by HBM and, at 17 MB (10 us),
 //   by its start. A session that gives up a handful of rows in place (one per step at the budget) is compacted by the selecting CTA itself: one launch.
 #include "tt_sm100.h"
@@ -32,6 +32,7 @@ constexpr uint32_t kBins = 2048;
 constexpr uint32_t kMaxCluster = 16;               // above 8: the non-portable size, allowed for this kernel
 constexpr uint32_t kFusedMoves = 1024;             // most rows a selecting CTA moves itself
 constexpr uint32_t kSelSliceKeys = 50000;          // keys a CTA holds: 200,000 bytes beside the histogram and the counters
+constexpr uint32_t kRanked = 256;                  // keys that are compared with one another
 constexpr uint32_t kHoleFlag = 0x80000000u;
 
 struct EvictSession {
@@ -100,7 +101,7 @@ struct __align__(16) SelShared {
     uint32_t counts[4];          // this CTA's ties, holes, fills (read by the cluster)
     uint32_t before[4];          // ... of the CTAs before this one
     uint32_t owner[2];           // the CTA whose bins hold the wanted rank, keys above its bins
-    uint32_t pick[2];            // the bin that holds it, keys above it
+    uint32_t pick[3];            // the bin that holds it, keys above it, keys in it
     uint32_t hole_rows[kFusedMoves], fill_rows[kFusedMoves];
 };
 
@@ -168,6 +169,8 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
     // ---- the budget-th largest key: three rounds over its bits from the top ----
     uint32_t prefix = 0, want = p.budget;                  // key bits fixed so far; rank wanted among the keys that share them
     const uint32_t share = CLUSTER ? kBins / size : kBins;      // bins whose counts a CTA adds up
+    // One CTA alone: where few keys share the bits of the first round they are compared with one another instead of counted
+    // twice more (4096 rows: 13.1 us to 11.7).
 #pragma unroll 1
     for (int round = 0; round < 3; ++round) {
         const uint32_t bits = round < 2 ? 11u : 10u, shift = round == 0 ? 21u : round == 1 ? 10u : 0u;
@@ -249,14 +252,53 @@ kv_evict_select_kernel(const __grid_constant__ EvictTable table, EvictParams p, 
         uint32_t total;
         const uint32_t above = above0 + block_scan<kSelWarps>(mine, sh.warp_sums, &total);
         if (above < want && want <= above + mine) {
-            uint32_t seen = above, x = 0;
-            while (x + 1 < kPer && seen + c[x] < want) seen += c[x++];
-            sh.pick[0] = first_bin + share - 1 - kPer * threadIdx.x - x;
+            uint32_t seen = above, nth = 0, in_bin = c[0];
+#pragma unroll
+            for (uint32_t x = 1; x < kPer; ++x)
+                if (seen + in_bin < want) { seen += in_bin; in_bin = c[x]; nth = x; }
+            sh.pick[0] = first_bin + share - 1 - kPer * threadIdx.x - nth;
             sh.pick[1] = seen;
+            sh.pick[2] = in_bin;
         }
+        if constexpr (!CLUSTER)
+            if (threadIdx.x == 0) sh.owner[0] = 0;
         __syncthreads();
         prefix = (prefix << bits) | sh.pick[0];
         want -= sh.pick[1];
+        if constexpr (!CLUSTER) {
+            const uint32_t left = sh.pick[2];
+            uint32_t *some = sh.sum[0];                    // which only clusters use
+            if (round == 0 && left <= kRanked) {
+                for (uint32_t i0 = 0; i0 < n; i0 += kSelThreads) {
+                    const uint32_t i = i0 + threadIdx.x;
+                    const uint32_t key = i < n ? key_of(i) : 0u;
+                    const bool is = i < n && key >> shift == prefix;
+                    const uint32_t found = __ballot_sync(0xffffffffu, is);
+                    if (found == 0) continue;
+                    uint32_t at = 0;
+                    if ((threadIdx.x & 31) == 0) at = atomicAdd(&sh.owner[0], (uint32_t)__popc(found));
+                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(found & ((1u << (threadIdx.x & 31)) - 1));
+                    if (is) some[at] = key;
+                }
+                if (threadIdx.x >= left && threadIdx.x < (left + 3) / 4 * 4) some[threadIdx.x] = 0;          // above no key
+                __syncthreads();
+                if (threadIdx.x < left) {
+                    const uint32_t mine = some[threadIdx.x];
+                    uint32_t above = 0, same = 0;
+                    for (uint32_t j = 0; j < left; j += 4) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(some + j);
+                        above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+                        same += (x.x == mine) + (x.y == mine) + (x.z == mine) + (x.w == mine);
+                    }
+                    if (above < want && want <= above + same) { sh.pick[0] = mine; sh.pick[1] = above; }          // one key does
+                }
+                __syncthreads();
+                prefix = sh.pick[0];
+                want -= sh.pick[1];
+                __syncthreads();
+                break;
+            }
+        }
         __syncthreads();
     }
     const uint32_t threshold = prefix, ties_kept = want;   // keys above it stay, and the first `ties_kept` equal to it
