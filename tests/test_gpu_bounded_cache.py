@@ -562,6 +562,24 @@ def test_evict_special_weights_and_ties():
     assert (p[..., :100] == torch.arange(100, device="cuda", dtype=torch.int32)).all() and (k[0, :100, 0, 0] == torch.arange(100, device="cuda")).all()
 
 
+@pytest.mark.parametrize("close", [1, 2, 5, 255, 256, 257, 600])        # rows whose weights share their leading bits: compared or counted
+@pytest.mark.parametrize("values", ["different", "two", "zero"])
+def test_evict_threshold_among_close_weights(close, values):
+    rows, hkv, hd = 1500, 1, 64
+    g = torch.Generator().manual_seed(close)
+    apart = torch.cat([torch.linspace(2.0, 900.0, 500), torch.linspace(-3.0, -900.0, rows - 500 - close)])
+    near = {"different": 1.0 + 0.2 * torch.rand(close, generator=g), "two": 1.0 + 0.125 * (torch.rand(close, generator=g) < 0.5).float(),
+            "zero": torch.zeros(close)}[values]
+    w = torch.cat([apart, near])[torch.randperm(rows, generator=g)]
+    for kept in sorted({1, (close + 1) // 2, close}):
+        budget = 500 + kept                                  # the threshold is the kept-th largest of the close ones
+        k = torch.arange(rows, dtype=torch.float32)[None, :, None, None].expand(1, rows, hkv, hd).to(BF16).cuda().contiguous()
+        p = torch.zeros(1, hkv, rows, dtype=torch.int32, device="cuda")
+        tt.evict_kv_rows(context(), k, k.clone(), w[None, None].cuda(), rows, budget, positions_out=p)
+        done()
+        assert p[0, 0, :budget].tolist() == evict(w.tolist(), list(range(rows)), rows, budget, 0, 0, rows)
+
+
 def test_evict_positions_default_to_the_rows():
     run_evict([400, 90], 80, 4, 20, keep_positions=False, in_place=False)
     run_evict([400, 90], 80, 4, 20, keep_positions=False)
