@@ -1,0 +1,21 @@
+"""Calls at the edges of the bounded- and shared-cache operators on the GPU, against plain 64-bit references."""
+import pytest
+import torch
+
+import tinytitan_b200 as tt
+from test_gpu_bounded_cache import BF16, F16, run_sink_decode
+
+pytestmark = pytest.mark.gpu
+
+
+# Draft rows over a plain sliding window (no sinks) whose keys fill an odd number of 64-key halves: the spare half of the last
+# tile belongs to no row, and the cache's first row, long behind the window, holds NaN like every row that nobody sees.
+@pytest.mark.parametrize("hd,hq,hkv,sessions", [(256, 16, 2, 3), (128, 16, 2, 40), (64, 32, 1, 40), (128, 64, 1, 3)])
+@pytest.mark.parametrize("window,ring", [(130, 0), (520, 0), (1024, 0), (130, 1100), (520, 1100)])
+def test_draft_rows_behind_a_window_without_sinks(hd, hq, hkv, sessions, window, ring):
+    rows = 4                                                     # window + 3 keys: 3, 9 and 17 halves
+    lens = [window + 777 + i % 5 for i in range(sessions)]       # in the ring: wrapped (1800 of 1100) or not yet, the window in one piece
+    if ring:
+        lens = [1800 + i % 5 for i in range(sessions)]
+        assert all((n - window - 3) % ring + window + 3 <= ring for n in lens)
+    run_sink_decode(hd, hq, hkv, F16 if window == 520 else BF16, rows, lens, 0, window, ring)

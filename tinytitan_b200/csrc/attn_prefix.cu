@@ -193,7 +193,10 @@ struct SinkRowsForm : PrefixForm {
         static_cast<PrefixForm::Item &>(it) = PrefixForm::item(block, hd, rows);
         it.s = session[it.session_begin];
         it.sink_keys = it.s.windowed ? (sink + 63) / 64 * 64 : 0u;
-        it.straight_keys = (it.s.straight + 63) / 64 * 64;
+        // with nothing behind the ring's end the first range also takes the numbers past its last half: of a cache without sinks
+        // they would else be row 0 of the last range's map, which cannot be empty, and a spare half of the last tile would read it
+        const bool behind = it.s.seq_len - it.s.base > it.s.straight;
+        it.straight_keys = behind ? (it.s.straight + 63) / 64 * 64 : 0xffffffffu;
         it.v_ends = reinterpret_cast<const CUtensorMap *>(table.maps[kSinkRowSessions + it.session_begin].m[0]);
         return it;
     }
