@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import tinytitan_b200 as tt
-from test_gpu_bounded_cache import BF16, F16, run_sink_decode
+from test_gpu_bounded_cache import BF16, F16, run_accumulate, run_sink_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +19,12 @@ def test_draft_rows_behind_a_window_without_sinks(hd, hq, hkv, sessions, window,
         lens = [1800 + i % 5 for i in range(sessions)]
         assert all((n - window - 3) % ring + window + 3 <= ring for n in lens)
     run_sink_decode(hd, hq, hkv, F16 if window == 520 else BF16, rows, lens, 0, window, ring)
+
+
+@pytest.mark.parametrize("max_sessions", [1, 3])
+def test_accumulate_takes_more_sessions_than_its_context_has_places(max_sessions):
+    ctx = tt.Context(0, max_sessions=max_sessions)
+    lens = [5 + 9 * i for i in range(10)]
+    run_accumulate(64, 8, 2, F16, [1 + i % 3 for i in range(10)], lens, [1 + i % 3 for i in range(10)], ctx=ctx)
+    run_accumulate(256, 16, 2, BF16, [1] * 70, [1 + i for i in range(70)], [0] * 70, ctx=ctx)
+    ctx.close()

@@ -213,6 +213,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
     // The scores of one pass share the workspace with its split partials: at most half of it. A batch that needs more
     // is taken in several passes, by sessions first, then by the query rows of one session.
     const size_t score_budget = ctx->workspace_bytes / 2 / 16 * 16;
+    const uint32_t pass_sessions = ctx->max_sessions < kParamSessions ? ctx->max_sessions : kParamSessions;      // the context's tables hold no more
     static thread_local AccTable table;
     uint32_t i = 0, row_done = 0;
     while (i < n_sessions) {
@@ -225,7 +226,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
             // pass 0: with 8-row padding when every session of the call fits it; pass 1: 16-row padding
             const uint32_t pad = pass == 0 ? 8u : 16u;
             bytes = 0; count = 0; wide_rows = false;
-            for (uint32_t k = i; k < n_sessions && count < kParamSessions; ++k) {
+            for (uint32_t k = i; k < n_sessions && count < pass_sessions; ++k) {
                 uint32_t rows = sessions[k].q_rows - (k == i ? row_done : 0u);
                 auto need = [&](uint32_t r) {
                     return (size_t)params->n_kv_heads * sessions[k].seq_len * ((r * group + pad - 1) / pad * pad) * sizeof(float);
