@@ -3,7 +3,8 @@ import pytest
 import torch
 
 import tinytitan_b200 as tt
-from test_gpu_bounded_cache import BF16, F16, run_accumulate, run_sink_decode
+from bounded_cache_reference import attend
+from test_gpu_bounded_cache import BF16, F16, NAN, check, normal, run_accumulate, run_sink_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -27,4 +28,24 @@ def test_accumulate_takes_more_sessions_than_its_context_has_places(max_sessions
     lens = [5 + 9 * i for i in range(10)]
     run_accumulate(64, 8, 2, F16, [1 + i % 3 for i in range(10)], lens, [1 + i % 3 for i in range(10)], ctx=ctx)
     run_accumulate(256, 16, 2, BF16, [1] * 70, [1 + i for i in range(70)], [0] * 70, ctx=ctx)
+    ctx.close()
+
+
+def test_accumulate_cut_by_rows_with_a_narrowly_padded_output():
+    # an output row stride that keeps rows 8-byte aligned: passes behind the first start at such rows
+    hd, hq, hkv, rows, m, pad = 64, 32, 2, 3, 2000, 4            # one row a pass
+    ctx = tt.Context(0, workspace_bytes=900_000)
+    q, k, v = normal(1, rows, hq, hd), normal(2, m, hkv, hd), normal(3, m, hkv, hd)
+    out, w = torch.full((rows, hq * hd + pad), NAN, dtype=F16, device="cuda"), torch.zeros(1, hkv, m, device="cuda")
+    d = [x.cuda() for x in (q, k, v)]
+    tt.Attention(ctx).encode_accumulate([tt.DecodeSession(d[0], out, d[1], d[2], m, rows)], w, hd, hq, hkv, out_row_stride_elements=hq * hd + pad)
+    torch.cuda.synchronize()
+    added = torch.zeros(hkv, m, dtype=torch.float64)
+    for r in range(rows):
+        end = m - (rows - 1 - r)
+        o, p, bound = attend(q[r], k[:end], v[:end])
+        check(out[r, :hq * hd].reshape(hq, hd), o, bound)
+        added[:, :end] += p.reshape(hkv, hq // hkv, end).sum(1)
+    # 32-bit scores, exponentials and normaliser (2e-5, see attend), and one rounding of 2^-24 per added weight
+    assert ((w[0].cpu().double() - added).abs() <= (2e-5 + (1 + rows * hq // hkv) * 2.0 ** -24) * added).all()
     ctx.close()

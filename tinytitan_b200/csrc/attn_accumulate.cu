@@ -254,7 +254,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
             const uint32_t skip = c == 0 ? row_done : 0u, rows = c == 0 ? rows_of_first : s.q_rows;
             TTDecodeSession &d = tmp[c];
             d.q = reinterpret_cast<const unsigned char *>(s.q) + (size_t)skip * params->q_row_stride_elements * 2;
-            d.out = reinterpret_cast<unsigned char *>(s.out) + (size_t)skip * params->out_row_stride_elements * 2;
+            d.out = s.out;                   // pass 1 leaves it alone
             if (s.q == nullptr || s.out == nullptr) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has a null buffer", i + c);
             d.k = s.k; d.v = s.v;
             d.seq_len = s.seq_len - (s.q_rows - skip - rows); d.q_rows = rows; d.kv_start = 0;
@@ -265,7 +265,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
             a.seq_len = d.seq_len; a.total_len = s.seq_len; a.q_rows = rows;
             a.fresh_begin = skip == 0 ? s.seq_len - weight_rows[i + c].fresh_rows : s.seq_len;
             a.end_position = weight_rows[i + c].end_position;
-            a.out = d.out;
+            a.out = reinterpret_cast<unsigned char *>(s.out) + (size_t)skip * params->out_row_stride_elements * 2;
             table.first_cta[c] = blocks;
             table.first_row[c] = query_rows;
             query_rows += rows;
