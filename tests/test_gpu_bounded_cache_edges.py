@@ -31,6 +31,36 @@ def test_accumulate_takes_more_sessions_than_its_context_has_places(max_sessions
     ctx.close()
 
 
+def test_accumulate_refused_calls_add_nothing():
+    """A call that takes several passes is refused before the first of them, whichever session is at fault."""
+    hd, hq, hkv, n, cap = 64, 8, 2, 70, 40
+    q, k, w = torch.zeros(n, 1, hq, hd, dtype=F16, device="cuda"), torch.ones(n, cap, hkv, hd, dtype=F16, device="cuda"), torch.zeros(n, hkv, cap, device="cuda")
+    out = torch.full_like(q, 7.0)
+    a = tt.Attention(tt.Context(0))
+    good = [tt.DecodeSession(q[i], out[i], k[i], k[i], 30) for i in range(n)]
+    last = n - 1
+    for error, bad in ((tt.InvalidArgument, tt.DecodeSession(q[last], out[last], None, k[last], 30)),
+                       (tt.InvalidArgument, tt.DecodeSession(q[last], None, k[last], k[last], 30)),
+                       (tt.UnsupportedShape, tt.DecodeSession(q[last], out[last], k[last], k[last], 30, v_offset=2)),
+                       (tt.UnsupportedShape, tt.DecodeSession(q[last], out[last], k[last], k[last], 30, q_offset=8))):
+        with pytest.raises(error):
+            a.encode_accumulate(good[:last] + [bad], w, hd, hq, hkv, fresh_rows=1)
+    torch.cuda.synchronize()
+    assert (w == 0).all() and (out == 7).all()
+    # the last session's scores, then its partials, do not fit the workspace
+    for length, rows, room in ((5000, 1, 1 << 17), (4, 64, 1 << 17)):
+        small = tt.Context(0, workspace_bytes=room)
+        lens = [30] * 3 + [length]
+        qs, ks = torch.zeros(4, rows, hq, hd, dtype=F16, device="cuda"), torch.zeros(4, max(lens), hkv, hd, dtype=F16, device="cuda")
+        ws, outs = torch.zeros(4, hkv, max(lens), device="cuda"), torch.full((4, rows, hq, hd), 7.0, dtype=F16, device="cuda")
+        sessions = [tt.DecodeSession(qs[i], outs[i], ks[i], ks[i], max(lens[i], rows - 1), rows if i == 3 else 1) for i in range(4)]
+        with pytest.raises(tt.TinyTitanError):
+            tt.Attention(small).encode_accumulate(sessions, ws, hd, hq, hkv)
+        torch.cuda.synchronize()
+        assert (ws == 0).all() and (outs == 7).all()
+        small.close()
+
+
 def test_accumulate_cut_by_rows_with_a_narrowly_padded_output():
     # an output row stride that keeps rows 8-byte aligned: passes behind the first start at such rows
     hd, hq, hkv, rows, m, pad = 64, 32, 2, 3, 2000, 4            # one row a pass

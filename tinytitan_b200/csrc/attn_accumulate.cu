@@ -193,6 +193,8 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
     if (params->n_kv_heads == 0 || params->n_q_heads == 0 || params->n_q_heads % params->n_kv_heads != 0)
         return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_q_heads must be a multiple of n_kv_heads");
     if (params->n_q_heads > 96) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_q_heads exceeds 96");
+    if (params->head_dim != 64 && params->head_dim != 128 && params->head_dim != 256)
+        return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "decode attention supports head_dim 64/128/256, got %u", params->head_dim);
     if (!(params->scale > 0.f)) return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "accumulated weights need a positive scale");
     const uint32_t group = params->n_q_heads / params->n_kv_heads;
     for (uint32_t i = 0; i < n_sessions; ++i) {
@@ -202,6 +204,10 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
         if (s.q_rows == 0 || s.q_rows > 64) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: q_rows must be in 1..64", i);
         if (s.seq_len > (uint32_t)INT32_MAX || s.seq_len + 1 < s.q_rows)
             return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: seq_len %u cannot hold %u query rows", i, s.seq_len, s.q_rows);
+        if (s.q == nullptr || s.k == nullptr || s.v == nullptr || s.out == nullptr)
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has a null buffer", i);
+        if (((uintptr_t)s.q | (uintptr_t)s.k | (uintptr_t)s.v | (uintptr_t)s.out) & 15)
+            return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "session %u: buffers must be 16-byte aligned", i);
         if (w.weights == nullptr) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has no weight row", i);
         if (((uintptr_t)w.weights | (uintptr_t)w.positions) & 3)
             return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: weight and position rows must be 4-byte aligned", i);
@@ -214,38 +220,71 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
     // is taken in several passes, by sessions first, then by the query rows of one session.
     const size_t score_budget = ctx->workspace_bytes / 2 / 16 * 16;
     const uint32_t pass_sessions = ctx->max_sessions < kParamSessions ? ctx->max_sessions : kParamSessions;      // the context's tables hold no more
-    static thread_local AccTable table;
-    uint32_t i = 0, row_done = 0;
-    while (i < n_sessions) {
-        bool wide_rows = false;
-        // rows taken per session decide the padding (8 packed rows, or 16 as soon as one session has more)
-        size_t bytes = 0;
-        uint32_t count = 0, rows_of_first = 0;
-        TTDecodeSession *tmp = ctx->h_sessions_in;
-        for (uint32_t pass = 0; pass < 2; ++pass) {
-            // pass 0: with 8-row padding when every session of the call fits it; pass 1: 16-row padding
-            const uint32_t pad = pass == 0 ? 8u : 16u;
-            bytes = 0; count = 0; wide_rows = false;
-            for (uint32_t k = i; k < n_sessions && count < pass_sessions; ++k) {
-                uint32_t rows = sessions[k].q_rows - (k == i ? row_done : 0u);
+    struct Pass { uint32_t count, rows_of_first, pad; size_t bytes; };
+    auto reserved = [](const Pass &pass) { return (pass.bytes + 255) / 256 * 256 + 16; };
+    // the pass from query row `row_done` of session i on; no sessions: the scores of session i do not fit
+    auto pass_from = [&](uint32_t i, uint32_t row_done) {
+        Pass pass = {0, 0, 8, 0};
+        // with 8-row padding when every session of the pass fits it, else with 16-row padding
+        for (uint32_t pad = 8; pad <= 16; pad += 8) {
+            bool wide_rows = false;
+            pass.bytes = 0; pass.count = 0;
+            for (uint32_t k = i; k < n_sessions && pass.count < pass_sessions; ++k) {
+                const uint32_t all = sessions[k].q_rows - (k == i ? row_done : 0u);
+                uint32_t rows = all;
                 auto need = [&](uint32_t r) {
                     return (size_t)params->n_kv_heads * sessions[k].seq_len * ((r * group + pad - 1) / pad * pad) * sizeof(float);
                 };
-                if (bytes + need(rows) > score_budget) {
-                    if (count != 0) break;
+                if (pass.bytes + need(rows) > score_budget) {
+                    if (pass.count != 0) break;
                     while (rows > 1 && need(rows) > score_budget) --rows;
-                    if (need(rows) > score_budget)
-                        return tt_set_error(ctx, TT_ERR_OOM, "the scores of session %u do not fit the context workspace", k);
+                    if (need(rows) > score_budget) return pass;
                 }
-                bytes += (need(rows) + 15) / 16 * 16;
+                pass.bytes += (need(rows) + 15) / 16 * 16;
                 wide_rows |= rows * group > 8;
-                if (count == 0) rows_of_first = rows;
-                ++count;
-                if (rows != sessions[k].q_rows - (k == i ? row_done : 0u)) break;      // a session cut by rows ends its pass
+                if (pass.count == 0) pass.rows_of_first = rows;
+                ++pass.count;
+                if (rows != all) break;                  // a session cut by rows ends its pass
             }
+            pass.pad = wide_rows ? 16u : 8u;             // what pass 1 pads these sessions to
             if (!wide_rows) break;
         }
-        const uint32_t pad = wide_rows ? 16u : 8u;
+        return pass;
+    };
+    // the rest of a cut session, or the sessions behind it
+    auto advance = [&](const Pass &pass, uint32_t &i, uint32_t &row_done) {
+        if (pass.count == 1 && row_done + pass.rows_of_first < sessions[i].q_rows) {
+            row_done += pass.rows_of_first;
+        } else {
+            i += pass.count;
+            row_done = 0;
+        }
+    };
+    // A call whose later pass does not fit is refused before its first one has added to a statistic (a call of one pass is
+    // refused by tt_launch_decode, before it launches).
+    for (uint32_t i = 0, row_done = 0; i < n_sessions;) {
+        const Pass pass = pass_from(i, row_done);
+        if (pass.count == 0) return tt_set_error(ctx, TT_ERR_OOM, "the scores of session %u do not fit the context workspace", i);
+        if (pass.count == n_sessions && pass.rows_of_first == sessions[0].q_rows) break;
+        size_t room = ctx->workspace_bytes;
+        room = room > reserved(pass) ? (room - reserved(pass)) / (params->head_dim + 4) * (params->head_dim + 2) : 0;
+        for (uint32_t c = 0; c < pass.count; ++c) {
+            const uint32_t skip = c == 0 ? row_done : 0u;
+            ctx->h_rows[c] = c == 0 ? pass.rows_of_first : sessions[i + c].q_rows;
+            ctx->h_keys[c] = sessions[i + c].seq_len - (sessions[i + c].q_rows - skip - ctx->h_rows[c]);
+        }
+        if (room == 0 || tt_attn_plan_splits(ctx->h_keys, ctx->h_rows, pass.count, params->head_dim, params->n_q_heads, params->n_kv_heads,
+                                             (uint32_t)ctx->sm_count, room, nullptr, nullptr) != TT_OK)
+            return tt_set_error(ctx, TT_ERR_OOM, "the partials of session %u do not fit the context workspace", i);
+        advance(pass, i, row_done);
+    }
+    static thread_local AccTable table;
+    uint32_t i = 0, row_done = 0;
+    while (i < n_sessions) {
+        const Pass pass = pass_from(i, row_done);
+        const uint32_t count = pass.count, rows_of_first = pass.rows_of_first, pad = pass.pad;
+        const size_t bytes = pass.bytes;
+        TTDecodeSession *tmp = ctx->h_sessions_in;
         float *scores = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->partials) + (ctx->workspace_bytes / 16 * 16 - (bytes + 255) / 256 * 256));
         table.n = count;
         uint32_t blocks = 0, max_rows = 0, query_rows = 0;
@@ -255,7 +294,6 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
             TTDecodeSession &d = tmp[c];
             d.q = reinterpret_cast<const unsigned char *>(s.q) + (size_t)skip * params->q_row_stride_elements * 2;
             d.out = s.out;                   // pass 1 leaves it alone
-            if (s.q == nullptr || s.out == nullptr) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u has a null buffer", i + c);
             d.k = s.k; d.v = s.v;
             d.seq_len = s.seq_len - (s.q_rows - skip - rows); d.q_rows = rows; d.kv_start = 0;
             d.n_parts = 0; d.partial_base = 0; d.ring_capacity = 0; d.keep = nullptr; d.scores = scores;
@@ -277,7 +315,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
         TTDecodeForm form;
         form.form = kPassScores;
         form.partials_only = true;
-        form.reserved_bytes = (bytes + 255) / 256 * 256 + 16;
+        form.reserved_bytes = reserved(pass);
         int rc = tt_launch_decode(ctx, (cudaStream_t)stream, tmp, count, params, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &form);
         if (rc != TT_OK) return rc;
         uint32_t max_parts = 0;
@@ -298,13 +336,7 @@ TT_API int tt_attn_decode_accumulate(tt_context *ctx, tt_stream stream, const tt
                                                          : launch_accumulate<__nv_bfloat16>((cudaStream_t)stream, params->head_dim, ctas, smem, table, p);
         if (e != cudaSuccess) return tt_check_cuda(ctx, e, "attn_accumulate launch");
         ctx->launches++;
-        // the next pass: the rest of a cut session, or the sessions behind it
-        if (count == 1 && row_done + rows_of_first < sessions[i].q_rows) {
-            row_done += rows_of_first;
-        } else {
-            i += count;
-            row_done = 0;
-        }
+        advance(pass, i, row_done);
     }
     return TT_OK;
 }
