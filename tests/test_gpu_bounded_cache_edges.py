@@ -79,3 +79,20 @@ def test_accumulate_cut_by_rows_with_a_narrowly_padded_output():
     # 32-bit scores, exponentials and normaliser (2e-5, see attend), and one rounding of 2^-24 per added weight
     assert ((w[0].cpu().double() - added).abs() <= (2e-5 + (1 + rows * hq // hkv) * 2.0 ** -24) * added).all()
     ctx.close()
+
+
+def test_evict_refused_calls_move_nothing():
+    """A call whose last session's row map does not fit the workspace is refused before any session gives up a row."""
+    ctx = tt.Context(0, workspace_bytes=6000)                    # 1500 map entries: a session of 1001 rows needs 1001, one of 2000 rows 2000
+    n, cap, budget = 3, 2000, 1000
+    k = normal(1, n, cap, 1, 64).cuda()
+    v, w = k.clone(), torch.rand(n, 1, cap, generator=torch.Generator().manual_seed(2)).cuda()
+    before = [x.clone() for x in (k, v, w)]
+    with pytest.raises(tt.TinyTitanError):
+        tt.evict_kv_rows(ctx, k, v, w, [1001, 1001, 2000], budget)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip((k, v, w), before))
+    tt.evict_kv_rows(ctx, k, v, w, [1001, 1001, 1400], budget)   # each fits alone: one launch a session
+    torch.cuda.synchronize()
+    assert not any(torch.equal(w[i], before[2][i]) for i in range(n))
+    ctx.close()

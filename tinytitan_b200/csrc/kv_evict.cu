@@ -488,6 +488,11 @@ uint32_t cluster_size(uint32_t max_rows, uint32_t pairs, uint32_t sm_count) {
 // 614 given up: 32 CTAs 21.9 both ways, 64 25.3 against 39.1; 1024: 33.9 against 42.4).
 uint32_t fused_moves(uint32_t pairs) { return pairs >= 64 ? kFusedMoves : pairs >= 32 ? kFusedMoves / 2 : kFusedMoves / 4; }
 
+// entries of a head's map: a source for every kept row, and the list of the rows that fill holes
+uint64_t map_entries(uint32_t rows, uint32_t budget) {
+    return rows <= budget ? 0 : (uint64_t)budget + (rows - budget < budget ? rows - budget : budget);
+}
+
 bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return x < y + b_bytes && y < x + a_bytes;
@@ -566,6 +571,9 @@ TT_API int tt_kv_evict(tt_context *ctx, tt_stream stream, const tt_kv_evict_sess
     const uint32_t weight_out_stride = q.weight_out_head_stride ? q.weight_out_head_stride : q.weight_head_stride;
     if (in_stride < width || out_stride < width) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "a row stride is smaller than its tight width");
     if (in_stride % 8 || out_stride % 8) return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "row strides must keep rows 16-byte aligned");
+    // the maps of one launch pair live in the workspace; a batch that needs more is taken in several
+    uint64_t map_room = ctx->workspace_bytes / sizeof(uint32_t);
+    if (map_room > UINT32_MAX) map_room = UINT32_MAX;
     for (uint32_t i = 0; i < n_sessions; ++i) {
         const tt_kv_evict_session &s = sessions[i];
         if (s.k == nullptr || s.v == nullptr || s.weights == nullptr)
@@ -593,14 +601,15 @@ TT_API int tt_kv_evict(tt_context *ctx, tt_stream stream, const tt_kv_evict_sess
             (!w_in && overlaps(s.weights, w_bytes, s.weights_out, wo_bytes)) ||
             (s.positions != nullptr && !p_in && overlaps(s.positions, w_bytes, s.positions_out, wo_bytes)))
             return tt_set_error(ctx, TT_ERR_INVALID_ARG, "session %u: an output overlaps its input without being it", i);
+        // before the first launch: a call refused behind it would have emptied some caches and not others
+        if (map_entries(s.rows, q.budget) * q.n_kv_heads > map_room)
+            return tt_set_error(ctx, TT_ERR_OOM, "the row map of session %u does not fit the context workspace", i);
     }
     EvictParams p;
     p.budget = q.budget; p.sink = q.sink_tokens; p.recent = q.recent_tokens; p.n_kv_heads = q.n_kv_heads;
     p.weight_stride = q.weight_head_stride; p.weight_out_stride = weight_out_stride;
     p.row_bytes = q.head_dim * 2; p.held_keys = 0;
     p.in_stride = in_stride * 2; p.out_stride = out_stride * 2;
-    // the maps of one launch pair live in the workspace; a batch that needs more is taken in several
-    const uint64_t map_room = ctx->workspace_bytes / sizeof(uint32_t);
     static thread_local EvictTable table;
     uint32_t i = 0;
     while (i < n_sessions) {
@@ -610,12 +619,8 @@ TT_API int tt_kv_evict(tt_context *ctx, tt_stream stream, const tt_kv_evict_sess
         table.n = 0;
         for (; i < n_sessions && table.n < kParamSessions; ++i) {
             const tt_kv_evict_session &s = sessions[i];
-            uint64_t pitch = 0;
-            if (s.rows > q.budget) pitch = (uint64_t)q.budget + (s.rows - q.budget < q.budget ? s.rows - q.budget : q.budget);
-            if (used + pitch * q.n_kv_heads > map_room || used + pitch * q.n_kv_heads > UINT32_MAX) {
-                if (table.n != 0) break;
-                return tt_set_error(ctx, TT_ERR_OOM, "the row map of session %u does not fit the context workspace", i);
-            }
+            const uint64_t pitch = map_entries(s.rows, q.budget);
+            if (used + pitch * q.n_kv_heads > map_room) break;           // each alone fits
             EvictSession &d = table.s[table.n++];
             d.k = (const unsigned char *)s.k; d.v = (const unsigned char *)s.v;
             d.k_out = (unsigned char *)(s.k_out ? s.k_out : s.k); d.v_out = (unsigned char *)(s.v_out ? s.v_out : s.v);
