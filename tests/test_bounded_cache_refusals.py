@@ -1,0 +1,73 @@
+"""What the wrappers over bounded and shared caches refuse before they reach the library. No GPU."""
+import pytest
+import torch
+
+import tinytitan_b200 as tt
+
+H, B = torch.float16, torch.bfloat16
+
+
+class LibraryCalled(Exception):
+    pass
+
+
+class HostContext:
+    """A context whose device is the host's, so that every check but the library's own is passed on the way to it."""
+    handle, device = None, -1
+
+    def check(self, status):
+        raise LibraryCalled
+
+    check_device = tt.Context.check_device
+    stream = tt.Context.stream
+
+
+def attention():
+    return tt.Attention(HostContext())
+
+
+def cache(n=3, rows=20, hkv=2, hd=64, dtype=H, pad=0):
+    """[n, rows, hkv, hd], rows `pad` heads wider than that."""
+    return torch.zeros(n, rows, hkv + pad, hd, dtype=dtype)[:, :, :hkv]
+
+
+def queries(n=3, rows=1, hq=8, hd=64, dtype=H):
+    return torch.zeros(n, rows, hq, hd, dtype=dtype)
+
+
+def sessions(k=None, q=None, lens=4):
+    k, q = cache() if k is None else k, queries() if q is None else q
+    return tt.SessionTable.over_cache(q, q, k, k, lens)
+
+
+def refused(call, *args, **kw):
+    with pytest.raises(tt.InvalidArgument):
+        call(*args, command_buffer=0, **kw)
+
+
+def reaches_the_library(call, *args, **kw):
+    with pytest.raises(LibraryCalled):
+        call(*args, command_buffer=0, **kw)
+
+
+def test_prefix_tables_must_match_their_sessions():
+    shared = attention().encode_shared_prefix
+    prefix = tt.PrefixTable.over_cache(cache(1), cache(1), 7, 3)
+    reaches_the_library(shared, prefix, sessions(), 64, 8, 2)
+    wide = tt.PrefixTable.over_cache(cache(1, pad=1), cache(1, pad=1), 7, 3)
+    refused(shared, wide, sessions(), 64, 8, 2)                                          # rows of another stride
+    refused(shared, prefix, sessions(cache(pad=1)), 64, 8, 2)
+    reaches_the_library(shared, wide, sessions(cache(pad=1)), 64, 8, 2)
+    refused(shared, prefix, sessions(cache(dtype=B), queries(dtype=B)), 64, 8, 2)        # of another type
+    refused(shared, tt.PrefixTable.over_cache(cache(1, hkv=1), cache(1, hkv=1), 7, 3), sessions(), 64, 8, 2)    # other heads
+    refused(shared, tt.PrefixTable.over_cache(cache(1, hkv=1, hd=128), cache(1, hkv=1, hd=128), 7, 3), sessions(), 64, 8, 2)
+    # lists of sessions have the strides and the type that the call says
+    q, k = queries(), cache()
+    each = [tt.DecodeSession(q[i], q[i], k[i], k[i], 4) for i in range(3)]
+    reaches_the_library(shared, prefix, each, 64, 8, 2)
+    reaches_the_library(shared, wide, each, 64, 8, 2, kv_token_stride_elements=192)
+    refused(shared, wide, each, 64, 8, 2)
+    refused(shared, prefix, each, 64, 8, 2, kv_token_stride_elements=192)
+    refused(shared, prefix, each, 64, 8, 2, io_dtype=tt.TT_BF16)
+    # one row has no stride
+    reaches_the_library(shared, tt.PrefixTable.over_cache(cache(1, 1, pad=1), cache(1, 1, pad=1), 1, 3), sessions(), 64, 8, 2)

@@ -316,8 +316,9 @@ class PrefixTable:
 
     record = np.dtype([("k", "u8"), ("v", "u8"), ("prefix_len", "u4"), ("n_sessions", "u4")])
 
-    def __init__(self, words, device=None):
+    def __init__(self, words, device=None, kv_stride=None, io_dtype=None, heads=None):
         self.words, self.device = words, device
+        self.kv_stride, self.io_dtype, self.heads = kv_stride, io_dtype, heads      # heads: (n_kv_heads, head_dim)
 
     def __len__(self):
         return len(self.words) // 3
@@ -337,14 +338,26 @@ class PrefixTable:
     def over_cache(cls, k, v, prefix_lens, n_sessions) -> "PrefixTable":
         """k, v: [groups, capacity, n_kv_heads, head_dim]; n_sessions: per group, or one number for all."""
         shape, k_strides, v_strides = _pair("k and v", k, v)
-        _half_dtype("k and v", k.dtype)
+        io_dtype = _half_dtype("k and v", k.dtype)
         if v_strides[1] != k_strides[1]:
             _refuse("v must be laid out like k")
         g = shape[0]
         lens, counts = _counts("prefix_lens", prefix_lens, g), _counts("n_sessions", n_sessions, g)
         if max(lens, default=0) > shape[1]:
             _refuse(f"a prefix is longer than the {shape[1]} rows of its slot")
-        return cls(_block(g, ((k.data_ptr(), 2 * k_strides[0]), (v.data_ptr(), 2 * v_strides[0])), lens, counts), k.get_device())
+        words = _block(g, ((k.data_ptr(), 2 * k_strides[0]), (v.data_ptr(), 2 * v_strides[0])), lens, counts)
+        return cls(words, k.get_device(), k_strides[1] if shape[1] > 1 else None, io_dtype, (shape[2], shape[3]))
+
+    def check_rows(self, p: "L.AttnBatchParams"):
+        """Refuses a call that would read the prefixes' rows by another stride, type or number of heads than they have."""
+        if self.heads is None:
+            return
+        if self.kv_stride not in (None, p.kv_token_stride_elements):
+            _refuse(f"the prefixes' rows are {self.kv_stride} elements apart, the sessions' {p.kv_token_stride_elements}")
+        if self.io_dtype != p.io_dtype:
+            _refuse("the prefixes and the sessions must share one dtype")
+        if self.heads != (p.n_kv_heads, p.head_dim):
+            _refuse(f"the prefixes have {self.heads[0]} heads of {self.heads[1]}, the call {p.n_kv_heads} of {p.head_dim}")
 
     @classmethod
     def of(cls, groups) -> "PrefixTable":
@@ -491,6 +504,7 @@ class Attention:
         t.check_capacity()
         p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                      out_row_stride_elements, scale, io_dtype)
+        g.check_rows(p)
         self.context.check(L.lib().tt_attn_decode_shared_prefix(
             self.context.handle, self.context.stream(command_buffer), g.pointer, len(g), t.pointer, len(t), C.byref(p)))
 
