@@ -71,3 +71,32 @@ def test_prefix_tables_must_match_their_sessions():
     refused(shared, prefix, each, 64, 8, 2, io_dtype=tt.TT_BF16)
     # one row has no stride
     reaches_the_library(shared, tt.PrefixTable.over_cache(cache(1, 1, pad=1), cache(1, 1, pad=1), 1, 3), sessions(), 64, 8, 2)
+
+
+def test_session_tables_must_match_their_call():
+    weights = torch.zeros(3, 2, 20)
+    for call, tail in ((attention().encode_sink_window, (4, 8)), (attention().encode_accumulate, None)):
+        def args(t, hd=64, hq=8, hkv=2):
+            return (t, hd, hq, hkv) + tail if tail else (t, weights if hkv == 2 else torch.zeros(3, hkv, 20), hd, hq, hkv)
+        reaches_the_library(call, *args(sessions()))
+        wide = sessions(cache(pad=2), torch.zeros(3, 1, 12, 64, dtype=H)[:, :, :8])      # room for the heads that are not there
+        reaches_the_library(call, *args(wide))
+        refused(call, *args(wide, hkv=4))
+        refused(call, *args(wide, hq=12))
+        refused(call, *args(sessions(), hq=4))
+        refused(call, *args(sessions(), hd=32))
+        refused(call, *args(sessions(), hd=128, hq=4, hkv=1))
+        # what the tensors say is not to be contradicted, but may be said again
+        two = sessions(cache(pad=1), queries(rows=2))
+        reaches_the_library(call, *args(two), kv_token_stride_elements=192, q_row_stride_elements=512, out_row_stride_elements=512, io_dtype=tt.TT_F16)
+        for bad in (dict(kv_token_stride_elements=128), dict(q_row_stride_elements=520), dict(out_row_stride_elements=1024), dict(io_dtype=tt.TT_BF16)):
+            refused(call, *args(two), **bad)
+
+
+def test_one_row_has_no_stride():
+    call = attention().encode_sink_window
+    one = torch.zeros(3, 5, 8, 64, dtype=H)[:, 2:3]
+    reaches_the_library(call, sessions(q=one), 64, 8, 2, 4, 8, q_row_stride_elements=1024, out_row_stride_elements=520)
+    single = sessions(cache(rows=1), lens=1)
+    wide = tt.PrefixTable.over_cache(cache(1, pad=1), cache(1, pad=1), 7, 3)
+    reaches_the_library(attention().encode_shared_prefix, wide, single, 64, 8, 2)

@@ -242,9 +242,11 @@ class SessionTable:
     record = np.dtype([("q", "u8"), ("out", "u8"), ("k", "u8"), ("v", "u8"), ("seq_len", "u4"), ("q_rows", "u4"),
                        ("kv_start", "u4"), ("reserved", "u4")])
 
-    def __init__(self, words, longest=0, kv_stride=None, q_stride=None, out_stride=None, io_dtype=None, capacity=None, device=None):
+    def __init__(self, words, longest=0, kv_stride=None, q_stride=None, out_stride=None, io_dtype=None, capacity=None, device=None,
+                 heads=None):
         self.words, self.longest, self.kv_stride, self.q_stride, self.out_stride = words, longest, kv_stride, q_stride, out_stride
         self.io_dtype, self.capacity, self.device = io_dtype, capacity, device
+        self.heads = heads              # over whole tensors: (head_dim, n_q_heads, n_kv_heads)
 
     def __len__(self):
         return len(self.words) // 6
@@ -279,7 +281,12 @@ class SessionTable:
         places = ((q.data_ptr(), 2 * q_strides[0]), (out.data_ptr(), 2 * out_strides[0]),
                   (k.data_ptr(), 2 * k_strides[0]), (v.data_ptr(), 2 * v_strides[0]))
         words = _block(n, places, lens, q_rows, 1, None if slots is None else (None, None, slots, slots))
-        return cls(words, max(lens, default=0), k_strides[1], q_strides[1], out_strides[1], io_dtype, k_shape[1], device)
+        if q_shape[3] != k_shape[3]:
+            _refuse(f"q has heads of {q_shape[3]}, k of {k_shape[3]}")
+        kv_stride = k_strides[1] if k_shape[1] > 1 else None                       # one row has no stride
+        q_stride, out_stride = (q_strides[1], out_strides[1]) if q_rows > 1 else (None, None)
+        return cls(words, max(lens, default=0), kv_stride, q_stride, out_stride, io_dtype, k_shape[1], device,
+                   (k_shape[3], q_shape[2], k_shape[2]))
 
     @classmethod
     def of(cls, sessions) -> "SessionTable":
@@ -297,6 +304,15 @@ class SessionTable:
                out_row_stride_elements, scale, io_dtype) -> "L.AttnBatchParams":
         tight_q = num_q_heads * head_dim
         dtype = io_dtype if io_dtype is not None else self.io_dtype
+        if self.heads is not None:      # the call may repeat what the tensors say, not contradict it
+            if self.heads != (head_dim, num_q_heads, num_kv_heads):
+                _refuse("the tensors have heads of %d, %d of q, %d of k; " % self.heads + f"the call {head_dim}, {num_q_heads}, {num_kv_heads}")
+            if dtype != self.io_dtype:
+                _refuse("io_dtype is not the type of the tensors")
+            for name, given, known in (("kv_token", kv_token_stride_elements, self.kv_stride), ("q_row", q_row_stride_elements, self.q_stride),
+                                       ("out_row", out_row_stride_elements, self.out_stride)):
+                if given and known and given != known:
+                    _refuse(f"{name}_stride_elements {given}, but the tensors' rows are {known} apart")
         return L.AttnBatchParams(head_dim, num_q_heads, num_kv_heads,
                                  kv_token_stride_elements or self.kv_stride or num_kv_heads * head_dim,
                                  q_row_stride_elements or self.q_stride or tight_q,
@@ -502,6 +518,8 @@ class Attention:
         t, g = self._table(sessions), PrefixTable.of(groups)
         self.context.check_device(g)
         t.check_capacity()
+        if t.heads is not None and t.kv_stride is None:
+            kv_token_stride_elements = kv_token_stride_elements or g.kv_stride
         p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                      out_row_stride_elements, scale, io_dtype)
         g.check_rows(p)
