@@ -100,3 +100,56 @@ def test_one_row_has_no_stride():
     single = sessions(cache(rows=1), lens=1)
     wide = tt.PrefixTable.over_cache(cache(1, pad=1), cache(1, pad=1), 7, 3)
     reaches_the_library(attention().encode_shared_prefix, wide, single, 64, 8, 2)
+
+
+def test_expanded_tensors():
+    """Tensors that show one row, head or session several times: read where the layout can say so, else refused, never written."""
+    over = tt.SessionTable.over_cache
+    q, k = queries(rows=2), cache()
+    one_row = cache(rows=1).expand(3, 20, 2, 64)                # one row shown twenty times
+    with pytest.raises(tt.InvalidArgument):
+        over(q, q, one_row, one_row, 4)
+    with pytest.raises(tt.InvalidArgument):
+        tt.PrefixTable.over_cache(one_row, one_row, 4, 1)
+    with pytest.raises(tt.InvalidArgument):
+        over(queries(rows=1).expand(3, 2, 8, 64), q, k, k, 4)
+    with pytest.raises(tt.InvalidArgument):
+        over(q, queries(rows=1).expand(3, 2, 8, 64), k, k, 4)
+    with pytest.raises(tt.InvalidArgument):
+        over(q, queries(1, 2).expand(3, 2, 8, 64), k, k, 4)     # outputs of all sessions in one place
+    shared = cache(1).expand(3, 20, 2, 64)                      # one cache read by all sessions
+    over(queries(1, 2).expand(3, 2, 8, 64), q, shared, shared, 4)
+    tt.PrefixTable.over_cache(shared, shared, 4, 1)
+    accumulate, w = attention().encode_accumulate, torch.zeros(3, 2, 20)
+    reaches_the_library(accumulate, over(q, q, k, k, 4), w, 64, 8, 2, positions=w.int())
+    for bad in (w[:1].expand(3, 2, 20), w[:, :1].expand(3, 2, 20)):
+        refused(accumulate, over(q, q, k, k, 4), bad, 64, 8, 2)
+        refused(accumulate, over(q, q, k, k, 4), w, 64, 8, 2, positions=bad.int()[:1].expand(3, 2, 20))
+    single = torch.zeros(1, 2, 20)
+    reaches_the_library(accumulate, over(q[:1], q[:1], k[:1], k[:1], 4), single.expand(1, 2, 20), 64, 8, 2)
+
+
+def test_expanded_tensors_in_evictions():
+    k, w = cache(), torch.zeros(3, 2, 20)
+    p = w.int()
+    outs = dict(k_out=cache(rows=8), v_out=cache(rows=8), weights_out=torch.zeros(3, 2, 8), positions_out=torch.zeros(3, 2, 8, dtype=torch.int32))
+
+    def evict(k=k, w=w, **kw):
+        tt.evict_kv_rows(HostContext(), k, k, w, 20, 8, command_buffer=kw.pop("command_buffer"), **kw)
+    reaches_the_library(evict)
+    reaches_the_library(evict, positions=p, **outs)
+    shared, flat = cache(1).expand(3, 20, 2, 64), cache(rows=1).expand(3, 20, 2, 64)
+    refused(evict, k=shared)                                                            # in place, all sessions in one
+    refused(evict, k=flat)
+    refused(evict, k=flat, **outs)
+    reaches_the_library(evict, k=shared, w=w[:1].expand(3, 2, 20), positions=p[:1].expand(3, 2, 20), **outs)
+    refused(evict, w=w[:1].expand(3, 2, 20))
+    refused(evict, w=w[:, :1].expand(3, 2, 20))
+    refused(evict, positions=p[:1].expand(3, 2, 20))
+    for name in outs:
+        t = outs[name]
+        refused(evict, positions=p, **{**outs, name: t[:1].expand_as(t)})
+    for name in ("weights_out", "positions_out"):
+        refused(evict, positions=p, **{name: outs[name][:, :1].expand_as(outs[name])})
+    for name in ("k_out", "v_out"):
+        refused(evict, **{name: cache(rows=1).expand(3, 8, 2, 64)})

@@ -179,9 +179,17 @@ def _pair(what: str, a, b):
     shape, s, t = a.shape, a.stride(), b.stride()
     if b.shape != shape or len(shape) != 4 or s[3] != 1 or t[3] != 1 or s[2] != shape[3] or t[2] != shape[3]:
         _refuse(f"{what} must be [batch, rows, heads, head_dim] of one shape with tight rows")
+    if shape[1] > 1 and (s[1] < shape[2] * shape[3] or t[1] < shape[2] * shape[3]):
+        _refuse(f"the rows of {what} overlap")
     if b.dtype is not a.dtype or a.get_device() != b.get_device():
         _refuse(f"{what} must share one dtype and one device")
     return shape, s, t
+
+
+def _check_apart(what: str, n: int, *steps):
+    """Refuses results of n sessions that lie in one place (an expanded tensor)."""
+    if n > 1 and 0 in steps:
+        _refuse(f"the sessions share {what}")
 
 
 def _half_dtype(what: str, dtype) -> int:
@@ -272,6 +280,7 @@ class SessionTable:
         if k.dtype is not q.dtype or q.get_device() != device or v_strides[1] != k_strides[1]:
             _refuse("q and k must share one dtype and one device, and v be laid out like k")
         n, q_rows = q_shape[0], q_shape[1]
+        _check_apart("out", n, out_strides[0])
         if slots is None:
             if k_shape[0] < n:
                 _refuse(f"{n} sessions, but the cache has {k_shape[0]} slots")
@@ -654,12 +663,16 @@ def quantize_kv_rows(context: Context, source, destination, element_count: int, 
         group_size, tokens))
 
 
-def _statistic(name: str, t, dtype: str, n: int, num_kv_heads: int, context: Context):
+def _statistic(name: str, t, dtype: str, n: int, num_kv_heads: int, context: Context, written: bool = True):
     """A [sessions, n_kv_heads, rows] tensor of one 32-bit number per cache row: elements between its heads, and
     (address, bytes between sessions)."""
     shape, stride = t.shape, t.stride()
     if str(t.dtype) != dtype or len(shape) != 3 or shape[0] < n or shape[1] != num_kv_heads or (shape[2] > 1 and stride[2] != 1):
         _refuse(f"{name} must be {dtype} [{n}, {num_kv_heads}, rows], rows contiguous")
+    if num_kv_heads > 1 and stride[1] < shape[2]:
+        _refuse(f"the heads of {name} overlap")
+    if written:
+        _check_apart(name, n, stride[0])
     if t.get_device() != context.device:
         context.check_device(t)
     return stride[1] if num_kv_heads > 1 else shape[2], (t.data_ptr(), 4 * stride[0])
@@ -689,6 +702,10 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
     if most > capacity:
         _refuse(f"a session has more rows than the {capacity} of its slot")
     # destinations of K and V
+    if k_out is None:
+        _check_apart("k", n, k_strides[0])
+    if v_out is None:
+        _check_apart("v", n, v_strides[0])
     out_stride, at_k, at_v = in_stride, _nowhere, _nowhere
     if k_out is not None or v_out is not None:
         a, b = (v_out if k_out is None else k_out), (k_out if v_out is None else v_out)
@@ -697,15 +714,16 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
         if (a.dtype is not k.dtype or a.get_device() != k.get_device() or room[0] < n or room[1] < kept or room[2] != num_kv_heads or
                 room[3] != head_dim or b_strides[1] != out_stride):
             _refuse(f"k_out and v_out must hold the kept rows of {n} sessions, in the layout of k and v")
+        _check_apart("k_out or v_out", n, a_strides[0], b_strides[0])
         if k_out is not None:
             at_k = (k_out.data_ptr(), 2 * a_strides[0])
         if v_out is not None:
             at_v = (v_out.data_ptr(), 2 * b_strides[0])
     # the statistic and the positions, then where they go
-    stat, at_w = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context)
+    stat, at_w = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context, weights_out is None)
     at_p, at_wo, at_po, stat_out = _nowhere, _nowhere, _nowhere, None
     if positions is not None:
-        stride, at_p = _statistic("positions", positions, "torch.int32", n, num_kv_heads, context)
+        stride, at_p = _statistic("positions", positions, "torch.int32", n, num_kv_heads, context, positions_out is None)
         if stride != stat or positions.shape[2] < most:
             _refuse(f"positions must be laid out like weights and hold {most} rows")
     if weights.shape[2] < most:
