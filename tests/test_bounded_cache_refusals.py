@@ -153,3 +153,25 @@ def test_expanded_tensors_in_evictions():
         refused(evict, positions=p, **{name: outs[name][:, :1].expand_as(outs[name])})
     for name in ("k_out", "v_out"):
         refused(evict, **{name: cache(rows=1).expand(3, 8, 2, 64)})
+
+
+@pytest.mark.parametrize("bad", [-1, 2 ** 32, 2 ** 32 + 64, -2 ** 32 + 64, 1.5, None, "4"])
+def test_counts_that_32_bits_do_not_hold(bad):
+    k, q, w = cache(), queries(), torch.zeros(3, 2, 20)
+    sink = attention().encode_sink_window
+    refused(sink, sessions(), 64, 8, 2, bad, 8)
+    refused(sink, sessions(), 64, 8, 2, 4, bad)
+    refused(sink, sessions(), 64, 8, 2, 4, 8, ring_capacity=bad)
+    for i in range(3):
+        refused(tt.evict_kv_rows, HostContext(), k, k, w, 20, *[bad if i == x else 2 + 4 * (x == 0) for x in range(3)])
+    p = tt.PrefillAttentionParams(0, 3, 64, 8, 2, 3, 8, 128, 512, 512, 0.125)
+    prefill = tt.PrefillAttention(HostContext()).encode_sink_window
+    reaches_the_library(prefill, q, k, k, q, p, 4)
+    refused(prefill, q, k, k, q, p, bad)
+    refused(prefill, q, k, k, q, p, 4, kv_ring_capacity=bad)
+
+
+def test_counts_of_other_integer_types():
+    import numpy as np
+    reaches_the_library(attention().encode_sink_window, sessions(), 64, 8, 2, np.int64(4), torch.tensor(8), ring_capacity=np.uint32(16))
+    reaches_the_library(tt.evict_kv_rows, HostContext(), cache(), cache(), torch.zeros(3, 2, 20), 20, np.int32(8), np.int64(1), True)

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 from array import array
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -212,6 +213,19 @@ def _counts(name: str, values, n: int) -> array:
         found = None
     if found is None or len(found) != n:
         _refuse(f"{name} must be {n} numbers in 0..2^32-1")
+    return found
+
+
+def _count(name: str, value) -> int:
+    """A number in 0..2^32-1, which is what ctypes would make of any other without a word."""
+    if type(value) is int and 0 <= value <= 0xffffffff:
+        return value
+    try:
+        found = operator.index(value)
+    except TypeError:
+        found = -1
+    if not 0 <= found <= 0xffffffff:
+        _refuse(f"{name} must be in 0..2^32-1, not {value!r}")
     return found
 
 
@@ -511,6 +525,7 @@ class Attention:
         (tt_attn_decode_sink_window). `sessions`: DecodeSession list or SessionTable; with `ring_capacity` R a
         session's cache has sink_tokens + R rows and key j >= sink_tokens is row sink_tokens + (j - sink_tokens) % R."""
         t = self._table(sessions)
+        sink_tokens, window, ring_capacity = _count("sink_tokens", sink_tokens), _count("window", window), _count("ring_capacity", ring_capacity)
         t.check_capacity(sink_tokens + ring_capacity if ring_capacity else None)
         p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                      out_row_stride_elements, scale, io_dtype)
@@ -689,6 +704,7 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
     positions: int32 like weights, None = row j holds position j; end_positions: position of the next token (default:
     rows). *_out: None for in place, or tensors of the same kind with room for min(rows, budget) rows. Afterwards
     session i has min(rows[i], budget) rows per head."""
+    budget, sink_tokens, recent_tokens = _count("budget", budget), _count("sink_tokens", sink_tokens), _count("recent_tokens", recent_tokens)
     shape, k_strides, v_strides = _pair("k and v", k, v)
     _half_dtype("k and v", k.dtype)
     context.check_device(k)
@@ -797,6 +813,7 @@ class PrefillAttention:
         """Causal prefill over the first `sink_tokens` keys and a sliding window of params.sliding_window
         (tt_attn_prefill_sink_window); a ring lies behind the sinks' rows as in Attention.encode_sink_window."""
         self.context.check_device(q, k, v, out)
+        sink_tokens, kv_ring_capacity = _count("sink_tokens", sink_tokens), _count("kv_ring_capacity", kv_ring_capacity)
         self.context.check(L.lib().tt_attn_prefill_sink_window(
             self.context.handle, self.context.stream(command_buffer), _addr(q, q_offset), _addr(k, k_offset),
             _addr(v, v_offset), _addr(out, out_offset), C.byref(params.to_c()), sink_tokens, kv_ring_capacity,
