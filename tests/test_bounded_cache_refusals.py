@@ -175,3 +175,41 @@ def test_counts_of_other_integer_types():
     import numpy as np
     reaches_the_library(attention().encode_sink_window, sessions(), 64, 8, 2, np.int64(4), torch.tensor(8), ring_capacity=np.uint32(16))
     reaches_the_library(tt.evict_kv_rows, HostContext(), cache(), cache(), torch.zeros(3, 2, 20), 20, np.int32(8), np.int64(1), True)
+
+
+class ElsewhereTensor:
+    """What a list of sessions looks at in a tensor, on a device of its own."""
+    dtype = H
+
+    def __init__(self, device):
+        self.get_device = lambda: device
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+def test_lists_over_tensors_of_another_device():
+    a, here, there = attention(), ElsewhereTensor(-1), ElsewhereTensor(1)
+
+    def session(**kw):
+        return tt.DecodeSession(**{**dict(q=here, out=here, k=here, v=here, seq_len=4), **kw})
+    reaches_the_library(a.encode_sink_window, [session()], 64, 8, 2, 4, 8)
+    reaches_the_library(a.encode_sink_window, [session(q=1 << 20, out=1 << 20, k=1 << 20, v=1 << 20)], 64, 8, 2, 4, 8)       # addresses
+    weights = torch.zeros(2, 2, 20)
+    prefix = [tt.PrefixGroup(here, here, 7, 2)]
+    reaches_the_library(a.encode_shared_prefix, prefix, [session()] * 2, 64, 8, 2)
+    for name in ("q", "out", "k", "v"):
+        some = [session(), session(**{name: there})]
+        refused(a.encode_sink_window, some, 64, 8, 2, 4, 8)
+        refused(a.encode_accumulate, some, weights, 64, 8, 2)
+        refused(a.encode_shared_prefix, prefix, some, 64, 8, 2)
+    refused(a.encode_shared_prefix, [tt.PrefixGroup(there, here, 7, 1), tt.PrefixGroup(here, here, 7, 1)], [session()] * 2, 64, 8, 2)
+    refused(a.encode_shared_prefix, [tt.PrefixGroup(here, there, 7, 2)], [session()] * 2, 64, 8, 2)
+
+
+def test_lists_with_lengths_that_32_bits_do_not_hold():
+    a, k = attention(), cache()
+    for bad in (-1, 2 ** 32, None):
+        refused(a.encode_sink_window, [tt.DecodeSession(k, k, k, k, bad)], 64, 8, 2, 4, 8)
+        refused(a.encode_sink_window, [tt.DecodeSession(k, k, k, k, 4, q_rows=bad)], 64, 8, 2, 4, 8)
+        refused(a.encode_shared_prefix, [tt.PrefixGroup(k, k, bad, 1)], [tt.DecodeSession(k, k, k, k, 4)], 64, 8, 2)

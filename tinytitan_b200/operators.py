@@ -174,6 +174,14 @@ def _refuse(message: str):
     raise L.InvalidArgument(L.TT_ERR_INVALID_ARG, message)
 
 
+def _device_of(buffers):
+    """The device of those that are tensors (None: all are addresses)."""
+    found = {t.get_device() for t in buffers if hasattr(t, "get_device")}
+    if len(found) > 1:
+        _refuse(f"the buffers of a call are on devices {sorted(found)}")
+    return found.pop() if found else None
+
+
 def _pair(what: str, a, b):
     """Of two [batch, rows, heads, head_dim] tensors of one shape, type and device with tight rows: the shape and their
     strides."""
@@ -319,9 +327,10 @@ class SessionTable:
         r = np.frombuffer(words, dtype=cls.record)
         for i, s in enumerate(sessions):
             r[i] = (_addr(s.q, s.q_offset), _addr(s.out, s.out_offset), _addr(s.k, s.k_offset), _addr(s.v, s.v_offset),
-                    s.seq_len, s.q_rows, s.kv_start, 0)
+                    _count("seq_len", s.seq_len), _count("q_rows", s.q_rows), _count("kv_start", s.kv_start), 0)
         return cls(words, max((s.seq_len for s in sessions), default=0),
-                   io_dtype=_dtype_of(sessions[0].q) if len(sessions) else None)
+                   io_dtype=_dtype_of(sessions[0].q) if len(sessions) else None,
+                   device=_device_of(t for s in sessions for t in (s.q, s.out, s.k, s.v)))
 
     def params(self, attention, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
                out_row_stride_elements, scale, io_dtype) -> "L.AttnBatchParams":
@@ -405,8 +414,8 @@ class PrefixTable:
         words = array("Q", bytes(24 * len(groups)))
         r = np.frombuffer(words, dtype=cls.record)
         for i, g in enumerate(groups):
-            r[i] = (_addr(g.k, g.k_offset), _addr(g.v, g.v_offset), g.prefix_len, g.n_sessions)
-        return cls(words)
+            r[i] = (_addr(g.k, g.k_offset), _addr(g.v, g.v_offset), _count("prefix_len", g.prefix_len), _count("n_sessions", g.n_sessions))
+        return cls(words, _device_of(t for g in groups for t in (g.k, g.v)))
 
 
 class Attention:
