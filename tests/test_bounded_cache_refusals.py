@@ -213,3 +213,14 @@ def test_lists_with_lengths_that_32_bits_do_not_hold():
         refused(a.encode_sink_window, [tt.DecodeSession(k, k, k, k, bad)], 64, 8, 2, 4, 8)
         refused(a.encode_sink_window, [tt.DecodeSession(k, k, k, k, 4, q_rows=bad)], 64, 8, 2, 4, 8)
         refused(a.encode_shared_prefix, [tt.PrefixGroup(k, k, bad, 1)], [tt.DecodeSession(k, k, k, k, 4)], 64, 8, 2)
+
+
+def test_plain_decode_takes_session_tables():
+    a = attention()
+    reaches_the_library(a.encode_batched, sessions(), 64, 8, 2)
+    refused(a.encode_batched, sessions(), 64, 8, 4)
+    refused(a.encode_batched, sessions(lens=21), 64, 8, 2)
+    words, n, p = a.prepare_batch(sessions(cache(pad=1), queries(rows=2), lens=[4, 5, 6]), 64, 8, 2)
+    assert n == 3 and [s.seq_len for s in words] == [4, 5, 6] and {s.q_rows for s in words} == {2}
+    assert (p.kv_token_stride_elements, p.q_row_stride_elements, p.io_dtype) == (192, 512, tt.TT_F16)
+    assert a.prepare_batch(sessions(torch.zeros(0, 20, 2, 64, dtype=H), queries(0)), 64, 8, 2)[1] == 0

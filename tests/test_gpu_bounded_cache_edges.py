@@ -4,6 +4,7 @@ import torch
 
 import tinytitan_b200 as tt
 from bounded_cache_reference import attend
+from gpu_util import context
 from test_gpu_bounded_cache import BF16, F16, NAN, check, normal, run_accumulate, run_sink_decode
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +97,20 @@ def test_evict_refused_calls_move_nothing():
     torch.cuda.synchronize()
     assert not any(torch.equal(w[i], before[2][i]) for i in range(n))
     ctx.close()
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+def test_plain_decode_over_session_tables(rows):
+    # the rows that an eviction leaves, by plain decode: a table gives what a list of sessions does
+    n, hq, hkv, hd, cap = 5, 16, 2, 256, 300
+    q, k, v = (normal(i, *x).cuda() for i, x in enumerate([(n, rows, hq, hd), (n, cap, hkv, hd), (n, cap, hkv, hd)]))
+    w, lens, a = torch.rand(n, hkv, cap, generator=torch.Generator().manual_seed(3)).cuda(), [300, 150, 64, 99, 7], tt.Attention(context())
+    tt.evict_kv_rows(context(), k, v, w, lens, 64)
+    left = [min(x, 64) for x in lens]
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    a.encode_batched([tt.DecodeSession(q[i], outs[0][i], k[i], v[i], left[i], rows) for i in range(n)], hd, hq, hkv)
+    a.encode_batched(tt.SessionTable.over_cache(q, outs[1], k, v, left), hd, hq, hkv)
+    a.encode_prepared(a.prepare_batch(tt.SessionTable.over_cache(q, outs[2], k, v, left), hd, hq, hkv))
+    torch.cuda.synchronize()
+    assert context().poll_status() == 0
+    assert outs[0].any() and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])

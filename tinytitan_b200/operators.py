@@ -485,6 +485,11 @@ class Attention:
                        kv_token_stride_elements=None, q_row_stride_elements=None, out_row_stride_elements=None,
                        scale=None, io_dtype=None, command_buffer=None):
         """All rows of a batched decode / verify step in one launch pair (tt_attn_decode_batched)."""
+        if isinstance(sessions, SessionTable):
+            batch = self.prepare_batch(sessions, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
+                                       out_row_stride_elements, scale, io_dtype)
+            self.encode_prepared(batch, self.context.stream(command_buffer))
+            return
         n = len(sessions)
         arr = (L.AttnSession * max(n, 1))()
         for i, s in enumerate(sessions):
@@ -504,6 +509,12 @@ class Attention:
                       scale=None, io_dtype=None):
         """The argument block of encode_batched built once, for a step that is replayed with the
         same buffers (the reference re-encodes the same bindings every token as well)."""
+        if isinstance(sessions, SessionTable):
+            t = self._table(sessions)
+            t.check_capacity()
+            p = t.params(self, head_dim, num_q_heads, num_kv_heads, kv_token_stride_elements, q_row_stride_elements,
+                         out_row_stride_elements, scale, io_dtype)
+            return ((L.AttnSession * max(len(t), 1)).from_buffer_copy(t.words if len(t) else bytes(C.sizeof(L.AttnSession))), len(t), p)
         n = len(sessions)
         arr = (L.AttnSession * max(n, 1))()
         for i, s in enumerate(sessions):
