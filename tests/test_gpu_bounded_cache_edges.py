@@ -5,7 +5,7 @@ import torch
 import tinytitan_b200 as tt
 from bounded_cache_reference import attend
 from gpu_util import context
-from test_gpu_bounded_cache import BF16, F16, NAN, check, normal, run_accumulate, run_sink_decode
+from test_gpu_bounded_cache import BF16, F16, NAN, check, normal, run_accumulate, run_evict, run_sink_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,10 @@ def test_plain_decode_over_session_tables(rows):
     torch.cuda.synchronize()
     assert context().poll_status() == 0
     assert outs[0].any() and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_more_keys_than_a_cluster_holds(in_place):
+    # 16 CTAs hold 800,000 selection keys; beyond, every round reads the statistic and the positions again
+    run_evict([810_003, 800_000], 500_000, 4, 1000, hkv=1, hd=64, in_place=in_place)
+    run_evict([810_003], 900, 0, 0, hkv=1, hd=64, in_place=in_place, mix=True, keep_positions=False)
