@@ -5,7 +5,7 @@ import torch
 import tinytitan_b200 as tt
 from bounded_cache_reference import attend
 from gpu_util import context
-from test_gpu_bounded_cache import BF16, F16, NAN, check, normal, run_accumulate, run_evict, run_sink_decode
+from test_gpu_bounded_cache import BF16, F16, NAN, check, normal, run_accumulate, run_evict, run_prefix, run_sink_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +121,17 @@ def test_evict_more_keys_than_a_cluster_holds(in_place):
     # 16 CTAs hold 800,000 selection keys; beyond, every round reads the statistic and the positions again
     run_evict([810_003, 800_000], 500_000, 4, 1000, hkv=1, hd=64, in_place=in_place)
     run_evict([810_003], 900, 0, 0, hkv=1, hd=64, in_place=in_place, mix=True, keep_positions=False)
+
+
+# Tables of 24 and of 72 groups travel in the parameters: prefixes and sessions on both sides, draft rows of 12 and 36 sessions.
+@pytest.mark.parametrize("sessions", [16, 17, 32])
+def test_prefix_tables_on_both_sides_of_their_sizes(sessions):
+    per = [sessions // 8 + (i < sessions % 8) for i in range(8)]
+    run_prefix(128, 16, 2, F16, [130 + 9 * i for i in range(8)], per, [1] * sessions, [(11 * i) % 140 for i in range(sessions)])
+    run_prefix(256, 16, 2, BF16, [7 + 40 * i for i in range(8)], per, [3] * sessions, [2 + (13 * i) % 90 for i in range(sessions)])
+
+
+@pytest.mark.parametrize("sessions", [12, 13, 36, 37])
+def test_draft_rows_on_both_sides_of_the_table_sizes(sessions):
+    run_sink_decode(128, 16, 2, F16, 4, [700 + 31 * (i % 9) for i in range(sessions)], 4, 400, 0)
+    run_sink_decode(256, 16, 2, BF16, 3, [900 + 31 * (i % 9) for i in range(sessions)], 3, 300, 333)

@@ -27,7 +27,9 @@ namespace {
 
 constexpr uint32_t kParamGroups = 8;
 constexpr uint32_t kFusedSessions = kParamSessions;                // sessions whose own rows may join the prefix pass
-constexpr uint32_t kTableGroups = kParamGroups + kFusedSessions;
+// What the parameters have room for: a launch pays for their size (25 KB against 9: 1.4 us of host time a launch, a prefix call of
+// one session that is waited for 27.9 us against 25.0), so a form takes the smaller table where that is enough.
+constexpr uint32_t kTableGroups = kParamGroups + kFusedSessions, kFewGroups = kParamGroups + 16;
 
 // Query rows of one session, in call order.
 struct PrefixSession {
@@ -56,16 +58,18 @@ struct alignas(64) PrefixMaps { unsigned char m[2][128]; };    // K and V tensor
 
 // Calls of up to kParamGroups groups and kParamSessions sessions carry their tables and tensor maps in the kernel
 // parameters; larger ones read the copies the host uploaded.
+template <uint32_t GROUPS>
 struct alignas(64) PrefixTable {
     uint32_t n_groups, n_sessions;
     uint32_t in_params;
-    uint32_t item_begin[kTableGroups];
-    PrefixGroup g[kTableGroups];
-    PrefixMaps maps[kTableGroups];
+    uint32_t item_begin[GROUPS];
+    PrefixGroup g[GROUPS];
+    PrefixMaps maps[GROUPS];
     PrefixSession s[kParamSessions];
 };
 
 // The prefix pass's items for attn_rows_kernel.
+template <uint32_t GROUPS>
 struct PrefixForm {
     static constexpr bool kPartials = true;
     // what every CTA reads first stands first and together: every line of the parameters it touches costs a miss, some 600
@@ -76,7 +80,7 @@ struct PrefixForm {
     const PrefixSession *sessions;
     const PrefixMaps *maps;
     float *part_o, *part_m, *part_l;
-    PrefixTable table;
+    PrefixTable<GROUPS> table;
 
     struct Item : RowsItem {
         const CUtensorMap *maps;
@@ -177,27 +181,29 @@ struct PrefixForm {
 // every session is a group, and its keys are numbered in whole halves of 64: those over [0, sink), those of the windows from
 // `base` on up to the ring's end, those behind it. Nothing that no row sees is multiplied: V has a map for each of the three
 // ranges that ends with it. (What K has there makes scores that are replaced.)
-constexpr uint32_t kSinkRowSessions = kTableGroups / 2;      // two groups' maps each
-struct SinkRowsForm : PrefixForm {
+template <uint32_t GROUPS>
+struct SinkRowsForm : PrefixForm<GROUPS> {
+    using Base = PrefixForm<GROUPS>;
+    static constexpr uint32_t kSessions = GROUPS / 2;            // two groups' maps each
     uint32_t sink, window;
     // keys base .. base + straight - 1 are rows first_row on, the later ones rows sink on
-    struct Session { uint32_t seq_len, q_rows, base, windowed, first_row, straight; } session[kSinkRowSessions];
+    struct Session { uint32_t seq_len, q_rows, base, windowed, first_row, straight; } session[kSessions];
 
-    struct Item : PrefixForm::Item {
+    struct Item : Base::Item {
         Session s;
         uint32_t sink_keys, straight_keys;      // key numbers that stand for the sinks, for the first range of the window
         const CUtensorMap *v_ends;              // of the sinks, of the range behind the ring's end
     };
     __device__ __forceinline__ Item item(uint32_t block, int hd, int rows) const {
         Item it;
-        static_cast<PrefixForm::Item &>(it) = PrefixForm::item(block, hd, rows);
+        static_cast<typename Base::Item &>(it) = Base::item(block, hd, rows);
         it.s = session[it.session_begin];
         it.sink_keys = it.s.windowed ? (sink + 63) / 64 * 64 : 0u;
         // with nothing behind the ring's end the first range also takes the numbers past its last half: of a cache without sinks
         // they would else be row 0 of the last range's map, which cannot be empty, and a spare half of the last tile would read it
         const bool behind = it.s.seq_len - it.s.base > it.s.straight;
         it.straight_keys = behind ? (it.s.straight + 63) / 64 * 64 : 0xffffffffu;
-        it.v_ends = reinterpret_cast<const CUtensorMap *>(table.maps[kSinkRowSessions + it.session_begin].m[0]);
+        it.v_ends = reinterpret_cast<const CUtensorMap *>(this->table.maps[kSessions + it.session_begin].m[0]);
         return it;
     }
     __device__ __forceinline__ const CUtensorMap *box(const Item &it, uint32_t tile, uint32_t half, bool is_k, int &row) const {
@@ -224,7 +230,7 @@ struct SinkRowsForm : PrefixForm {
         return key + kBK + it.s.q_rows - 1 > it.s.seq_len || (it.s.windowed && key < max(sink, it.s.seq_len - window));
     }
     __device__ __forceinline__ void visible(const Item &it, uint32_t row, uint32_t tile, uint32_t (&bits)[4]) const {
-        const uint32_t w = min((it.row0 + row) / (n_q_heads / n_kv_heads), it.s.q_rows - 1);
+        const uint32_t w = min((it.row0 + row) / (this->n_q_heads / this->n_kv_heads), it.s.q_rows - 1);
         const uint32_t end = it.s.seq_len - (it.s.q_rows - 1 - w);
         const uint32_t from = it.s.windowed ? max(sink, end > window ? end - window : 0u) : 0u;
 #pragma unroll
@@ -323,9 +329,9 @@ cudaError_t launch_prefix(cudaStream_t stream, uint32_t head_dim, uint32_t rows,
 #undef TT_X
 }
 
-template <typename T>
+template <typename T, class Form>
 cudaError_t launch_merge(cudaStream_t stream, uint32_t head_dim, uint32_t rows, uint32_t parts, const MergeTable &table, const MergeSession *dev,
-                         const uint32_t *dev_first_row, uint32_t n_sessions, const PrefixForm &kp, const TTDecodeForm &own,
+                         const uint32_t *dev_first_row, uint32_t n_sessions, const Form &kp, const TTDecodeForm &own,
                          uint32_t n_q_heads, uint32_t out_row_stride, uint32_t sm_count) {
     uint32_t grid = 0;
     const uint32_t groups = merge_groups(rows, parts, head_dim, sm_count, &grid);
@@ -386,45 +392,14 @@ TT_API int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_
     return TT_OK;
 }
 
-TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const tt_attn_prefix *groups, uint32_t n_groups,
-                                        const tt_attn_session *sessions, uint32_t n_sessions, const tt_attn_batch_params *params) {
-    TT_ENTER(ctx);
-    if (params == nullptr || ((sessions == nullptr || groups == nullptr) && n_sessions != 0))
-        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "groups, sessions and params must not be null");
-    if (n_sessions > ctx->max_sessions)
-        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_sessions %u exceeds the context's max_sessions %u", n_sessions, ctx->max_sessions);
-    if (n_groups > ctx->max_sessions)
-        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_groups %u exceeds the context's max_sessions %u", n_groups, ctx->max_sessions);
-    if (n_sessions == 0) return TT_OK;
+// The launches of a call whose groups are checked; `fused`: the sessions' own rows are groups of the prefix pass too.
+template <uint32_t GROUPS>
+static int shared_prefix(tt_context *ctx, tt_stream stream, const tt_attn_prefix *groups, uint32_t n_groups, const tt_attn_session *sessions,
+                         uint32_t n_sessions, const tt_attn_batch_params *params, bool in_params, bool fused) {
     const tt_attn_batch_params &q = *params;
-    if (q.n_kv_heads == 0 || q.n_q_heads == 0 || q.n_q_heads % q.n_kv_heads != 0)
-        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_q_heads must be a multiple of n_kv_heads");
-    if (q.head_dim != 64 && q.head_dim != 128 && q.head_dim != 256)
-        return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "decode attention supports head_dim 64/128/256, got %u", q.head_dim);
-    if (!(q.scale > 0.f)) return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "a shared prefix needs a positive scale");
-    if (q.kv_token_stride_elements % 8 || q.kv_token_stride_elements < q.n_kv_heads * q.head_dim)
-        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "kv_token_stride_elements must hold a row and be a multiple of 8");
-    uint64_t covered = 0;
-    for (uint32_t g = 0; g < n_groups; ++g) {
-        if (groups[g].n_sessions == 0) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "group %u has no sessions", g);
-        if (groups[g].prefix_len > (uint32_t)INT32_MAX) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "group %u: the prefix is too long", g);
-        if (groups[g].prefix_len != 0 && (groups[g].k == nullptr || groups[g].v == nullptr))
-            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "group %u has a null buffer", g);
-        if (((uintptr_t)groups[g].k | (uintptr_t)groups[g].v) & 15)
-            return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "group %u: buffers must be 16-byte aligned", g);
-        covered += groups[g].n_sessions;
-    }
-    if (covered != n_sessions)
-        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "the groups have %llu sessions, the call %u", (unsigned long long)covered, n_sessions);
-
-    const bool in_params = n_groups <= kParamGroups && n_sessions <= kParamSessions;
-    if (!in_params && tt_stream_is_capturing((cudaStream_t)stream))
-        return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE,
-                            "more than %u groups or %u sessions cannot be captured: their tables are uploaded from host memory",
-                            kParamGroups, kParamSessions);
     // host tables: the parameter blocks, or the staging copy of what is uploaded
-    static thread_local PrefixForm kp;
-    PrefixTable &table = kp.table;
+    static thread_local PrefixForm<GROUPS> kp;
+    PrefixTable<GROUPS> &table = kp.table;
     static thread_local MergeTable merge;
     const size_t off_groups = sizeof(PrefixMaps) * (size_t)n_groups, off_sessions = off_groups + sizeof(PrefixGroup) * (size_t)n_groups;
     const size_t off_merge = (off_sessions + sizeof(PrefixSession) * (size_t)n_sessions + 15) / 16 * 16;
@@ -459,26 +434,8 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
         d.n_parts = 0; d.partial_base = 0; d.ring_capacity = 0; d.keep = nullptr; d.row_index = nullptr;
         total_rows += s.q_rows;
     }
-    // The sessions' own rows as groups of one session each in the prefix pass: one launch less, no second pass that starts
-    // when the first one ends, and the tensor cores for draft rows. Up to 16 sessions always: 4 of short keys 18.5 -> 13 us,
-    // 16 of 4000 to 8000 keys 52 -> 48, of 4 rows of 16 heads 176 -> 82. Up to 64, whose maps and groups make the parameters
-    // 26 KB (10 us more of host time), with more than the 16 packed rows a split-KV item takes: 64 sessions of 4 rows and 800
-    // to 1600 keys 220 -> 123 us, of 4 to 300 98 -> 94. Up to 32 otherwise unless a few rows would have items of 256:
-    // head_dim 128, 32 sessions of 800 to 1600 keys 29 -> 23; head_dim 256, 16/2 heads, 4000 to 8000 keys 79 -> 115.
-    bool fused = in_params && n_sessions <= 16;
-    if (in_params && !fused) {
-        uint32_t group_rows = 0, most_rows = 0, most_own = 0;
-        for (uint32_t g = 0, i = 0; g < n_groups; ++g, group_rows = 0)
-            for (uint32_t x = 0; x < groups[g].n_sessions; ++x, ++i) {
-                group_rows += sessions[i].q_rows;
-                most_rows = std::max(most_rows, group_rows);
-                most_own = std::max(most_own, sessions[i].q_rows);
-            }
-        const uint32_t heads = q.n_q_heads / q.n_kv_heads, rows_tile = rows_per_tile(&most_rows, 1, heads, q.head_dim);
-        fused = most_own * heads > 16 || (n_sessions <= 32 && rows_tile < 256);
-    }
     const uint32_t n_table = fused ? n_groups + n_sessions : n_groups;
-    uint32_t fused_lens[kTableGroups], fused_rows[kTableGroups];
+    uint32_t fused_lens[GROUPS], fused_rows[GROUPS];
     uint32_t *lens = fused ? fused_lens : ctx->h_prefix_lens, *rows = fused ? fused_rows : ctx->h_prefix_rows;
     for (uint32_t g = 0, first = 0; g < n_groups; ++g) {
         lens[g] = groups[g].prefix_len;
@@ -621,6 +578,65 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
     return TT_OK;
 }
 
+TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const tt_attn_prefix *groups, uint32_t n_groups,
+                                        const tt_attn_session *sessions, uint32_t n_sessions, const tt_attn_batch_params *params) {
+    TT_ENTER(ctx);
+    if (params == nullptr || ((sessions == nullptr || groups == nullptr) && n_sessions != 0))
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "groups, sessions and params must not be null");
+    if (n_sessions > ctx->max_sessions)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_sessions %u exceeds the context's max_sessions %u", n_sessions, ctx->max_sessions);
+    if (n_groups > ctx->max_sessions)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_groups %u exceeds the context's max_sessions %u", n_groups, ctx->max_sessions);
+    if (n_sessions == 0) return TT_OK;
+    const tt_attn_batch_params &q = *params;
+    if (q.n_kv_heads == 0 || q.n_q_heads == 0 || q.n_q_heads % q.n_kv_heads != 0)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "n_q_heads must be a multiple of n_kv_heads");
+    if (q.head_dim != 64 && q.head_dim != 128 && q.head_dim != 256)
+        return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "decode attention supports head_dim 64/128/256, got %u", q.head_dim);
+    if (!(q.scale > 0.f)) return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "a shared prefix needs a positive scale");
+    if (q.kv_token_stride_elements % 8 || q.kv_token_stride_elements < q.n_kv_heads * q.head_dim)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "kv_token_stride_elements must hold a row and be a multiple of 8");
+    uint64_t covered = 0;
+    for (uint32_t g = 0; g < n_groups; ++g) {
+        if (groups[g].n_sessions == 0) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "group %u has no sessions", g);
+        if (groups[g].prefix_len > (uint32_t)INT32_MAX) return tt_set_error(ctx, TT_ERR_INVALID_ARG, "group %u: the prefix is too long", g);
+        if (groups[g].prefix_len != 0 && (groups[g].k == nullptr || groups[g].v == nullptr))
+            return tt_set_error(ctx, TT_ERR_INVALID_ARG, "group %u has a null buffer", g);
+        if (((uintptr_t)groups[g].k | (uintptr_t)groups[g].v) & 15)
+            return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE, "group %u: buffers must be 16-byte aligned", g);
+        covered += groups[g].n_sessions;
+    }
+    if (covered != n_sessions)
+        return tt_set_error(ctx, TT_ERR_INVALID_ARG, "the groups have %llu sessions, the call %u", (unsigned long long)covered, n_sessions);
+
+    const bool in_params = n_groups <= kParamGroups && n_sessions <= kParamSessions;
+    if (!in_params && tt_stream_is_capturing((cudaStream_t)stream))
+        return tt_set_error(ctx, TT_ERR_UNSUPPORTED_SHAPE,
+                            "more than %u groups or %u sessions cannot be captured: their tables are uploaded from host memory",
+                            kParamGroups, kParamSessions);
+    // The sessions' own rows as groups of one session each in the prefix pass: one launch less, no second pass that starts
+    // when the first one ends, and the tensor cores for draft rows. Up to 16 sessions always: 4 of short keys 18.5 -> 13 us,
+    // 16 of 4000 to 8000 keys 52 -> 48, of 4 rows of 16 heads 176 -> 82. Up to 64, whose maps and groups make the parameters
+    // 26 KB (10 us more of host time), with more than the 16 packed rows a split-KV item takes: 64 sessions of 4 rows and 800
+    // to 1600 keys 220 -> 123 us, of 4 to 300 98 -> 94. Up to 32 otherwise unless a few rows would have items of 256:
+    // head_dim 128, 32 sessions of 800 to 1600 keys 29 -> 23; head_dim 256, 16/2 heads, 4000 to 8000 keys 79 -> 115.
+    bool fused = in_params && n_sessions <= 16;
+    if (in_params && !fused) {
+        uint32_t group_rows = 0, most_rows = 0, most_own = 0;
+        for (uint32_t g = 0, i = 0; g < n_groups; ++g, group_rows = 0)
+            for (uint32_t x = 0; x < groups[g].n_sessions; ++x, ++i) {
+                group_rows += sessions[i].q_rows;
+                most_rows = std::max(most_rows, group_rows);
+                most_own = std::max(most_own, sessions[i].q_rows);
+            }
+        const uint32_t heads = q.n_q_heads / q.n_kv_heads, rows_tile = rows_per_tile(&most_rows, 1, heads, q.head_dim);
+        fused = most_own * heads > 16 || (n_sessions <= 32 && rows_tile < 256);
+    }
+    return !in_params || n_groups + (fused ? n_sessions : 0u) <= kFewGroups
+               ? shared_prefix<kFewGroups>(ctx, stream, groups, n_groups, sessions, n_sessions, params, in_params, fused)
+               : shared_prefix<kTableGroups>(ctx, stream, groups, n_groups, sessions, n_sessions, params, in_params, fused);
+}
+
 // Whether the tensor cores take a sink call: more packed rows than a split-KV item has (which reads K and V again for every
 // 16 of them; 16 sessions of 4 rows of 8 heads, 1024 keys: 25.2 us against 14.9, 4096 keys 70 against 34; of 16 heads 143 against
 // 35). Sessions beyond one launch's tables need more than a tile or two of keys (64 sessions of 64 keys,
@@ -632,15 +648,18 @@ bool tt_sink_rows_form(const TTDecodeSession *sessions, uint32_t n_sessions, con
         most_rows = std::max(most_rows, sessions[i].q_rows);
         most_keys = std::max(most_keys, sessions[i].seq_len - std::min(sessions[i].seq_len, sessions[i].kv_start));
     }
-    return most_rows * (p->n_q_heads / p->n_kv_heads) > 16 && (n_sessions <= kSinkRowSessions || most_keys > 2 * kBK);
+    return most_rows * (p->n_q_heads / p->n_kv_heads) > 16 && (n_sessions <= SinkRowsForm<kTableGroups>::kSessions || most_keys > 2 * kBK);
 }
 
 // One launch and merge of that form.
+template <uint32_t GROUPS>
 static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form,
                             const tt_attn_batch_params *p) {
     const tt_attn_batch_params &q = *p;
     const uint32_t group = q.n_q_heads / q.n_kv_heads;
-    static thread_local SinkRowsForm f;
+    using Form = SinkRowsForm<GROUPS>;
+    constexpr uint32_t kSessions = Form::kSessions;
+    static thread_local Form f;
     static thread_local MergeTable merge;
     f.n_q_heads = q.n_q_heads; f.n_kv_heads = q.n_kv_heads; f.q_row_stride = q.q_row_stride_elements; f.behind_own_rows = 0;
     f.groups = nullptr; f.sessions = nullptr; f.maps = nullptr;
@@ -648,10 +667,10 @@ static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecode
     f.table.n_groups = n_sessions; f.table.n_sessions = n_sessions; f.table.in_params = 1;
     merge.n = n_sessions; merge.q_rows = sessions[0].q_rows;
     // the longest first
-    uint32_t order[kSinkRowSessions] = {}, keys[kSinkRowSessions] = {}, lens[kSinkRowSessions] = {}, rows[kSinkRowSessions] = {}, total_rows = 0;
+    uint32_t order[kSessions] = {}, keys[kSessions] = {}, lens[kSessions] = {}, rows[kSessions] = {}, total_rows = 0;
     for (uint32_t i = 0; i < n_sessions; ++i) {
         const TTDecodeSession &s = sessions[i];
-        SinkRowsForm::Session &d = f.session[i];
+        typename Form::Session &d = f.session[i];
         d.seq_len = s.seq_len; d.q_rows = s.q_rows;
         d.windowed = s.seq_len > form.window && s.seq_len - form.window > form.sink ? 1u : 0u;
         d.base = d.windowed ? s.kv_start : 0u;
@@ -699,7 +718,7 @@ static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecode
         partial += d.n_parts * s.q_rows * q.n_q_heads;
         parts = std::max(parts, d.n_parts);
         if (lens[g] == 0) continue;
-        const SinkRowsForm::Session &e = f.session[x];
+        const typename Form::Session &e = f.session[x];
         const uint64_t cached = s.ring_capacity != 0 ? std::min<uint64_t>(s.seq_len, (uint64_t)form.sink + s.ring_capacity) : s.seq_len;
         const uint64_t sinks = std::max<uint64_t>(1, std::min<uint64_t>(form.sink, cached));
         const uint64_t behind = form.sink + (uint64_t)(s.seq_len - e.base - e.straight);
@@ -707,8 +726,8 @@ static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecode
             return tt_make_tensor_map_2d(reinterpret_cast<CUtensorMap *>(map), from, q.io_dtype, width, count, q.kv_token_stride_elements, 64);
         };
         if (!encode(f.table.maps[g].m[0], s.k, cached) || !encode(f.table.maps[g].m[1], s.v, (uint64_t)e.first_row + e.straight) ||
-            !encode(f.table.maps[kSinkRowSessions + x].m[0], s.v, sinks) ||
-            !encode(f.table.maps[kSinkRowSessions + x].m[1], s.v, std::max<uint64_t>(1, std::min(behind, cached))))
+            !encode(f.table.maps[kSessions + x].m[0], s.v, sinks) ||
+            !encode(f.table.maps[kSessions + x].m[1], s.v, std::max<uint64_t>(1, std::min(behind, cached))))
             return tt_set_error(ctx, TT_ERR_CUDA, "cuTensorMapEncodeTiled failed for the decode operands");
     }
     f.part_o = ctx->partials; f.part_m = f.part_o + (size_t)partial * q.head_dim; f.part_l = f.part_m + partial;
@@ -738,9 +757,11 @@ static int launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecode
 // of the rows' windows behind the sinks.
 int tt_launch_sink_rows(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *sessions, uint32_t n_sessions, const TTDecodeForm &form,
                         const tt_attn_batch_params *p) {
-    const uint32_t passes = ceil_div(n_sessions, kSinkRowSessions), each = ceil_div(n_sessions, passes);
+    const uint32_t passes = ceil_div(n_sessions, SinkRowsForm<kTableGroups>::kSessions), each = ceil_div(n_sessions, passes);
     for (uint32_t i = 0; i < n_sessions; i += each) {
-        const int rc = launch_sink_rows(ctx, stream, sessions + i, std::min(each, n_sessions - i), form, p);
+        const uint32_t n = std::min(each, n_sessions - i);
+        const int rc = n <= SinkRowsForm<kFewGroups>::kSessions ? launch_sink_rows<kFewGroups>(ctx, stream, sessions + i, n, form, p)
+                                                               : launch_sink_rows<kTableGroups>(ctx, stream, sessions + i, n, form, p);
         if (rc != TT_OK) return rc;
     }
     return TT_OK;
