@@ -135,3 +135,9 @@ def test_prefix_tables_on_both_sides_of_their_sizes(sessions):
 def test_draft_rows_on_both_sides_of_the_table_sizes(sessions):
     run_sink_decode(128, 16, 2, F16, 4, [700 + 31 * (i % 9) for i in range(sessions)], 4, 400, 0)
     run_sink_decode(256, 16, 2, BF16, 3, [900 + 31 * (i % 9) for i in range(sessions)], 3, 300, 333)
+
+
+# Own rows in a pass of their own whose streams leave the machine four places each, two, or one, and heads of all sizes.
+@pytest.mark.parametrize("hd,hq,hkv,n", [(256, 8, 4, 33), (256, 8, 4, 64), (256, 8, 8, 64), (128, 8, 8, 40), (128, 3, 3, 40), (64, 8, 8, 64), (64, 3, 1, 64)])
+def test_prefix_streams_of_own_rows(hd, hq, hkv, n):
+    run_prefix(hd, hq, hkv, F16, [140], [n], [1] * n, [[3, 900, 64, 65, 400][i % 5] + i for i in range(n)])

@@ -827,6 +827,24 @@ static bool plan_wide(tt_context *ctx, const TTDecodeSession *in_sessions, uint3
 // mode 0: write normalised outputs to the sessions' `out`; mode 1: one merged triple for a
 // single session (m_out/d_out/o_out); mode 2: a single one-row session whose local merge is fused
 // with the cross-GPU exchange (`exchange`).
+// Waves of items of the sessions' own rows behind shared prefixes. Three waves, plan_splits' own rule for ragged sessions, make items
+// of 64 keys of what usually follows a prefix, some hundred keys, whose start-up and partials cost more than the balance is
+// worth; one wave cannot balance streams that fill the machine. Whole calls behind 2000 shared keys, us, with 1 / 2 / 3 waves:
+//   head_dim 256, 2 KV heads, 64 sessions (4.6 places a stream) of 1..1024 keys 30 / 32 / 32, of 256..4096 53 / 54 / 57, of
+//   1024..32768 186 / 185 / 184; 100 sessions (3 places) 48 / 51 / 54, 80 / 82 / 84, 340 / 322 / 320; 8 KV heads, 64 sessions
+//   (1.2 places) 87 / 68 / 64, 272 / 155 / 145, 1352 / 899 / 812;
+//   head_dim 128, where more than two CTAs of two heads fit an SM: 8 KV heads, 64 sessions 83 / 43 / 48, 245 / 89 / 103,
+//   1667 / 457 / 557; one KV head, 100 sessions 36 / 32 / 32, 48 / 51 / 49, 160 / 162 / 128; head_dim 64, 2 KV heads, 64 sessions 26 / 19 / 19,
+//   49 / 32 / 27, 201 / 112 / 81.
+static uint32_t waves_behind_prefix(const uint32_t *rows, uint32_t n_sessions, const tt_attn_batch_params *p, uint32_t sm_count, uint32_t hpc) {
+    const uint32_t group = p->n_q_heads / p->n_kv_heads;
+    if (p->head_dim < 256) return p->head_dim == 128 && hpc == 2 ? 2u : 3u;
+    uint64_t streams = 0;
+    for (uint32_t i = 0; i < n_sessions; ++i) streams += (uint64_t)(p->n_kv_heads / hpc) * ceil_div_u32((uint64_t)rows[i] * group, 16);
+    const uint64_t slots = (uint64_t)sm_count * (4u / hpc);
+    return streams * 4 <= slots ? 1u : streams * 2 <= slots ? 2u : 3u;
+}
+
 int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession *in_sessions,
                      uint32_t n_sessions, const tt_attn_batch_params *p, int mode, float *m_out,
                      float *d_out, float *o_out, const TTKvQuant *quant, const tt_attn_exchange *exchange,
@@ -928,10 +946,7 @@ int tt_launch_decode(tt_context *ctx, cudaStream_t stream, const TTDecodeSession
     if (!wide) {
         int rc = plan_splits(keys, rows, n_sessions, p->head_dim, p->n_q_heads, p->n_kv_heads, (uint32_t)ctx->sm_count,
                              partial_bytes, hpc, &keys_per_item, &n_items,
-                             // sessions of some hundred keys (what follows a shared prefix): three waves would be items of
-                             // 64 keys, whose start-up and partials cost more than the balance is worth (64 sessions of
-                             // 1..1024 keys behind 32768 shared ones: 63.5 us a call, 60.2 us with one wave)
-                             form != nullptr && form->short_sessions ? 1u : 3u);
+                             form != nullptr && form->short_sessions ? waves_behind_prefix(rows, n_sessions, p, (uint32_t)ctx->sm_count, hpc) : 3u);
         if (rc != TT_OK) return tt_set_error(ctx, rc, "split-KV partials do not fit the context workspace");
         if (!in_params && n_items > ctx->max_items)
             return tt_set_error(ctx, TT_ERR_OOM, "%u work items exceed the context's item table (%u)", n_items,

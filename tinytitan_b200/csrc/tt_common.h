@@ -201,7 +201,7 @@ struct TTDecodeForm {
     uint32_t sink = 0, window = 0;   // kPassSink
     size_t reserved_bytes = 0;       // the end of the workspace, which the caller keeps for itself
     bool partials_only = false;      // leave the split partials for the caller to merge
-    bool short_sessions = false;     // split into one wave of items at most (see plan_splits)
+    bool short_sessions = false;     // the rows behind a shared prefix (see waves_behind_prefix)
     // out: where this call's partials are
     float *part_o = nullptr, *part_m = nullptr, *part_l = nullptr;
     float *part_m2 = nullptr, *part_l2 = nullptr;   // kPassScores
