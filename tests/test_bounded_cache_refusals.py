@@ -224,3 +224,17 @@ def test_plain_decode_takes_session_tables():
     assert n == 3 and [s.seq_len for s in words] == [4, 5, 6] and {s.q_rows for s in words} == {2}
     assert (p.kv_token_stride_elements, p.q_row_stride_elements, p.io_dtype) == (192, 512, tt.TT_F16)
     assert a.prepare_batch(sessions(torch.zeros(0, 20, 2, 64, dtype=H), queries(0)), 64, 8, 2)[1] == 0
+
+
+def test_evictions_into_one_buffer_are_refused():
+    k, v, w, one = cache(), cache(), torch.zeros(3, 2, 20), cache(rows=8)
+
+    def evict(k, v, **kw):
+        tt.evict_kv_rows(HostContext(), k, v, w, 20, 8, **kw)
+    refused(evict, k, v, k_out=one, v_out=one)
+    refused(evict, k, v, k_out=v)
+    refused(evict, k, v, v_out=k)
+    reaches_the_library(evict, k, k)                             # keys that are the values too
+    reaches_the_library(evict, k, k, k_out=one, v_out=one)
+    reaches_the_library(evict, k, v, k_out=k, v_out=v)
+    reaches_the_library(evict, k, v, k_out=one)

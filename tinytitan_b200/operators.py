@@ -755,6 +755,9 @@ def evict_kv_rows(context: Context, k, v, weights, rows, budget: int, sink_token
             at_k = (k_out.data_ptr(), 2 * a_strides[0])
         if v_out is not None:
             at_v = (v_out.data_ptr(), 2 * b_strides[0])
+    to_k, to_v = k if k_out is None else k_out, v if v_out is None else v_out
+    if kept and to_k.data_ptr() == to_v.data_ptr() and k.data_ptr() != v.data_ptr():
+        _refuse("K and V would go to one place")
     # the statistic and the positions, then where they go
     stat, at_w = _statistic("weights", weights, "torch.float32", n, num_kv_heads, context, weights_out is None)
     at_p, at_wo, at_po, stat_out = _nowhere, _nowhere, _nowhere, None
