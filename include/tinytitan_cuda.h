@@ -371,7 +371,8 @@ int tt_attn_prefill_causal_selected(tt_context *ctx, tt_stream stream, const voi
  * 256 for decode. Batches of any size up to max_sessions; during a stream capture, decode batches of
  * up to 64 sessions (8 prefix groups), whose tables travel in the kernel parameters (larger ones
  * are refused with TT_ERR_UNSUPPORTED_SHAPE where their tables would be uploaded; accumulate and
- * evict take any). Captured calls use the
+ * evict take any number of sessions, captured or not, in as many launches as that needs, and a call of
+ * theirs that is refused has changed nothing). Captured calls use the
  * context's workspace when replayed: like calls, graphs of one context must not overlap on the GPU. */
 
 /* The tables of these calls (tt_attn_session, tt_attn_prefix, tt_attn_weight_rows, tt_kv_evict_session)
@@ -385,7 +386,8 @@ void tt_table_fill(uint64_t *words, uint32_t n, uint32_t width, uint32_t spare, 
  * (j < sink_tokens or j >= e - window); window 0 = no window. A row without visible keys gives
  * zeros. Key j is cache row j, or with ring_capacity R > 0 (window > 0 then) row
  * j < sink_tokens ? j : sink_tokens + (j - sink_tokens) % R, a cache of sink_tokens + R rows for an
- * endless session; R >= window + q_rows - 1 once a session has wrapped. kv_start must be 0. Cache
+ * endless session; R >= window + q_rows - 1 once a session has wrapped, and the same R in every call
+ * over a cache. kv_start must be 0. Cache
  * rows that no query row sees are not read and may hold anything. */
 int tt_attn_decode_sink_window(tt_context *ctx, tt_stream stream, const tt_attn_session *sessions,
                                uint32_t n_sessions, const tt_attn_batch_params *params,

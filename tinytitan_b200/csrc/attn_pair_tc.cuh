@@ -20,8 +20,8 @@
 // groups of four warps take the tiles in turn and hand the running maximum on, as in attn_rows_tc.cuh.
 //
 // Measured: 2600 clocks a tile behind a prefix of 32768 keys, 2400 in a prompt's chunk whose keys are in L2 (the products
-// alone 2130; TMA writes and the weights' stores share the port they are read through), 0.83 of the sustained rate of a
-// library product of 8192^3 over a prompt of 8192 tokens, and 13,000 to 15,000 clocks an item besides its tiles: 3300 to the
+// alone 2130; TMA writes and the weights' stores share the port they are read through), 212 to 247 us over a prompt of 8192
+// tokens on different machines, 0.83 to 0.71 of the sustained rate of a library product of 8192^3, and 13,000 to 15,000 clocks an item besides its tiles: 3300 to the
 // cluster barrier, 1100 for Q, 3500 to 5000 to the first scores, 5500 for the output.
 //
 // Every mbarrier wait is bounded; all threads of both CTAs meet at the cluster barrier before TMEM is released.

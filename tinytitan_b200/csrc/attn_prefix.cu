@@ -617,7 +617,7 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
     // The sessions' own rows as groups of one session each in the prefix pass: one launch less, no second pass that starts
     // when the first one ends, and the tensor cores for draft rows. Up to 16 sessions always: 4 of short keys 18.5 -> 13 us,
     // 16 of 4000 to 8000 keys 52 -> 48, of 4 rows of 16 heads 176 -> 82. Up to 64, whose maps and groups make the parameters
-    // 26 KB (10 us more of host time), with more than the 16 packed rows a split-KV item takes: 64 sessions of 4 rows and 800
+    // 25 KB (8 us more of host time than 16 sessions), with more than the 16 packed rows a split-KV item takes: 64 sessions of 4 rows and 800
     // to 1600 keys 220 -> 123 us, of 4 to 300 98 -> 94. Up to 32 otherwise unless a few rows would have items of 256:
     // head_dim 128, 32 sessions of 800 to 1600 keys 29 -> 23; head_dim 256, 16/2 heads, 4000 to 8000 keys 79 -> 115.
     bool fused = in_params && n_sessions <= 16;
