@@ -615,22 +615,31 @@ TT_API int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const
                             "more than %u groups or %u sessions cannot be captured: their tables are uploaded from host memory",
                             kParamGroups, kParamSessions);
     // The sessions' own rows as groups of one session each in the prefix pass: one launch less, no second pass that starts
-    // when the first one ends, and the tensor cores for draft rows. Up to 16 sessions always: 4 of short keys 18.5 -> 13 us,
-    // 16 of 4000 to 8000 keys 52 -> 48, of 4 rows of 16 heads 176 -> 82. Up to 64, whose maps and groups make the parameters
-    // 25 KB (8 us more of host time than 16 sessions), with more than the 16 packed rows a split-KV item takes: 64 sessions of 4 rows and 800
-    // to 1600 keys 220 -> 123 us, of 4 to 300 98 -> 94. Up to 32 otherwise unless a few rows would have items of 256:
-    // head_dim 128, 32 sessions of 800 to 1600 keys 29 -> 23; head_dim 256, 16/2 heads, 4000 to 8000 keys 79 -> 115.
-    bool fused = in_params && n_sessions <= 16;
-    if (in_params && !fused) {
-        uint32_t group_rows = 0, most_rows = 0, most_own = 0;
+    // when the first one ends, and the tensor cores for draft rows. Us a call with a pass of their own, then so:
+    //   more than the 16 packed rows a split-KV item takes, up to 64 sessions (whose maps and groups make the parameters 25 KB,
+    //     8 us more of host time than 16 sessions): 16 sessions of 4 rows of 16 heads 176, 82; 64 of 4 rows and 800 to 1600
+    //     keys 220, 123, of 4 to 300 98, 94;
+    //   head_dim 256: up to 16 sessions (4 of short keys 18.5, 13; 16 of 4000 to 8000 46, 43, with 8 KV heads 122, 118), and up to
+    //     32 where items of 128 rows do (8 KV heads, 32 of 1 to 1024 keys 42, 44, of 1024 to 32768 389, 380) but not of 256 (2
+    //     KV heads, 32 of 4000 to 8000 76, 101);
+    //   head_dim 64 and 128: up to 32 sessions whose streams, one a KV head, leave half of the SMs free (128, 2 KV heads, 32 of
+    //     800 to 1600 keys 26, 19; 8 KV heads, 8 of 4000 to 8000 69, 45, but 10 50, 56 and 24 100, 130; 64, 8 KV heads, 8 33,
+    //     20, 24 of 800 to 1600 25, 31), or up to one an SM of at most 1024 keys (4 KV heads, 24 20.5, 19.0; 8, 16 20.3, 21.0, of 64 17.8, 16.5).
+    bool fused = false;
+    if (in_params) {
+        uint32_t group_rows = 0, most_rows = 0, most_own = 0, longest = 0;
         for (uint32_t g = 0, i = 0; g < n_groups; ++g, group_rows = 0)
             for (uint32_t x = 0; x < groups[g].n_sessions; ++x, ++i) {
                 group_rows += sessions[i].q_rows;
                 most_rows = std::max(most_rows, group_rows);
                 most_own = std::max(most_own, sessions[i].q_rows);
+                longest = std::max(longest, sessions[i].seq_len);
             }
-        const uint32_t heads = q.n_q_heads / q.n_kv_heads, rows_tile = rows_per_tile(&most_rows, 1, heads, q.head_dim);
-        fused = most_own * heads > 16 || (n_sessions <= 32 && rows_tile < 256);
+        const uint32_t heads = q.n_q_heads / q.n_kv_heads, sms = (uint32_t)ctx->sm_count;
+        const uint64_t streams = (uint64_t)n_sessions * q.n_kv_heads;
+        fused = most_own * heads > 16 ? true
+                : q.head_dim == 256 ? n_sessions <= 16 || (n_sessions <= 32 && rows_per_tile(&most_rows, 1, heads, q.head_dim) < 256)
+                                    : n_sessions <= 32 && (streams * 2 <= sms || (streams <= sms && longest <= 1024));
     }
     return !in_params || n_groups + (fused ? n_sessions : 0u) <= kFewGroups
                ? shared_prefix<kFewGroups>(ctx, stream, groups, n_groups, sessions, n_sessions, params, in_params, fused)
