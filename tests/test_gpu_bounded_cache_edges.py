@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import tinytitan_b200 as tt
-from bounded_cache_reference import attend
+from bounded_cache_reference import attend, sink_keys
 from gpu_util import context
 from test_gpu_bounded_cache import BF16, F16, NAN, check, normal, run_accumulate, run_evict, run_prefix, run_sink_decode
 
@@ -141,3 +141,112 @@ def test_draft_rows_on_both_sides_of_the_table_sizes(sessions):
 @pytest.mark.parametrize("hd,hq,hkv,n", [(256, 8, 4, 33), (256, 8, 4, 64), (256, 8, 8, 64), (128, 8, 8, 40), (128, 3, 3, 40), (64, 8, 8, 64), (64, 3, 1, 64)])
 def test_prefix_streams_of_own_rows(hd, hq, hkv, n):
     run_prefix(hd, hq, hkv, F16, [140], [n], [1] * n, [[3, 900, 64, 65, 400][i % 5] + i for i in range(n)])
+
+
+# ------------------------------------------------------------------ caches of more than 4 GiB (rows of 1 KB)
+
+LONG = 4_300_000
+
+
+@pytest.fixture(scope="module")
+def long_cache():
+    cache = [torch.empty(LONG, 2, 256, dtype=F16, device="cuda") for _ in range(2)]
+    yield cache
+    cache.clear()
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("hq", [8, 16])
+def test_sink_decode_beyond_four_gigabytes(long_cache, hq, rows):
+    hd, hkv, sink, window = 256, 2, 5, 700
+    k, v = normal(1, window + rows, hkv, hd), normal(2, window + rows, hkv, hd)
+    ks, vs, q = normal(3, sink, hkv, hd), normal(4, sink, hkv, hd), normal(5, rows, hq, hd)
+    first = LONG - window - rows
+    for cache, near, far in ((long_cache[0], ks, k), (long_cache[1], vs, v)):
+        cache[:sink], cache[first:] = near.cuda(), far.cuda()
+        cache[sink:first:1009] = NAN
+    out = torch.empty(1, rows, hq, hd, dtype=F16, device="cuda")
+    t = tt.SessionTable.over_cache(q.cuda()[None], out, long_cache[0][None], long_cache[1][None], LONG)
+    tt.Attention(context()).encode_sink_window(t, hd, hq, hkv, sink, window)
+    torch.cuda.synchronize()
+    assert context().poll_status() == 0
+    for r in range(rows):
+        at = torch.tensor([j - first for j in sink_keys(LONG - (rows - 1 - r), sink, window) if j >= sink])
+        o, _, bound = attend(q[r], torch.cat([ks, k[at]]), torch.cat([vs, v[at]]))
+        check(out[0, r], o, bound)
+
+
+def test_sink_prefill_beyond_four_gigabytes(long_cache):
+    hd, hq, hkv, sink, window, tokens = 256, 8, 2, 70, 300, 50
+    start = LONG - tokens
+    first = start + 1 - window
+    k, v = normal(1, LONG - first, hkv, hd), normal(2, LONG - first, hkv, hd)
+    ks, vs, q = normal(3, sink, hkv, hd), normal(4, sink, hkv, hd), normal(5, tokens, hq, hd)
+    for cache, near, far in ((long_cache[0], ks, k), (long_cache[1], vs, v)):
+        cache[:sink], cache[first:] = near.cuda(), far.cuda()
+    out = torch.empty(tokens, hq, hd, dtype=F16, device="cuda")
+    p = tt.PrefillAttentionParams(start, tokens, hd, hq, hkv, LONG, window, hkv * hd, hq * hd, hq * hd, hd ** -0.5)
+    tt.PrefillAttention(context()).encode_sink_window(q.cuda(), long_cache[0], long_cache[1], out, p, sink)
+    torch.cuda.synchronize()
+    assert context().poll_status() == 0
+    for t in (0, 1, 31, 32, 49):
+        at = torch.tensor([j - first for j in sink_keys(start + t + 1, sink, window) if j >= sink])
+        o, _, bound = attend(q[t], torch.cat([ks, k[at]]), torch.cat([vs, v[at]]))
+        check(out[t], o, bound)
+
+
+def test_prefix_and_accumulate_beyond_four_gigabytes(long_cache):
+    # all keys but a few near the end score far below them: the few weigh everything, the others nothing
+    hd, hq, hkv = 256, 8, 2
+    few = torch.tensor([LONG - 1, LONG - 2, LONG - 130, LONG - 5000])
+    q, kf, vf = normal(5, hq, hd), normal(6, len(few), hkv, hd), normal(7, len(few), hkv, hd)
+    q[:, 0], kf[:, :, 0] = 16.0, 16.0                                # a score of 16 against one of -160 * 16 / 16
+    for cache in long_cache:
+        cache.zero_()
+    long_cache[0][:, :, 0] = -160.0
+    long_cache[0][few.cuda()], long_cache[1][few.cuda()] = kf.cuda(), vf.cuda()
+    out = torch.empty(2, 1, 1, hq, hd, dtype=F16, device="cuda")
+    ctx = tt.Context(0, workspace_bytes=1 << 30)                     # the scores of so many keys
+    a, qd, w = tt.Attention(ctx), q.cuda()[None, None], torch.zeros(1, hkv, LONG, device="cuda")
+    k, v = long_cache[0][None], long_cache[1][None]
+    a.encode_shared_prefix(tt.PrefixTable.over_cache(k, v, LONG, 1), tt.SessionTable.over_cache(qd, out[0], k, v, 0), hd, hq, hkv)
+    a.encode_accumulate(tt.SessionTable.over_cache(qd, out[1], k, v, LONG), w, hd, hq, hkv)
+    torch.cuda.synchronize()
+    assert ctx.poll_status() == 0
+    o, p, bound = attend(q, kf, vf)
+    added = p.reshape(hkv, hq // hkv, -1).sum(1)
+    assert (p > 0).all()
+    for x in out:
+        check(x[0, 0], o, bound)
+    # 32-bit scores, exponentials and normaliser (2e-5, see attend); exp(-160) is below every 32-bit number that counts
+    assert ((w[0].cpu()[:, few].double() - added).abs() <= 2e-5 * added + 1e-30).all()
+    w[0][:, few.cuda()] = 0
+    assert (w < 1e-30).all()
+    ctx.close()
+
+
+def test_evict_beyond_four_gigabytes(long_cache):
+    given_up, budget = 100_000, LONG - 100_000
+    row = torch.arange(LONG, device="cuda")
+    for cache, shift in zip(long_cache, (0, 1)):
+        for h in range(2):
+            for digit in range(3):                                   # rows by their digits to the base 256
+                cache[:, h, digit] = ((row + shift + h >> 8 * digit) & 255).half()
+    w = torch.rand(1, 2, LONG, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    before, p = w.clone(), torch.zeros(1, 2, LONG, dtype=torch.int32, device="cuda")
+    ctx = tt.Context(0)
+    tt.evict_kv_rows(ctx, long_cache[0][None], long_cache[1][None], w, LONG, budget, positions_out=p)
+    torch.cuda.synchronize()
+    assert ctx.poll_status() == 0
+    for h in range(2):
+        order = before[0, h].sort(descending=True, stable=True).indices[:budget]
+        keep = torch.zeros(LONG, dtype=torch.bool, device="cuda")
+        keep[order] = True
+        src, fills = row[:budget].clone(), row[keep & (row >= budget)]
+        src[~keep[:budget]] = fills
+        assert len(fills) and torch.equal(p[0, h, :budget].long(), src) and torch.equal(w[0, h, :budget], before[0, h, src])
+        for cache, shift in zip(long_cache, (0, 1)):
+            held = sum(cache[:budget, h, digit].long() << 8 * digit for digit in range(3))
+            assert torch.equal(held, src + shift + h)
+    ctx.close()
