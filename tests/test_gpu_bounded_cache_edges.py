@@ -250,3 +250,52 @@ def test_evict_beyond_four_gigabytes(long_cache):
             held = sum(cache[:budget, h, digit].long() << 8 * digit for digit in range(3))
             assert torch.equal(held, src + shift + h)
     ctx.close()
+
+
+# ------------------------------------------------------------------ layouts
+
+@pytest.mark.parametrize("layout", ["interleaved", "token-major"])
+@pytest.mark.parametrize("rows", [1, 4])
+def test_layouts_give_the_same_bits(layout, rows):
+    """K beside V in every row, or the sessions' rows side by side: what the contiguous cache gives, bit for bit."""
+    n, cap, hq, hkv, hd = 4, 300, 16, 2, 256
+    q, k, v, w0 = normal(1, n, rows, hq, hd).cuda(), normal(2, n, cap, hkv, hd).cuda(), normal(3, n, cap, hkv, hd).cuda(), torch.rand(n, hkv, cap, generator=torch.Generator().manual_seed(4)).cuda()
+    lens, a = [300, 77, 200, rows], tt.Attention(context())
+
+    def lay(x, y):
+        if layout == "interleaved":
+            both = torch.stack([x, y], dim=2)
+            return both[:, :, 0], both[:, :, 1]
+        return tuple(t.transpose(0, 1).contiguous().transpose(0, 1) for t in (x, y))
+    got = []
+    for kk, vv in ((k.clone(), v.clone()), lay(k, v)):
+        outs, w = [torch.zeros_like(q) for _ in range(4)], w0.clone()
+        table = [tt.SessionTable.over_cache(q, o, kk, vv, lens) for o in outs]
+        a.encode_sink_window(table[0], hd, hq, hkv, 4, 100)
+        a.encode_shared_prefix(tt.PrefixTable.over_cache(kk[1:2], vv[1:2], 250, n), table[1], hd, hq, hkv)
+        a.encode_accumulate(table[2], w, hd, hq, hkv, fresh_rows=rows)
+        a.encode_batched(table[3], hd, hq, hkv)
+        tt.evict_kv_rows(context(), kk, vv, w, lens, 90, 2, 10)
+        torch.cuda.synchronize()
+        assert context().poll_status() == 0
+        got.append(outs + [w, kk.contiguous(), vv.contiguous()])
+    assert all(x.any() and torch.equal(x, y) for x, y in zip(*got))
+
+
+def test_sessions_that_read_one_slot():
+    # the branches of one search: several sessions over one slot, each with queries and a length of its own
+    n, cap, hq, hkv, hd, slots, lens = 5, 200, 8, 2, 128, [1, 1, 0, 1, 0], [200, 150, 33, 150, 200]
+    q, k, v, a = normal(1, n, 1, hq, hd), normal(2, 2, cap, hkv, hd), normal(3, 2, cap, hkv, hd), tt.Attention(context())
+    d = [x.cuda() for x in (q, k, v)]
+    out, w = [torch.zeros_like(d[0]) for _ in range(2)], torch.zeros(n, hkv, cap, device="cuda")
+    a.encode_sink_window(tt.SessionTable.over_cache(d[0], out[0], d[1], d[2], lens, slots=slots), hd, hq, hkv, 3, 60)
+    a.encode_accumulate(tt.SessionTable.over_cache(d[0], out[1], d[1], d[2], lens, slots=slots), w, hd, hq, hkv)
+    torch.cuda.synchronize()
+    for i in range(n):
+        at = torch.tensor(sink_keys(lens[i], 3, 60))
+        o, _, bound = attend(q[i, 0], k[slots[i], at], v[slots[i], at])
+        check(out[0][i, 0], o, bound)
+        o, p, bound = attend(q[i, 0], k[slots[i], :lens[i]], v[slots[i], :lens[i]])
+        check(out[1][i, 0], o, bound)
+        added = p.reshape(hkv, hq // hkv, -1).sum(1)             # 32-bit scores to normaliser 2e-5 (see attend), four sums of 2^-24
+        assert ((w[i, :, :lens[i]].cpu().double() - added).abs() <= (2e-5 + 5 * 2.0 ** -24) * added).all()
