@@ -425,7 +425,7 @@ int tt_attn_decode_shared_prefix(tt_context *ctx, tt_stream stream, const tt_att
                                  uint32_t n_sessions, const tt_attn_batch_params *params);
 /* The split of the prefix pass (host arithmetic): keys per work item (a multiple of 128) for groups
  * of the given prefix lengths and query rows (sessions x q_rows), and the number of items. Where
- * the sessions' own rows join that pass (up to 16 sessions, or 64 with draft rows), each is one more group.
+ * the sessions' own rows join that pass (draft rows, and batches of few sessions), each is one more group.
  * TT_ERR_OOM when the partials do not fit workspace_bytes (0 = no limit). */
 int tt_attn_plan_prefix_splits(const uint32_t *prefix_lens, const uint32_t *query_rows,
                                uint32_t n_groups, uint32_t head_dim, uint32_t n_q_heads,
